@@ -189,8 +189,9 @@ def _in_8bit(x):
     full[:, :cols] = x
     full = full.view(rows, groups, 128)
     amax = full.abs().amax(-1, keepdim=True).clamp_min(1e-12)
-    codes = (full * (448.0 / amax)).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
-    return (codes.float() * (amax / 448.0)).view(rows, groups * 128)[:, :cols]
+    most = torch.full_like(amax, 448.0)      # (two divisions of tensors: a division by or of a number is a product with a reciprocal)
+    codes = (full * (most / amax)).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
+    return (codes.float() * (amax / most)).view(rows, groups * 128)[:, :cols]
 
 
 def _plain(s):
