@@ -16,8 +16,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "hpfp8", "libhpfp8.so")
 NATIVE = os.path.join(HERE, "hpfp8", "_native.so")
 NATIVE_SOURCE = os.path.join(CSRC, "torch_ops.cpp")
-SOURCES = ["capi.hip", "quantize.hip", "bucket.hip", "grouped.hip", "gemm.hip", "gemm_skinny.hip"]
-HEADERS = ["gemm_skinny.h", "gemm_tile.h", "hpfp8_device.h", "hpfp8_host.h", os.path.join("..", "..", "include", "hpfp8.h")]
+SOURCES = ["capi.hip", "quantize.hip", "bucket.hip", "grouped.hip", "gemm.hip", "gemm_skinny.hip", "activation.hip", "norm.hip", "cross_entropy.hip"]
+HEADERS = ["rows.h", "gemm_skinny.h", "gemm_tile.h", "hpfp8_device.h", "hpfp8_host.h", os.path.join("..", "..", "include", "hpfp8.h")]
 
 
 def _flags():

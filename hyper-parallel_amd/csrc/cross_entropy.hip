@@ -1,0 +1,607 @@
+// Softmax cross entropy of a linear's output over a large vocabulary, with its gradients, in pieces of the vocabulary: the logits
+// l = x W^T [tokens, vocab] exist as accumulators only.
+//
+//   lse = log sum_v exp(l_v),  loss = lse - (1 - s) l_target - s mean_v(l_v)                 (s: label smoothing)
+//   dl  = c (exp(l - lse) - s / V - (1 - s) [v = target]),  dx = dl W,  dW = dl^T x          (c: the row's share of the loss's gradient)
+//
+// Forward: one product whose tiles leave, for each row and 128 columns, the largest logit and the sum of exp(l - largest) in fp32; a second
+// launch joins them.  Backward, a piece of the vocabulary at a time: the same product again, whose tiles leave dl rounded to bf16 (8
+// bits of a value that is a difference of probabilities: an error of 2^-9 relative in each of dx's and dW's summands, and half of that of the
+// result's own rounding in their sum), row-major and transposed, then both gradients in one launch.  Recomputing the logits is a quarter of the
+// step's products; keeping them would be tokens x vocab.
+//
+// All three are one kernel: c[m, n] = sum_k a[m, k] b[n, k] in bf16 with both operands contiguous along k, 256 x 256 tiles, 8 waves
+// of 64 x 128, v_mfma_f32_16x16x32_bf16.  64 values of k are 128 bytes of a row: LDS holds two such slabs of a and three of b, written
+// by direct loads (rows past the end read as zeros) with 16-byte chunks swizzled by row, so that fragments are read without bank conflicts.
+// The rows of a slab are permuted on their way into LDS so that a lane's sums are four neighbouring rows by eight neighbouring
+// columns: results leave as 16 bytes of a row, transposed ones as 8 bytes of a column, without a pass through LDS.
+#include "gemm_tile.h"
+#include "hpfp8_host.h"
+
+namespace hpfp8 {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4_st __attribute__((ext_vector_type(4)));
+
+constexpr int kTile = 256;
+constexpr int kSlab = 64;                     // values of k in a slab: 128 bytes of a row
+constexpr int kSlabBytes = kTile * 2 * kSlab;
+constexpr float kLog2e = 1.44269504f;
+
+enum Epilogue { kStats = 0, kDlogits = 1, kGrads = 2 };
+enum Store { kBf16 = 0, kF32 = 1, kF32Add = 2 };
+
+// One product c[M, N] = a[M, K] b[N, K]^T; lda and ldb in bytes.
+struct Product {
+  const uint8_t* a;
+  const uint8_t* b;
+  int64_t lda, ldb;
+  int M, N, K;
+  void* c;
+  int64_t ldc;           // elements
+  int store;
+  int tiles;
+};
+
+struct CeParams {
+  Product part[2];       // (kGrads: two products that share the grid; otherwise the first alone)
+  // kStats
+  float2* stats;         // [2 tiles of N][rows_padded] largest logit and sum
+  float* sums;           // the same for the sum of the logits, or null
+  float* target_logit;   // [M]
+  // kStats and kDlogits
+  const int64_t* target; // [M]
+  int64_t rows_padded;
+  // kDlogits
+  const float* lse;      // [M]
+  const float* grad;     // of the loss: one value, or one for each row with stride grad_stride
+  int64_t grad_stride;
+  const float* count;    // rows that count, when the loss is their mean; null otherwise
+  int64_t ignore_index;
+  float smoothing;
+  int64_t vocab;         // the whole of it
+  int64_t first;         // the piece's first column
+  uint16_t* dl;          // [rows_padded][ld_dl]
+  int64_t ld_dl;
+  uint16_t* dl_t;        // [N padded][rows_padded]
+};
+
+// Tile number -> (m tile, n tile): consecutive numbers cover rectangles of 32 tiles, an XCD's compute units at any moment, so that its L2
+// serves each slab to several of them; the longer side of the rectangle goes along the shorter side of the grid.
+__device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int gm = tiles_m > tiles_n ? 4 : 8, gn_full = 32 / gm;
+  const int per = gn_full * tiles_m;
+  const int ng = t / per, rest = t - ng * per;
+  const int gn = tiles_n - ng * gn_full < gn_full ? tiles_n - ng * gn_full : gn_full;
+  const int mg = rest / (gm * gn), r = rest - mg * gm * gn;
+  tm = mg * gm + r / gn;
+  tn = ng * gn_full + r % gn;
+}
+
+// The XCD that a workgroup runs on gets a contiguous run of the tiles.
+__device__ __forceinline__ int tile_of_workgroup(int pid, int tiles) {
+  const int xcd = pid % kXcds, i = pid / kXcds, base = tiles / kXcds, more = tiles % kXcds;
+  return xcd * base + (xcd < more ? xcd : more) + i;
+}
+
+// column (of the wave's 128) of sum r of subtile i in the lanes of group g, and the row of b that therefore goes to row p of LDS
+__device__ __forceinline__ int column_of(int i, int g, int r) { return 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r; }
+
+template <int EPI>
+__global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[5 * kSlabBytes];
+  uint8_t* const a_lds = lds;
+  uint8_t* const b_lds = lds + 2 * kSlabBytes;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pid = blockIdx.x;
+  const bool second = EPI == kGrads && pid >= p.part[0].tiles;
+  const Product q = second ? p.part[1] : p.part[0];
+  int tm, tn;
+  tile_at(tile_of_workgroup(second ? pid - p.part[0].tiles : pid, q.tiles), (q.M + kTile - 1) / kTile, (q.N + kTile - 1) / kTile, tm, tn);
+  const int m0 = tm * kTile, n0 = tn * kTile;
+  const int slabs = (q.K + kSlab - 1) / kSlab;
+
+  // ---- transfers: one is 8 rows x 128 bytes of LDS per wave, four per wave and slab
+  auto resource = [](const uint8_t* base, int64_t rows, int64_t ld, int K) {
+    const int64_t bytes = (rows - 1) * ld + (int64_t)K * 2;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(bytes < 0x7FFFF000 ? bytes : 0x7FFFF000), 0x00020000);
+  };
+  const __amdgpu_buffer_rsrc_t rsrc_a = resource(q.a + (int64_t)m0 * q.lda, q.M - m0, q.lda, q.K);
+  const __amdgpu_buffer_rsrc_t rsrc_b = resource(q.b + (int64_t)n0 * q.ldb, q.N - n0, q.ldb, q.K);
+  uint32_t a_off[4], b_off[4], past[2];
+  const int whole = q.K / kSlab;               // slabs that are not cut off by the end of k
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = (wave * 4 + i) * 8 + (lane >> 3);
+    const int chunk = (lane & 7) ^ row_swizzle(r);
+    const int ra = (r & ~63) + (r & 15) * 4 + ((r >> 4) & 3);
+    const int rb = (r & ~127) + column_of((r >> 4) & 7, (r >> 2) & 3, r & 3);
+    a_off[i] = (uint32_t)ra * (uint32_t)q.lda + chunk * 16;
+    b_off[i] = (uint32_t)rb * (uint32_t)q.ldb + chunk * 16;
+    // (a chunk behind the end of k is read from beyond the resource, as zeros; the swizzle has two patterns over i)
+    if (i < 2) past[i] = chunk * 8 >= q.K % kSlab ? 0x80000000u : 0u;
+  }
+  auto load = [&](const __amdgpu_buffer_rsrc_t& rs, uint32_t off, uint8_t* to, int slab, int i) {
+    // (behind the last slab the last one again: those are never used)
+    const int s = slab < slabs ? slab : slabs - 1;
+    const uint32_t o = off + (s >= whole ? past[i & 1] : 0u);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(to + (wave * 4 + i) * 1024), 16, o, s * 128, 0, 0);
+  };
+  auto load_a = [&](int buf, int slab, int i) { load(rsrc_a, a_off[i], a_lds + buf * kSlabBytes, slab, i); };
+  auto load_b = [&](int buf, int slab, int i) { load(rsrc_b, b_off[i], b_lds + buf * kSlabBytes, slab, i); };
+
+  const int wn = wave & 1, wm = wave >> 1, l16 = lane & 15, g = lane >> 4;
+  int frag_lo = l16 * 128 + ((2 * g) ^ row_swizzle(l16)) * 16, frag_hi = frag_lo ^ 16;
+  asm volatile("" : "+v"(frag_lo), "+v"(frag_hi));
+  const int a_frag = wm * 64 * 128, b_frag = wn * 128 * 128;
+
+  const v4f zero = {0.f, 0.f, 0.f, 0.f};
+  v4f acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = zero;
+
+  // ---- slab 0 of both, slab 1 of b, the first half of slab 1 of a
+#pragma unroll
+  for (int i = 0; i < 4; ++i) load_a(0, 0, i);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) load_b(0, 0, i);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) load_b(1, 1, i);
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0F70 | 4);      // all but the last four have landed
+  __syncthreads();
+  load_a(1, 1, 0);
+  load_a(1, 1, 1);
+
+  v8i xf[4], wf_n0, wf_n1;
+  wf_n0 = frag_read(b_lds + b_frag, frag_lo, frag_hi);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) xf[j] = frag_read(a_lds + a_frag + j * 16 * 128, frag_lo, frag_hi);
+  wf_n1 = frag_read(b_lds + b_frag + 16 * 128, frag_lo, frag_hi);
+
+  auto halves = [](const v8i& f, int h) {
+    return __builtin_bit_cast(bf16x8, v4i{f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]});
+  };
+  // One slab.  Its barrier sits before its last two subtiles: what follows it, the fragments of the next slab, is covered by the matrix
+  // instructions that are left.  Transfers, one per subtile: the rest of the next slab of a, the slab after next of b, and behind
+  // the barrier the first half of the slab after next of a into the buffer that every wave has just left.
+  int abuf = 0, bbuf = 0;
+  for (int s = 0; s < slabs; ++s) {
+    const int bnext = bbuf == 2 ? 0 : bbuf + 1, bnew = bnext == 2 ? 0 : bnext + 1;
+    const uint8_t* const bcur = b_lds + bbuf * kSlabBytes;
+    const uint8_t* const bnxt = b_lds + bnext * kSlabBytes;
+    const uint8_t* const anxt = a_lds + (abuf ^ 1) * kSlabBytes;
+    v8i wf[3];
+    wf[0] = wf_n0;
+    wf[1] = wf_n1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i == 6) {
+        __builtin_amdgcn_s_waitcnt(0x0070 | 4);         // vmcnt(4) lgkmcnt(0): b's slab after next may be under way
+        __builtin_amdgcn_s_barrier();
+      }
+      wf[(i + 2) % 3] = i < 6 ? frag_read(bcur + b_frag + (i + 2) * 16 * 128, frag_lo, frag_hi)
+                              : frag_read(bnxt + b_frag + (i - 6) * 16 * 128, frag_lo, frag_hi);
+      if (i < 2) load_a(abuf ^ 1, s + 1, i + 2);
+      else if (i < 6) load_b(bnew, s + 2, i - 2);
+      else load_a(abuf, s + 2, i - 6);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(halves(wf[i % 3], 0), halves(xf[j], 0), acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(halves(wf[i % 3], 1), halves(xf[j], 1), acc[i][j], 0, 0, 0);
+        if (i == 7) xf[j] = frag_read(anxt + a_frag + j * 16 * 128, frag_lo, frag_hi);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wf_n0 = wf[8 % 3];
+    wf_n1 = wf[9 % 3];
+    abuf ^= 1;
+    bbuf = bnext;
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);          // vmcnt(0): the last transfers write to this workgroup's LDS
+
+  // ---- the tile's sums: lane (l16, g) has rows m + j and columns n + column_of(i, g, r)
+  const int m = m0 + wm * 64 + l16 * 4, n = n0 + wn * 128;
+  const bool cut = n + 128 > q.N;              // columns behind the end (their sums are zeros)
+  if constexpr (EPI == kStats) {
+    float2 out[4];
+    float total[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t t = m + j < q.M ? p.target[m + j] : -1;
+      const int own = t >= 0 && t < q.N ? (int)t : -1;
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int c = n + column_of(i, g, r);
+          if (cut && c >= q.N) acc[i][j][r] = -INFINITY;
+          top = fmaxf(top, acc[i][j][r]);
+          if (own == c) p.target_logit[m + j] = acc[i][j][r];
+        }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float from = top == -INFINITY ? 0.f : top;      // (nothing but -inf: the sum is 0)
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f((acc[i][j][r] - from) * kLog2e);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      out[j] = make_float2(top, sum);
+      if (p.sums) {
+        float all = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) all += cut && n + column_of(i, g, r) >= q.N ? 0.f : acc[i][j][r];
+        all += __shfl_xor(all, 16);
+        all += __shfl_xor(all, 32);
+        total[j] = all;
+      }
+    }
+    if (g == 0) {
+      const int64_t at = (int64_t)(tn * 2 + wn) * p.rows_padded + m;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p.stats[at + j] = out[j];
+        if (p.sums) p.sums[at + j] = total[j];
+      }
+    }
+  } else if constexpr (EPI == kDlogits) {
+    const float flat = p.smoothing / (float)p.vocab, one = 1.0f - p.smoothing;
+    uint32_t pk[4][8][2];                      // [j][i][r / 2]: bf16 pairs along the columns
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool row = m + j < q.M;
+      const int64_t t = row ? p.target[m + j] : p.ignore_index;
+      float c = 0.f, lse = 0.f;
+      if (t != p.ignore_index) {
+        lse = p.lse[m + j];
+        c = p.grad[(int64_t)(m + j) * p.grad_stride];
+        if (p.count) c /= p.count[0];
+        if (t < 0 || t >= p.vocab) c = NAN;
+      }
+      const int own = t >= p.first && t < p.first + q.N ? (int)(t - p.first) : -1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float d[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int col = n + column_of(i, g, r);
+          float v = __builtin_amdgcn_exp2f((acc[i][j][r] - lse) * kLog2e) - flat;
+          if (own == col) v -= one;
+          d[r] = t == p.ignore_index || (cut && col >= q.N) ? 0.f : c * v;
+        }
+        pk[j][i][0] = pack_bf16x2(d[0], d[1]);
+        pk[j][i][1] = pack_bf16x2(d[2], d[3]);
+      }
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const u32x4_st v = {pk[j][2 * h][0], pk[j][2 * h][1], pk[j][2 * h + 1][0], pk[j][2 * h + 1][1]};
+        *reinterpret_cast<u32x4_st*>(p.dl + (int64_t)(m + j) * p.ld_dl + n + 32 * h + 8 * g) = v;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t sel = r & 1 ? 0x07060302u : 0x05040100u;       // the upper or the lower halves of two words
+        uint2 v;
+        v.x = __builtin_amdgcn_perm(pk[1][i][r >> 1], pk[0][i][r >> 1], sel);
+        v.y = __builtin_amdgcn_perm(pk[3][i][r >> 1], pk[2][i][r >> 1], sel);
+        *reinterpret_cast<uint2*>(p.dl_t + (int64_t)(n + column_of(i, g, r)) * p.rows_padded + m) = v;
+      }
+  } else {
+    if (q.store == kBf16) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (m + j >= q.M) break;
+        uint16_t* const row = reinterpret_cast<uint16_t*>(q.c) + (int64_t)(m + j) * q.ldc;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int col = n + 32 * h + 8 * g;
+          const u32x4_st v = {pack_bf16x2(acc[2 * h][j][0], acc[2 * h][j][1]), pack_bf16x2(acc[2 * h][j][2], acc[2 * h][j][3]),
+                              pack_bf16x2(acc[2 * h + 1][j][0], acc[2 * h + 1][j][1]), pack_bf16x2(acc[2 * h + 1][j][2], acc[2 * h + 1][j][3])};
+          if (col < q.N) *reinterpret_cast<u32x4_st*>(row + col) = v;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (m + j >= q.M) break;
+        float* const row = reinterpret_cast<float*>(q.c) + (int64_t)(m + j) * q.ldc;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int col = n + column_of(i, g, 0);
+          if (col >= q.N) continue;
+          v4f v = acc[i][j];
+          if (q.store == kF32Add) v += *reinterpret_cast<const v4f*>(row + col);
+          *reinterpret_cast<v4f*>(row + col) = v;
+        }
+      }
+    }
+  }
+}
+
+// ---- joins the forward's partial results: 64 rows per workgroup, 16 waves that share the parts
+__global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ stats, const float* __restrict__ sums,
+                                                       const float* __restrict__ target_logit, const int64_t* __restrict__ target, int parts,
+                                                       int64_t rows, int64_t rows_padded, int64_t ignore_index, int64_t vocab, float smoothing,
+                                                       float* __restrict__ lse, float* __restrict__ loss) {
+  __shared__ float tops[16][64], each[16][64], totals[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x * 64 + lane;
+  float top = -INFINITY, sum = 0.f, total = 0.f;
+  if (row < rows) {
+    int k = wave;
+    auto add = [&](float2 s) {
+      const float t = fmaxf(top, s.x), from = t == -INFINITY ? 0.f : t;
+      sum = sum * __builtin_amdgcn_exp2f((top - from) * kLog2e) + s.y * __builtin_amdgcn_exp2f((s.x - from) * kLog2e);
+      top = t;
+    };
+    for (; k + 112 < parts; k += 128) {
+      float2 s[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s[u] = stats[(int64_t)(k + 16 * u) * rows_padded + row];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) add(s[u]);
+    }
+    for (; k < parts; k += 16) add(stats[(int64_t)k * rows_padded + row]);
+    if (sums)
+      for (k = wave; k < parts; k += 16) total += sums[(int64_t)k * rows_padded + row];
+  }
+  tops[wave][lane] = top;
+  each[wave][lane] = sum;
+  totals[wave][lane] = total;
+  __syncthreads();
+  if (wave != 0 || row >= rows) return;
+  for (int k = 1; k < 16; ++k) top = fmaxf(top, tops[k][lane]);
+  const float from = top == -INFINITY ? 0.f : top;
+  sum = 0.f;
+  total = 0.f;
+  for (int k = 0; k < 16; ++k) {
+    sum += each[k][lane] * __builtin_amdgcn_exp2f((tops[k][lane] - from) * kLog2e);
+    total += totals[k][lane];
+  }
+  const float l = from + logf(sum);
+  if (lse) lse[row] = l;
+  const int64_t t = target[row];
+  float out = 0.f;
+  if (t != ignore_index) {
+    out = t < 0 || t >= vocab ? NAN : l - (1.0f - smoothing) * target_logit[row];
+    if (smoothing != 0.f) out -= smoothing * (total / (float)vocab);
+  }
+  loss[row] = out;
+}
+
+// ---- the rows' losses, their sum or mean, and how many count: one workgroup, in a fixed order
+__global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* __restrict__ loss, const int64_t* __restrict__ target, int64_t rows,
+                                                         int64_t ignore_index, int mean, float* __restrict__ out, float* __restrict__ count) {
+  __shared__ double sums[16];
+  __shared__ int64_t counts[16];
+  double s = 0.0;
+  int64_t n = 0;
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+    s += (double)loss[r];
+    n += target[r] != ignore_index;
+  }
+  for (int d = 1; d < 64; d *= 2) {
+    s += __shfl_xor(s, d);
+    n += __shfl_xor(n, d);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    sums[threadIdx.x >> 6] = s;
+    counts[threadIdx.x >> 6] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    n = 0;
+    for (int k = 0; k < 16; ++k) {
+      s += sums[k];
+      n += counts[k];
+    }
+    *out = (float)(mean ? s / (double)n : s);
+    *count = (float)n;
+  }
+}
+
+// ---- out[c, r] = in[r, c], bf16, 64 x 64 per workgroup; columns of out from rows to the next multiple of 64 are zeros, and so are those of
+// rows whose target is ignored (what such a row holds, NaN in padding too, then meets a gradient of 0 as 0)
+__global__ __launch_bounds__(256) void ce_transpose_kernel(const uint16_t* __restrict__ in, int64_t ld, int64_t rows, int64_t cols,
+                                                           const int64_t* __restrict__ target, int64_t ignore_index, uint16_t* __restrict__ out,
+                                                           int64_t ld_out) {
+  __shared__ uint16_t tile[64][66];
+  const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = threadIdx.x / 8 + 32 * h, c = threadIdx.x % 8 * 8;
+    u32x4_st v = {0, 0, 0, 0};
+    if (r0 + r < rows && c0 + c < cols && !(target && target[r0 + r] == ignore_index)) v = *reinterpret_cast<const u32x4_st*>(in + (r0 + r) * ld + c0 + c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) *reinterpret_cast<uint32_t*>(&tile[r][c + 2 * k]) = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int c = threadIdx.x / 8 + 32 * h, r = threadIdx.x % 8 * 8;
+    if (c0 + c >= cols) continue;
+    u32x4_st v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (uint32_t)tile[r + 2 * k][c] | (uint32_t)tile[r + 2 * k + 1][c] << 16;
+    *reinterpret_cast<u32x4_st*>(out + (c0 + c) * ld_out + r0 + r) = v;
+  }
+}
+
+// ---- fp32 -> bf16
+__global__ __launch_bounds__(256) void ce_round_kernel(const float* __restrict__ in, int64_t n8, uint16_t* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n8) return;
+  const v4f a = reinterpret_cast<const v4f*>(in)[2 * i], b = reinterpret_cast<const v4f*>(in)[2 * i + 1];
+  reinterpret_cast<u32x4_st*>(out)[i] = u32x4_st{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])};
+}
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+int tiles_of(int64_t m, int64_t n) { return (int)((m + kTile - 1) / kTile * ((n + kTile - 1) / kTile)); }
+
+int check(int64_t tokens, int64_t hidden, int64_t vocab, int64_t ld_x, int64_t ld_w) {
+  HPFP8_REQUIRE(tokens >= 0 && hidden > 0 && vocab > 0, HPFP8_ERR_SHAPE, "tokens=%lld hidden=%lld vocab=%lld", (long long)tokens, (long long)hidden, (long long)vocab);
+  HPFP8_REQUIRE(hidden % 8 == 0 && ld_x % 8 == 0 && ld_w % 8 == 0, HPFP8_ERR_SHAPE, "hidden and the row strides must be multiples of 8");
+  HPFP8_REQUIRE(ld_x >= hidden && ld_w >= hidden, HPFP8_ERR_SHAPE, "a row stride is below hidden");
+  HPFP8_REQUIRE(ld_x < (1 << 22) && ld_w < (1 << 22), HPFP8_ERR_SHAPE, "rows of 8 MiB and more");
+  HPFP8_REQUIRE(tokens <= (1 << 22) && vocab <= (1 << 24), HPFP8_ERR_SHAPE, "tokens=%lld vocab=%lld: at most 2^22 and 2^24", (long long)tokens, (long long)vocab);
+  return HPFP8_OK;
+}
+
+Product product(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N, int64_t K, void* c, int64_t ldc, int store) {
+  Product q = {};
+  q.a = (const uint8_t*)a;
+  q.b = (const uint8_t*)b;
+  q.lda = lda * 2;
+  q.ldb = ldb * 2;
+  q.M = (int)M;
+  q.N = (int)N;
+  q.K = (int)K;
+  q.c = c;
+  q.ldc = ldc;
+  q.store = store;
+  q.tiles = tiles_of(M, N);
+  return q;
+}
+
+}  // namespace
+}  // namespace hpfp8
+
+using namespace hpfp8;
+
+extern "C" {
+
+int64_t hpfp8_cross_entropy_parts(int64_t vocab) { return vocab > 0 ? 2 * ((vocab + kTile - 1) / kTile) : 0; }
+int64_t hpfp8_cross_entropy_padded_rows(int64_t tokens) { return tokens > 0 ? up(tokens, kTile) : 0; }
+
+int hpfp8_linear_cross_entropy_forward(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t tokens,
+                                       int64_t hidden, int64_t vocab, int64_t ignore_index, float smoothing, int reduction, float* stats,
+                                       float* sums, float* target_logit, float* lse, float* loss, float* out, float* count,
+                                       hpfp8_stream_t stream) {
+  const int bad = check(tokens, hidden, vocab, ld_x, ld_w);
+  if (bad != HPFP8_OK) return bad;
+  HPFP8_REQUIRE(reduction >= 0 && reduction <= 2, HPFP8_ERR_ARG, "unknown reduction %d", reduction);
+  HPFP8_REQUIRE(smoothing >= 0.f && smoothing <= 1.f, HPFP8_ERR_ARG, "label smoothing must be in [0, 1]");
+  HPFP8_REQUIRE(reduction == 0 || (out && count), HPFP8_ERR_ARG, "null buffer");
+  const hipStream_t s = (hipStream_t)stream;
+  if (tokens > 0) {
+    HPFP8_REQUIRE(x && w && target && stats && target_logit && loss && (smoothing == 0.f || sums), HPFP8_ERR_ARG, "null buffer");
+    HPFP8_REQUIRE(aligned16(x) && aligned16(w) && aligned16(stats), HPFP8_ERR_ALIGN, "a buffer is not 16-byte aligned");
+    CeParams p = {};
+    p.part[0] = product(x, ld_x, w, ld_w, tokens, vocab, hidden, nullptr, 0, 0);
+    p.stats = (float2*)stats;
+    p.sums = smoothing != 0.f ? sums : nullptr;
+    p.target_logit = target_logit;
+    p.target = target;
+    p.rows_padded = up(tokens, kTile);
+    ce_gemm_kernel<kStats><<<p.part[0].tiles, 512, 0, s>>>(p);
+    int rc = check_launch("linear_cross_entropy_forward");
+    if (rc != HPFP8_OK) return rc;
+    ce_join_kernel<<<(unsigned)((tokens + 63) / 64), 1024, 0, s>>>(p.stats, p.sums, target_logit, target, (int)hpfp8_cross_entropy_parts(vocab), tokens,
+                                                                 p.rows_padded, ignore_index, vocab, smoothing, lse, loss);
+    rc = check_launch("linear_cross_entropy_forward (join)");
+    if (rc != HPFP8_OK) return rc;
+  }
+  return reduction != 0 ? hpfp8_linear_cross_entropy_reduce(loss, target, tokens, ignore_index, reduction, out, count, stream) : HPFP8_OK;
+}
+
+int hpfp8_linear_cross_entropy_reduce(const float* loss, const int64_t* target, int64_t tokens, int64_t ignore_index, int reduction, float* out,
+                                      float* count, hpfp8_stream_t stream) {
+  HPFP8_REQUIRE(tokens >= 0, HPFP8_ERR_SHAPE, "tokens=%lld", (long long)tokens);
+  HPFP8_REQUIRE(reduction == 1 || reduction == 2, HPFP8_ERR_ARG, "unknown reduction %d", reduction);
+  HPFP8_REQUIRE(out && count && (tokens == 0 || (loss && target)), HPFP8_ERR_ARG, "null buffer");
+  ce_reduce_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(loss, target, tokens, ignore_index, reduction == 1, out, count);
+  return check_launch("linear_cross_entropy_reduce");
+}
+
+int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_t, const void* w, int64_t ld_w, const int64_t* target,
+                                     int64_t tokens, int64_t hidden, int64_t vocab, int64_t first, int64_t width, int64_t ignore_index,
+                                     float smoothing, const float* lse, const float* grad, int64_t grad_stride, const float* count, void* dl,
+                                     void* dl_t, void* w_t, float* dx, int dx_add, void* dw, int dw_type, int dw_add, hpfp8_stream_t stream) {
+  const int bad = check(tokens, hidden, vocab, ld_x, ld_w);
+  if (bad != HPFP8_OK) return bad;
+  HPFP8_REQUIRE(first >= 0 && width > 0 && first + width <= vocab, HPFP8_ERR_SHAPE, "piece %lld + %lld of %lld", (long long)first, (long long)width, (long long)vocab);
+  HPFP8_REQUIRE(dw_type == HPFP8_OUT_BF16 || dw_type == HPFP8_OUT_F32, HPFP8_ERR_ARG, "unknown output type %d", dw_type);
+  HPFP8_REQUIRE(!dw_add || dw_type == HPFP8_OUT_F32, HPFP8_ERR_ARG, "only fp32 is added onto");
+  if (tokens == 0) return HPFP8_OK;
+  HPFP8_REQUIRE(x && w && target && lse && grad && dl && dl_t && (!dx == !w_t) && (!dw == !x_t), HPFP8_ERR_ARG, "null buffer");
+  HPFP8_REQUIRE(aligned16(x) && aligned16(w) && aligned16(dl) && aligned16(dl_t) && aligned16(w_t) && aligned16(x_t) && aligned16(dx) && aligned16(dw),
+                HPFP8_ERR_ALIGN, "a buffer is not 16-byte aligned");
+  const hipStream_t s = (hipStream_t)stream;
+  const int64_t rows_padded = up(tokens, kTile), cols_padded = up(width, kTile);
+  const uint16_t* const piece = (const uint16_t*)w + first * ld_w;
+  CeParams p = {};
+  p.part[0] = product(x, ld_x, piece, ld_w, tokens, width, hidden, nullptr, 0, 0);
+  p.target = target;
+  p.rows_padded = rows_padded;
+  p.lse = lse;
+  p.grad = grad;
+  p.grad_stride = grad_stride;
+  p.count = count;
+  p.ignore_index = ignore_index;
+  p.smoothing = smoothing;
+  p.vocab = vocab;
+  p.first = first;
+  p.dl = (uint16_t*)dl;
+  p.ld_dl = cols_padded;
+  p.dl_t = (uint16_t*)dl_t;
+  ce_gemm_kernel<kDlogits><<<p.part[0].tiles, 512, 0, s>>>(p);
+  int rc = check_launch("linear_cross_entropy_piece");
+  if (rc != HPFP8_OK) return rc;
+  CeParams g = {};
+  int n = 0;
+  if (dx) {
+    ce_transpose_kernel<<<dim3((unsigned)((width + 63) / 64), (unsigned)((hidden + 63) / 64)), 256, 0, s>>>(piece, ld_w, width, hidden, nullptr, 0, (uint16_t*)w_t,
+                                                                                                       cols_padded);
+    rc = check_launch("linear_cross_entropy_piece (transpose)");
+    if (rc != HPFP8_OK) return rc;
+    g.part[n++] = product(dl, cols_padded, w_t, cols_padded, tokens, hidden, up(width, kSlab), dx, hidden, dx_add ? kF32Add : kF32);
+  }
+  if (dw) {
+    void* const to = (uint8_t*)dw + first * hidden * (dw_type == HPFP8_OUT_F32 ? 4 : 2);
+    g.part[n++] = product(dl_t, rows_padded, x_t, rows_padded, width, hidden, up(tokens, kSlab), to, hidden,
+                          dw_type == HPFP8_OUT_BF16 ? kBf16 : (dw_add ? kF32Add : kF32));
+  }
+  if (n == 0) return HPFP8_OK;
+  ce_gemm_kernel<kGrads><<<g.part[0].tiles + g.part[1].tiles, 512, 0, s>>>(g);
+  return check_launch("linear_cross_entropy_piece (gradients)");
+}
+
+int hpfp8_linear_cross_entropy_rows_t(const void* x, int64_t rows, int64_t cols, int64_t ld, const int64_t* target, int64_t ignore_index, void* x_t,
+                                      int64_t ld_t, hpfp8_stream_t stream) {
+  HPFP8_REQUIRE(rows >= 0 && cols >= 0 && cols % 8 == 0 && ld % 8 == 0 && ld >= cols, HPFP8_ERR_SHAPE, "rows=%lld cols=%lld ld=%lld", (long long)rows,
+                (long long)cols, (long long)ld);
+  HPFP8_REQUIRE(ld_t % 8 == 0 && ld_t >= up(rows, 64), HPFP8_ERR_SHAPE, "ld_t=%lld does not hold %lld values and the zeros behind them", (long long)ld_t,
+                (long long)rows);
+  if (rows == 0 || cols == 0) return HPFP8_OK;
+  HPFP8_REQUIRE(x && x_t, HPFP8_ERR_ARG, "null buffer");
+  HPFP8_REQUIRE(aligned16(x) && aligned16(x_t), HPFP8_ERR_ALIGN, "a buffer is not 16-byte aligned");
+  HPFP8_REQUIRE((cols + 63) / 64 < 65536, HPFP8_ERR_SHAPE, "too many columns");
+  ce_transpose_kernel<<<dim3((unsigned)((rows + 63) / 64), (unsigned)((cols + 63) / 64)), 256, 0, (hipStream_t)stream>>>((const uint16_t*)x, ld, rows, cols, target, ignore_index,
+                                                                                                                    (uint16_t*)x_t, ld_t);
+  return check_launch("linear_cross_entropy_rows_t");
+}
+
+int hpfp8_linear_cross_entropy_round(const float* x, int64_t n, void* y, hpfp8_stream_t stream) {
+  HPFP8_REQUIRE(n >= 0 && n % 8 == 0, HPFP8_ERR_SHAPE, "n=%lld is no multiple of 8", (long long)n);
+  if (n == 0) return HPFP8_OK;
+  HPFP8_REQUIRE(x && y, HPFP8_ERR_ARG, "null buffer");
+  HPFP8_REQUIRE(aligned16(x) && aligned16(y), HPFP8_ERR_ALIGN, "a buffer is not 16-byte aligned");
+  ce_round_kernel<<<(unsigned)((n / 8 + 255) / 256), 256, 0, (hipStream_t)stream>>>(x, n / 8, (uint16_t*)y);
+  return check_launch("linear_cross_entropy_round");
+}
+
+}  // extern "C"

@@ -1,0 +1,451 @@
+// Layer norm over the last dimension, forward and backward, its normalised input kept for the backward in 8 bits if asked for.
+//
+//   hat = (x - mean(x)) / sqrt(mean((x - mean)^2) + eps),   y = hat w + b
+//   u = dy w,   dx = (u - mean(u) - hat mean(u hat)) / sqrt(...),   dw = sum over rows of dy hat,   db = sum over rows of dy
+//
+// One pass over memory each way, bound by it: a row is in the registers of a team of 64, 256 or 512 threads, eight neighbouring
+// values per thread and step, from its load to its results.  All sums are fp32; the variance is taken around the mean (each wave's
+// values around the wave's own mean, the waves joined by their counts), so an offset many times the spread costs nothing.
+// The workgroups stay for many rows: the weight's values are loaded once, the next row's loads are under way while a row is worked on,
+// and in the backward the two vectors' gradients grow in registers.  At the end a workgroup's teams are joined in LDS in their order and
+// its sums leave as one row of partial sums, at most 256 of them, which a second launch adds up in a fixed order: the same
+// bits every time, and for 4096 rows of 7168 14 MB of sums beside 176 MB of values.
+#include <type_traits>
+
+#include "hpfp8_host.h"
+#include "rows.h"
+
+namespace hpfp8 {
+namespace {
+
+constexpr int kMaxCols = 16384;
+constexpr int kBackwardThreads = 512;
+constexpr int kMaxPartials = 256;          // one workgroup of the backward per compute unit
+
+struct NormParams {
+  const void* x;
+  int64_t ld;            // elements between the rows of x
+  const void* w;         // may be null, as b
+  const void* b;
+  int wtype;             // element type of w and b: HPFP8_OUT_BF16, HPFP8_OUT_F32 or HPFP8_TYPE_F16
+  int64_t rows;
+  int cols;
+  float eps;
+  void* y;
+  float* mean;           // [rows], may be null
+  float* rstd;           // [rows], may be null
+  uint8_t* q;            // [rows, cols] codes of hat
+  float* scale_inv;      // [rows, ceil(cols / 128)]
+  const void* dy;
+  int64_t ld_dy;
+  void* dx;
+  float* partial;        // [workgroups][2][cols]: dw, db
+};
+
+__device__ __forceinline__ float wave_sum(float v) {
+  v += __uint_as_float(dpp_u32<kDppQuadXor1>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_u32<kDppQuadXor2>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_u32<kDppRowHalfMirror>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_u32<kDppRowMirror>(__float_as_uint(v)));
+  const int i = __builtin_bit_cast(int, v);
+  auto at = [&](int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, lane)); };
+  return (at(0) + at(16)) + (at(32) + at(48));
+}
+
+// eight of w's (or b's) values as fp32; `none` where there is no such vector
+__device__ __forceinline__ void load_vector8(const void* w, int type, int col, int left, float none, float v[8]) {
+  if (!w) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = none;
+  } else if (type == HPFP8_OUT_BF16) {
+    load8<Bf16, false>((const uint16_t*)w + col, left, v);
+  } else if (type == HPFP8_TYPE_F16) {
+    load8<F16, false>((const _Float16*)w + col, left, v);
+  } else {
+    load8<F32, false>((const float*)w + col, left, v);
+  }
+}
+
+// A row per team of TPR threads; thread t has the chunks of eight values t, t + TPR, ...: 16 neighbouring threads have one group of 128.
+template <typename E, int TPR, int NV, bool KEEP, bool TAIL>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(NormParams p) {
+  using raw = typename E::raw;
+  constexpr int kTeams = (TPR < 256 ? 256 : TPR) / TPR, kWaves = TPR / 64;
+  __shared__ v4f parts[2][kTeams][kWaves];
+  // (the same in a whole wave, so a row's address is a scalar)
+  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, wave = __builtin_amdgcn_readfirstlane(t / 64);
+  const int C = p.cols, groups = (C + kBlock - 1) / kBlock;
+  int left[NV];
+  float w[NV][8], b[NV][8];
+  int mine = 0;                                       // values of a row in this wave's hands
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    left[j] = C - (j * TPR + t) * 8;
+    const int first = (j * TPR + wave * 64) * 8;
+    mine += C - first < 0 ? 0 : (C - first < 512 ? C - first : 512);
+    load_vector8(p.w, p.wtype, (j * TPR + t) * 8, left[j], 1.f, w[j]);
+    load_vector8(p.b, p.wtype, (j * TPR + t) * 8, left[j], 0.f, b[j]);
+  }
+  const float n = (float)mine;
+  const int64_t step = (int64_t)gridDim.x * kTeams;
+  Pack8<E> next[NV];
+  auto fetch = [&](int64_t r) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      next[j] = load_pack8<E, true, TAIL>((const raw*)p.x + (r < p.rows ? r : 0) * p.ld + (j * TPR + t) * 8, r < p.rows ? left[j] : 0);
+  };
+  int64_t row = (int64_t)blockIdx.x * kTeams + team;
+  fetch(row);
+  int turn = 0;
+  for (int64_t at = (int64_t)blockIdx.x * kTeams; at < p.rows; at += step, row += step, turn ^= 1) {    // (as many turns for every team)
+    float v[NV][8];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) unpack8<E>(next[j], v[j]);
+    fetch(row + step);
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[j][i];
+    float mean = mine ? wave_sum(s) / n : 0.f;
+    float m2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = i < left[j] ? v[j][i] - mean : 0.f;
+        m2 = __builtin_fmaf(d, d, m2);
+      }
+    m2 = wave_sum(m2);
+    if constexpr (kWaves > 1) {
+      if ((t & 63) == 0) parts[turn][team][wave] = v4f{n, mean, m2, 0.f};
+      __syncthreads();                                // (one barrier: the next turn writes the other half)
+      v4f each[kWaves];
+      float total = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) {
+        each[k] = parts[turn][team][k];
+        total += each[k][0] * each[k][1];
+      }
+      mean = total / (float)C;
+      m2 = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) m2 += each[k][2] + each[k][0] * ((each[k][1] - mean) * (each[k][1] - mean));
+    }
+    const float rstd = 1.0f / sqrtf(m2 / (float)C + p.eps);
+    if (row >= p.rows) continue;
+    if (t == 0) {
+      if (p.mean) p.mean[row] = mean;
+      if (p.rstd) p.rstd[row] = rstd;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int col = (j * TPR + t) * 8;
+      float out[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[j][i] = i < left[j] ? (v[j][i] - mean) * rstd : 0.f;
+        out[i] = __builtin_fmaf(v[j][i], w[j][i], b[j][i]);
+      }
+      if (left[j] > 0) store8<E, true, TAIL>((raw*)p.y + row * C + col, left[j], out);
+      if constexpr (KEEP) {
+        float si;
+        const uint2 c = encode_group(v[j], si);
+        if (left[j] > 0) {
+          store_codes8<TAIL>(p.q + row * C + col, left[j], c);
+          if ((t & 15) == 0) p.scale_inv[row * groups + col / kBlock] = si;
+        }
+      }
+    }
+  }
+}
+
+template <typename E, int TPR, int NV, bool KEEP, bool TAIL>
+__global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(NormParams p) {
+  using raw = typename E::raw;
+  constexpr int kTeams = kBackwardThreads / TPR, kWaves = TPR / 64, kChunks = TPR * NV;
+  __shared__ v2f parts[2][kTeams][kWaves];
+  __shared__ v4f joined[kTeams > 1 ? 2 * kChunks * 2 : 1];
+  // (the same in a whole wave, so a row's address is a scalar)
+  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, wave = __builtin_amdgcn_readfirstlane(t / 64);
+  const int C = p.cols, groups = (C + kBlock - 1) / kBlock;
+  int left[NV];
+  float w[NV][8], dw[NV][8], db[NV][8];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    left[j] = C - (j * TPR + t) * 8;
+    load_vector8(p.w, p.wtype, (j * TPR + t) * 8, left[j], 1.f, w[j]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dw[j][i] = db[j][i] = 0.f;
+  }
+  const int64_t step = (int64_t)gridDim.x * kTeams;
+  Pack8<E> next_dy[NV], next_x[KEEP ? 1 : NV];
+  uint2 next_q[KEEP ? NV : 1];
+  float next_s[KEEP ? NV : 1], next_mean = 0.f, next_rstd = 0.f;
+  auto fetch = [&](int64_t r) {
+    const bool in = r < p.rows;
+    const int64_t at = in ? r : 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int col = (j * TPR + t) * 8, n = in ? left[j] : 0;
+      next_dy[j] = load_pack8<E, true, TAIL>((const raw*)p.dy + at * p.ld_dy + col, n);
+      if constexpr (KEEP) {
+        next_q[j] = load_codes8<TAIL>(p.q + at * C + col, n);
+        next_s[j] = n > 0 ? (p.scale_inv + at * groups)[col / kBlock] : 0.f;
+      } else {
+        next_x[j] = load_pack8<E, true, TAIL>((const raw*)p.x + at * p.ld + col, n);
+      }
+    }
+    if (!KEEP) next_mean = in ? p.mean[r] : 0.f;
+    next_rstd = in ? p.rstd[r] : 0.f;
+  };
+  int64_t row = (int64_t)blockIdx.x * kTeams + team;
+  fetch(row);
+  int turn = 0;
+  for (int64_t at = (int64_t)blockIdx.x * kTeams; at < p.rows; at += step, row += step, turn ^= 1) {
+    float go[NV][8], hat[NV][8];
+    const float rstd = next_rstd;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      unpack8<E>(next_dy[j], go[j]);
+      if constexpr (KEEP) {
+        decode8(next_q[j], next_s[j], hat[j]);
+      } else {
+        unpack8<E>(next_x[j], hat[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) hat[j][i] = i < left[j] ? (hat[j][i] - next_mean) * rstd : 0.f;
+      }
+    }
+    fetch(row + step);
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        dw[j][i] = __builtin_fmaf(go[j][i], hat[j][i], dw[j][i]);
+        db[j][i] += go[j][i];
+        go[j][i] *= w[j][i];                          // from here on u
+        s1 += go[j][i];
+        s2 = __builtin_fmaf(go[j][i], hat[j][i], s2);
+      }
+    }
+    s1 = wave_sum(s1);
+    s2 = wave_sum(s2);
+    if constexpr (kWaves > 1) {
+      if ((t & 63) == 0) parts[turn][team][wave] = v2f{s1, s2};
+      __syncthreads();
+      s1 = s2 = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) {
+        s1 += parts[turn][team][k].x;
+        s2 += parts[turn][team][k].y;
+      }
+    }
+    if (row >= p.rows) continue;
+    const float m1 = s1 / (float)C, m2 = s2 / (float)C;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float out[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i] = (go[j][i] - m1 - hat[j][i] * m2) * rstd;
+      if (left[j] > 0) store8<E, true, TAIL>((raw*)p.dx + row * C + (j * TPR + t) * 8, left[j], out);
+    }
+  }
+  // the teams' sums, one after the other
+  float* const to = p.partial + (int64_t)blockIdx.x * 2 * C;
+  for (int k = 0; k < kTeams; ++k) {
+    if (team == k) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int chunk = j * TPR + t;
+        if constexpr (kTeams > 1) {
+          v4f* const a = joined + chunk * 2;
+          v4f* const b = joined + (kChunks + chunk) * 2;
+          if (k > 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              dw[j][i] = a[i / 4][i % 4] + dw[j][i];
+              db[j][i] = b[i / 4][i % 4] + db[j][i];
+            }
+          }
+          if (k < kTeams - 1) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              a[h] = v4f{dw[j][4 * h], dw[j][4 * h + 1], dw[j][4 * h + 2], dw[j][4 * h + 3]};
+              b[h] = v4f{db[j][4 * h], db[j][4 * h + 1], db[j][4 * h + 2], db[j][4 * h + 3]};
+            }
+          }
+        }
+        if (k == kTeams - 1 && left[j] > 0) {
+          store8<F32, false, TAIL>(to + chunk * 8, left[j], dw[j]);
+          store8<F32, false, TAIL>(to + C + chunk * 8, left[j], db[j]);
+        }
+      }
+    }
+    if (kTeams > 1) __syncthreads();
+  }
+}
+
+// dw and db from the workgroups' partial sums: 64 columns per workgroup, each of its 16 waves every sixteenth partial sum, then the waves in order.
+__global__ __launch_bounds__(1024) void norm_join_kernel(const float* __restrict__ partial, int count, int cols, void* __restrict__ dw,
+                                                         void* __restrict__ db, int wtype) {
+  __shared__ float parts[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t col = (int64_t)blockIdx.x * 64 + lane, all = 2 * (int64_t)cols;
+  float s = 0.f;
+  if (col < all) {
+    int k = wave;
+    for (; k + 48 < count; k += 64) {
+      float v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = partial[(k + 16 * u) * all + col];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s += v[u];
+    }
+    for (; k < count; k += 16) s += partial[k * all + col];
+  }
+  parts[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && col < all) {
+    float total = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) total += parts[k][lane];
+    void* const to = col < cols ? dw : db;
+    const int64_t i = col < cols ? col : col - cols;
+    if (!to) return;
+    if (wtype == HPFP8_OUT_BF16) ((uint16_t*)to)[i] = from_f32<Bf16>(total);
+    else if (wtype == HPFP8_TYPE_F16) ((_Float16*)to)[i] = (_Float16)total;
+    else ((float*)to)[i] = total;
+  }
+}
+
+// The smallest team that holds a row, and its steps.  f(E, threads per row, steps).
+template <typename E, typename F>
+void by_width(int cols, F&& f) {
+  const int chunks = (cols + 7) / 8;
+  if (chunks <= 64) f(E(), std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+  else if (chunks <= 128) f(E(), std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+  else if (chunks <= 512) f(E(), std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+  else if (chunks <= 1024) f(E(), std::integral_constant<int, 512>(), std::integral_constant<int, 2>());
+  else f(E(), std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
+}
+template <typename F>
+void by_type_and_width(int dtype, int cols, F&& f) {
+  if (dtype == HPFP8_OUT_BF16) by_width<Bf16>(cols, f);
+  else if (dtype == HPFP8_TYPE_F16) by_width<F16>(cols, f);
+  else by_width<F32>(cols, f);
+}
+
+template <typename F>
+void by_form(bool keep, bool tail, F&& f) {
+  if (keep && tail) f(std::true_type(), std::true_type());
+  else if (keep) f(std::true_type(), std::false_type());
+  else if (tail) f(std::false_type(), std::true_type());
+  else f(std::false_type(), std::false_type());
+}
+
+int team_threads(int64_t cols) {
+  const int64_t chunks = (cols + 7) / 8;
+  return chunks <= 128 ? 64 : (chunks <= 512 ? 256 : 512);
+}
+
+bool at_element(const void* p, int dtype) { return ((uintptr_t)p & (dtype == HPFP8_OUT_F32 ? 3 : 1)) == 0; }
+
+int check(int dtype, int wtype, int64_t rows, int64_t cols) {
+  HPFP8_REQUIRE(dtype >= 0 && dtype <= 2 && wtype >= 0 && wtype <= 2, HPFP8_ERR_ARG, "unknown element type (%d, weight %d)", dtype, wtype);
+  HPFP8_REQUIRE(rows >= 0 && cols > 0, HPFP8_ERR_SHAPE, "rows=%lld cols=%lld", (long long)rows, (long long)cols);
+  HPFP8_REQUIRE(cols <= kMaxCols, HPFP8_ERR_SHAPE, "a row of %lld values is longer than %d", (long long)cols, kMaxCols);
+  return HPFP8_OK;
+}
+
+}  // namespace
+}  // namespace hpfp8
+
+using namespace hpfp8;
+
+extern "C" {
+
+int64_t hpfp8_layer_norm_partials(int64_t rows, int64_t cols) {
+  if (rows <= 0 || cols <= 0 || cols > kMaxCols) return 0;
+  const int64_t teams = kBackwardThreads / team_threads(cols), blocks = (rows + teams - 1) / teams;
+  return blocks < kMaxPartials ? blocks : kMaxPartials;
+}
+
+int hpfp8_layer_norm_forward(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* w, const void* b, int wtype, float eps,
+                             void* y, float* mean, float* rstd, void* q, float* scale_inv, hpfp8_stream_t stream) {
+  const int bad = check(dtype, wtype, rows, cols);
+  if (bad != HPFP8_OK) return bad;
+  if (rows == 0) return HPFP8_OK;
+  HPFP8_REQUIRE(x && y && (!q == !scale_inv), HPFP8_ERR_ARG, "null buffer, or codes without scales");
+  HPFP8_REQUIRE(ld >= 0, HPFP8_ERR_SHAPE, "negative stride");
+  HPFP8_REQUIRE(at_element(x, dtype) && at_element(y, dtype) && at_element(w, wtype) && at_element(b, wtype), HPFP8_ERR_ALIGN,
+                "a tensor is not aligned to its elements");
+  NormParams p = {};
+  p.x = x;
+  p.ld = ld;
+  p.w = w;
+  p.b = b;
+  p.wtype = wtype;
+  p.rows = rows;
+  p.cols = (int)cols;
+  p.eps = eps;
+  p.y = y;
+  p.mean = mean;
+  p.rstd = rstd;
+  p.q = (uint8_t*)q;
+  p.scale_inv = scale_inv;
+  by_type_and_width(dtype, (int)cols, [&](auto e, auto tpr, auto nv) {
+    using E = decltype(e);
+    constexpr int kThreads = tpr < 256 ? 256 : tpr, kTeams = kThreads / tpr;
+    const int64_t blocks = (rows + kTeams - 1) / kTeams, most = 256 * (1024 / kThreads);   // every compute unit full once
+    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    auto launch = [&](auto keep, auto tail) { norm_forward_kernel<E, tpr, nv, keep, tail><<<grid, kThreads, 0, (hipStream_t)stream>>>(p); };
+    by_form(q != nullptr, cols % 8 != 0, launch);
+  });
+  return check_launch("layer_norm_forward");
+}
+
+int hpfp8_layer_norm_backward(const void* dy, int64_t ld_dy, const void* x, int64_t ld, const float* mean, const void* q, const float* scale_inv,
+                              const float* rstd, int dtype, int64_t rows, int64_t cols, const void* w, int wtype, void* dx, void* dw, void* db,
+                              float* partial, hpfp8_stream_t stream) {
+  const int bad = check(dtype, wtype, rows, cols);
+  if (bad != HPFP8_OK) return bad;
+  if (rows > 0) {
+    HPFP8_REQUIRE(dy && dx && rstd && partial && (!q == !scale_inv) && (q || (x && mean)), HPFP8_ERR_ARG,
+                  "null buffer, codes without scales, or neither codes nor x and its mean");
+    HPFP8_REQUIRE(ld >= 0 && ld_dy >= 0, HPFP8_ERR_SHAPE, "negative stride");
+    HPFP8_REQUIRE(at_element(dy, dtype) && at_element(x, dtype) && at_element(dx, dtype) && at_element(w, wtype) && at_element(dw, wtype) &&
+                      at_element(db, wtype), HPFP8_ERR_ALIGN, "a tensor is not aligned to its elements");
+    NormParams p = {};
+    p.x = x;
+    p.ld = ld;
+    p.w = w;
+    p.wtype = wtype;
+    p.rows = rows;
+    p.cols = (int)cols;
+    p.mean = const_cast<float*>(mean);
+    p.rstd = const_cast<float*>(rstd);
+    p.q = (uint8_t*)const_cast<void*>(q);
+    p.scale_inv = const_cast<float*>(scale_inv);
+    p.dy = dy;
+    p.ld_dy = ld_dy;
+    p.dx = dx;
+    p.partial = partial;
+    const dim3 grid((unsigned)hpfp8_layer_norm_partials(rows, cols));
+    by_type_and_width(dtype, (int)cols, [&](auto e, auto tpr, auto nv) {
+      using E = decltype(e);
+      by_form(q != nullptr, cols % 8 != 0,
+              [&](auto keep, auto tail) { norm_backward_kernel<E, tpr, nv, keep, tail><<<grid, kBackwardThreads, 0, (hipStream_t)stream>>>(p); });
+    });
+    const int rc = check_launch("layer_norm_backward");
+    if (rc != HPFP8_OK) return rc;
+  }
+  if (dw || db) {      // (no rows: zeros)
+    norm_join_kernel<<<(unsigned)((2 * cols + 63) / 64), 1024, 0, (hipStream_t)stream>>>(partial, (int)hpfp8_layer_norm_partials(rows, cols), (int)cols,
+                                                                                      dw, db, wtype);
+    return check_launch("layer_norm_backward (join)");
+  }
+  return HPFP8_OK;
+}
+
+}  // extern "C"

@@ -14,6 +14,9 @@ from .linear import (fp8_linear, Fp8Linear, fp8_grouped_linear, fp8_swiglu_mlp, 
                      quantize_weight, quantize_grouped_weight, invalidate_fp8_caches, attach_optimizer)
 from . import fsdp, checkpoint  # noqa: E402
 from .bucket import quantize_bucket, dequantize_bucket, Fp8GradBucket  # noqa: E402
+from .kept import Fp8Activation, activation, keep_activations_8bit, quantize_activation  # noqa: E402
+from .norm import LayerNorm, layer_norm  # noqa: E402
+from .loss import linear_cross_entropy  # noqa: E402
 from .policy import Fp8MixedPrecisionPolicy, Fp8Tensor, cast_fp_tensor, tensor_type_cast  # noqa: E402
 
 __all__ = [
@@ -24,4 +27,5 @@ __all__ = [
     "dequantize_1x128", "dequantize_1x128_accumulate", "dequantize_128x128", "dequantize_per_tensor", "gemm_blockwise", "gemm_blockwise_swiglu_quantize", "gemm_per_tensor",
     "gemm_grouped_blockwise", "fp8_linear", "Fp8Linear", "fp8_grouped_linear", "fp8_swiglu_mlp", "Fp8SwiGLUMLP",
     "quantize_bucket", "dequantize_bucket", "Fp8GradBucket",
+    "layer_norm", "LayerNorm", "quantize_activation", "Fp8Activation", "keep_activations_8bit", "activation", "linear_cross_entropy",
 ]

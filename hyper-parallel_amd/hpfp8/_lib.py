@@ -77,6 +77,18 @@ SIGNATURES = {
     "hpfp8_quantize_128x1_t_grouped_bf16": [_vp, _i64, _i64, _vp, _int, _vp, _i64, _vp, _vp, _vp, _vp],
     "hpfp8_gemm_grouped_wgrad": [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _i64, _i64, _i64, _vp, _int, _vp],
     "hpfp8_grouped_zero_unrouted_rows_bf16": [_vp, _i64, _vp, _int, _i64, _i64, _vp],
+    "hpfp8_quantize_rows": [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp],
+    "hpfp8_dequantize_rows": [_vp, _vp, _i64, _i64, _vp, _int, _vp],
+    "hpfp8_activation_forward": [_vp, _int, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp],
+    "hpfp8_activation_backward": [_vp, _vp, _i64, _vp, _vp, _int, _i64, _i64, _int, _vp, _vp],
+    "hpfp8_linear_cross_entropy_forward": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _f32, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "hpfp8_linear_cross_entropy_piece": [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _i64, _vp, _vp,
+                                         _vp, _vp, _vp, _int, _vp, _int, _int, _vp],
+    "hpfp8_linear_cross_entropy_reduce": [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp],
+    "hpfp8_linear_cross_entropy_rows_t": [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp],
+    "hpfp8_linear_cross_entropy_round": [_vp, _i64, _vp, _vp],
+    "hpfp8_layer_norm_forward": [_vp, _int, _i64, _i64, _i64, _vp, _vp, _int, _f32, _vp, _vp, _vp, _vp, _vp, _vp],
+    "hpfp8_layer_norm_backward": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _int, _i64, _i64, _vp, _int, _vp, _vp, _vp, _vp, _vp],
 }
 # functions that return a size, not a status
 SIZE_FUNCTIONS = {
@@ -84,6 +96,9 @@ SIZE_FUNCTIONS = {
     "hpfp8_grouped_layout_words": [_int, _i64],
     "hpfp8_gemm_few_rows": [_i64],
     "hpfp8_linear_few_rows": [_i64, _i64],
+    "hpfp8_layer_norm_partials": [_i64, _i64],
+    "hpfp8_cross_entropy_parts": [_i64],
+    "hpfp8_cross_entropy_padded_rows": [_i64],
 }
 
 OUT_BF16, OUT_F32 = 0, 1

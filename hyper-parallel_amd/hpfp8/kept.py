@@ -1,0 +1,180 @@
+"""Activations kept in 8 bits between forward and backward.
+
+An activation that is only needed again in the backward can wait there as E4M3 codes with one fp32 scale for each 128 values of its last
+dimension: 1.03 bytes a value instead of two or four.  `fp8_linear` keeps its input that way by itself; this module does it for the rest
+of a model:
+
+  `quantize_activation(x)`     codes and scales of any floating tensor, `.dequantize()` what they stand for
+  `keep_activations_8bit()`    around any torch code: what its backward nodes save is kept so
+  `activation(x, kind)`        silu, gelu, gelu_tanh or swiglu, the codes written in the pass that computes the result, and the derivative
+                               taken from them in the pass that computes the gradient
+"""
+from __future__ import annotations
+
+import contextlib
+from typing import Callable, NamedTuple, Optional, Sequence
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, ops
+from .linear import _hand_off
+
+_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+KINDS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "swiglu": 3}
+
+
+def _check_rows(x, name: str) -> None:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if x.dtype not in _TYPES:
+        raise TypeError(f"{name} must be bfloat16, float16 or float32, got {x.dtype}")
+    ops._check_device(x, name)
+
+
+def _as_rows(x: torch.Tensor, cols: int) -> torch.Tensor:
+    """x as [rows, cols] with unit stride along a row: a view where x's strides allow it."""
+    x = x.reshape(x.numel() // cols if cols else 0, cols)
+    return x if cols == 1 or x.stride(1) == 1 else x.contiguous()
+
+
+def _groups(cols: int) -> int:
+    return (cols + ops.BLOCK - 1) // ops.BLOCK
+
+
+class Fp8Activation(NamedTuple):
+    """A tensor in 8 bits: what `quantize_activation` makes."""
+    codes: torch.Tensor                 # e4m3, the tensor's shape
+    scale_inv: torch.Tensor             # fp32 [..., ceil(C / 128)]
+    dtype: torch.dtype                  # of the tensor it was made from
+
+    def dequantize(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """The values that the codes stand for, rounded once to ``dtype`` (default: that of the original)."""
+        dtype = self.dtype if dtype is None else dtype
+        if dtype not in _TYPES:
+            raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
+        ops._check_device(self.codes, "codes")
+        x = torch.empty(self.codes.shape, dtype=dtype, device=self.codes.device)
+        cols = x.shape[-1]
+        _lib.call("hpfp8_dequantize_rows", ops._ptr(self.codes), ops._ptr(self.scale_inv), x.numel() // max(cols, 1), cols, ops._ptr(x),
+                  _TYPES[dtype], ops._stream())
+        return x
+
+    def __repr__(self) -> str:          # (shapes, never values: see Fp8Weight)
+        return f"Fp8Activation({tuple(self.codes.shape)}@{self.codes.data_ptr():#x}, {self.dtype})"
+
+
+def quantize_activation(x: torch.Tensor) -> Fp8Activation:
+    """x[..., C] (bfloat16, float16 or float32; any C, any strides) in 8 bits: E4M3 codes, one scale for each 128 values of the last
+    dimension, the last group of a row being what is left.  For bf16 rows of a multiple of 128 values the codes and scales of
+    `quantize_1x128`."""
+    _check_rows(x, "x")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    cols = x.shape[-1]
+    x2 = _as_rows(x, cols)
+    codes = torch.empty(x.shape, dtype=ops.FP8, device=x.device)
+    scale_inv = torch.empty(x.shape[:-1] + (_groups(cols),), dtype=torch.float32, device=x.device)
+    _lib.call("hpfp8_quantize_rows", ops._ptr(x2), _TYPES[x.dtype], x2.shape[0], cols, x2.stride(0), ops._ptr(codes), ops._ptr(scale_inv),
+              ops._stream())
+    return Fp8Activation(codes, scale_inv, x.dtype)
+
+
+def _is_parameter(t: torch.Tensor) -> bool:
+    base = t if t._base is None else t._base
+    return base.is_leaf and base.requires_grad
+
+
+@contextlib.contextmanager
+def keep_activations_8bit(min_elements: int = 1 << 16, dtypes: Sequence[torch.dtype] = (torch.bfloat16, torch.float16),
+                          select: Optional[Callable[[torch.Tensor], bool]] = None):
+    """Inside this context the tensors that backward nodes save are kept in 8 bits until the backward reads them.
+
+    Kept so are GPU tensors of ``min_elements`` values and more in one of ``dtypes`` (by default the 16-bit types: an fp32 tensor is
+    more often a statistic or a scale than an activation), unless they are parameters or views of one (leaves that require a gradient) or
+    ``select(tensor)`` says no.  Everything else is kept as it is.  The backward may run after the context has ended."""
+    for d in dtypes:
+        if d not in _TYPES:
+            raise TypeError(f"dtypes must be bfloat16, float16 or float32, got {d}")
+
+    def pack(t):
+        if (type(t) is not torch.Tensor or not t.is_cuda or t.dtype not in dtypes or t.dim() < 1 or t.numel() < min_elements
+                or _is_parameter(t) or (select is not None and not select(t))):
+            return t
+        with torch.cuda.device(t.device):
+            return quantize_activation(t.detach())
+
+    def unpack(kept):
+        if not isinstance(kept, Fp8Activation):
+            return kept
+        with torch.cuda.device(kept.codes.device):
+            return kept.dequantize()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        yield
+
+
+def _forward(x2, kind: int, cols: int, keep: bool):
+    """(y[rows, cols], codes, scale_inv): the last two None unless x is kept."""
+    rows, halves = x2.shape[0], 2 if kind == 3 else 1
+    y = torch.empty((rows, cols), dtype=x2.dtype, device=x2.device)
+    codes = scale_inv = None
+    if keep:
+        codes = torch.empty((rows, halves * cols), dtype=ops.FP8, device=x2.device)
+        scale_inv = torch.empty((rows, halves, _groups(cols)), dtype=torch.float32, device=x2.device)
+    _lib.call("hpfp8_activation_forward", ops._ptr(x2), _TYPES[x2.dtype], rows, cols, x2.stride(0), kind, ops._ptr(y), ops._ptr(codes),
+              ops._ptr(scale_inv), ops._stream())
+    return y, codes, scale_inv
+
+
+class _Activation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, kind, keep):
+        cols = x.shape[-1] // (2 if kind == 3 else 1)
+        x2 = _as_rows(x, x.shape[-1])
+        y, codes, scale_inv = _forward(x2, kind, cols, keep)
+        # (as it was: x itself, so that a write to it in between is noticed)
+        ctx.save_for_backward(*((codes, scale_inv) if keep else (x,)))
+        ctx.kind, ctx.keep, ctx.cols, ctx.shape = kind, keep, cols, x.shape
+        return y.reshape(x.shape[:-1] + (cols,))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        codes = scale_inv = x2 = None
+        if ctx.keep:
+            codes, scale_inv = ctx.saved_tensors
+        else:
+            x2 = _as_rows(ctx.saved_tensors[0], ctx.shape[-1])
+        go = grad_out.contiguous()
+        dx = torch.empty(ctx.shape, dtype=go.dtype, device=go.device)
+        rows = go.numel() // max(ctx.cols, 1)
+        _lib.call("hpfp8_activation_backward", ops._ptr(go), ops._ptr(x2), 0 if x2 is None else x2.stride(0), ops._ptr(codes),
+                  ops._ptr(scale_inv), _TYPES[go.dtype], rows, ctx.cols, ctx.kind, ops._ptr(dx), ops._stream())
+        return dx, None, None
+
+
+_ACTIVATION_DEFAULTS = dict(keep_8bit=True)
+
+
+def activation(input: torch.Tensor, kind: str, *, keep_8bit: bool = True) -> torch.Tensor:
+    """An activation function whose input waits for the backward in 8 bits.
+
+    kind: "silu", "gelu", "gelu_tanh" (the tanh form), or "swiglu": input [..., 2C] = gate | up, result silu(gate) * up [..., C].
+    bfloat16, float16 or float32, any width; computed in fp32 and rounded once.  The result is that of the input as it is; the
+    gradient is taken where the codes are (each half of a SwiGLU input has scaling groups of its own).  ``keep_8bit=False`` keeps the
+    input itself."""
+    if torch.overrides.has_torch_function((input,)):
+        return _hand_off(activation, (input,), (input, kind), dict(keep_8bit=keep_8bit), _ACTIVATION_DEFAULTS)
+    if kind not in KINDS:
+        raise ValueError(f"kind must be one of {tuple(KINDS)}, got {kind!r}")
+    _check_rows(input, "input")
+    if input.dim() < 1:
+        raise ValueError("input must have at least one dimension")
+    if kind == "swiglu" and input.shape[-1] % 2:
+        raise ValueError(f"swiglu takes gate | up in the last dimension, which is {input.shape[-1]}")
+    k = KINDS[kind]
+    if torch.is_grad_enabled() and input.requires_grad:
+        return _Activation.apply(input, k, bool(keep_8bit))
+    cols = input.shape[-1] // (2 if kind == "swiglu" else 1)
+    return _forward(_as_rows(input.detach(), input.shape[-1]), k, cols, False)[0].reshape(input.shape[:-1] + (cols,))

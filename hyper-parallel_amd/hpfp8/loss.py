@@ -1,0 +1,171 @@
+"""The loss at the end of a language model: the head's linear and the softmax cross entropy over its vocabulary in one operator, which
+never holds the logits."""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, ops
+from .linear import _hand_off
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+_TILE = 256
+# The forward takes this many tokens at a time: its per-tile results (16 bytes for 256 columns of a row) stay below 128 MiB for 131072 columns
+_FORWARD_ROWS = 16384
+# What the backward's workspaces for a piece of the vocabulary may take: the gradient of its logits, twice, and its transposed weight
+_PIECE_BYTES = 512 << 20
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x[..., C] as [rows, C] the kernels can read: unit stride along a row, rows 16 bytes apart and aligned."""
+    x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.stride(0) >= x.shape[1] and x.data_ptr() % 16 == 0 else x.contiguous()
+
+
+def _forward(x, weight, target, ignore_index, reduction, smoothing, want_lse):
+    """(loss, lse, count): loss [tokens] or 0-dim, lse None unless asked for, count None unless the loss is reduced."""
+    lib = _lib.load()
+    tokens, vocab = x.shape[0], weight.shape[0]
+    f32 = dict(dtype=torch.float32, device=x.device)
+    most = min(tokens, _FORWARD_ROWS)
+    parts, padded = lib.hpfp8_cross_entropy_parts(vocab), lib.hpfp8_cross_entropy_padded_rows(most)
+    stats = torch.empty((parts, padded, 2), **f32)
+    sums = torch.empty((parts, padded), **f32) if smoothing else None
+    own = torch.empty((most,), **f32)
+    loss = torch.empty((tokens,), **f32)
+    lse = torch.empty((tokens,), **f32) if want_lse else None
+    out = count = None
+    if reduction:
+        out, count = torch.empty((), **f32), torch.empty((), **f32)
+    last = max(0, (tokens - 1) // _FORWARD_ROWS * _FORWARD_ROWS)
+    for at in range(0, max(tokens, 1), _FORWARD_ROWS):
+        n = min(tokens - at, _FORWARD_ROWS)
+        whole = last == 0            # (in several pieces the losses are reduced behind the last of them, over all of them)
+        _lib.call("hpfp8_linear_cross_entropy_forward", ops._ptr(x[at:]), x.stride(0), ops._ptr(weight), weight.stride(0), ops._ptr(target[at:]), n,
+                  x.shape[1], vocab, ignore_index, smoothing, reduction if whole else 0, ops._ptr(stats), ops._ptr(sums), ops._ptr(own),
+                  None if lse is None else ops._ptr(lse[at:]), ops._ptr(loss[at:]), ops._ptr(out), ops._ptr(count), ops._stream())
+    if reduction and last:
+        _lib.call("hpfp8_linear_cross_entropy_reduce", ops._ptr(loss), ops._ptr(target), tokens, ignore_index, reduction, ops._ptr(out),
+                  ops._ptr(count), ops._stream())
+    return (out if reduction else loss), lse, count
+
+
+def _pieces(tokens: int, hidden: int, vocab: int, budget: int):
+    """[(first, width)]: pieces of the vocabulary, of equal width but for the last, whole tiles wide, whose workspaces fit the budget."""
+    padded = (tokens + _TILE - 1) // _TILE * _TILE
+    most = max(_TILE, budget // (4 * padded + 2 * hidden) // _TILE * _TILE)
+    count = (vocab + most - 1) // most
+    width = ((vocab + count - 1) // count + _TILE - 1) // _TILE * _TILE
+    return [(at, min(width, vocab - at)) for at in range(0, vocab, width)]
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, target, ignore_index, reduction, smoothing, main_grad_of):
+        x2, w = _rows(x), _rows(weight)
+        loss, lse, count = _forward(x2, w, target, ignore_index, reduction, smoothing, True)
+        ctx.save_for_backward(x, weight, target, lse, count)
+        ctx.ignore_index, ctx.reduction, ctx.smoothing, ctx.main_grad_of = ignore_index, reduction, smoothing, main_grad_of
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        x, weight, target, lse, count = ctx.saved_tensors
+        need_dx, need_dw = ctx.needs_input_grad[:2]
+        x2, w = _rows(x), _rows(weight)
+        tokens, hidden = x2.shape
+        vocab = w.shape[0]
+        param = ctx.main_grad_of
+        main_grad = None if param is None else getattr(param, "main_grad", None)
+        if tokens == 0:
+            if need_dw and param is not None and main_grad is None:
+                param.main_grad = torch.zeros(weight.shape, dtype=torch.float32, device=w.device)
+            return (torch.zeros_like(x) if need_dx else None, torch.zeros_like(weight) if need_dw and param is None else None) + (None,) * 5
+        device = x2.device
+        bf16, f32 = dict(dtype=torch.bfloat16, device=device), dict(dtype=torch.float32, device=device)
+        grad = grad_out.reshape(-1).contiguous()
+        dw = dx = x_t = w_t = None
+        padded = _lib.load().hpfp8_cross_entropy_padded_rows(tokens)
+        pieces = _pieces(tokens, hidden, vocab, _PIECE_BYTES)
+        width = (pieces[0][1] + _TILE - 1) // _TILE * _TILE
+        dl, dl_t = torch.empty((padded, width), **bf16), torch.empty((width, padded), **bf16)
+        if need_dw:
+            dw = torch.empty((vocab, hidden), **bf16) if param is None else main_grad
+            if dw is None:
+                dw = torch.empty((vocab, hidden), **f32)
+            x_t = torch.empty((hidden, padded), **bf16)
+            _lib.call("hpfp8_linear_cross_entropy_rows_t", ops._ptr(x2), tokens, hidden, x2.stride(0), ops._ptr(target), ctx.ignore_index,
+                      ops._ptr(x_t), padded, ops._stream())
+        if need_dx:
+            dx = torch.empty((tokens, hidden), **f32)
+            w_t = torch.empty((hidden, width), **bf16)
+        for first, n in pieces:
+            _lib.call("hpfp8_linear_cross_entropy_piece", ops._ptr(x2), x2.stride(0), ops._ptr(x_t), ops._ptr(w), w.stride(0), ops._ptr(target),
+                      tokens, hidden, vocab, first, n, ctx.ignore_index, ctx.smoothing, ops._ptr(lse), ops._ptr(grad),
+                      0 if ctx.reduction else 1, ops._ptr(count) if ctx.reduction == 1 else None, ops._ptr(dl), ops._ptr(dl_t), ops._ptr(w_t),
+                      ops._ptr(dx), int(first > 0), ops._ptr(dw), _lib.OUT_BF16 if param is None else _lib.OUT_F32, int(main_grad is not None),
+                      ops._stream())
+        if need_dx:
+            rounded = torch.empty(x.shape, **bf16)
+            _lib.call("hpfp8_linear_cross_entropy_round", ops._ptr(dx), dx.numel(), ops._ptr(rounded), ops._stream())
+            dx = rounded
+        if need_dw and param is not None:
+            if main_grad is None:
+                param.main_grad = dw
+            dw = None
+        return dx, dw, None, None, None, None, None
+
+
+_DEFAULTS = dict(ignore_index=-100, reduction="mean", label_smoothing=0.0, apply_grad_on_fp32_main_grad=False)
+
+
+def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100,
+                         reduction: str = "mean", label_smoothing: float = 0.0,
+                         apply_grad_on_fp32_main_grad: bool = False) -> torch.Tensor:
+    """F.cross_entropy(F.linear(input, weight), target) without the logits: input [..., hidden] and weight [vocab, hidden] in bfloat16
+    (hidden a multiple of 8, any vocabulary up to 2^24), target int64 of input's leading shape.
+
+    The logits are fp32 accumulators of the tensors' products and are not rounded; the loss is fp32: [...] with reduction "none" (0 where
+    target is ``ignore_index``), its sum, or its mean over the tokens that are not ignored (NaN if all are), summed in a fixed order.
+    A target that is neither ``ignore_index`` nor in [0, vocab) makes its token's loss and gradients NaN.  In the backward the logits are
+    computed again, a piece of the vocabulary at a time, their gradient rounded to bfloat16 for the products of both gradients.
+
+    ``apply_grad_on_fp32_main_grad`` as in `fp8_linear`: the weight's gradient goes to ``weight.main_grad`` (fp32), created by the first
+    backward and added onto by every later one."""
+    if torch.overrides.has_torch_function((input, weight, target)):
+        return _hand_off(linear_cross_entropy, (input, weight, target), (input, weight, target),
+                         dict(ignore_index=ignore_index, reduction=reduction, label_smoothing=label_smoothing,
+                              apply_grad_on_fp32_main_grad=apply_grad_on_fp32_main_grad), _DEFAULTS)
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {tuple(_REDUCTIONS)}, got {reduction!r}")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
+    for name, t in (("input", input), ("weight", weight)):
+        ops._check_bf16(t, name, contiguous=False)
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[0] > 1 << 24:
+        raise ValueError("weight must be [vocab, hidden] with 1 to 2^24 rows")
+    hidden = weight.shape[1]
+    if input.dim() < 1 or input.shape[-1] != hidden:
+        raise ValueError(f"input {tuple(input.shape)} does not end with weight's hidden size {hidden}")
+    if hidden < 8 or hidden % 8 or hidden >= 1 << 22:
+        raise ValueError(f"hidden must be a multiple of 8 below 2^22, got {hidden}")
+    if not isinstance(target, torch.Tensor) or target.dtype != torch.int64:
+        raise TypeError("target must be an int64 tensor")
+    ops._check_device(target, "target")
+    if target.shape != input.shape[:-1]:
+        raise ValueError(f"target must have input's leading shape {tuple(input.shape[:-1])}, got {tuple(target.shape)}")
+    if target.numel() > 1 << 22:
+        raise ValueError(f"at most 2^22 tokens in a call, got {target.numel()}")
+    if apply_grad_on_fp32_main_grad:
+        mg = getattr(weight, "main_grad", None)
+        if mg is not None and (mg.dtype != torch.float32 or mg.shape != weight.shape or not mg.is_contiguous()):
+            raise ValueError("weight.main_grad must be a contiguous float32 tensor of the weight's shape")
+    flat = target.reshape(-1).contiguous()
+    r = _REDUCTIONS[reduction]
+    if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad):
+        loss = _LinearCrossEntropy.apply(input, weight, flat, int(ignore_index), r, float(label_smoothing),
+                                         weight if apply_grad_on_fp32_main_grad else None)
+    else:
+        loss = _forward(_rows(input.detach()), _rows(weight.detach()), flat, int(ignore_index), r, float(label_smoothing), False)[0]
+    return loss if r else loss.reshape(target.shape)

@@ -46,6 +46,8 @@ enum {
 
 /* Output element type of the GEMMs. */
 enum { HPFP8_OUT_BF16 = 0, HPFP8_OUT_F32 = 1 };
+/* The third element type of the row-wise operators (layer norm, activations kept in 8 bits), whose `dtype` is one of all three. */
+enum { HPFP8_TYPE_F16 = 2 };
 
 /* Library version (major*10000 + minor*100 + patch). */
 int hpfp8_version(void);
@@ -502,6 +504,71 @@ int hpfp8_gemm_grouped_wgrad(const void* a, int64_t lda, const float* sa, const 
                              int out_type, hpfp8_stream_t stream);
 int hpfp8_grouped_zero_unrouted_rows_bf16(void* out, int64_t ld, const int32_t* offs, int experts, int64_t total_m,
                                           int64_t cols, hpfp8_stream_t stream);
+
+/* ---- what stands around the linears of a training step -------------------------------------------------------------
+ * Row-wise operators on bf16, fp16 or fp32 tensors (`dtype`: HPFP8_OUT_BF16, HPFP8_OUT_F32 or HPFP8_TYPE_F16).  A tensor's base and
+ * rows may start at any multiple of its element's size; `ld` is the stride between the rows of an input in elements (0 reads one row for
+ * all), outputs are contiguous.  In the reference these are aten calls on local shards, as the linear is
+ * (hyper_parallel/core/shard/_op_dispatch.py:277-283). */
+
+/* x[rows, cols] -> codes[rows, cols] and scale_inv[rows, ceil(cols / 128)], a scale for each 128 values of a row and one for what is left;
+ * for bf16 rows that are a multiple of 128 the codes and scales of hpfp8_quantize_1x128_bf16. */
+int hpfp8_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, void* q, float* scale_inv, hpfp8_stream_t stream);
+/* x[r, c] = code * scale_inv, rounded once to dtype. */
+int hpfp8_dequantize_rows(const void* q, const float* scale_inv, int64_t rows, int64_t cols, void* x, int dtype, hpfp8_stream_t stream);
+
+/* y = f(x), in fp32, rounded once; kind 0 silu, 1 gelu, 2 gelu (tanh form), 3 SwiGLU: x[rows, 2 cols] = gate | up, y = silu(gate) up.
+ * cols is y's width.  q and scale_inv (both or neither NULL) receive x in 8 bits: [rows, cols] as above, for SwiGLU [rows, 2, cols] and
+ * [rows, 2, ceil(cols / 128)], each half with groups of its own. */
+int hpfp8_activation_forward(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, int kind, void* y, void* q, float* scale_inv,
+                             hpfp8_stream_t stream);
+/* dx = dy f'(x) with x as it was, or from its codes (exactly one of x and q; dy contiguous). */
+int hpfp8_activation_backward(const void* dy, const void* x, int64_t ld, const void* q, const float* scale_inv, int dtype, int64_t rows,
+                              int64_t cols, int kind, void* dx, hpfp8_stream_t stream);
+
+/* y = (x - mean) rstd w + b over rows of up to 16384 values; w and b [cols] of element type wtype, each may be NULL.  mean and rstd
+ * (fp32 [rows], may be NULL) are what the backward needs; q and scale_inv (both or neither) receive (x - mean) rstd in 8 bits, for a
+ * backward without x and mean. */
+int hpfp8_layer_norm_forward(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* w, const void* b, int wtype, float eps,
+                             void* y, float* mean, float* rstd, void* q, float* scale_inv, hpfp8_stream_t stream);
+/* dx, and dw and db (element type wtype; each may be NULL) summed over the rows in a fixed order.  partial: fp32
+ * [hpfp8_layer_norm_partials(rows, cols), 2, cols], written and read by the call. */
+int hpfp8_layer_norm_backward(const void* dy, int64_t ld_dy, const void* x, int64_t ld, const float* mean, const void* q, const float* scale_inv,
+                              const float* rstd, int dtype, int64_t rows, int64_t cols, const void* w, int wtype, void* dx, void* dw, void* db,
+                              float* partial, hpfp8_stream_t stream);
+int64_t hpfp8_layer_norm_partials(int64_t rows, int64_t cols);
+
+/* Softmax cross entropy of the linear l = x w^T over a vocabulary, without the logits in memory.  x[tokens, hidden] and w[vocab, hidden] are
+ * bf16, row strides ld_x and ld_w in elements, hidden and the strides multiples of 8; target[tokens] is int64.
+ *   loss[t] = lse(l_t) - (1 - smoothing) l_t[target] - smoothing mean(l_t);  0 where target is ignore_index, NaN where it is neither that
+ *   nor in [0, vocab).  reduction 0: nothing more; 1: out[0] = their mean over the count[0] rows that are not ignored; 2: their sum.
+ * Workspaces, fp32: stats[hpfp8_cross_entropy_parts(vocab), hpfp8_cross_entropy_padded_rows(tokens), 2], sums (with smoothing only) half of
+ * that, target_logit[tokens].  lse[tokens] (may be NULL) is what the backward needs; out and count may be NULL with reduction 0. */
+int64_t hpfp8_cross_entropy_parts(int64_t vocab);
+int64_t hpfp8_cross_entropy_padded_rows(int64_t tokens);
+int hpfp8_linear_cross_entropy_forward(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t tokens,
+                                       int64_t hidden, int64_t vocab, int64_t ignore_index, float smoothing, int reduction, float* stats,
+                                       float* sums, float* target_logit, float* lse, float* loss, float* out, float* count,
+                                       hpfp8_stream_t stream);
+/* The reduction by itself (1 mean, 2 sum), for losses that several calls wrote. */
+int hpfp8_linear_cross_entropy_reduce(const float* loss, const int64_t* target, int64_t tokens, int64_t ignore_index, int reduction, float* out,
+                                      float* count, hpfp8_stream_t stream);
+/* The backward's part of the vocabulary's columns [first, first + width): the gradient of the logits, rounded to bf16, and with it
+ * dx (fp32 [tokens, hidden]; dx_add: added onto) and rows [first, first + width) of dw ([vocab, hidden], dw_type HPFP8_OUT_*; dw_add: added onto,
+ * fp32 only).  Either may be NULL.  grad is the loss's gradient, one value with grad_stride 0 or one for each row; count as the
+ * forward wrote it for reduction 1, otherwise NULL.  x_t is what hpfp8_linear_cross_entropy_rows_t makes of x, with row stride
+ * padded_rows(tokens) (needed for dw).  Workspaces, bf16: dl and dl_t [padded_rows(tokens) * width rounded up to 256], w_t [hidden, width rounded
+ * up to 256] (needed for dx). */
+int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_t, const void* w, int64_t ld_w, const int64_t* target,
+                                     int64_t tokens, int64_t hidden, int64_t vocab, int64_t first, int64_t width, int64_t ignore_index,
+                                     float smoothing, const float* lse, const float* grad, int64_t grad_stride, const float* count, void* dl,
+                                     void* dl_t, void* w_t, float* dx, int dx_add, void* dw, int dw_type, int dw_add, hpfp8_stream_t stream);
+/* x[rows, cols] -> x_t[cols, ld_t], bf16, zeros behind the rows up to a multiple of 64 and in place of rows whose target (may be NULL) is
+ * ignore_index. */
+int hpfp8_linear_cross_entropy_rows_t(const void* x, int64_t rows, int64_t cols, int64_t ld, const int64_t* target, int64_t ignore_index, void* x_t,
+                                      int64_t ld_t, hpfp8_stream_t stream);
+/* The sum of the pieces' dx, rounded to bf16 (n a multiple of 8). */
+int hpfp8_linear_cross_entropy_round(const float* x, int64_t n, void* y, hpfp8_stream_t stream);
 
 #ifdef __cplusplus
 }

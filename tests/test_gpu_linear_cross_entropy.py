@@ -1,0 +1,230 @@
+"""Softmax cross entropy of a linear, without its logits, against 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+IGNORE = -100
+H = 2.0 ** -8        # half a step of bf16, relative
+U = 2.0 ** -24
+
+
+def make(tokens, hidden, vocab, seed, ignored=0.1):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((tokens, hidden), generator=g).to(torch.bfloat16)
+    w = (torch.randn((vocab, hidden), generator=g) * 2 / math.sqrt(hidden)).to(torch.bfloat16)
+    t = torch.randint(vocab, (tokens,), generator=g)
+    if tokens > 1:
+        t = torch.where(torch.rand((tokens,), generator=g) < ignored, IGNORE, t)
+        t[0] = vocab - 1
+    return x, w, t
+
+
+def reference(x, w, t, smoothing, coefficient):
+    """(loss per row, dx, dw, bounds of the three) in 64 bits; coefficient [tokens]: each row's share of the loss's gradient.
+    A logit is a chain of hidden / 32 accumulations of 32 products each, at most a step of fp32 lost in each: `off`."""
+    x, w = x.double(), w.double()
+    vocab, hidden = w.shape
+    l = x @ w.t()
+    off = (hidden / 32 + 32) * 2 * U * (x.abs() @ w.abs().t()).amax(1)
+    lse = torch.logsumexp(l, 1)
+    counted = t != IGNORE
+    at = torch.where(counted, t, 0)
+    rows = lse - (1 - smoothing) * l.gather(1, at[:, None])[:, 0] - smoothing * l.mean(1)
+    rows = torch.where(counted, rows, 0.0)
+    # the logits' error reaches lse and the target's logit; 64 roundings of sums of exponentials (relative: absolute in lse); a few of the result's
+    b_rows = 2 * off + 64 * U + 8 * U * (lse.abs() + l.abs().amax(1)) + (vocab / 256 + 64) * U * smoothing * l.abs().mean(1)
+    p = torch.exp(l - lse[:, None])
+    c = torch.where(counted, coefficient.double(), 0.0)[:, None]
+    dl = p - smoothing / vocab
+    dl.scatter_add_(1, at[:, None], torch.full_like(dl, -(1 - smoothing))[:, :1])
+    size = (p + smoothing / vocab)
+    size.scatter_add_(1, at[:, None], torch.full_like(dl, 1 - smoothing)[:, :1])
+    # dl: rounded to bf16; its probability is off by the logits' and lse's errors, relative
+    b_dl = H * dl.abs() + size * (4 * off[:, None] + 64 * U + 4 * U * l.abs().amax())
+    dl, b_dl = c * dl, c.abs() * b_dl * 1.01
+    dx, dw = dl @ w, dl.t() @ x
+    b_dx = b_dl @ w.abs() + (vocab / 32 + 64) * 2 * U * (dl.abs() @ w.abs())
+    b_dw = b_dl.t() @ x.abs() + (x.shape[0] / 32 + 64) * 2 * U * (dl.abs().t() @ x.abs())
+    return rows, dx, dw, b_rows, b_dx, b_dw
+
+
+def within(got, want, bound, half=0.0):
+    off = (got.double().cpu() - want).abs()
+    limit = half * want.abs() + bound
+    assert (off <= limit).all(), float((off - limit).max())
+
+
+SIZES = [(1, 8, 1), (1, 64, 256), (2, 8, 300), (5, 128, 1000), (64, 72, 257), (255, 256, 511), (256, 512, 512), (300, 200, 1111), (513, 320, 2049)]
+
+
+@pytest.mark.parametrize("tokens,hidden,vocab", SIZES)
+@pytest.mark.parametrize("reduction,smoothing", [("mean", 0.0), ("sum", 0.1), ("none", 0.0), ("none", 0.3)])
+def test_loss_and_gradients(gpu, tokens, hidden, vocab, reduction, smoothing):
+    import hpfp8
+    x, w, t = make(tokens, hidden, vocab, 1)
+    xg, wg = x.to(gpu).requires_grad_(), w.to(gpu).requires_grad_()
+    loss = hpfp8.linear_cross_entropy(xg, wg, t.to(gpu), reduction=reduction, label_smoothing=smoothing)
+    assert loss.dtype == torch.float32
+    counted = t != IGNORE
+    go = torch.randn((tokens,), generator=torch.Generator().manual_seed(2)) if reduction == "none" else torch.tensor(0.7)
+    coefficient = go if reduction == "none" else (go / counted.sum() if reduction == "mean" else go).expand(tokens)
+    dx, dw = torch.autograd.grad(loss, (xg, wg), go.to(gpu))
+    rows, rdx, rdw, b_rows, b_dx, b_dw = reference(x, w, t, smoothing, coefficient)
+    if reduction == "none":
+        within(loss.detach(), rows, b_rows)
+        assert (loss.detach().cpu()[~counted] == 0).all()
+    else:
+        n = counted.sum() if reduction == "mean" else 1
+        within(loss.detach(), rows.sum() / n, (b_rows * counted).sum() / n + U * (rows.sum() / n).abs())
+    within(dx, rdx, b_dx, H)
+    within(dw, rdw, b_dw, H)
+    assert (dx.cpu()[~counted] == 0).all()
+    with torch.no_grad():
+        assert torch.equal(hpfp8.linear_cross_entropy(xg, wg, t.to(gpu), reduction=reduction, label_smoothing=smoothing), loss)
+
+
+@pytest.mark.parametrize("budget", [1 << 20, 1 << 16])
+def test_pieces_of_the_vocabulary(gpu, budget, monkeypatch):
+    """Several pieces, a last one that is no whole tile: the weight's gradient has the bits of one piece, x's is summed in fp32."""
+    import hpfp8
+    from hpfp8 import loss as module
+    x, w, t = make(130, 256, 2000, 3)
+    assert len(module._pieces(130, 256, 2000, budget)) > 1
+    both = []
+    for b in (1 << 30, budget):
+        monkeypatch.setattr(module, "_PIECE_BYTES", b)
+        xg, wg = x.to(gpu).requires_grad_(), w.to(gpu).requires_grad_()
+        both.append(torch.autograd.grad(hpfp8.linear_cross_entropy(xg, wg, t.to(gpu)), (xg, wg)))
+    _, rdx, _, _, b_dx, _ = reference(x, w, t, 0.0, torch.full((130,), 1.0) / (t != IGNORE).sum())
+    within(both[1][0], rdx, b_dx, H)
+    assert torch.equal(both[0][1], both[1][1])
+
+
+def test_pieces_cover_the_vocabulary_once():
+    from hpfp8.loss import _pieces
+    for tokens, hidden, vocab, budget in ((1, 8, 1, 1), (4096, 7168, 131072, 512 << 20), (1 << 22, 8, 1 << 24, 512 << 20), (300, 64, 50001, 1 << 20)):
+        pieces = _pieces(tokens, hidden, vocab, budget)
+        assert pieces[0][0] == 0 and sum(n for _, n in pieces) == vocab
+        assert all(a + n == b for (a, n), (b, _) in zip(pieces, pieces[1:])) and all(n % 256 == 0 for _, n in pieces[:-1])
+
+
+def test_tokens_in_several_forwards(gpu, monkeypatch):
+    import hpfp8
+    from hpfp8 import loss as module
+    x, w, t = (v.to(gpu) for v in make(600, 64, 500, 4))
+    want = [hpfp8.linear_cross_entropy(x, w, t, reduction=r, label_smoothing=0.1) for r in ("none", "mean", "sum")]
+    monkeypatch.setattr(module, "_FORWARD_ROWS", 256)
+    got = [hpfp8.linear_cross_entropy(x, w, t, reduction=r, label_smoothing=0.1) for r in ("none", "mean", "sum")]
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_rows_that_are_ignored_may_hold_anything(gpu):
+    import hpfp8
+    x, w, t = make(100, 128, 700, 5, 0.3)
+    grads = []
+    for junk in (0.0, math.nan, math.inf):
+        y = x.clone()
+        y[t == IGNORE] = junk
+        xg, wg = y.to(gpu).requires_grad_(), w.to(gpu).requires_grad_()
+        loss = hpfp8.linear_cross_entropy(xg, wg, t.to(gpu))
+        grads.append((loss.detach(),) + torch.autograd.grad(loss, (xg, wg)))
+    for other in grads[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(grads[0], other))
+
+
+def test_all_rows_ignored_and_no_rows(gpu):
+    import hpfp8
+    x, w, t = make(20, 64, 100, 6)
+    for n in (20, 0):
+        xg, wg = x[:n].to(gpu).requires_grad_(), w.to(gpu).requires_grad_()
+        tg = torch.full((n,), IGNORE, device=gpu)
+        assert hpfp8.linear_cross_entropy(xg, wg, tg).isnan()
+        loss = hpfp8.linear_cross_entropy(xg, wg, tg, reduction="sum")
+        dx, dw = torch.autograd.grad(loss, (xg, wg))
+        assert loss == 0 and dx.shape == (n, 64) and (dx == 0).all() and (dw == 0).all()
+        assert hpfp8.linear_cross_entropy(xg, wg, tg, reduction="none").shape == (n,)
+
+
+def test_targets_out_of_range_and_logits_that_are_not_finite(gpu):
+    import hpfp8
+    x, w, t = make(40, 64, 300, 7, 0.0)
+    t[3], t[4] = 300, -5
+    x[7, 0] = math.nan
+    xg = x.to(gpu).requires_grad_()
+    loss = hpfp8.linear_cross_entropy(xg, w.to(gpu), t.to(gpu), reduction="none")
+    bad = torch.zeros(40, dtype=torch.bool)
+    bad[[3, 4, 7]] = True
+    assert torch.equal(loss.isnan().cpu(), bad)
+    dx, = torch.autograd.grad(loss.sum(), xg)
+    assert torch.equal(dx.isnan().any(1).cpu(), bad)
+    # another value that is ignored
+    t[3], t[4] = 7, 7
+    loss = hpfp8.linear_cross_entropy(x.to(gpu), w.to(gpu), t.to(gpu), reduction="none", ignore_index=7)
+    assert (loss.cpu()[t == 7] == 0).all()
+
+
+def test_large_logits(gpu):
+    """Logits of +-500: the largest is subtracted before the exponential."""
+    import hpfp8
+    x, w, t = make(50, 64, 400, 8)
+    x = x * 60
+    loss = hpfp8.linear_cross_entropy(x.to(gpu), w.to(gpu), t.to(gpu), reduction="none")
+    rows, _, _, b_rows, _, _ = reference(x, w, t, 0.0, torch.ones(50))
+    within(loss, rows, b_rows)
+
+
+def test_shapes_strides_and_starts_between_vectors(gpu):
+    import hpfp8
+    g = torch.Generator().manual_seed(9)
+    base = torch.randn((6, 50, 80), generator=g).to(torch.bfloat16).to(gpu)
+    weight = torch.randn((333, 96), generator=g).to(torch.bfloat16).to(gpu)
+    t = torch.randint(333, (6, 50), generator=g).to(gpu)
+    for x, w in ((base[:, :, :64], weight[:, :64]), (base[:, :, 3:67], weight[:, 1:65]), (base[::2, 5:20, 16:], weight[:, 32:]),
+                 (base.transpose(0, 1)[:, :, 8:72], weight[:, 8:72])):
+        tt = t.reshape(-1)[:x.shape[0] * x.shape[1]].reshape(x.shape[:2])
+        a = [v.detach().requires_grad_() for v in (x, w)]
+        b = [v.detach().clone(memory_format=torch.contiguous_format).requires_grad_() for v in (x, w)]
+        got, want = hpfp8.linear_cross_entropy(*a, tt, reduction="none"), hpfp8.linear_cross_entropy(*b, tt, reduction="none")
+        assert got.shape == tt.shape and torch.equal(got, want)
+        for p, q in zip(torch.autograd.grad(got.sum(), a), torch.autograd.grad(want.sum(), b)):
+            assert torch.equal(p, q)
+
+
+def test_gradient_of_one_alone_and_main_grad(gpu):
+    import hpfp8
+    x, w, t = (v.to(gpu) for v in make(70, 64, 900, 10))
+    leaves = [v.clone().requires_grad_() for v in (x, w)]
+    dx, dw = torch.autograd.grad(hpfp8.linear_cross_entropy(*leaves, t), leaves)
+    for k in range(2):
+        some = [v.clone().requires_grad_(i == k) for i, v in enumerate((x, w))]
+        assert torch.equal(torch.autograd.grad(hpfp8.linear_cross_entropy(*some, t), some[k])[0], (dx, dw)[k])
+    p = torch.nn.Parameter(w.clone())
+    xg = x.clone().requires_grad_()
+    for step in (1, 2):
+        hpfp8.linear_cross_entropy(xg, p, t, apply_grad_on_fp32_main_grad=True).backward()
+        assert p.grad is None and p.main_grad.dtype == torch.float32
+        if step == 1:
+            once = p.main_grad.clone()
+            assert torch.equal(once.to(torch.bfloat16), dw)
+    assert ((p.main_grad - 2 * once).abs() <= 4 * U * once.abs()).all()
+
+
+def test_gradient_against_differences(gpu):
+    import hpfp8
+    x, w, t = make(3, 16, 50, 11, 0.0)
+    xg = x.to(gpu).requires_grad_()
+    dx, = torch.autograd.grad(hpfp8.linear_cross_entropy(xg, w.to(gpu), t.to(gpu), reduction="sum"), xg)
+    with torch.no_grad():
+        for c in range(16):
+            up, down = x.clone(), x.clone()
+            up[:, c] += 0.0625
+            down[:, c] -= 0.0625
+            step = (up[:, c].double() - down[:, c].double())
+            d = (hpfp8.linear_cross_entropy(up.to(gpu), w.to(gpu), t.to(gpu), reduction="none")
+                 - hpfp8.linear_cross_entropy(down.to(gpu), w.to(gpu), t.to(gpu), reduction="none")).double().cpu() / step
+            # the loss's third derivative along c is below 8 (a moment of weights below 2); bf16 rounds dl's 50 summands
+            limit = 8 / 6 * 0.0625 ** 2 * 1.2 + 2.0 ** -7 * 2 * float(w.abs().max()) + 1e-4 + (step - 0.125).abs() * 8
+            assert ((d - dx.double().cpu()[:, c]).abs() <= limit).all()
