@@ -42,6 +42,7 @@ struct Product {
   int64_t ldc;           // elements
   int store;
   int tiles;
+  int splits;            // parts of k, each with a c of its own, M ldc elements behind the one before
 };
 
 struct CeParams {
@@ -53,11 +54,12 @@ struct CeParams {
   // kStats and kDlogits
   const int64_t* target; // [M]
   int64_t rows_padded;
-  // kDlogits
-  const float* lse;      // [M]
-  const float* grad;     // of the loss: one value, or one for each row with stride grad_stride
+  // kDlogits and kGrads: the gradient of the loss, one value, or one for each row with stride grad_stride
+  const float* grad;
   int64_t grad_stride;
   const float* count;    // rows that count, when the loss is their mean; null otherwise
+  // kDlogits
+  const float* lse;      // [M]
   int64_t ignore_index;
   float smoothing;
   int64_t vocab;         // the whole of it
@@ -95,10 +97,20 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
   uint8_t* const b_lds = lds + 2 * kSlabBytes;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pid = blockIdx.x;
-  const bool second = EPI == kGrads && pid >= p.part[0].tiles;
-  const Product q = second ? p.part[1] : p.part[0];
-  int tm, tn;
-  tile_at(tile_of_workgroup(second ? pid - p.part[0].tiles : pid, q.tiles), (q.M + kTile - 1) / kTile, (q.N + kTile - 1) / kTile, tm, tn);
+  const int before = EPI == kGrads ? p.part[0].tiles * p.part[0].splits : 0;
+  const bool second = EPI == kGrads && pid >= before;
+  Product q = second ? p.part[1] : p.part[0];
+  int t = tile_of_workgroup(second ? pid - before : pid, q.tiles * q.splits), tm, tn;
+  if (EPI == kGrads && q.splits > 1) {
+    const int split = t / q.tiles, all = (q.K + kSlab - 1) / kSlab;
+    t -= split * q.tiles;
+    const int from = (int)((int64_t)all * split / q.splits), to = (int)((int64_t)all * (split + 1) / q.splits);
+    q.a += (int64_t)from * kSlab * 2;
+    q.b += (int64_t)from * kSlab * 2;
+    q.K = (to < all ? to * kSlab : q.K) - from * kSlab;
+    q.c = reinterpret_cast<float*>(q.c) + (int64_t)split * q.M * q.ldc;
+  }
+  tile_at(t, (q.M + kTile - 1) / kTile, (q.N + kTile - 1) / kTile, tm, tn);
   const int m0 = tm * kTile, n0 = tn * kTile;
   const int slabs = (q.K + kSlab - 1) / kSlab;
 
@@ -265,8 +277,7 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
       float c = 0.f, lse = 0.f;
       if (t != p.ignore_index) {
         lse = p.lse[m + j];
-        c = p.grad[(int64_t)(m + j) * p.grad_stride];
-        if (p.count) c /= p.count[0];
+        c = p.grad_stride ? p.grad[(int64_t)(m + j) * p.grad_stride] : 1.f;
         if (t < 0 || t >= p.vocab) c = NAN;
       }
       const int own = t >= p.first && t < p.first + q.N ? (int)(t - p.first) : -1;
@@ -300,6 +311,15 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
         *reinterpret_cast<uint2*>(p.dl_t + (int64_t)(n + column_of(i, g, r)) * p.rows_padded + m) = v;
       }
   } else {
+    if (p.grad) {
+      // (one factor for all rows is applied here, so that what was rounded is a difference of probabilities: of c (p - 1) the most
+      // frequent value by far, -c, would be rounded the same way in every row)
+      const float c = p.grad[0] / (p.count ? p.count[0] : 1.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] *= c;
+    }
     if (q.store == kBf16) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -441,11 +461,17 @@ __global__ __launch_bounds__(256) void ce_transpose_kernel(const uint16_t* __res
   }
 }
 
-// ---- fp32 -> bf16
-__global__ __launch_bounds__(256) void ce_round_kernel(const float* __restrict__ in, int64_t n8, uint16_t* __restrict__ out) {
+// ---- the sum of the parts, in order, rounded to bf16
+__global__ __launch_bounds__(256) void ce_round_kernel(const float* __restrict__ in, int64_t n8, int parts, uint16_t* __restrict__ out) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n8) return;
-  const v4f a = reinterpret_cast<const v4f*>(in)[2 * i], b = reinterpret_cast<const v4f*>(in)[2 * i + 1];
+  const v4f* at = reinterpret_cast<const v4f*>(in) + 2 * i;
+  v4f a = at[0], b = at[1];
+  for (int k = 1; k < parts; ++k) {
+    at += 2 * n8;
+    a += at[0];
+    b += at[1];
+  }
   reinterpret_cast<u32x4_st*>(out)[i] = u32x4_st{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])};
 }
 
@@ -474,6 +500,7 @@ Product product(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t 
   q.ldc = ldc;
   q.store = store;
   q.tiles = tiles_of(M, N);
+  q.splits = 1;
   return q;
 }
 
@@ -485,6 +512,18 @@ using namespace hpfp8;
 extern "C" {
 
 int64_t hpfp8_cross_entropy_parts(int64_t vocab) { return vocab > 0 ? 2 * ((vocab + kTile - 1) / kTile) : 0; }
+// dx's product contracts over the whole piece and has few tiles, so with few tokens a few of its tiles would still be at work long after
+// dw's are done.  Its contraction is split until one part takes at most half of what all of the launch takes the 256 compute units
+// together (in slabs; a tile's start and end cost about six).  us of the launch unsplit / split: 512 tokens, 4096, 32000 736 / 256,
+// 1531, 2048, 50001 1112 / 541.
+int64_t hpfp8_cross_entropy_splits(int64_t tokens, int64_t hidden, int64_t width, int with_dw) {
+  if (tokens <= 0 || hidden <= 0 || width <= 0) return 1;
+  const int64_t slabs_x = (width + kSlab - 1) / kSlab, slabs_w = (tokens + kSlab - 1) / kSlab;
+  const int64_t all = tiles_of(tokens, hidden) * (slabs_x + 6) + (with_dw ? tiles_of(width, hidden) * (slabs_w + 6) : 0);
+  const int64_t half = all / 512 > 24 ? all / 512 : 24;
+  const int64_t splits = (slabs_x + half - 1) / half;
+  return splits < 16 ? splits : 16;
+}
 int64_t hpfp8_cross_entropy_padded_rows(int64_t tokens) { return tokens > 0 ? up(tokens, kTile) : 0; }
 
 int hpfp8_linear_cross_entropy_forward(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t tokens,
@@ -530,11 +569,15 @@ int hpfp8_linear_cross_entropy_reduce(const float* loss, const int64_t* target, 
 int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_t, const void* w, int64_t ld_w, const int64_t* target,
                                      int64_t tokens, int64_t hidden, int64_t vocab, int64_t first, int64_t width, int64_t ignore_index,
                                      float smoothing, const float* lse, const float* grad, int64_t grad_stride, const float* count, void* dl,
-                                     void* dl_t, void* w_t, float* dx, int dx_add, void* dw, int dw_type, int dw_add, hpfp8_stream_t stream) {
+                                     void* dl_t, void* w_t, float* dx, int splits, int dx_add, void* dw, int dw_type, int dw_add,
+                                     hpfp8_stream_t stream) {
   const int bad = check(tokens, hidden, vocab, ld_x, ld_w);
   if (bad != HPFP8_OK) return bad;
   HPFP8_REQUIRE(first >= 0 && width > 0 && first + width <= vocab, HPFP8_ERR_SHAPE, "piece %lld + %lld of %lld", (long long)first, (long long)width, (long long)vocab);
   HPFP8_REQUIRE(dw_type == HPFP8_OUT_BF16 || dw_type == HPFP8_OUT_F32, HPFP8_ERR_ARG, "unknown output type %d", dw_type);
+  HPFP8_REQUIRE(!dx || (splits >= 1 && splits <= 16), HPFP8_ERR_ARG, "dx in %d parts", splits);
+  const int64_t slabs = (width + kSlab - 1) / kSlab;
+  HPFP8_REQUIRE(!dx || dx_add || splits <= slabs, HPFP8_ERR_ARG, "dx in %d parts of %lld slabs", splits, (long long)slabs);
   HPFP8_REQUIRE(!dw_add || dw_type == HPFP8_OUT_F32, HPFP8_ERR_ARG, "only fp32 is added onto");
   if (tokens == 0) return HPFP8_OK;
   HPFP8_REQUIRE(x && w && target && lse && grad && dl && dl_t && (!dx == !w_t) && (!dw == !x_t), HPFP8_ERR_ARG, "null buffer");
@@ -568,7 +611,8 @@ int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_
                                                                                                        cols_padded);
     rc = check_launch("linear_cross_entropy_piece (transpose)");
     if (rc != HPFP8_OK) return rc;
-    g.part[n++] = product(dl, cols_padded, w_t, cols_padded, tokens, hidden, up(width, kSlab), dx, hidden, dx_add ? kF32Add : kF32);
+    g.part[n] = product(dl, cols_padded, w_t, cols_padded, tokens, hidden, up(width, kSlab), dx, hidden, dx_add ? kF32Add : kF32);
+    g.part[n++].splits = (int)(splits < slabs ? splits : slabs);      // (a narrower piece adds onto fewer parts)
   }
   if (dw) {
     void* const to = (uint8_t*)dw + first * hidden * (dw_type == HPFP8_OUT_F32 ? 4 : 2);
@@ -576,7 +620,9 @@ int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_
                           dw_type == HPFP8_OUT_BF16 ? kBf16 : (dw_add ? kF32Add : kF32));
   }
   if (n == 0) return HPFP8_OK;
-  ce_gemm_kernel<kGrads><<<g.part[0].tiles + g.part[1].tiles, 512, 0, s>>>(g);
+  g.grad = grad_stride ? nullptr : grad;
+  g.count = count;
+  ce_gemm_kernel<kGrads><<<g.part[0].tiles * g.part[0].splits + g.part[1].tiles * g.part[1].splits, 512, 0, s>>>(g);
   return check_launch("linear_cross_entropy_piece (gradients)");
 }
 
@@ -595,12 +641,13 @@ int hpfp8_linear_cross_entropy_rows_t(const void* x, int64_t rows, int64_t cols,
   return check_launch("linear_cross_entropy_rows_t");
 }
 
-int hpfp8_linear_cross_entropy_round(const float* x, int64_t n, void* y, hpfp8_stream_t stream) {
+int hpfp8_linear_cross_entropy_round(const float* x, int64_t n, int parts, void* y, hpfp8_stream_t stream) {
+  HPFP8_REQUIRE(parts >= 1, HPFP8_ERR_ARG, "%d parts", parts);
   HPFP8_REQUIRE(n >= 0 && n % 8 == 0, HPFP8_ERR_SHAPE, "n=%lld is no multiple of 8", (long long)n);
   if (n == 0) return HPFP8_OK;
   HPFP8_REQUIRE(x && y, HPFP8_ERR_ARG, "null buffer");
   HPFP8_REQUIRE(aligned16(x) && aligned16(y), HPFP8_ERR_ALIGN, "a buffer is not 16-byte aligned");
-  ce_round_kernel<<<(unsigned)((n / 8 + 255) / 256), 256, 0, (hipStream_t)stream>>>(x, n / 8, (uint16_t*)y);
+  ce_round_kernel<<<(unsigned)((n / 8 + 255) / 256), 256, 0, (hipStream_t)stream>>>(x, n / 8, parts, (uint16_t*)y);
   return check_launch("linear_cross_entropy_round");
 }
 

@@ -83,10 +83,10 @@ SIGNATURES = {
     "hpfp8_activation_backward": [_vp, _vp, _i64, _vp, _vp, _int, _i64, _i64, _int, _vp, _vp],
     "hpfp8_linear_cross_entropy_forward": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _f32, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "hpfp8_linear_cross_entropy_piece": [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _i64, _vp, _vp,
-                                         _vp, _vp, _vp, _int, _vp, _int, _int, _vp],
+                                         _vp, _vp, _vp, _int, _int, _vp, _int, _int, _vp],
     "hpfp8_linear_cross_entropy_reduce": [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp],
     "hpfp8_linear_cross_entropy_rows_t": [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp],
-    "hpfp8_linear_cross_entropy_round": [_vp, _i64, _vp, _vp],
+    "hpfp8_linear_cross_entropy_round": [_vp, _i64, _int, _vp, _vp],
     "hpfp8_layer_norm_forward": [_vp, _int, _i64, _i64, _i64, _vp, _vp, _int, _f32, _vp, _vp, _vp, _vp, _vp, _vp],
     "hpfp8_layer_norm_backward": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _int, _i64, _i64, _vp, _int, _vp, _vp, _vp, _vp, _vp],
 }
@@ -98,6 +98,7 @@ SIZE_FUNCTIONS = {
     "hpfp8_linear_few_rows": [_i64, _i64],
     "hpfp8_layer_norm_partials": [_i64, _i64],
     "hpfp8_cross_entropy_parts": [_i64],
+    "hpfp8_cross_entropy_splits": [_i64, _i64, _i64, _int],
     "hpfp8_cross_entropy_padded_rows": [_i64],
 }
 

@@ -86,6 +86,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         bf16, f32 = dict(dtype=torch.bfloat16, device=device), dict(dtype=torch.float32, device=device)
         grad = grad_out.reshape(-1).contiguous()
         dw = dx = x_t = w_t = None
+        splits = 1
         padded = _lib.load().hpfp8_cross_entropy_padded_rows(tokens)
         pieces = _pieces(tokens, hidden, vocab, _PIECE_BYTES)
         width = (pieces[0][1] + _TILE - 1) // _TILE * _TILE
@@ -98,17 +99,18 @@ class _LinearCrossEntropy(torch.autograd.Function):
             _lib.call("hpfp8_linear_cross_entropy_rows_t", ops._ptr(x2), tokens, hidden, x2.stride(0), ops._ptr(target), ctx.ignore_index,
                       ops._ptr(x_t), padded, ops._stream())
         if need_dx:
-            dx = torch.empty((tokens, hidden), **f32)
+            splits = _lib.load().hpfp8_cross_entropy_splits(tokens, hidden, pieces[0][1], int(need_dw))
+            dx = torch.empty((splits, tokens, hidden), **f32)
             w_t = torch.empty((hidden, width), **bf16)
         for first, n in pieces:
             _lib.call("hpfp8_linear_cross_entropy_piece", ops._ptr(x2), x2.stride(0), ops._ptr(x_t), ops._ptr(w), w.stride(0), ops._ptr(target),
                       tokens, hidden, vocab, first, n, ctx.ignore_index, ctx.smoothing, ops._ptr(lse), ops._ptr(grad),
                       0 if ctx.reduction else 1, ops._ptr(count) if ctx.reduction == 1 else None, ops._ptr(dl), ops._ptr(dl_t), ops._ptr(w_t),
-                      ops._ptr(dx), int(first > 0), ops._ptr(dw), _lib.OUT_BF16 if param is None else _lib.OUT_F32, int(main_grad is not None),
+                      ops._ptr(dx), splits, int(first > 0), ops._ptr(dw), _lib.OUT_BF16 if param is None else _lib.OUT_F32, int(main_grad is not None),
                       ops._stream())
         if need_dx:
             rounded = torch.empty(x.shape, **bf16)
-            _lib.call("hpfp8_linear_cross_entropy_round", ops._ptr(dx), dx.numel(), ops._ptr(rounded), ops._stream())
+            _lib.call("hpfp8_linear_cross_entropy_round", ops._ptr(dx), tokens * hidden, splits, ops._ptr(rounded), ops._stream())
             dx = rounded
         if need_dw and param is not None:
             if main_grad is None:

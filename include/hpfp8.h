@@ -554,21 +554,24 @@ int hpfp8_linear_cross_entropy_forward(const void* x, int64_t ld_x, const void* 
 int hpfp8_linear_cross_entropy_reduce(const float* loss, const int64_t* target, int64_t tokens, int64_t ignore_index, int reduction, float* out,
                                       float* count, hpfp8_stream_t stream);
 /* The backward's part of the vocabulary's columns [first, first + width): the gradient of the logits, rounded to bf16, and with it
- * dx (fp32 [tokens, hidden]; dx_add: added onto) and rows [first, first + width) of dw ([vocab, hidden], dw_type HPFP8_OUT_*; dw_add: added onto,
+ * dx (fp32 [splits, tokens, hidden], the parts of a sum; dx_add: added onto) and rows [first, first + width) of dw ([vocab, hidden], dw_type HPFP8_OUT_*; dw_add: added onto,
  * fp32 only).  Either may be NULL.  grad is the loss's gradient, one value with grad_stride 0 or one for each row; count as the
  * forward wrote it for reduction 1, otherwise NULL.  x_t is what hpfp8_linear_cross_entropy_rows_t makes of x, with row stride
  * padded_rows(tokens) (needed for dw).  Workspaces, bf16: dl and dl_t [padded_rows(tokens) * width rounded up to 256], w_t [hidden, width rounded
- * up to 256] (needed for dx). */
+ * up to 256] (needed for dx).  splits: what hpfp8_cross_entropy_splits says for the widest piece, or another number from 1 to 16 up to its
+ * slabs of 64 columns. */
+int64_t hpfp8_cross_entropy_splits(int64_t tokens, int64_t hidden, int64_t width, int with_dw);
 int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_t, const void* w, int64_t ld_w, const int64_t* target,
                                      int64_t tokens, int64_t hidden, int64_t vocab, int64_t first, int64_t width, int64_t ignore_index,
                                      float smoothing, const float* lse, const float* grad, int64_t grad_stride, const float* count, void* dl,
-                                     void* dl_t, void* w_t, float* dx, int dx_add, void* dw, int dw_type, int dw_add, hpfp8_stream_t stream);
+                                     void* dl_t, void* w_t, float* dx, int splits, int dx_add, void* dw, int dw_type, int dw_add,
+                                     hpfp8_stream_t stream);
 /* x[rows, cols] -> x_t[cols, ld_t], bf16, zeros behind the rows up to a multiple of 64 and in place of rows whose target (may be NULL) is
  * ignore_index. */
 int hpfp8_linear_cross_entropy_rows_t(const void* x, int64_t rows, int64_t cols, int64_t ld, const int64_t* target, int64_t ignore_index, void* x_t,
                                       int64_t ld_t, hpfp8_stream_t stream);
-/* The sum of the pieces' dx, rounded to bf16 (n a multiple of 8). */
-int hpfp8_linear_cross_entropy_round(const float* x, int64_t n, void* y, hpfp8_stream_t stream);
+/* The sum of dx's parts x[parts, n], rounded to bf16 (n a multiple of 8). */
+int hpfp8_linear_cross_entropy_round(const float* x, int64_t n, int parts, void* y, hpfp8_stream_t stream);
 
 #ifdef __cplusplus
 }
