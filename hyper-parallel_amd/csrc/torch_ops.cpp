@@ -17,6 +17,7 @@
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
@@ -38,7 +39,9 @@ constexpr int64_t kBlock = 128;
   X(hpfp8_quantize_per_tensor_t_bf16) X(hpfp8_transpose_codes) X(hpfp8_gemm_blockwise) X(hpfp8_gemm_blockwise_pow2) X(hpfp8_gemm_per_tensor) \
   X(hpfp8_quantize_per_tensor_sync_bf16) X(hpfp8_gemm_few_rows) X(hpfp8_linear_few_rows) X(hpfp8_linear_few_rows_bf16) X(hpfp8_linear_backward) X(hpfp8_quantize_two_per_tensor_t_bf16) X(hpfp8_gemm_blockwise_swiglu_quantize) X(hpfp8_swiglu_quantize_1x128_bf16) \
   X(hpfp8_swiglu_quantize_1x128_pow2_bf16) X(hpfp8_swiglu_quantize_1x128_fast_bf16) X(hpfp8_gemm_grouped_blockwise) \
-  X(hpfp8_bucket_pack_quantize_bf16) X(hpfp8_bucket_unpack_dequantize_bf16)
+  X(hpfp8_bucket_pack_quantize_bf16) X(hpfp8_bucket_unpack_dequantize_bf16) \
+  X(hpfp8_quantize_rows) X(hpfp8_dequantize_rows) X(hpfp8_activation_forward) X(hpfp8_activation_backward) X(hpfp8_layer_norm_forward) \
+  X(hpfp8_layer_norm_backward) X(hpfp8_layer_norm_partials)
 struct Library {
 #define HPFP8_POINTER(name) decltype(&::name) name = nullptr;
   HPFP8_FUNCTIONS(HPFP8_POINTER)
@@ -893,6 +896,323 @@ PyObject* bucket_unpack(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------
+// layer norm and activations, and tensors in 8 bits
+// ------------------------------------------------------------------------------------------------
+PyObject* norm_backward_function = nullptr;         // the Python backwards, for what the nodes below do not take
+PyObject* activation_backward_function = nullptr;
+
+int type_code(at::ScalarType t) { return t == at::kBFloat16 ? HPFP8_OUT_BF16 : t == at::kFloat ? HPFP8_OUT_F32 : t == at::kHalf ? HPFP8_TYPE_F16 : -1; }
+at::ScalarType type_of(int code) { return code == HPFP8_OUT_BF16 ? at::kBFloat16 : code == HPFP8_OUT_F32 ? at::kFloat : at::kHalf; }
+
+bool rows_of_values(PyObject* o, int64_t device, const at::Tensor*& t) {      // contiguous, one of the three types, with a last dimension
+  return plain(o, device, t) && type_code(t->scalar_type()) >= 0 && t->dim() >= 1 && t->is_contiguous();
+}
+// Nothing is under way that a Python autograd function would answer in its own way (or refuse).
+bool ordinary(std::initializer_list<const at::Tensor*> tensors) {
+  if (!no_modes() || torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode))
+    return false;
+  for (const at::Tensor* t : tensors)
+    if (t && t->_fw_grad(0).defined()) return false;
+  return true;
+}
+bool to_train(std::initializer_list<const at::Tensor*> tensors) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : tensors)
+    if (t && t->requires_grad()) return true;
+  return false;
+}
+int64_t groups_of(int64_t cols) { return (cols + kBlock - 1) / kBlock; }
+// a saved tensor is still what forward saved, whatever hooks did with it in between
+bool again(const at::Tensor& t, const at::Tensor& go, at::ScalarType type, int64_t numel) {
+  return t.defined() && t.is_cuda() && t.get_device() == go.get_device() && t.layout() == at::kStrided && !at::isTensorSubclassLike(t) &&
+         t.scalar_type() == type && t.numel() == numel && t.is_contiguous();
+}
+// Results of a backward that has no derivative of its own: using one for a second derivative raises.
+torch::autograd::variable_list once(torch::autograd::variable_list grads, const at::Tensor& go) {
+  if (!c10::GradMode::is_enabled() || !go.requires_grad()) return grads;
+  auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable",
+                                                               (int64_t)grads.size());
+  for (at::Tensor& g : grads)
+    if (g.defined()) g.set_requires_grad(true);          // (the error has a place in the graph of what requires a gradient alone)
+  return (*error)(std::move(grads));
+}
+torch::autograd::variable_list from_python(PyObject* function, const pybind11::tuple& args, size_t count) {
+  const auto grads = pybind11::reinterpret_steal<pybind11::object>(PyObject_CallObject(function, args.ptr()));
+  if (!grads) raise_python_error();
+  torch::autograd::variable_list out(count);
+  const pybind11::tuple each(grads);
+  for (size_t i = 0; i < each.size(); ++i)
+    if (!each[i].is_none()) out[i] = each[i].cast<at::Tensor>();
+  return out;
+}
+pybind11::tuple as_tuple(const std::vector<int64_t>& v) {
+  pybind11::tuple t(v.size());
+  for (size_t i = 0; i < v.size(); ++i) t[i] = v[i];
+  return t;
+}
+pybind11::object or_none(const at::Tensor& t) { return t.defined() ? pybind11::cast(t) : pybind11::object(pybind11::none()); }
+
+struct Norm {
+  at::Tensor y, kept, other, rstd;       // kept, other: x and its mean, or the codes and scales of its normalised values
+  int64_t cols;
+  bool keep;
+};
+
+struct NormNode : torch::autograd::Function<NormNode> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& weight,
+                            const std::optional<at::Tensor>& bias, const Norm& made) {
+    ctx->save_for_backward({made.keep ? made.kept : x, made.other, made.rstd, weight ? *weight : at::Tensor()});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    const std::optional<at::Tensor>& vector = weight ? weight : bias;
+    if (vector) ctx->saved_data["vector"] = vector->sizes().vec();
+    ctx->saved_data["flags"] = (int64_t)(made.keep | type_code(x.scalar_type()) << 1 | (vector ? type_code(vector->scalar_type()) : 1) << 3 | weight.has_value() << 5 |
+                                            bias.has_value() << 6);
+    ctx->saved_data["cols"] = made.cols;
+    return made.y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &kept = saved[0], &other = saved[1], &rstd = saved[2], &weight = saved[3];
+    const int64_t flags = ctx->saved_data["flags"].toInt(), cols = ctx->saved_data["cols"].toInt();
+    const bool keep = flags & 1;
+    const int type = flags >> 1 & 3, vtype = flags >> 3 & 3;
+    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+    const std::vector<int64_t> vector = ctx->saved_data.count("vector") ? ctx->saved_data["vector"].toIntVector() : std::vector<int64_t>();
+    const bool has_w = flags >> 5 & 1, has_b = flags >> 6 & 1;       // (an input that is not there has no edge)
+    const bool need_dw = has_w && ctx->needs_input_grad(1), need_db = has_b && ctx->needs_input_grad(has_w ? 2 : 1);
+    const at::Tensor& grad = grads[0];
+    const int64_t n = grad.numel(), rows = n / cols;
+    bool as_made = no_modes() && grad.is_cuda() && grad.layout() == at::kStrided && !at::isTensorSubclassLike(grad) &&
+                   again(rstd, grad, at::kFloat, rows) && (!weight.defined() || again(weight, grad, type_of(vtype), cols));
+    if (keep) as_made = as_made && again(kept, grad, at::kFloat8_e4m3fn, n) && again(other, grad, at::kFloat, rows * groups_of(cols));
+    else as_made = as_made && again(kept, grad, type_of(type), n) && again(other, grad, at::kFloat, rows);
+    if (!as_made) {
+      pybind11::gil_scoped_acquire held;
+      return from_python(norm_backward_function,
+                         pybind11::make_tuple(grad, kept, other, rstd, or_none(weight), keep, cols, as_tuple(shape), type,
+                                              ctx->saved_data.count("vector") ? pybind11::object(as_tuple(vector)) : pybind11::object(pybind11::none()), vtype,
+                                              need_dw, need_db), 4);
+    }
+    const at::Tensor go = grad.contiguous();
+    void* const stream = c10::hip::getCurrentHIPStream(go.get_device()).stream();
+    const at::TensorOptions plain_options = go.options().requires_grad(false);
+    at::Tensor dx = at::empty(shape, plain_options), dw, db;
+    if (need_dw) dw = at::empty(vector, plain_options.dtype(type_of(vtype)));
+    if (need_db) db = at::empty(vector, plain_options.dtype(type_of(vtype)));
+    const at::Tensor partial = at::empty({lib.hpfp8_layer_norm_partials(rows, cols), 2, cols}, plain_options.dtype(at::kFloat));
+    Call call;
+    HPFP8_CALL(call, hpfp8_layer_norm_backward, go.data_ptr(), cols, keep ? nullptr : kept.data_ptr(), cols, keep ? nullptr : f32(other),
+               keep ? kept.data_ptr() : nullptr, keep ? f32(other) : nullptr, f32(rstd), type, rows, cols,
+               weight.defined() ? weight.data_ptr() : nullptr, vtype, dx.data_ptr(), need_dw ? dw.data_ptr() : nullptr,
+               need_db ? db.data_ptr() : nullptr, f32(partial), stream);
+    if (!call.ok()) raise(call);
+    return once({dx, dw, db, at::Tensor()}, grad);
+  }
+};
+
+// (x, normalized_shape, weight or None, bias or None, eps, keep, device, stream) -> y, with its place in the graph where it has one
+PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 8);
+  const Where at_ = where(args, n_args);
+  const double eps = PyFloat_AsDouble(args[4]);
+  if (PyErr_Occurred()) throw python_error();
+  bool keep = truth(args[5]);
+  const at::Tensor *x, *v[2] = {nullptr, nullptr};
+  if (!rows_of_values(args[0], at_.device, x) || x->numel() == 0 || !PyTuple_Check(args[1])) Py_RETURN_NONE;
+  const Py_ssize_t dims = PyTuple_GET_SIZE(args[1]);
+  if (dims < 1 || dims > x->dim()) Py_RETURN_NONE;
+  int64_t cols = 1;
+  for (Py_ssize_t i = 0; i < dims; ++i) {
+    const int64_t size = PyLong_AsLongLong(PyTuple_GET_ITEM(args[1], i));
+    if (PyErr_Occurred()) throw python_error();
+    if (size != x->size(x->dim() - dims + i)) Py_RETURN_NONE;
+    cols *= size;
+  }
+  if (cols < 1 || lib.hpfp8_layer_norm_partials(1, cols) == 0) Py_RETURN_NONE;
+  for (int i = 0; i < 2; ++i) {
+    if (args[2 + i] == Py_None) continue;
+    if (!rows_of_values(args[2 + i], at_.device, v[i]) || v[i]->sizes() != x->sizes().slice(x->dim() - dims)) Py_RETURN_NONE;
+  }
+  if ((v[0] && v[1] && v[0]->scalar_type() != v[1]->scalar_type()) || !ordinary({x, v[0], v[1]})) Py_RETURN_NONE;
+  const bool train = to_train({x, v[0], v[1]});
+  keep = keep && train;
+  Norm made;
+  Call call;
+  {
+    pybind11::gil_scoped_release free;
+    at::NoGradGuard no_grad;
+    const int64_t rows = x->numel() / cols;
+    const at::TensorOptions options = x->options().requires_grad(false), floats = options.dtype(at::kFloat);
+    made.y = at::empty(x->sizes(), options);
+    made.keep = keep;
+    made.cols = cols;
+    if (train) made.rstd = at::empty({rows}, floats);
+    if (keep) {
+      made.kept = at::empty({rows, cols}, options.dtype(at::kFloat8_e4m3fn));
+      made.other = at::empty({rows, groups_of(cols)}, floats);
+    } else if (train) {
+      made.other = at::empty({rows}, floats);
+    }
+    const at::Tensor* const vector = v[0] ? v[0] : v[1];
+    HPFP8_CALL(call, hpfp8_layer_norm_forward, x->data_ptr(), type_code(x->scalar_type()), rows, cols, cols, v[0] ? v[0]->data_ptr() : nullptr,
+               v[1] ? v[1]->data_ptr() : nullptr, vector ? type_code(vector->scalar_type()) : HPFP8_OUT_BF16, (float)eps, made.y.data_ptr(),
+               train && !keep ? f32(made.other) : nullptr, train ? f32(made.rstd) : nullptr, keep ? made.kept.data_ptr() : nullptr,
+               keep ? f32(made.other) : nullptr, at_.stream);
+  }
+  if (!call.ok()) return failed(call);
+  if (!train) return THPVariable_Wrap(made.y);
+  return THPVariable_Wrap(NormNode::apply(*x, v[0] ? std::optional<at::Tensor>(*v[0]) : std::nullopt,
+                                          v[1] ? std::optional<at::Tensor>(*v[1]) : std::nullopt, made));
+  END_HANDLE_TH_ERRORS
+}
+
+struct Activated {
+  at::Tensor y, codes, scales;
+  int kind;
+  bool keep;
+};
+
+struct ActivationNode : torch::autograd::Function<ActivationNode> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const Activated& made) {
+    if (made.keep) ctx->save_for_backward({made.codes, made.scales});
+    else ctx->save_for_backward({x});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["flags"] = (int64_t)(made.keep | made.kind << 1 | type_code(x.scalar_type()) << 3);
+    return made.y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    const bool keep = flags & 1;
+    const int kind = flags >> 1 & 3, type = flags >> 3 & 3;
+    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+    const int64_t halves = kind == 3 ? 2 : 1, cols = shape.back() / halves;
+    const at::Tensor& grad = grads[0];
+    const int64_t n = grad.numel(), rows = n / cols;
+    bool as_made = no_modes() && grad.is_cuda() && grad.layout() == at::kStrided && !at::isTensorSubclassLike(grad);
+    if (keep) as_made = as_made && again(saved[0], grad, at::kFloat8_e4m3fn, halves * n) && again(saved[1], grad, at::kFloat, rows * halves * groups_of(cols));
+    else as_made = as_made && again(saved[0], grad, type_of(type), halves * n);
+    if (!as_made) {
+      pybind11::gil_scoped_acquire held;
+      return from_python(activation_backward_function,
+                         pybind11::make_tuple(grad, saved[0], keep ? or_none(saved[1]) : pybind11::object(pybind11::none()), keep, kind, as_tuple(shape)), 2);
+    }
+    const at::Tensor go = grad.contiguous();
+    at::Tensor dx = at::empty(shape, go.options().requires_grad(false));
+    Call call;
+    HPFP8_CALL(call, hpfp8_activation_backward, go.data_ptr(), keep ? nullptr : saved[0].data_ptr(), keep ? 0 : halves * cols,
+               keep ? saved[0].data_ptr() : nullptr, keep ? f32(saved[1]) : nullptr, type, rows, cols, kind, dx.data_ptr(),
+               c10::hip::getCurrentHIPStream(go.get_device()).stream());
+    if (!call.ok()) raise(call);
+    return once({dx, at::Tensor()}, grad);
+  }
+};
+
+// (x, kind, keep, device, stream) -> y, with its place in the graph where it has one
+PyObject* activation(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 5);
+  const Where at_ = where(args, n_args);
+  Activated made;
+  made.kind = (int)PyLong_AsLongLong(args[1]);
+  if (PyErr_Occurred()) throw python_error();
+  made.keep = truth(args[2]);
+  const at::Tensor* x;
+  const int64_t halves = made.kind == 3 ? 2 : 1;
+  if (!rows_of_values(args[0], at_.device, x) || x->numel() == 0 || x->size(-1) % halves || !ordinary({x})) Py_RETURN_NONE;
+  const bool train = to_train({x});
+  made.keep = made.keep && train;
+  Call call;
+  {
+    pybind11::gil_scoped_release free;
+    at::NoGradGuard no_grad;
+    const int64_t width = x->size(-1), cols = width / halves, rows = x->numel() / width;
+    const at::TensorOptions options = x->options().requires_grad(false);
+    std::vector<int64_t> shape = x->sizes().vec();
+    shape.back() = cols;
+    made.y = at::empty(shape, options);
+    if (made.keep) {
+      made.codes = at::empty({rows, width}, options.dtype(at::kFloat8_e4m3fn));
+      made.scales = at::empty({rows, halves, groups_of(cols)}, options.dtype(at::kFloat));
+    }
+    HPFP8_CALL(call, hpfp8_activation_forward, x->data_ptr(), type_code(x->scalar_type()), rows, cols, width, made.kind, made.y.data_ptr(),
+               made.keep ? made.codes.data_ptr() : nullptr, made.keep ? f32(made.scales) : nullptr, at_.stream);
+  }
+  if (!call.ok()) return failed(call);
+  return THPVariable_Wrap(train ? ActivationNode::apply(*x, made) : made.y);
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, device, stream) -> (codes, scale_inv)
+PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 3);
+  const Where at_ = where(args, n_args);
+  const at::Tensor* x;
+  if (!rows_of_values(args[0], at_.device, x) || x->numel() == 0 || !no_modes()) Py_RETURN_NONE;
+  at::Tensor codes, scales;
+  Call call;
+  {
+    pybind11::gil_scoped_release free;
+    at::NoGradGuard no_grad;
+    const int64_t cols = x->size(-1);
+    std::vector<int64_t> shape = x->sizes().vec();
+    const at::TensorOptions options = x->options().requires_grad(false);
+    codes = at::empty(shape, options.dtype(at::kFloat8_e4m3fn));
+    shape.back() = groups_of(cols);
+    scales = at::empty(shape, options.dtype(at::kFloat));
+    HPFP8_CALL(call, hpfp8_quantize_rows, x->data_ptr(), type_code(x->scalar_type()), x->numel() / cols, cols, cols, codes.data_ptr(), f32(scales),
+               at_.stream);
+  }
+  return call.ok() ? tuple_of(std::move(codes), std::move(scales)) : failed(call);
+  END_HANDLE_TH_ERRORS
+}
+
+// (codes, scale_inv, element type, device, stream) -> x
+PyObject* dequantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 5);
+  const Where at_ = where(args, n_args);
+  const int type = (int)PyLong_AsLongLong(args[2]);
+  if (PyErr_Occurred()) throw python_error();
+  const at::Tensor *codes, *scales;
+  if (!plain(args[0], at_.device, codes) || codes->scalar_type() != at::kFloat8_e4m3fn || codes->dim() < 1 || codes->numel() == 0 ||
+      !codes->is_contiguous() || !floats(args[1], at_.device, scales) || !scales->is_contiguous() ||
+      scales->numel() != codes->numel() / codes->size(-1) * groups_of(codes->size(-1)) || !no_modes())
+    Py_RETURN_NONE;
+  at::Tensor x;
+  Call call;
+  {
+    pybind11::gil_scoped_release free;
+    at::NoGradGuard no_grad;
+    x = at::empty(codes->sizes(), codes->options().dtype(type_of(type)));
+    const int64_t cols = codes->size(-1);
+    HPFP8_CALL(call, hpfp8_dequantize_rows, codes->data_ptr(), f32(*scales), codes->numel() / cols, cols, x.data_ptr(), type, at_.stream);
+  }
+  return call.ok() ? THPVariable_Wrap(std::move(x)) : failed(call);
+  END_HANDLE_TH_ERRORS
+}
+
+// (the Python functions that NormNode's and ActivationNode's backwards call where they do not apply themselves)
+PyObject* bind_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 1);
+  Py_INCREF(args[0]);
+  norm_backward_function = args[0];
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+PyObject* bind_activation_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 1);
+  Py_INCREF(args[0]);
+  activation_backward_function = args[0];
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // (handle of the loaded library, function that raises for a name and a status, torch.nn.Parameter)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -930,6 +1250,8 @@ PyMethodDef methods[] = {HPFP8_METHOD(built_for), HPFP8_METHOD(bind), HPFP8_METH
                          HPFP8_METHOD(quantize_128x128), HPFP8_METHOD(quantize_per_tensor_t), HPFP8_METHOD(gemm_blockwise),
                          HPFP8_METHOD(gemm_per_tensor), HPFP8_METHOD(trains), HPFP8_METHOD(linear_node), HPFP8_METHOD(linear_train), HPFP8_METHOD(linear_infer), HPFP8_METHOD(linear_backward),
                          HPFP8_METHOD(swiglu_mlp_infer), HPFP8_METHOD(grouped_infer), HPFP8_METHOD(bucket_pack), HPFP8_METHOD(bucket_unpack),
+                         HPFP8_METHOD(layer_norm), HPFP8_METHOD(activation), HPFP8_METHOD(quantize_rows), HPFP8_METHOD(dequantize_rows),
+                         HPFP8_METHOD(bind_norm_backward), HPFP8_METHOD(bind_activation_backward),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -53,6 +53,11 @@ class Fp8Activation(NamedTuple):
         dtype = self.dtype if dtype is None else dtype
         if dtype not in _TYPES:
             raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
+        if ops._gpu(self.codes):
+            device = ops._device()
+            x = ops._native.dequantize_rows(self.codes, self.scale_inv, _TYPES[dtype], device, ops._raw_stream(device))
+            if x is not None:
+                return x
         ops._check_device(self.codes, "codes")
         x = torch.empty(self.codes.shape, dtype=dtype, device=self.codes.device)
         cols = x.shape[-1]
@@ -68,6 +73,11 @@ def quantize_activation(x: torch.Tensor) -> Fp8Activation:
     """x[..., C] (bfloat16, float16 or float32; any C, any strides) in 8 bits: E4M3 codes, one scale for each 128 values of the last
     dimension, the last group of a row being what is left.  For bf16 rows of a multiple of 128 values the codes and scales of
     `quantize_1x128`."""
+    if ops._gpu(x):
+        device = ops._device()
+        made = ops._native.quantize_rows(x, device, ops._raw_stream(device))
+        if made is not None:
+            return Fp8Activation(*made, x.dtype)
     _check_rows(x, "x")
     if x.dim() < 1:
         raise ValueError("x must have at least one dimension")
@@ -141,17 +151,26 @@ class _Activation(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        codes = scale_inv = x2 = None
-        if ctx.keep:
-            codes, scale_inv = ctx.saved_tensors
-        else:
-            x2 = _as_rows(ctx.saved_tensors[0], ctx.shape[-1])
-        go = grad_out.contiguous()
-        dx = torch.empty(ctx.shape, dtype=go.dtype, device=go.device)
-        rows = go.numel() // max(ctx.cols, 1)
-        _lib.call("hpfp8_activation_backward", ops._ptr(go), ops._ptr(x2), 0 if x2 is None else x2.stride(0), ops._ptr(codes),
-                  ops._ptr(scale_inv), _TYPES[go.dtype], rows, ctx.cols, ctx.kind, ops._ptr(dx), ops._stream())
-        return dx, None, None
+        return _backward(grad_out, *(ctx.saved_tensors if ctx.keep else (*ctx.saved_tensors, None)), ctx.keep, ctx.kind, ctx.shape), None, None
+
+
+def _backward(grad_out, kept, scale_inv, keep, kind, shape):
+    """dx.  kept: x, or its codes with their scales."""
+    cols = shape[-1] // (2 if kind == 3 else 1)
+    x2 = None
+    if keep:                # (hooks on saved tensors may have handed them back with other strides)
+        kept, scale_inv = kept.contiguous(), scale_inv.contiguous()
+    else:
+        x2 = _as_rows(kept, shape[-1])
+    go = grad_out.contiguous()
+    dx = torch.empty(shape, dtype=go.dtype, device=go.device)
+    _lib.call("hpfp8_activation_backward", ops._ptr(go), ops._ptr(x2), 0 if x2 is None else x2.stride(0), ops._ptr(kept) if keep else None,
+              ops._ptr(scale_inv), _TYPES[go.dtype], go.numel() // max(cols, 1), cols, kind, ops._ptr(dx), ops._stream())
+    return dx
+
+
+if ops._native is not None:
+    ops._native.bind_activation_backward(lambda *args: (_backward(*args),))
 
 
 _ACTIVATION_DEFAULTS = dict(keep_8bit=True)
@@ -168,6 +187,11 @@ def activation(input: torch.Tensor, kind: str, *, keep_8bit: bool = True) -> tor
         return _hand_off(activation, (input,), (input, kind), dict(keep_8bit=keep_8bit), _ACTIVATION_DEFAULTS)
     if kind not in KINDS:
         raise ValueError(f"kind must be one of {tuple(KINDS)}, got {kind!r}")
+    if ops._gpu(input):
+        device = ops._device()
+        y = ops._native.activation(input, KINDS[kind], keep_8bit, device, ops._raw_stream(device))
+        if y is not None:
+            return y
     _check_rows(input, "input")
     if input.dim() < 1:
         raise ValueError("input must have at least one dimension")

@@ -72,6 +72,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out):
         x, weight, target, lse, count = ctx.saved_tensors
+        target, lse = target.contiguous(), lse.contiguous()      # (hooks on saved tensors may have handed them back with other strides)
         need_dx, need_dw = ctx.needs_input_grad[:2]
         x2, w = _rows(x), _rows(weight)
         tokens, hidden = x2.shape

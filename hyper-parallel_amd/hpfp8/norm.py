@@ -12,6 +12,7 @@ from .kept import _TYPES, _as_rows, _check_rows, _groups
 from .linear import _hand_off
 
 MAX_WIDTH = 16384
+_OF_CODE = {code: dtype for dtype, code in _TYPES.items()}
 
 
 def _forward(x2, weight, bias, eps, stats: bool, keep: bool):
@@ -52,22 +53,30 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        kept, other, rstd, weight = ctx.saved_tensors
-        cols = ctx.cols
-        go = _as_rows(grad_out, cols)
-        rows = go.shape[0]
-        dx = torch.empty(ctx.shape, dtype=ctx.dtype, device=go.device)
-        shape, vtype = ctx.vector if ctx.vector is not None else (None, torch.float32)
-        dw = torch.empty(shape, dtype=vtype, device=go.device) if ctx.needs_input_grad[1] else None
-        db = torch.empty(shape, dtype=vtype, device=go.device) if ctx.needs_input_grad[2] else None
-        partial = torch.empty((_lib.load().hpfp8_layer_norm_partials(rows, cols), 2, cols), dtype=torch.float32, device=go.device)
-        w = None if weight is None else weight.reshape(-1).contiguous()
-        x2 = None if ctx.keep else _as_rows(kept, cols)
-        _lib.call("hpfp8_layer_norm_backward", ops._ptr(go), go.stride(0), ops._ptr(x2), 0 if x2 is None else x2.stride(0),
-                  None if ctx.keep else ops._ptr(other), ops._ptr(kept) if ctx.keep else None, ops._ptr(other) if ctx.keep else None,
-                  ops._ptr(rstd), _TYPES[ctx.dtype], rows, cols, ops._ptr(w), _TYPES[vtype], ops._ptr(dx), ops._ptr(dw), ops._ptr(db),
-                  ops._ptr(partial), ops._stream())
-        return dx, dw, db, None, None, None
+        shape, dtype = ctx.vector if ctx.vector is not None else (None, torch.float32)
+        return _backward(grad_out, *ctx.saved_tensors, ctx.keep, ctx.cols, ctx.shape, _TYPES[ctx.dtype], shape, _TYPES[dtype],
+                         ctx.needs_input_grad[1], ctx.needs_input_grad[2]) + (None, None, None)
+
+
+def _backward(grad_out, kept, other, rstd, weight, keep, cols, shape, dtype, vector, vector_dtype, need_dw, need_db):
+    """(dx, dw, db).  kept, other: x and its mean, or the codes and scales of its normalised values; vector: the shape of weight and bias."""
+    go = _as_rows(grad_out, cols)
+    rows = go.shape[0]
+    # (hooks on saved tensors may have handed them back with other strides)
+    kept, other, rstd = kept.contiguous() if keep else kept, other.contiguous(), rstd.contiguous()
+    dx = torch.empty(shape, dtype=_OF_CODE[dtype], device=go.device)
+    dw, db = (torch.empty(vector, dtype=_OF_CODE[vector_dtype], device=go.device) if need else None for need in (need_dw, need_db))
+    partial = torch.empty((_lib.load().hpfp8_layer_norm_partials(rows, cols), 2, cols), dtype=torch.float32, device=go.device)
+    w = None if weight is None else weight.reshape(-1).contiguous()
+    x2 = None if keep else _as_rows(kept, cols)
+    _lib.call("hpfp8_layer_norm_backward", ops._ptr(go), go.stride(0), ops._ptr(x2), 0 if x2 is None else x2.stride(0),
+              None if keep else ops._ptr(other), ops._ptr(kept) if keep else None, ops._ptr(other) if keep else None, ops._ptr(rstd), dtype, rows,
+              cols, ops._ptr(w), vector_dtype, ops._ptr(dx), ops._ptr(dw), ops._ptr(db), ops._ptr(partial), ops._stream())
+    return dx, dw, db
+
+
+if ops._native is not None:
+    ops._native.bind_norm_backward(_backward)
 
 
 _LAYER_NORM_DEFAULTS = dict(weight=None, bias=None, eps=1e-5, keep_8bit=False)
@@ -85,8 +94,14 @@ def layer_norm(input: torch.Tensor, normalized_shape: Union[int, Sequence[int]],
     if torch.overrides.has_torch_function(tensors):
         return _hand_off(layer_norm, tensors, (input, normalized_shape), dict(weight=weight, bias=bias, eps=eps, keep_8bit=keep_8bit),
                          _LAYER_NORM_DEFAULTS)
+    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
+    if ops._gpu(input):
+        device = ops._device()
+        y = ops._native.layer_norm(input, shape, weight, bias, eps, keep_8bit, device, ops._raw_stream(device))
+        if y is not None:
+            return y
     _check_rows(input, "input")
-    shape = torch.Size((normalized_shape,) if isinstance(normalized_shape, int) else normalized_shape)
+    shape = torch.Size(shape)
     if len(shape) < 1 or input.shape[-len(shape):] != shape:
         raise ValueError(f"input {tuple(input.shape)} does not end with normalized_shape {tuple(shape)}")
     cols = shape.numel()

@@ -266,3 +266,24 @@ def test_second_derivatives_are_refused(gpu):
     g, = torch.autograd.grad(hpfp8.activation(x, "silu").sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("keep", [False, True])
+def test_the_python_form_and_hooks_on_what_is_saved(gpu, keep, monkeypatch):
+    import hpfp8
+    from hpfp8 import ops
+    x, go = randn((21, 390), 15, torch.float16).to(gpu), randn((21, 195), 16, torch.float16).to(gpu)
+
+    def step():
+        a = x.clone().requires_grad_()
+        y = hpfp8.activation(a, "swiglu", keep_8bit=keep)
+        return y.detach(), torch.autograd.grad(y, a, go)[0]
+    want = step()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(gpu)):
+        got = step()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    kept = hpfp8.quantize_activation(x)
+    monkeypatch.setattr(ops, "_native", None)
+    assert all(torch.equal(p, q) for p, q in zip(step(), want))
+    again = hpfp8.quantize_activation(x)
+    assert torch.equal(again.codes.view(torch.uint8), kept.codes.view(torch.uint8)) and torch.equal(again.dequantize(), kept.dequantize())

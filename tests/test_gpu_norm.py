@@ -222,3 +222,59 @@ def test_gradient_against_differences(gpu):
             d = ((hpfp8.layer_norm(x + e, 24, w, b) - hpfp8.layer_norm(x - e, 24, w, b)) * go).sum(1) / (2 * step)
             # fp32 results of size 4 by 24 summands off by 2^-22 each, over 2 step; curvature: step^2 times third derivatives (below 2 per unit of go)
             assert ((d - dx[:, c]).abs() <= 24 * 4 * 4 * 2.0 ** -22 / (2 * step) + 2 * step ** 2 * go.abs().sum(1)).all()
+
+
+@pytest.mark.parametrize("keep", [False, True])
+def test_the_python_form_and_other_ways_through_the_graph(gpu, keep, monkeypatch):
+    """Without the native host path, under a dispatch mode, and with hooks on saved tensors: the same results."""
+    import hpfp8
+    from hpfp8 import ops
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x, w, b, go = (t.to(gpu) for t in make(33, 300, torch.bfloat16, torch.float32, 11))
+
+    def step(around_forward=None, around_backward=None):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        if around_forward is None:
+            y = hpfp8.layer_norm(leaves[0], 300, leaves[1], leaves[2], keep_8bit=keep)
+        else:
+            with around_forward:
+                y = hpfp8.layer_norm(leaves[0], 300, leaves[1], leaves[2], keep_8bit=keep)
+        if around_backward is None:
+            grads = torch.autograd.grad(y, leaves, go)
+        else:
+            with around_backward:
+                grads = torch.autograd.grad(y, leaves, go)
+        return (y.detach(),) + grads
+    want = step()
+    hooks = torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(gpu))
+    strided = torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.stack((t, t), -1)[..., 0])
+    for got in (step(Mode()), step(None, Mode()), step(hooks), step(strided) if not keep else want):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    with torch.no_grad():
+        monkeypatch.setattr(ops, "_native", None)
+        assert torch.equal(hpfp8.layer_norm(x, 300, w, b), want[0])
+    assert all(torch.equal(p, q) for p, q in zip(step(), want))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_second_derivatives_are_refused_and_writes_in_between_noticed(gpu, native, monkeypatch):
+    import hpfp8
+    from hpfp8 import ops
+    if not native:
+        monkeypatch.setattr(ops, "_native", None)
+    x = torch.randn((4, 64), device=gpu, requires_grad=True)
+    go = torch.ones((4, 64), device=gpu, requires_grad=True)
+    for f in (lambda t: hpfp8.layer_norm(t, 64), lambda t: hpfp8.activation(t, "silu")):
+        g, = torch.autograd.grad(f(x), x, go, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            g.sum().backward()
+    t = x * 1.0
+    y = hpfp8.layer_norm(t, 64)
+    t.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
