@@ -70,7 +70,7 @@ __device__ __forceinline__ void load_vector8(const void* w, int type, int col, i
 template <typename E, int TPR, int NV, bool KEEP, bool TAIL>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(NormParams p) {
   using raw = typename E::raw;
-  constexpr int kTeams = (TPR < 256 ? 256 : TPR) / TPR, kWaves = TPR / 64;
+  constexpr int kTeams = (TPR < 256 ? 256 : TPR) / TPR, kWaves = TPR / 64, kAhead = 2;
   __shared__ v4f parts[2][kTeams][kWaves];
   // (the same in a whole wave, so a row's address is a scalar)
   const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, wave = __builtin_amdgcn_readfirstlane(t / 64);
@@ -88,20 +88,16 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(Nor
   }
   const float n = (float)mine;
   const int64_t step = (int64_t)gridDim.x * kTeams;
-  Pack8<E> next[NV];
-  auto fetch = [&](int64_t r) {
+  Pack8<E> next[kAhead][NV];
+  auto fetch = [&](Pack8<E> (&to)[NV], int64_t r) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      next[j] = load_pack8<E, true, TAIL>((const raw*)p.x + (r < p.rows ? r : 0) * p.ld + (j * TPR + t) * 8, r < p.rows ? left[j] : 0);
+      to[j] = load_pack8<E, true, TAIL>((const raw*)p.x + (r < p.rows ? r : 0) * p.ld + (j * TPR + t) * 8, r < p.rows ? left[j] : 0);
   };
-  int64_t row = (int64_t)blockIdx.x * kTeams + team;
-  fetch(row);
-  int turn = 0;
-  for (int64_t at = (int64_t)blockIdx.x * kTeams; at < p.rows; at += step, row += step, turn ^= 1) {    // (as many turns for every team)
+  auto work = [&](const Pack8<E> (&packed)[NV], int64_t row, int turn) {
     float v[NV][8];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) unpack8<E>(next[j], v[j]);
-    fetch(row + step);
+    for (int j = 0; j < NV; ++j) unpack8<E>(packed[j], v[j]);
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -120,20 +116,19 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(Nor
     if constexpr (kWaves > 1) {
       if ((t & 63) == 0) parts[turn][team][wave] = v4f{n, mean, m2, 0.f};
       __syncthreads();                                // (one barrier: the next turn writes the other half)
-      v4f each[kWaves];
       float total = 0.f;
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k) {
-        each[k] = parts[turn][team][k];
-        total += each[k][0] * each[k][1];
-      }
+      for (int k = 0; k < kWaves; ++k) total += parts[turn][team][k][0] * parts[turn][team][k][1];
       mean = total / (float)C;
       m2 = 0.f;
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k) m2 += each[k][2] + each[k][0] * ((each[k][1] - mean) * (each[k][1] - mean));
+      for (int k = 0; k < kWaves; ++k) {
+        const v4f each = parts[turn][team][k];
+        m2 += each[2] + each[0] * ((each[1] - mean) * (each[1] - mean));
+      }
     }
     const float rstd = 1.0f / sqrtf(m2 / (float)C + p.eps);
-    if (row >= p.rows) continue;
+    if (row >= p.rows) return;
     if (t == 0) {
       if (p.mean) p.mean[row] = mean;
       if (p.rstd) p.rstd[row] = rstd;
@@ -157,74 +152,91 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(Nor
         }
       }
     }
+  };
+  const int64_t first = (int64_t)blockIdx.x * kTeams;
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) fetch(next[u], first + team + u * step);
+  int turn = 0;
+  for (int64_t at = first; at < p.rows; at += kAhead * step) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u, turn ^= 1) {
+      const int64_t from = at + u * step;             // (as many turns for every team)
+      if (from >= p.rows) break;
+      Pack8<E> packed[NV];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) packed[j] = next[u][j];
+      fetch(next[u], from + team + kAhead * step);
+      work(packed, from + team, turn);
+    }
   }
 }
 
 template <typename E, int TPR, int NV, bool KEEP, bool TAIL>
 __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(NormParams p) {
   using raw = typename E::raw;
-  constexpr int kTeams = kBackwardThreads / TPR, kWaves = TPR / 64, kChunks = TPR * NV;
+  constexpr int kTeams = kBackwardThreads / TPR, kWaves = TPR / 64, kChunks = TPR * NV, kAhead = NV <= 2 ? 3 : 1;
+  constexpr bool kHoldWeight = NV <= 2;      // (four steps' weights beside four steps' sums: over 256 registers)
   __shared__ v2f parts[2][kTeams][kWaves];
   __shared__ v4f joined[kTeams > 1 ? 2 * kChunks * 2 : 1];
   // (the same in a whole wave, so a row's address is a scalar)
   const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, wave = __builtin_amdgcn_readfirstlane(t / 64);
   const int C = p.cols, groups = (C + kBlock - 1) / kBlock;
   int left[NV];
-  float w[NV][8], dw[NV][8], db[NV][8];
+  float w[kHoldWeight ? NV : 1][8], dw[NV][8], db[NV][8];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     left[j] = C - (j * TPR + t) * 8;
-    load_vector8(p.w, p.wtype, (j * TPR + t) * 8, left[j], 1.f, w[j]);
+    if (kHoldWeight) load_vector8(p.w, p.wtype, (j * TPR + t) * 8, left[j], 1.f, w[j]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[j][i] = db[j][i] = 0.f;
   }
   const int64_t step = (int64_t)gridDim.x * kTeams;
-  Pack8<E> next_dy[NV], next_x[KEEP ? 1 : NV];
-  uint2 next_q[KEEP ? NV : 1];
-  float next_s[KEEP ? NV : 1], next_mean = 0.f, next_rstd = 0.f;
-  auto fetch = [&](int64_t r) {
+  struct Row {
+    Pack8<E> dy[NV], x[KEEP ? 1 : NV];
+    uint2 q[KEEP ? NV : 1];
+    float s[KEEP ? NV : 1], mean, rstd;
+  };
+  Row next[kAhead];
+  auto fetch = [&](Row& to, int64_t r) {
     const bool in = r < p.rows;
     const int64_t at = in ? r : 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int col = (j * TPR + t) * 8, n = in ? left[j] : 0;
-      next_dy[j] = load_pack8<E, true, TAIL>((const raw*)p.dy + at * p.ld_dy + col, n);
+      to.dy[j] = load_pack8<E, true, TAIL>((const raw*)p.dy + at * p.ld_dy + col, n);
       if constexpr (KEEP) {
-        next_q[j] = load_codes8<TAIL>(p.q + at * C + col, n);
-        next_s[j] = n > 0 ? (p.scale_inv + at * groups)[col / kBlock] : 0.f;
+        to.q[j] = load_codes8<TAIL>(p.q + at * C + col, n);
+        to.s[j] = n > 0 ? (p.scale_inv + at * groups)[col / kBlock] : 0.f;
       } else {
-        next_x[j] = load_pack8<E, true, TAIL>((const raw*)p.x + at * p.ld + col, n);
+        to.x[j] = load_pack8<E, true, TAIL>((const raw*)p.x + at * p.ld + col, n);
       }
     }
-    if (!KEEP) next_mean = in ? p.mean[r] : 0.f;
-    next_rstd = in ? p.rstd[r] : 0.f;
+    to.mean = !KEEP && in ? p.mean[r] : 0.f;
+    to.rstd = in ? p.rstd[r] : 0.f;
   };
-  int64_t row = (int64_t)blockIdx.x * kTeams + team;
-  fetch(row);
-  int turn = 0;
-  for (int64_t at = (int64_t)blockIdx.x * kTeams; at < p.rows; at += step, row += step, turn ^= 1) {
+  auto work = [&](const Row& from, int64_t row, int turn) {
     float go[NV][8], hat[NV][8];
-    const float rstd = next_rstd;
+    const float rstd = from.rstd;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      unpack8<E>(next_dy[j], go[j]);
+      unpack8<E>(from.dy[j], go[j]);
       if constexpr (KEEP) {
-        decode8(next_q[j], next_s[j], hat[j]);
+        decode8(from.q[j], from.s[j], hat[j]);
       } else {
-        unpack8<E>(next_x[j], hat[j]);
+        unpack8<E>(from.x[j], hat[j]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) hat[j][i] = i < left[j] ? (hat[j][i] - next_mean) * rstd : 0.f;
+        for (int i = 0; i < 8; ++i) hat[j][i] = i < left[j] ? (hat[j][i] - from.mean) * rstd : 0.f;
       }
     }
-    fetch(row + step);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      if (!kHoldWeight) load_vector8(p.w, p.wtype, (j * TPR + t) * 8, left[j], 1.f, w[0]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         dw[j][i] = __builtin_fmaf(go[j][i], hat[j][i], dw[j][i]);
         db[j][i] += go[j][i];
-        go[j][i] *= w[j][i];                          // from here on u
+        go[j][i] *= w[kHoldWeight ? j : 0][i];        // from here on u
         s1 += go[j][i];
         s2 = __builtin_fmaf(go[j][i], hat[j][i], s2);
       }
@@ -241,7 +253,7 @@ __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(NormPar
         s2 += parts[turn][team][k].y;
       }
     }
-    if (row >= p.rows) continue;
+    if (row >= p.rows) return;
     const float m1 = s1 / (float)C, m2 = s2 / (float)C;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -249,6 +261,20 @@ __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(NormPar
 #pragma unroll
       for (int i = 0; i < 8; ++i) out[i] = (go[j][i] - m1 - hat[j][i] * m2) * rstd;
       if (left[j] > 0) store8<E, true, TAIL>((raw*)p.dx + row * C + (j * TPR + t) * 8, left[j], out);
+    }
+  };
+  const int64_t first = (int64_t)blockIdx.x * kTeams;
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) fetch(next[u], first + team + u * step);
+  int turn = 0;
+  for (int64_t at = first; at < p.rows; at += kAhead * step) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u, turn ^= 1) {
+      const int64_t from = at + u * step;             // (as many turns for every team)
+      if (from >= p.rows) break;
+      const Row row = next[u];
+      fetch(next[u], from + team + kAhead * step);
+      work(row, from + team, turn);
     }
   }
   // the teams' sums, one after the other
