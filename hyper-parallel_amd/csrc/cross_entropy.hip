@@ -48,12 +48,13 @@ struct Product {
 struct CeParams {
   Product part[2];       // (kGrads: two products that share the grid; otherwise the first alone)
   // kStats
-  float2* stats;         // [2 tiles of N][rows_padded] largest logit and sum
+  float2* stats;         // [M][parts] largest logit and sum of each tile of N
+  int parts;
   float* sums;           // the same for the sum of the logits, or null
   float* target_logit;   // [M]
   // kStats and kDlogits
   const int64_t* target; // [M]
-  int64_t rows_padded;
+  int64_t rows_padded;   // stride of dl_t
   // kDlogits and kGrads: the gradient of the loss, one value, or one for each row with stride grad_stride
   const float* grad;
   int64_t grad_stride;
@@ -90,6 +91,167 @@ __device__ __forceinline__ int tile_of_workgroup(int pid, int tiles) {
 // column (of the wave's 128) of sum r of subtile i in the lanes of group g, and the row of b that therefore goes to row p of LDS
 __device__ __forceinline__ int column_of(int i, int g, int r) { return 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r; }
 
+// an operand's rows from `base` to its last one: a transfer from behind it reads zeros
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const uint8_t* base, int64_t rows, int64_t ld, int K) {
+  const int64_t bytes = (rows - 1) * ld + (int64_t)K * 2;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(bytes < 0x7FFFF000 ? bytes : 0x7FFFF000), 0x00020000);
+}
+// 32 values of k out of a fragment's 64
+__device__ __forceinline__ bf16x8 half_of(const v8i& f, int h) {
+  return __builtin_bit_cast(bf16x8, v4i{f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]});
+}
+
+// The end of a tile of TM rows: lane (l16, g) of a wave has the sums of rows m + j and columns n + column_of(i, g, r).
+template <int EPI, int NS, int TM>
+__device__ __forceinline__ void finish_tile(const CeParams& p, const Product& q, v4f (&acc)[NS][4], int m0, int n0, int m, int n, int g, uint8_t* lds) {
+  const bool cut = n + 16 * NS > q.N;          // columns behind the end (their sums are zeros)
+  if constexpr (EPI == kStats) {
+    float2 out[4];
+    float total[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t t = m + j < q.M ? p.target[m + j] : -1;
+      const int own = t >= 0 && t < q.N ? (int)t : -1;
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int c = n + column_of(i, g, r);
+          if (cut && c >= q.N) acc[i][j][r] = -INFINITY;
+          top = fmaxf(top, acc[i][j][r]);
+          if (own == c) p.target_logit[m + j] = acc[i][j][r];
+        }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float from = top == -INFINITY ? 0.f : top;      // (nothing but -inf: the sum is 0)
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f((acc[i][j][r] - from) * kLog2e);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      out[j] = make_float2(top, sum);
+      if (p.sums) {
+        float all = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) all += cut && n + column_of(i, g, r) >= q.N ? 0.f : acc[i][j][r];
+        all += __shfl_xor(all, 16);
+        all += __shfl_xor(all, 32);
+        total[j] = all;
+      }
+    }
+    // the waves that share these rows, joined in LDS
+    __syncthreads();
+    float4* const each = reinterpret_cast<float4*>(lds);          // [waves along n][rows of the tile]
+    if (g == 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) each[(n - n0) / (16 * NS) * TM + m - m0 + j] = make_float4(out[j].x, out[j].y, p.sums ? total[j] : 0.f, 0.f);
+    }
+    __syncthreads();
+    const int row = m0 + (int)threadIdx.x;
+    if ((int)threadIdx.x < TM && row < q.M) {
+      float top = -INFINITY, sum = 0.f, all = 0.f;
+#pragma unroll
+      for (int k = 0; k < kTile / (16 * NS); ++k) top = fmaxf(top, each[k * TM + threadIdx.x].x);
+      const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int k = 0; k < kTile / (16 * NS); ++k) {
+        const float4 v = each[k * TM + threadIdx.x];
+        sum += v.y * __builtin_amdgcn_exp2f((v.x - from) * kLog2e);
+        all += v.z;
+      }
+      const int64_t at = (int64_t)row * p.parts + n0 / kTile;
+      p.stats[at] = make_float2(top, sum);
+      if (p.sums) p.sums[at] = all;
+    }
+  } else if constexpr (EPI == kDlogits) {
+    const float flat = p.smoothing / (float)p.vocab, one = 1.0f - p.smoothing;
+    uint32_t pk[4][NS][2];                      // [j][i][r / 2]: bf16 pairs along the columns
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool row = m + j < q.M;
+      const int64_t t = row ? p.target[m + j] : p.ignore_index;
+      float c = 0.f, lse = 0.f;
+      if (t != p.ignore_index) {
+        lse = p.lse[m + j];
+        c = p.grad_stride ? p.grad[(int64_t)(m + j) * p.grad_stride] : 1.f;
+        if (t < 0 || t >= p.vocab) c = NAN;
+      }
+      const int own = t >= p.first && t < p.first + q.N ? (int)(t - p.first) : -1;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        float d[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int col = n + column_of(i, g, r);
+          float v = __builtin_amdgcn_exp2f((acc[i][j][r] - lse) * kLog2e) - flat;
+          if (own == col) v -= one;
+          d[r] = t == p.ignore_index || (cut && col >= q.N) ? 0.f : c * v;
+        }
+        pk[j][i][0] = pack_bf16x2(d[0], d[1]);
+        pk[j][i][1] = pack_bf16x2(d[2], d[3]);
+      }
+#pragma unroll
+      for (int h = 0; h < NS / 2; ++h) {
+        const u32x4_st v = {pk[j][2 * h][0], pk[j][2 * h][1], pk[j][2 * h + 1][0], pk[j][2 * h + 1][1]};
+        *reinterpret_cast<u32x4_st*>(p.dl + (int64_t)(m + j) * p.ld_dl + n + 32 * h + 8 * g) = v;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t sel = r & 1 ? 0x07060302u : 0x05040100u;       // the upper or the lower halves of two words
+        uint2 v;
+        v.x = __builtin_amdgcn_perm(pk[1][i][r >> 1], pk[0][i][r >> 1], sel);
+        v.y = __builtin_amdgcn_perm(pk[3][i][r >> 1], pk[2][i][r >> 1], sel);
+        *reinterpret_cast<uint2*>(p.dl_t + (int64_t)(n + column_of(i, g, r)) * p.rows_padded + m) = v;
+      }
+  } else {
+    if (p.grad) {
+      // (one factor for all rows is applied here, so that what was rounded is a difference of probabilities: of c (p - 1) the most
+      // frequent value by far, -c, would be rounded the same way in every row)
+      const float c = p.grad[0] / (p.count ? p.count[0] : 1.f);
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] *= c;
+    }
+    if (q.store == kBf16) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (m + j >= q.M) break;
+        uint16_t* const row = reinterpret_cast<uint16_t*>(q.c) + (int64_t)(m + j) * q.ldc;
+#pragma unroll
+        for (int h = 0; h < NS / 2; ++h) {
+          const int col = n + 32 * h + 8 * g;
+          const u32x4_st v = {pack_bf16x2(acc[2 * h][j][0], acc[2 * h][j][1]), pack_bf16x2(acc[2 * h][j][2], acc[2 * h][j][3]),
+                              pack_bf16x2(acc[2 * h + 1][j][0], acc[2 * h + 1][j][1]), pack_bf16x2(acc[2 * h + 1][j][2], acc[2 * h + 1][j][3])};
+          if (col < q.N) *reinterpret_cast<u32x4_st*>(row + col) = v;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (m + j >= q.M) break;
+        float* const row = reinterpret_cast<float*>(q.c) + (int64_t)(m + j) * q.ldc;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          const int col = n + column_of(i, g, 0);
+          if (col >= q.N) continue;
+          v4f v = acc[i][j];
+          if (q.store == kF32Add) v += *reinterpret_cast<const v4f*>(row + col);
+          *reinterpret_cast<v4f*>(row + col) = v;
+        }
+      }
+    }
+  }
+}
+
 template <int EPI>
 __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[5 * kSlabBytes];
@@ -115,10 +277,6 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
   const int slabs = (q.K + kSlab - 1) / kSlab;
 
   // ---- transfers: one is 8 rows x 128 bytes of LDS per wave, four per wave and slab
-  auto resource = [](const uint8_t* base, int64_t rows, int64_t ld, int K) {
-    const int64_t bytes = (rows - 1) * ld + (int64_t)K * 2;
-    return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(bytes < 0x7FFFF000 ? bytes : 0x7FFFF000), 0x00020000);
-  };
   const __amdgpu_buffer_rsrc_t rsrc_a = resource(q.a + (int64_t)m0 * q.lda, q.M - m0, q.lda, q.K);
   const __amdgpu_buffer_rsrc_t rsrc_b = resource(q.b + (int64_t)n0 * q.ldb, q.N - n0, q.ldb, q.K);
   uint32_t a_off[4], b_off[4], past[2];
@@ -174,9 +332,6 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
   for (int j = 0; j < 4; ++j) xf[j] = frag_read(a_lds + a_frag + j * 16 * 128, frag_lo, frag_hi);
   wf_n1 = frag_read(b_lds + b_frag + 16 * 128, frag_lo, frag_hi);
 
-  auto halves = [](const v8i& f, int h) {
-    return __builtin_bit_cast(bf16x8, v4i{f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]});
-  };
   // One slab.  Its barrier sits before its last two subtiles: what follows it, the fragments of the next slab, is covered by the matrix
   // instructions that are left.  Transfers, one per subtile: the rest of the next slab of a, the slab after next of b, and behind
   // the barrier the first half of the slab after next of a into the buffer that every wave has just left.
@@ -202,10 +357,10 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
       else load_a(abuf, s + 2, i - 6);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(halves(wf[i % 3], 0), halves(xf[j], 0), acc[i][j], 0, 0, 0);
+      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(half_of(wf[i % 3], 0), half_of(xf[j], 0), acc[i][j], 0, 0, 0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(halves(wf[i % 3], 1), halves(xf[j], 1), acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(half_of(wf[i % 3], 1), half_of(xf[j], 1), acc[i][j], 0, 0, 0);
         if (i == 7) xf[j] = frag_read(anxt + a_frag + j * 16 * 128, frag_lo, frag_hi);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -216,182 +371,104 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
     bbuf = bnext;
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);          // vmcnt(0): the last transfers write to this workgroup's LDS
-
-  // ---- the tile's sums: lane (l16, g) has rows m + j and columns n + column_of(i, g, r)
-  const int m = m0 + wm * 64 + l16 * 4, n = n0 + wn * 128;
-  const bool cut = n + 128 > q.N;              // columns behind the end (their sums are zeros)
-  if constexpr (EPI == kStats) {
-    float2 out[4];
-    float total[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t t = m + j < q.M ? p.target[m + j] : -1;
-      const int own = t >= 0 && t < q.N ? (int)t : -1;
-      float top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int c = n + column_of(i, g, r);
-          if (cut && c >= q.N) acc[i][j][r] = -INFINITY;
-          top = fmaxf(top, acc[i][j][r]);
-          if (own == c) p.target_logit[m + j] = acc[i][j][r];
-        }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float from = top == -INFINITY ? 0.f : top;      // (nothing but -inf: the sum is 0)
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f((acc[i][j][r] - from) * kLog2e);
-      sum += __shfl_xor(sum, 16);
-      sum += __shfl_xor(sum, 32);
-      out[j] = make_float2(top, sum);
-      if (p.sums) {
-        float all = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) all += cut && n + column_of(i, g, r) >= q.N ? 0.f : acc[i][j][r];
-        all += __shfl_xor(all, 16);
-        all += __shfl_xor(all, 32);
-        total[j] = all;
-      }
-    }
-    if (g == 0) {
-      const int64_t at = (int64_t)(tn * 2 + wn) * p.rows_padded + m;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        p.stats[at + j] = out[j];
-        if (p.sums) p.sums[at + j] = total[j];
-      }
-    }
-  } else if constexpr (EPI == kDlogits) {
-    const float flat = p.smoothing / (float)p.vocab, one = 1.0f - p.smoothing;
-    uint32_t pk[4][8][2];                      // [j][i][r / 2]: bf16 pairs along the columns
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool row = m + j < q.M;
-      const int64_t t = row ? p.target[m + j] : p.ignore_index;
-      float c = 0.f, lse = 0.f;
-      if (t != p.ignore_index) {
-        lse = p.lse[m + j];
-        c = p.grad_stride ? p.grad[(int64_t)(m + j) * p.grad_stride] : 1.f;
-        if (t < 0 || t >= p.vocab) c = NAN;
-      }
-      const int own = t >= p.first && t < p.first + q.N ? (int)(t - p.first) : -1;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float d[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int col = n + column_of(i, g, r);
-          float v = __builtin_amdgcn_exp2f((acc[i][j][r] - lse) * kLog2e) - flat;
-          if (own == col) v -= one;
-          d[r] = t == p.ignore_index || (cut && col >= q.N) ? 0.f : c * v;
-        }
-        pk[j][i][0] = pack_bf16x2(d[0], d[1]);
-        pk[j][i][1] = pack_bf16x2(d[2], d[3]);
-      }
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const u32x4_st v = {pk[j][2 * h][0], pk[j][2 * h][1], pk[j][2 * h + 1][0], pk[j][2 * h + 1][1]};
-        *reinterpret_cast<u32x4_st*>(p.dl + (int64_t)(m + j) * p.ld_dl + n + 32 * h + 8 * g) = v;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t sel = r & 1 ? 0x07060302u : 0x05040100u;       // the upper or the lower halves of two words
-        uint2 v;
-        v.x = __builtin_amdgcn_perm(pk[1][i][r >> 1], pk[0][i][r >> 1], sel);
-        v.y = __builtin_amdgcn_perm(pk[3][i][r >> 1], pk[2][i][r >> 1], sel);
-        *reinterpret_cast<uint2*>(p.dl_t + (int64_t)(n + column_of(i, g, r)) * p.rows_padded + m) = v;
-      }
-  } else {
-    if (p.grad) {
-      // (one factor for all rows is applied here, so that what was rounded is a difference of probabilities: of c (p - 1) the most
-      // frequent value by far, -c, would be rounded the same way in every row)
-      const float c = p.grad[0] / (p.count ? p.count[0] : 1.f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] *= c;
-    }
-    if (q.store == kBf16) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (m + j >= q.M) break;
-        uint16_t* const row = reinterpret_cast<uint16_t*>(q.c) + (int64_t)(m + j) * q.ldc;
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int col = n + 32 * h + 8 * g;
-          const u32x4_st v = {pack_bf16x2(acc[2 * h][j][0], acc[2 * h][j][1]), pack_bf16x2(acc[2 * h][j][2], acc[2 * h][j][3]),
-                              pack_bf16x2(acc[2 * h + 1][j][0], acc[2 * h + 1][j][1]), pack_bf16x2(acc[2 * h + 1][j][2], acc[2 * h + 1][j][3])};
-          if (col < q.N) *reinterpret_cast<u32x4_st*>(row + col) = v;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (m + j >= q.M) break;
-        float* const row = reinterpret_cast<float*>(q.c) + (int64_t)(m + j) * q.ldc;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int col = n + column_of(i, g, 0);
-          if (col >= q.N) continue;
-          v4f v = acc[i][j];
-          if (q.store == kF32Add) v += *reinterpret_cast<const v4f*>(row + col);
-          *reinterpret_cast<v4f*>(row + col) = v;
-        }
-      }
-    }
-  }
+  finish_tile<EPI, 8, kTile>(p, q, acc, m0, n0, m0 + wm * 64 + l16 * 4, n0 + wn * 128, g, lds);
 }
 
-// ---- joins the forward's partial results: 64 rows per workgroup, 16 waves that share the parts
-__global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ stats, const float* __restrict__ sums,
-                                                       const float* __restrict__ target_logit, const int64_t* __restrict__ target, int parts,
-                                                       int64_t rows, int64_t rows_padded, int64_t ignore_index, int64_t vocab, float smoothing,
-                                                       float* __restrict__ lse, float* __restrict__ loss) {
-  __shared__ float tops[16][64], each[16][64], totals[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = (int64_t)blockIdx.x * 64 + lane;
+// Few rows: tiles of 64 x 256, a wave has all 64 rows and 32 columns.  What such a tile waits for is b, so LDS is four slabs of both operands
+// and three of them are on their way while the fourth is multiplied; one barrier per slab.
+constexpr int kNarrow = 64, kNarrowStages = 4, kNarrowStage = (kNarrow + kTile) * 128;
+template <int EPI>
+__global__ __launch_bounds__(512) void ce_gemm_narrow_kernel(CeParams p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kNarrowStages * kNarrowStage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Product q = p.part[0];
+  int tm, tn;
+  tile_at(tile_of_workgroup(blockIdx.x, q.tiles), (q.M + kNarrow - 1) / kNarrow, (q.N + kTile - 1) / kTile, tm, tn);
+  const int m0 = tm * kNarrow, n0 = tn * kTile, slabs = (q.K + kSlab - 1) / kSlab, whole = q.K / kSlab;
+  const __amdgpu_buffer_rsrc_t rsrc_a = resource(q.a + (int64_t)m0 * q.lda, q.M - m0, q.lda, q.K);
+  const __amdgpu_buffer_rsrc_t rsrc_b = resource(q.b + (int64_t)n0 * q.ldb, q.N - n0, q.ldb, q.K);
+  // a wave's transfers of a slab: one of a (rows 8 wave ...), four of b
+  uint32_t off[5], past[2];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    const int r = (i == 0 ? wave : wave * 4 + i - 1) * 8 + (lane >> 3);
+    const int chunk = (lane & 7) ^ row_swizzle(r);
+    const int from = i == 0 ? (r & 15) * 4 + (r >> 4) : (r & ~31) + column_of((r >> 4) & 1, (r >> 2) & 3, r & 3);
+    off[i] = (uint32_t)from * (uint32_t)(i == 0 ? q.lda : q.ldb) + chunk * 16;
+    // (behind the end of k: from beyond the resource, as zeros; the swizzle has two patterns, by whether r / 8 is odd)
+    if (i == 1 || i == 2) past[i - 1] = chunk * 8 >= q.K % kSlab ? 0x80000000u : 0u;
+  }
+  const uint32_t past_a = wave & 1 ? past[1] : past[0];
+  auto load = [&](int slab) {
+    uint8_t* const to = lds + slab % kNarrowStages * kNarrowStage;
+    const int s = slab < slabs ? slab : slabs - 1;        // (behind the last slab the last one again: those are never used)
+    const bool cut = s >= whole;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_a, (lds_ptr_t)(to + wave * 1024), 16, off[0] + (cut ? past_a : 0u), s * 128, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_b, (lds_ptr_t)(to + kNarrow * 128 + (wave * 4 + i) * 1024), 16, off[1 + i] + (cut ? past[i & 1] : 0u),
+                                               s * 128, 0, 0);
+  };
+  const int l16 = lane & 15, g = lane >> 4;
+  const int frag_lo = l16 * 128 + ((2 * g) ^ row_swizzle(l16)) * 16, frag_hi = frag_lo ^ 16;
+  const v4f zero = {0.f, 0.f, 0.f, 0.f};
+  v4f acc[2][4] = {{zero, zero, zero, zero}, {zero, zero, zero, zero}};
+  load(0);
+  load(1);
+  load(2);
+  for (int s = 0; s < slabs; ++s) {
+    asm volatile("s_waitcnt vmcnt(10)\n\ts_barrier" ::: "memory");       // slab s is there, and the one before has been read by all
+    load(s + 3);
+    const uint8_t* const a = lds + s % kNarrowStages * kNarrowStage;
+    const uint8_t* const b = a + kNarrow * 128 + wave * 32 * 128;
+    v8i wf[2], xf[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) wf[i] = frag_read(b + i * 16 * 128, frag_lo, frag_hi);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) xf[j] = frag_read(a + j * 16 * 128, frag_lo, frag_hi);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(half_of(wf[i], h), half_of(xf[j], h), acc[i][j], 0, 0, 0);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);          // vmcnt(0): the last transfers write to this workgroup's LDS
+  finish_tile<EPI, 2, kNarrow>(p, q, acc, m0, n0, m0 + l16 * 4, n0 + wave * 32, g, lds);
+}
+
+// ---- joins the forward's partial results, a wave for each row
+__global__ __launch_bounds__(256) void ce_join_kernel(const float2* __restrict__ stats, const float* __restrict__ sums,
+                                                      const float* __restrict__ target_logit, const int64_t* __restrict__ target, int parts,
+                                                      int64_t rows, int64_t ignore_index, int64_t vocab, float smoothing, float* __restrict__ lse,
+                                                      float* __restrict__ loss) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const float2* const s = stats + row * parts;
   float top = -INFINITY, sum = 0.f, total = 0.f;
-  if (row < rows) {
-    int k = wave;
-    auto add = [&](float2 s) {
-      const float t = fmaxf(top, s.x), from = t == -INFINITY ? 0.f : t;
-      sum = sum * __builtin_amdgcn_exp2f((top - from) * kLog2e) + s.y * __builtin_amdgcn_exp2f((s.x - from) * kLog2e);
-      top = t;
-    };
-    for (; k + 112 < parts; k += 128) {
-      float2 s[8];
+  auto add = [&](float2 v) {
+    const float t = fmaxf(top, v.x), from = t == -INFINITY ? 0.f : t;
+    sum = sum * __builtin_amdgcn_exp2f((top - from) * kLog2e) + v.y * __builtin_amdgcn_exp2f((v.x - from) * kLog2e);
+    top = t;
+  };
+  int k = lane;
+  for (; k + 448 < parts; k += 512) {
+    float2 v[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) s[u] = stats[(int64_t)(k + 16 * u) * rows_padded + row];
+    for (int u = 0; u < 8; ++u) v[u] = s[k + 64 * u];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) add(s[u]);
-    }
-    for (; k < parts; k += 16) add(stats[(int64_t)k * rows_padded + row]);
-    if (sums)
-      for (k = wave; k < parts; k += 16) total += sums[(int64_t)k * rows_padded + row];
+    for (int u = 0; u < 8; ++u) add(v[u]);
   }
-  tops[wave][lane] = top;
-  each[wave][lane] = sum;
-  totals[wave][lane] = total;
-  __syncthreads();
-  if (wave != 0 || row >= rows) return;
-  for (int k = 1; k < 16; ++k) top = fmaxf(top, tops[k][lane]);
-  const float from = top == -INFINITY ? 0.f : top;
-  sum = 0.f;
-  total = 0.f;
-  for (int k = 0; k < 16; ++k) {
-    sum += each[k][lane] * __builtin_amdgcn_exp2f((tops[k][lane] - from) * kLog2e);
-    total += totals[k][lane];
+  for (; k < parts; k += 64) add(s[k]);
+  if (sums)
+    for (k = lane; k < parts; k += 64) total += sums[row * parts + k];
+  for (int d = 1; d < 64; d *= 2) {
+    add(make_float2(__shfl_xor(top, d), __shfl_xor(sum, d)));
+    total += __shfl_xor(total, d);
   }
-  const float l = from + logf(sum);
+  if (lane != 0) return;
+  const float l = (top == -INFINITY ? 0.f : top) + logf(sum);
   if (lse) lse[row] = l;
   const int64_t t = target[row];
   float out = 0.f;
@@ -475,6 +552,10 @@ __global__ __launch_bounds__(256) void ce_round_kernel(const float* __restrict__
   reinterpret_cast<u32x4_st*>(out)[i] = u32x4_st{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])};
 }
 
+// Elements between the rows of the workspaces: whole tiles, and an odd number of 128-byte lines, so that the rows of a tile do not all lie
+// in the same few memory channels (the gradients' launch of 4096 tokens, 7168, 16384 columns: 1480 us with strides of 2^13 and 2^15 bytes).
+int64_t up(int64_t n, int64_t to);
+int64_t stride_of(int64_t n) { return up(n, kTile) + kSlab; }
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int tiles_of(int64_t m, int64_t n) { return (int)((m + kTile - 1) / kTile * ((n + kTile - 1) / kTile)); }
 
@@ -504,6 +585,22 @@ Product product(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t 
   return q;
 }
 
+// Tiles of 64 rows up to 64 rows, and wherever the compute units' rounds of them are shorter: a slab takes at least 0.85 us in a tile of 256
+// rows and 0.42 in one of 64.  us of a forward, 256 / 64 rows: 5 tokens, 7168, 131072 375 / 312, 128, 2048, 32000 60 / 44, 256, 2048, 32000
+// 62 / 66, 512, 896, 5165 30 / 27, 512, 4096, 32000 120 / 212.
+template <int EPI>
+void launch_logits(CeParams& p, hipStream_t s) {
+  Product& q = p.part[0];
+  const int64_t slabs = (q.K + kSlab - 1) / kSlab, narrow = (int64_t)((q.M + kNarrow - 1) / kNarrow) * ((q.N + kTile - 1) / kTile);
+  const int64_t cost = (q.tiles + 255) / 256 * (85 * slabs + 500), narrow_cost = (narrow + 255) / 256 * (42 * slabs + 400);
+  if (q.M <= kNarrow || narrow_cost < cost) {
+    q.tiles = (int)narrow;
+    ce_gemm_narrow_kernel<EPI><<<q.tiles, 512, 0, s>>>(p);
+  } else {
+    ce_gemm_kernel<EPI><<<q.tiles, 512, 0, s>>>(p);
+  }
+}
+
 }  // namespace
 }  // namespace hpfp8
 
@@ -511,7 +608,7 @@ using namespace hpfp8;
 
 extern "C" {
 
-int64_t hpfp8_cross_entropy_parts(int64_t vocab) { return vocab > 0 ? 2 * ((vocab + kTile - 1) / kTile) : 0; }
+int64_t hpfp8_cross_entropy_parts(int64_t vocab) { return vocab > 0 ? (vocab + kTile - 1) / kTile : 0; }
 // dx's product contracts over the whole piece and has few tiles, so with few tokens a few of its tiles would still be at work long after
 // dw's are done.  Its contraction is split until one part takes at most half of what all of the launch takes the 256 compute units
 // together (in slabs; a tile's start and end cost about six).  us of the launch unsplit / split: 512 tokens, 4096, 32000 736 / 256,
@@ -524,7 +621,7 @@ int64_t hpfp8_cross_entropy_splits(int64_t tokens, int64_t hidden, int64_t width
   const int64_t splits = (slabs_x + half - 1) / half;
   return splits < 16 ? splits : 16;
 }
-int64_t hpfp8_cross_entropy_padded_rows(int64_t tokens) { return tokens > 0 ? up(tokens, kTile) : 0; }
+int64_t hpfp8_cross_entropy_stride(int64_t n) { return n > 0 ? stride_of(n) : 0; }
 
 int hpfp8_linear_cross_entropy_forward(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t tokens,
                                        int64_t hidden, int64_t vocab, int64_t ignore_index, float smoothing, int reduction, float* stats,
@@ -545,12 +642,12 @@ int hpfp8_linear_cross_entropy_forward(const void* x, int64_t ld_x, const void* 
     p.sums = smoothing != 0.f ? sums : nullptr;
     p.target_logit = target_logit;
     p.target = target;
-    p.rows_padded = up(tokens, kTile);
-    ce_gemm_kernel<kStats><<<p.part[0].tiles, 512, 0, s>>>(p);
+    p.parts = (int)hpfp8_cross_entropy_parts(vocab);
+    launch_logits<kStats>(p, s);
     int rc = check_launch("linear_cross_entropy_forward");
     if (rc != HPFP8_OK) return rc;
-    ce_join_kernel<<<(unsigned)((tokens + 63) / 64), 1024, 0, s>>>(p.stats, p.sums, target_logit, target, (int)hpfp8_cross_entropy_parts(vocab), tokens,
-                                                                 p.rows_padded, ignore_index, vocab, smoothing, lse, loss);
+    ce_join_kernel<<<(unsigned)((tokens + 3) / 4), 256, 0, s>>>(p.stats, p.sums, target_logit, target, p.parts, tokens, ignore_index, vocab, smoothing,
+                                                              lse, loss);
     rc = check_launch("linear_cross_entropy_forward (join)");
     if (rc != HPFP8_OK) return rc;
   }
@@ -584,7 +681,7 @@ int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_
   HPFP8_REQUIRE(aligned16(x) && aligned16(w) && aligned16(dl) && aligned16(dl_t) && aligned16(w_t) && aligned16(x_t) && aligned16(dx) && aligned16(dw),
                 HPFP8_ERR_ALIGN, "a buffer is not 16-byte aligned");
   const hipStream_t s = (hipStream_t)stream;
-  const int64_t rows_padded = up(tokens, kTile), cols_padded = up(width, kTile);
+  const int64_t rows_padded = stride_of(tokens), cols_padded = stride_of(width);
   const uint16_t* const piece = (const uint16_t*)w + first * ld_w;
   CeParams p = {};
   p.part[0] = product(x, ld_x, piece, ld_w, tokens, width, hidden, nullptr, 0, 0);
@@ -601,7 +698,7 @@ int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_
   p.dl = (uint16_t*)dl;
   p.ld_dl = cols_padded;
   p.dl_t = (uint16_t*)dl_t;
-  ce_gemm_kernel<kDlogits><<<p.part[0].tiles, 512, 0, s>>>(p);
+  launch_logits<kDlogits>(p, s);
   int rc = check_launch("linear_cross_entropy_piece");
   if (rc != HPFP8_OK) return rc;
   CeParams g = {};

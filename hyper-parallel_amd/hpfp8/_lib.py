@@ -99,7 +99,7 @@ SIZE_FUNCTIONS = {
     "hpfp8_layer_norm_partials": [_i64, _i64],
     "hpfp8_cross_entropy_parts": [_i64],
     "hpfp8_cross_entropy_splits": [_i64, _i64, _i64, _int],
-    "hpfp8_cross_entropy_padded_rows": [_i64],
+    "hpfp8_cross_entropy_stride": [_i64],
 }
 
 OUT_BF16, OUT_F32 = 0, 1

@@ -10,7 +10,7 @@ from .linear import _hand_off
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 _TILE = 256
-# The forward takes this many tokens at a time: its per-tile results (16 bytes for 256 columns of a row) stay below 128 MiB for 131072 columns
+# The forward takes this many tokens at a time: its per-tile results (8 bytes for 256 columns of a row) stay at 64 MiB for 131072 columns
 _FORWARD_ROWS = 16384
 # What the backward's workspaces for a piece of the vocabulary may take: the gradient of its logits, twice, and its transposed weight
 _PIECE_BYTES = 512 << 20
@@ -28,9 +28,9 @@ def _forward(x, weight, target, ignore_index, reduction, smoothing, want_lse):
     tokens, vocab = x.shape[0], weight.shape[0]
     f32 = dict(dtype=torch.float32, device=x.device)
     most = min(tokens, _FORWARD_ROWS)
-    parts, padded = lib.hpfp8_cross_entropy_parts(vocab), lib.hpfp8_cross_entropy_padded_rows(most)
-    stats = torch.empty((parts, padded, 2), **f32)
-    sums = torch.empty((parts, padded), **f32) if smoothing else None
+    parts = lib.hpfp8_cross_entropy_parts(vocab)
+    stats = torch.empty((most, parts, 2), **f32)
+    sums = torch.empty((most, parts), **f32) if smoothing else None
     own = torch.empty((most,), **f32)
     loss = torch.empty((tokens,), **f32)
     lse = torch.empty((tokens,), **f32) if want_lse else None
@@ -88,21 +88,22 @@ class _LinearCrossEntropy(torch.autograd.Function):
         grad = grad_out.reshape(-1).contiguous()
         dw = dx = x_t = w_t = None
         splits = 1
-        padded = _lib.load().hpfp8_cross_entropy_padded_rows(tokens)
         pieces = _pieces(tokens, hidden, vocab, _PIECE_BYTES)
-        width = (pieces[0][1] + _TILE - 1) // _TILE * _TILE
-        dl, dl_t = torch.empty((padded, width), **bf16), torch.empty((width, padded), **bf16)
+        width = pieces[0][1]
+        row_t, row = (_lib.load().hpfp8_cross_entropy_stride(n) for n in (tokens, width))
+        dl = torch.empty(((tokens + _TILE - 1) // _TILE * _TILE, row), **bf16)
+        dl_t = torch.empty(((width + _TILE - 1) // _TILE * _TILE, row_t), **bf16)
         if need_dw:
             dw = torch.empty((vocab, hidden), **bf16) if param is None else main_grad
             if dw is None:
                 dw = torch.empty((vocab, hidden), **f32)
-            x_t = torch.empty((hidden, padded), **bf16)
+            x_t = torch.empty((hidden, row_t), **bf16)
             _lib.call("hpfp8_linear_cross_entropy_rows_t", ops._ptr(x2), tokens, hidden, x2.stride(0), ops._ptr(target), ctx.ignore_index,
-                      ops._ptr(x_t), padded, ops._stream())
+                      ops._ptr(x_t), row_t, ops._stream())
         if need_dx:
             splits = _lib.load().hpfp8_cross_entropy_splits(tokens, hidden, pieces[0][1], int(need_dw))
             dx = torch.empty((splits, tokens, hidden), **f32)
-            w_t = torch.empty((hidden, width), **bf16)
+            w_t = torch.empty((hidden, row), **bf16)
         for first, n in pieces:
             _lib.call("hpfp8_linear_cross_entropy_piece", ops._ptr(x2), x2.stride(0), ops._ptr(x_t), ops._ptr(w), w.stride(0), ops._ptr(target),
                       tokens, hidden, vocab, first, n, ctx.ignore_index, ctx.smoothing, ops._ptr(lse), ops._ptr(grad),

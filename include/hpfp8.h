@@ -542,10 +542,8 @@ int64_t hpfp8_layer_norm_partials(int64_t rows, int64_t cols);
  * bf16, row strides ld_x and ld_w in elements, hidden and the strides multiples of 8; target[tokens] is int64.
  *   loss[t] = lse(l_t) - (1 - smoothing) l_t[target] - smoothing mean(l_t);  0 where target is ignore_index, NaN where it is neither that
  *   nor in [0, vocab).  reduction 0: nothing more; 1: out[0] = their mean over the count[0] rows that are not ignored; 2: their sum.
- * Workspaces, fp32: stats[hpfp8_cross_entropy_parts(vocab), hpfp8_cross_entropy_padded_rows(tokens), 2], sums (with smoothing only) half of
- * that, target_logit[tokens].  lse[tokens] (may be NULL) is what the backward needs; out and count may be NULL with reduction 0. */
+ * Workspaces, fp32: stats[tokens, hpfp8_cross_entropy_parts(vocab), 2], sums (with smoothing only) half of that, target_logit[tokens].  lse[tokens] (may be NULL) is what the backward needs; out and count may be NULL with reduction 0. */
 int64_t hpfp8_cross_entropy_parts(int64_t vocab);
-int64_t hpfp8_cross_entropy_padded_rows(int64_t tokens);
 int hpfp8_linear_cross_entropy_forward(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t tokens,
                                        int64_t hidden, int64_t vocab, int64_t ignore_index, float smoothing, int reduction, float* stats,
                                        float* sums, float* target_logit, float* lse, float* loss, float* out, float* count,
@@ -557,9 +555,10 @@ int hpfp8_linear_cross_entropy_reduce(const float* loss, const int64_t* target, 
  * dx (fp32 [splits, tokens, hidden], the parts of a sum; dx_add: added onto) and rows [first, first + width) of dw ([vocab, hidden], dw_type HPFP8_OUT_*; dw_add: added onto,
  * fp32 only).  Either may be NULL.  grad is the loss's gradient, one value with grad_stride 0 or one for each row; count as the
  * forward wrote it for reduction 1, otherwise NULL.  x_t is what hpfp8_linear_cross_entropy_rows_t makes of x, with row stride
- * padded_rows(tokens) (needed for dw).  Workspaces, bf16: dl and dl_t [padded_rows(tokens) * width rounded up to 256], w_t [hidden, width rounded
- * up to 256] (needed for dx).  splits: what hpfp8_cross_entropy_splits says for the widest piece, or another number from 1 to 16 up to its
+ * S(tokens), S(n) = hpfp8_cross_entropy_stride(n) (needed for dw).  Workspaces, bf16, with R(n) = n rounded up to 256: dl [R(tokens), S(width)],
+ * dl_t [R(width), S(tokens)], w_t [hidden, S(width)] (needed for dx).  splits: what hpfp8_cross_entropy_splits says for the widest piece, or another number from 1 to 16 up to its
  * slabs of 64 columns. */
+int64_t hpfp8_cross_entropy_stride(int64_t n);
 int64_t hpfp8_cross_entropy_splits(int64_t tokens, int64_t hidden, int64_t width, int with_dw);
 int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_t, const void* w, int64_t ld_w, const int64_t* target,
                                      int64_t tokens, int64_t hidden, int64_t vocab, int64_t first, int64_t width, int64_t ignore_index,
