@@ -21,25 +21,24 @@ enum Kind { kSilu = 0, kGelu = 1, kGeluTanh = 2, kSwiglu = 3 };
 // 1 / (1 + exp(-x)): the hardware's base-2 exponential and reciprocal, each within one unit in the last place.
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f)); }
 
-// The normal distribution's density and cumulative function.  Phi(-|x|) = erfcx(|x| / sqrt 2) exp(-x^2 / 2) / 2, where the scaled
-// complementary error function erfcx(z) is t P(t), t = 1 / (1 + 0.4 z), with a polynomial of degree 8 fitted to it on t in [0, 1]
-// (least squares, reweighted to equal ripple: 1.3e-7 relative, 4.5e-7 in fp32).  The tail on the left keeps its relative precision, which
-// 1 + erf would lose, and the density costs one multiplication more.
-__device__ __forceinline__ void normal(float x, float& density, float& phi) {
-  const float e = __builtin_amdgcn_exp2f(x * x * -0.72134752f);             // exp(-x^2 / 2)
-  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(x), 0.28284271f, 1.0f));
-  float r = 0.05026565119624138f;
-  r = __builtin_fmaf(r, t, -0.182915598154068f);
-  r = __builtin_fmaf(r, t, 0.169108584523201f);
-  r = __builtin_fmaf(r, t, -0.0056274873204529285f);
-  r = __builtin_fmaf(r, t, 0.14144112169742584f);
-  r = __builtin_fmaf(r, t, 0.16853934526443481f);
-  r = __builtin_fmaf(r, t, 0.20784308016300201f);
-  r = __builtin_fmaf(r, t, 0.22566957771778107f);
-  r = __builtin_fmaf(r, t, 0.22567586600780487f);
-  const float tail = 0.5f * r * t * e;
-  phi = x < 0.f ? tail : 1.0f - tail;                                        // (a NaN comes through e)
-  density = e * 0.39894228f;
+// The normal distribution's Phi(-a) for 0 <= a <= kFar is erfcx(a / sqrt 2) exp(-a^2 / 2) / 2, where the scaled complementary error function
+// erfcx(z) is t P(t), t = 1 / (1 + 0.4 z), with a polynomial of degree 8 fitted to it on t in [0, 1] (least squares, reweighted to equal
+// ripple: 1.3e-7 relative, 4.5e-7 in fp32; the factor 1 / 2 is in its coefficients).  The tail keeps its relative precision, which
+// 1 + erf would lose, and the exponential is the density's too.
+constexpr float kFar = 30.0f;             // (exp(-a^2 / 2) has been 0 for long)
+__device__ __forceinline__ float normal_tail(float a, float& e) {
+  e = __builtin_amdgcn_exp2f(a * a * -0.72134752f);             // exp(-a^2 / 2)
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.28284271f, 1.0f));
+  float r = 0.025132825598120689f;
+  r = __builtin_fmaf(r, t, -0.091457799077034f);
+  r = __builtin_fmaf(r, t, 0.0845542922616005f);
+  r = __builtin_fmaf(r, t, -0.00281374366022646425f);
+  r = __builtin_fmaf(r, t, 0.07072056084871292f);
+  r = __builtin_fmaf(r, t, 0.084269682317972183f);
+  r = __builtin_fmaf(r, t, 0.10392154008150101f);
+  r = __builtin_fmaf(r, t, 0.11283478885889053f);
+  r = __builtin_fmaf(r, t, 0.11283793300390244f);
+  return r * t * e;
 }
 
 // x times a factor in [0, 1] that goes to zero faster than x grows: 0 for x = -inf, where the product would be NaN
@@ -49,9 +48,10 @@ template <int KIND>
 __device__ __forceinline__ float value(float x) {
   if constexpr (KIND == kSilu) return damped(x, sigmoid(x));
   if constexpr (KIND == kGelu) {
-    float density, phi;
-    normal(x, density, phi);
-    return damped(x, phi);
+    // x Phi(x) = max(x, 0) - |x| Phi(-|x|); a NaN comes through the maximum
+    const float a = fminf(fabsf(x), kFar);
+    float e;
+    return __builtin_elementwise_maximum(x, 0.f) - a * normal_tail(a, e);
   }
   // 0.5 x (1 + tanh(u)) = x sigmoid(2 u), u = sqrt(2 / pi) (x + 0.044715 x^3)
   return damped(x, sigmoid(x * __builtin_fmaf(x * x, 0.07135481f, 1.59576912f)));
@@ -59,9 +59,10 @@ __device__ __forceinline__ float value(float x) {
 template <int KIND>
 __device__ __forceinline__ float derivative(float x) {
   if constexpr (KIND == kGelu) {
-    float density, phi;
-    normal(x, density, phi);
-    return phi + damped(x, density);
+    const float near = __builtin_elementwise_maximum(__builtin_elementwise_minimum(x, kFar), -kFar);
+    float e;
+    const float tail = normal_tail(fabsf(near), e), phi = x < 0.f ? tail : 1.0f - tail;
+    return __builtin_fmaf(near * 0.39894228f, e, phi);
   }
   const float x2 = x * x;
   const float s = KIND == kSilu ? sigmoid(x) : sigmoid(x * __builtin_fmaf(x2, 0.07135481f, 1.59576912f));
@@ -255,22 +256,21 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(const typename
   }
 }
 
-// The workgroup's shape: as many groups along a row as leave the fewest of them idle, the wider of two that leave as many.
+// The workgroup's shape: as many groups along a row as leave at most a quarter of them idle (rows of 8200 values with one group of each of
+// 16 rows, which leaves none idle: 141 us where eight take 69).
 bool shape(int64_t rows, int64_t cols, Grid& g, dim3& grid) {
   const int64_t groups = (cols + kBlock - 1) / kBlock;
   g.rows = rows;
   g.cols = cols;
   g.groups = (int)groups;
-  int64_t least = INT64_MAX;
-  for (int across = 16; across >= 1; across /= 2) {
-    const int64_t taken = (groups + across - 1) / across * across;
-    if (taken < least) {
-      least = taken;
-      g.across = across;
-    }
+  int64_t taken = groups;
+  for (g.across = 16; g.across > 1; g.across /= 2) {
+    taken = (groups + g.across - 1) / g.across * g.across;
+    if (4 * (taken - groups) <= taken) break;
   }
+  if (g.across == 1) taken = groups;
   const int64_t down = (int64_t)(16 / g.across) * kUnroll, blocks = (rows + down - 1) / down;
-  grid = dim3((unsigned)(least / g.across), (unsigned)(blocks < 32768 ? blocks : 32768));
+  grid = dim3((unsigned)(taken / g.across), (unsigned)(blocks < 32768 ? blocks : 32768));
   return groups <= (int64_t)1 << 24;
 }
 

@@ -92,7 +92,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(Nor
   auto fetch = [&](Pack8<E> (&to)[NV], int64_t r) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      to[j] = load_pack8<E, true, TAIL>((const raw*)p.x + (r < p.rows ? r : 0) * p.ld + (j * TPR + t) * 8, r < p.rows ? left[j] : 0);
+      to[j] = load_pack8<E, kStream<E>, TAIL>((const raw*)p.x + (r < p.rows ? r : 0) * p.ld + (j * TPR + t) * 8, r < p.rows ? left[j] : 0);
   };
   auto work = [&](const Pack8<E> (&packed)[NV], int64_t row, int turn) {
     float v[NV][8];
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(Nor
         v[j][i] = i < left[j] ? (v[j][i] - mean) * rstd : 0.f;
         out[i] = __builtin_fmaf(v[j][i], w[j][i], b[j][i]);
       }
-      if (left[j] > 0) store8<E, true, TAIL>((raw*)p.y + row * C + col, left[j], out);
+      if (left[j] > 0) store8<E, kStream<E>, TAIL>((raw*)p.y + row * C + col, left[j], out);
       if constexpr (KEEP) {
         float si;
         const uint2 c = encode_group(v[j], si);
@@ -203,12 +203,12 @@ __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(NormPar
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int col = (j * TPR + t) * 8, n = in ? left[j] : 0;
-      to.dy[j] = load_pack8<E, true, TAIL>((const raw*)p.dy + at * p.ld_dy + col, n);
+      to.dy[j] = load_pack8<E, kStream<E>, TAIL>((const raw*)p.dy + at * p.ld_dy + col, n);
       if constexpr (KEEP) {
         to.q[j] = load_codes8<TAIL>(p.q + at * C + col, n);
         to.s[j] = n > 0 ? (p.scale_inv + at * groups)[col / kBlock] : 0.f;
       } else {
-        to.x[j] = load_pack8<E, true, TAIL>((const raw*)p.x + at * p.ld + col, n);
+        to.x[j] = load_pack8<E, kStream<E>, TAIL>((const raw*)p.x + at * p.ld + col, n);
       }
     }
     to.mean = !KEEP && in ? p.mean[r] : 0.f;
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(NormPar
       float out[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) out[i] = (go[j][i] - m1 - hat[j][i] * m2) * rstd;
-      if (left[j] > 0) store8<E, true, TAIL>((raw*)p.dx + row * C + (j * TPR + t) * 8, left[j], out);
+      if (left[j] > 0) store8<E, kStream<E>, TAIL>((raw*)p.dx + row * C + (j * TPR + t) * 8, left[j], out);
     }
   };
   const int64_t first = (int64_t)blockIdx.x * kTeams;
