@@ -565,13 +565,28 @@ def fp8_grouped_linear(input: torch.Tensor, weight: torch.Tensor, offs: torch.Te
     return _Fp8GroupedLinear.apply(input, weight, offs, None, None, None, torch.is_grad_enabled())
 
 
+def _keep(h, in_8_bits: bool):
+    """(what is saved of h[M, 2I], its scales): h itself and None, or its codes and their scales."""
+    if h is None or not in_8_bits:
+        return h, None
+    from .kept import quantize_activation
+    return quantize_activation(h)[:2]
+
+
+def _kept(saved, scales):
+    if scales is None:
+        return saved
+    from .kept import Fp8Activation
+    return Fp8Activation(saved, scales, torch.bfloat16).dequantize()
+
+
 class _Fp8SwiGLUDown(torch.autograd.Function):
     """y = F.linear(silu(gate) * up, w_down) for h = [gate | up] (blockwise recipe): the activation is computed and
     quantized for the GEMM in one pass over h, which also makes the activation's transposed 128x1 codes for wgrad;
     backward quantizes grad_out once for both of its GEMMs and ends with the gradient of SwiGLU itself."""
 
     @staticmethod
-    def forward(ctx, h, weight, fast=True, wq=None, sw=None, wqt=None):
+    def forward(ctx, h, weight, fast=True, wq=None, sw=None, wqt=None, keep_8bit=False):
         h2 = _flatten(h)
         m = h2.shape[0]
         # With a weight gradient to come the gate/up output is read once for both forms of the activation: its
@@ -589,7 +604,7 @@ class _Fp8SwiGLUDown(torch.autograd.Function):
         elif h.requires_grad and wqt is None:
             wqt = ops.transpose_codes(wq)
         y = ops.gemm_blockwise(aq, sa, wq, sw)
-        ctx.save_for_backward(h2 if h.requires_grad else None, wqt, sw, at, sat)
+        ctx.save_for_backward(*_keep(h2 if h.requires_grad else None, keep_8bit), wqt, sw, at, sat)
         ctx.h_shape = h.shape
         ctx.x_shape, ctx.w_shape, ctx.has_bias = h.shape, weight.shape, False
         ctx.need = (h.requires_grad, weight.requires_grad)
@@ -597,7 +612,7 @@ class _Fp8SwiGLUDown(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_out):
-        h2, wqt, sw, at, sat = ctx.saved_tensors
+        kept, scales, wqt, sw, at, sat = ctx.saved_tensors
         need_dh, need_dw = ctx.need
         go = _flatten(grad_out)
         if go.dtype != torch.bfloat16:
@@ -605,7 +620,7 @@ class _Fp8SwiGLUDown(torch.autograd.Function):
         go = go.contiguous()
         m = go.shape[0]
         if m == 0:
-            return _empty_batch_grads(ctx, go)[:2] + (None, None, None, None)
+            return _empty_batch_grads(ctx, go)[:2] + (None, None, None, None, None)
         dh = dw = None
         goq = sgo = got = sgot = None
         if need_dh and need_dw:
@@ -619,8 +634,8 @@ class _Fp8SwiGLUDown(torch.autograd.Function):
             dw = ops.gemm_blockwise(got, sgot, at, sat, sb_gran=1)
         if need_dh:
             dact = ops.gemm_blockwise(goq, sgo, wqt, sw.t())
-            dh = ops.swiglu_backward(h2, dact).reshape(ctx.h_shape)
-        return dh, dw, None, None, None, None
+            dh = ops.swiglu_backward(_kept(kept, scales), dact).reshape(ctx.h_shape)
+        return dh, dw, None, None, None, None, None
 
 
 class _Fp8SwiGLUMLPBlock(torch.autograd.Function):
@@ -631,7 +646,7 @@ class _Fp8SwiGLUMLPBlock(torch.autograd.Function):
     never written in bf16."""
 
     @staticmethod
-    def forward(ctx, x, w_gate_up, w_down, fast, gu8, dn8):
+    def forward(ctx, x, w_gate_up, w_down, fast, gu8, dn8, keep_8bit=False):
         x2 = _flatten(x)
         need_dx = x.requires_grad
         xq, sx, xt, sxt = _both_forms(x2)
@@ -645,27 +660,28 @@ class _Fp8SwiGLUMLPBlock(torch.autograd.Function):
         h = ops.gemm_blockwise(xq, sx, gq, gs)
         aq, sa, at, sat = ops.swiglu_quantize_1x128_and_128x1_t_rows(h, fast=fast)
         y = ops.gemm_blockwise(aq, sa, dq, ds)
-        ctx.save_for_backward(h, xt, sxt, gqt if need_dx else None, gs, dqt, ds, at, sat)
+        ctx.save_for_backward(*_keep(h, keep_8bit), xt, sxt, gqt if need_dx else None, gs, dqt, ds, at, sat)
         ctx.x_shape, ctx.need_dx = x.shape, need_dx
         return y.reshape(x.shape[:-1] + (w_down.shape[0],))
 
     @staticmethod
     def backward(ctx, grad_out):
-        h, xt, sxt, gqt, gs, dqt, ds, at, sat = ctx.saved_tensors
+        kept, scales, xt, sxt, gqt, gs, dqt, ds, at, sat = ctx.saved_tensors
         go = _flatten(grad_out)
         if go.dtype != torch.bfloat16:
             go = go.to(torch.bfloat16)
         goq, sgo, got, sgot = _both_forms(go)
         dact, dw_down = ops.linear_backward(goq, sgo, dqt, ds.t(), got, sgot, at, sat)
-        dhq, sdh, dht, sdht = ops.swiglu_backward_quantize_1x128_and_128x1_t_rows(h, dact)
+        dhq, sdh, dht, sdht = ops.swiglu_backward_quantize_1x128_and_128x1_t_rows(_kept(kept, scales), dact)
         if not ctx.need_dx:
-            return None, ops.gemm_blockwise(dht, sdht, xt, sxt, sb_gran=1), dw_down, None, None, None
+            return None, ops.gemm_blockwise(dht, sdht, xt, sxt, sb_gran=1), dw_down, None, None, None, None
         dx, dw_gate_up = ops.linear_backward(dhq, sdh, gqt, gs.t(), dht, sdht, xt, sxt)
-        return dx.reshape(ctx.x_shape), dw_gate_up, dw_down, None, None, None
+        return dx.reshape(ctx.x_shape), dw_gate_up, dw_down, None, None, None, None
 
 
 def fp8_swiglu_mlp(input: torch.Tensor, w_gate_up, w_down, *, fast: bool = True,
-                   gate_up_fp8: Optional[Fp8Weight] = None, down_fp8: Optional[Fp8Weight] = None) -> torch.Tensor:
+                   gate_up_fp8: Optional[Fp8Weight] = None, down_fp8: Optional[Fp8Weight] = None,
+                   keep_8bit: bool = False) -> torch.Tensor:
     """A SwiGLU MLP block (DeepSeekV3 dense MLP): ``F.linear(F.silu(gate) * up, w_down)`` with
     ``gate | up = F.linear(input, w_gate_up)`` -- in the reference two aten::linear calls dispatched at
     hyper_parallel/core/shard/_op_dispatch.py:277-283 with eager bf16 elementwise ops between them.  Here the
@@ -677,9 +693,10 @@ def fp8_swiglu_mlp(input: torch.Tensor, w_gate_up, w_down, *, fast: bool = True,
     enabled the result carries an autograd graph (blockwise recipe); ``gate_up_fp8`` / ``down_fp8`` are then the
     weights' FP8 forms made earlier by `quantize_weight` (e.g. once per optimizer step for all its micro-batches),
     as `fp8_linear`'s ``weight_fp8``.  ``fast`` selects the SwiGLU kernel that uses the hardware exponential and
-    reciprocal."""
+    reciprocal.  ``keep_8bit`` keeps the gate/up output, the block's largest activation, for the backward in 8 bits
+    (`quantize_activation`) instead of bf16: the result is the same, SwiGLU's gradient is taken where the codes are."""
     out = _hand_off(fp8_swiglu_mlp, tuple(t for t in (input, w_gate_up, w_down) if isinstance(t, torch.Tensor)),
-                    (input, w_gate_up, w_down), dict(fast=fast, gate_up_fp8=gate_up_fp8, down_fp8=down_fp8),
+                    (input, w_gate_up, w_down), dict(fast=fast, gate_up_fp8=gate_up_fp8, down_fp8=down_fp8, keep_8bit=keep_8bit),
                     _FP8_MLP_DEFAULTS)
     if out is not NotImplemented:
         return out
@@ -700,9 +717,9 @@ def fp8_swiglu_mlp(input: torch.Tensor, w_gate_up, w_down, *, fast: bool = True,
         rows = input.numel() // max(input.shape[-1], 1)
         if (w_gate_up.requires_grad and w_down.requires_grad and rows > 0
                 and input.dtype == torch.bfloat16 and w_gate_up.dtype == torch.bfloat16 and w_down.dtype == torch.bfloat16):
-            return _Fp8SwiGLUMLPBlock.apply(input, w_gate_up, w_down, fast, gate_up_fp8, d8)
+            return _Fp8SwiGLUMLPBlock.apply(input, w_gate_up, w_down, fast, gate_up_fp8, d8, keep_8bit)
         h = fp8_linear(input, w_gate_up, weight_fp8=gate_up_fp8)
-        return _Fp8SwiGLUDown.apply(h, w_down, fast, *((d8.codes, d8.scale_inv, d8.codes_t) if d8 is not None else ()))
+        return _Fp8SwiGLUDown.apply(h, w_down, fast, *((d8.codes, d8.scale_inv, d8.codes_t) if d8 is not None else (None, None, None)), keep_8bit)
     gu = w_gate_up if isinstance(w_gate_up, Fp8Weight) else (gate_up_fp8 or quantize_weight(w_gate_up.detach(), with_transpose=False))
     dn = w_down if isinstance(w_down, Fp8Weight) else (down_fp8 or quantize_weight(w_down.detach(), with_transpose=False))
     inter = gu.codes.shape[0] // 2
@@ -725,7 +742,7 @@ def fp8_swiglu_mlp(input: torch.Tensor, w_gate_up, w_down, *, fast: bool = True,
     return y.reshape(input.shape[:-1] + (dn.codes.shape[0],))
 
 
-_FP8_MLP_DEFAULTS = dict(fast=True, gate_up_fp8=None, down_fp8=None)
+_FP8_MLP_DEFAULTS = dict(fast=True, gate_up_fp8=None, down_fp8=None, keep_8bit=False)
 
 
 class Fp8SwiGLUMLP(nn.Module):
@@ -733,15 +750,15 @@ class Fp8SwiGLUMLP(nn.Module):
     first) and ``down_proj.weight`` [hidden, intermediate], computed by `fp8_swiglu_mlp`.  With
     ``cache_weight=True`` it keeps, like `Fp8Linear`, the FP8 forms of its weights until a parameter is written
     again, so the micro-batches of one optimizer step and inference calls quantize them once (the same opt-in
-    and the same contract: `_Fp8WeightCache`)."""
+    and the same contract: `_Fp8WeightCache`).  ``keep_8bit`` as in `fp8_swiglu_mlp`."""
 
     def __init__(self, hidden_size: int, intermediate_size: int, *, fast: bool = True, cache_weight: bool = False,
-                 device=None, dtype=torch.bfloat16):
+                 keep_8bit: bool = False, device=None, dtype=torch.bfloat16):
         super().__init__()
         if hidden_size % ops.BLOCK or intermediate_size % ops.BLOCK:
             raise ValueError("hidden_size and intermediate_size must be multiples of 128")
         self.hidden_size, self.intermediate_size, self.fast = hidden_size, intermediate_size, fast
-        self.cache_weight = cache_weight
+        self.cache_weight, self.keep_8bit = cache_weight, keep_8bit
         self.gate_up_proj = nn.Linear(hidden_size, 2 * intermediate_size, bias=False, device=device, dtype=dtype)
         self.down_proj = nn.Linear(intermediate_size, hidden_size, bias=False, device=device, dtype=dtype)
         self._cache = _Fp8WeightCache(2)
@@ -761,9 +778,9 @@ class Fp8SwiGLUMLP(nn.Module):
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         wgu, wd = self.gate_up_proj.weight, self.down_proj.weight
         if not self.cache_weight:
-            return fp8_swiglu_mlp(input, wgu, wd, fast=self.fast)
+            return fp8_swiglu_mlp(input, wgu, wd, fast=self.fast, keep_8bit=self.keep_8bit)
         return fp8_swiglu_mlp(input, wgu, wd, fast=self.fast, gate_up_fp8=self._weight_fp8(0, wgu),
-                              down_fp8=self._weight_fp8(1, wd))
+                              down_fp8=self._weight_fp8(1, wd), keep_8bit=self.keep_8bit)
 
     def extra_repr(self) -> str:
         return f"hidden_size={self.hidden_size}, intermediate_size={self.intermediate_size}, fast={self.fast}"
