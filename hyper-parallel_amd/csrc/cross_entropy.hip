@@ -42,6 +42,7 @@ struct Product {
   int64_t ldc;           // elements
   int store;
   int tiles;
+  int b_by_k;            // b is [K, N]
   int splits;            // parts of k, each with a c of its own, M ldc elements behind the one before
 };
 
@@ -91,9 +92,10 @@ __device__ __forceinline__ int tile_of_workgroup(int pid, int tiles) {
 // column (of the wave's 128) of sum r of subtile i in the lanes of group g, and the row of b that therefore goes to row p of LDS
 __device__ __forceinline__ int column_of(int i, int g, int r) { return 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r; }
 
-// an operand's rows from `base` to its last one: a transfer from behind it reads zeros
+// an operand's rows from `base` to its last one: a transfer from behind it reads zeros.  (A row ends with a whole 16-byte chunk: the workspaces
+// whose length is none hold zeros there.)
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const uint8_t* base, int64_t rows, int64_t ld, int K) {
-  const int64_t bytes = (rows - 1) * ld + (int64_t)K * 2;
+  const int64_t bytes = (rows - 1) * ld + (int64_t)((K + 7) & ~7) * 2;
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(bytes < 0x7FFFF000 ? bytes : 0x7FFFF000), 0x00020000);
 }
 // 32 values of k out of a fragment's 64
@@ -241,7 +243,7 @@ __device__ __forceinline__ void finish_tile(const CeParams& p, const Product& q,
         float* const row = reinterpret_cast<float*>(q.c) + (int64_t)(m + j) * q.ldc;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-          const int col = n + column_of(i, g, 0);
+          const int col = n + (q.b_by_k ? 16 * i + 4 * g : column_of(i, g, 0));
           if (col >= q.N) continue;
           v4f v = acc[i][j];
           if (q.store == kF32Add) v += *reinterpret_cast<const v4f*>(row + col);
@@ -252,34 +254,22 @@ __device__ __forceinline__ void finish_tile(const CeParams& p, const Product& q,
   }
 }
 
-template <int EPI>
-__global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[5 * kSlabBytes];
+// Slabs of a b that lies with its rows along k (BT) are 64 rows of 512 bytes, in 32-byte slots swizzled so that the eight rows that half a
+// wave reads at a time lie in different banks.
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ int slot_swizzle(int k) { return (k & 3) | (k >> 4 & 1) << 2; }
+
+// The sums of a tile.  BT: b is [K, N], its rows along k; its fragments are then gathered by transposing reads, and subtile i is columns
+// 16 i ... instead of column_of's.
+template <bool BT>
+__device__ __forceinline__ void multiply(const Product& q, int m0, int n0, uint8_t* lds, int lane, int wave, v4f (&acc)[8][4]) {
   uint8_t* const a_lds = lds;
   uint8_t* const b_lds = lds + 2 * kSlabBytes;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int pid = blockIdx.x;
-  const int before = EPI == kGrads ? p.part[0].tiles * p.part[0].splits : 0;
-  const bool second = EPI == kGrads && pid >= before;
-  Product q = second ? p.part[1] : p.part[0];
-  int t = tile_of_workgroup(second ? pid - before : pid, q.tiles * q.splits), tm, tn;
-  if (EPI == kGrads && q.splits > 1) {
-    const int split = t / q.tiles, all = (q.K + kSlab - 1) / kSlab;
-    t -= split * q.tiles;
-    const int from = (int)((int64_t)all * split / q.splits), to = (int)((int64_t)all * (split + 1) / q.splits);
-    q.a += (int64_t)from * kSlab * 2;
-    q.b += (int64_t)from * kSlab * 2;
-    q.K = (to < all ? to * kSlab : q.K) - from * kSlab;
-    q.c = reinterpret_cast<float*>(q.c) + (int64_t)split * q.M * q.ldc;
-  }
-  tile_at(t, (q.M + kTile - 1) / kTile, (q.N + kTile - 1) / kTile, tm, tn);
-  const int m0 = tm * kTile, n0 = tn * kTile;
   const int slabs = (q.K + kSlab - 1) / kSlab;
-
   // ---- transfers: one is 8 rows x 128 bytes of LDS per wave, four per wave and slab
   const __amdgpu_buffer_rsrc_t rsrc_a = resource(q.a + (int64_t)m0 * q.lda, q.M - m0, q.lda, q.K);
-  const __amdgpu_buffer_rsrc_t rsrc_b = resource(q.b + (int64_t)n0 * q.ldb, q.N - n0, q.ldb, q.K);
-  uint32_t a_off[4], b_off[4], past[2];
+  const __amdgpu_buffer_rsrc_t rsrc_b = BT ? resource(q.b + (int64_t)n0 * 2, q.K, q.ldb, q.N - n0) : resource(q.b + (int64_t)n0 * q.ldb, q.N - n0, q.ldb, q.K);
+  uint32_t a_off[4], b_off[4], past[2], past_b[BT ? 4 : 1];
   const int whole = q.K / kSlab;               // slabs that are not cut off by the end of k
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -289,25 +279,49 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
     const int rb = (r & ~127) + column_of((r >> 4) & 7, (r >> 2) & 3, r & 3);
     a_off[i] = (uint32_t)ra * (uint32_t)q.lda + chunk * 16;
     b_off[i] = (uint32_t)rb * (uint32_t)q.ldb + chunk * 16;
+    if constexpr (BT) {
+      const int k = (wave * 4 + i) * 2 + (lane >> 5);       // 2 rows x 512 bytes
+      b_off[i] = (uint32_t)k * (uint32_t)q.ldb + (((lane & 31) >> 1 ^ slot_swizzle(k)) * 2 + (lane & 1)) * 16;
+      past_b[i] = k >= q.K % kSlab ? 0x80000000u : 0u;
+    }
     // (a chunk behind the end of k is read from beyond the resource, as zeros; the swizzle has two patterns over i)
     if (i < 2) past[i] = chunk * 8 >= q.K % kSlab ? 0x80000000u : 0u;
   }
-  auto load = [&](const __amdgpu_buffer_rsrc_t& rs, uint32_t off, uint8_t* to, int slab, int i) {
+  const int b_step = BT ? kSlab * (int)q.ldb : 128;
+  auto load = [&](const __amdgpu_buffer_rsrc_t& rs, uint32_t off, uint32_t behind, uint8_t* to, int slab, int step, int i) {
     // (behind the last slab the last one again: those are never used)
     const int s = slab < slabs ? slab : slabs - 1;
-    const uint32_t o = off + (s >= whole ? past[i & 1] : 0u);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(to + (wave * 4 + i) * 1024), 16, o, s * 128, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(to + (wave * 4 + i) * 1024), 16, off + (s >= whole ? behind : 0u), s * step, 0, 0);
   };
-  auto load_a = [&](int buf, int slab, int i) { load(rsrc_a, a_off[i], a_lds + buf * kSlabBytes, slab, i); };
-  auto load_b = [&](int buf, int slab, int i) { load(rsrc_b, b_off[i], b_lds + buf * kSlabBytes, slab, i); };
+  auto load_a = [&](int buf, int slab, int i) { load(rsrc_a, a_off[i], past[i & 1], a_lds + buf * kSlabBytes, slab, 128, i); };
+  auto load_b = [&](int buf, int slab, int i) {
+    load(rsrc_b, b_off[i], BT ? past_b[i] : past[i & 1], b_lds + buf * kSlabBytes, slab, b_step, i);
+  };
 
   const int wn = wave & 1, wm = wave >> 1, l16 = lane & 15, g = lane >> 4;
   int frag_lo = l16 * 128 + ((2 * g) ^ row_swizzle(l16)) * 16, frag_hi = frag_lo ^ 16;
   asm volatile("" : "+v"(frag_lo), "+v"(frag_hi));
   const int a_frag = wm * 64 * 128, b_frag = wn * 128 * 128;
+  // BT: a lane's 8 bytes of four rows of k; the group's 16 lanes exchange them, so that each has four values of k of one column.  (Through the
+  // builtin every such read waits for all transfers under way.  The reads of two subtiles and their wait are one block.)
+  const uint32_t tr_row = (16 * g + (l16 >> 2)) * 512 + (l16 & 3) * 8 + (uint32_t)(uintptr_t)(lds_ptr_t)lds, tr_slot = slot_swizzle(16 * g + (l16 >> 2)) * 32;
+  auto read_two = [&](const uint8_t* slab, int i, v8i& f0, v8i& f1) {
+    const uint32_t at = tr_row + (uint32_t)(slab - lds);
+    const uint32_t at0 = at + (((wn * 8 + i) * 32) ^ tr_slot), at1 = at + (((wn * 8 + i + 1) * 32) ^ tr_slot);
+    i32x2 r[8];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:2048\n\tds_read_b64_tr_b16 %2, %8 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %3, %8 offset:6144\n\tds_read_b64_tr_b16 %4, %9\n\tds_read_b64_tr_b16 %5, %9 offset:2048\n\t"
+        "ds_read_b64_tr_b16 %6, %9 offset:4096\n\tds_read_b64_tr_b16 %7, %9 offset:6144\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+        : "v"(at0), "v"(at1)
+        : "memory");
+    f0 = v8i{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
+    f1 = v8i{r[4][0], r[4][1], r[5][0], r[5][1], r[6][0], r[6][1], r[7][0], r[7][1]};
+  };
+  auto read_b = [&](const uint8_t* slab, int i) { return frag_read(slab + b_frag + i * 16 * 128, frag_lo, frag_hi); };
 
   const v4f zero = {0.f, 0.f, 0.f, 0.f};
-  v4f acc[8][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -326,11 +340,12 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
   load_a(1, 1, 0);
   load_a(1, 1, 1);
 
-  v8i xf[4], wf_n0, wf_n1;
-  wf_n0 = frag_read(b_lds + b_frag, frag_lo, frag_hi);
+  v8i xf[4], wf[4];
+  if constexpr (BT) read_two(b_lds, 0, wf[0], wf[1]);
+  else wf[0] = read_b(b_lds, 0);
 #pragma unroll
   for (int j = 0; j < 4; ++j) xf[j] = frag_read(a_lds + a_frag + j * 16 * 128, frag_lo, frag_hi);
-  wf_n1 = frag_read(b_lds + b_frag + 16 * 128, frag_lo, frag_hi);
+  if (!BT) wf[1] = read_b(b_lds, 1);
 
   // One slab.  Its barrier sits before its last two subtiles: what follows it, the fragments of the next slab, is covered by the matrix
   // instructions that are left.  Transfers, one per subtile: the rest of the next slab of a, the slab after next of b, and behind
@@ -341,37 +356,57 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
     const uint8_t* const bcur = b_lds + bbuf * kSlabBytes;
     const uint8_t* const bnxt = b_lds + bnext * kSlabBytes;
     const uint8_t* const anxt = a_lds + (abuf ^ 1) * kSlabBytes;
-    v8i wf[3];
-    wf[0] = wf_n0;
-    wf[1] = wf_n1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (i == 6) {
         __builtin_amdgcn_s_waitcnt(0x0070 | 4);         // vmcnt(4) lgkmcnt(0): b's slab after next may be under way
         __builtin_amdgcn_s_barrier();
       }
-      wf[(i + 2) % 3] = i < 6 ? frag_read(bcur + b_frag + (i + 2) * 16 * 128, frag_lo, frag_hi)
-                              : frag_read(bnxt + b_frag + (i - 6) * 16 * 128, frag_lo, frag_hi);
+      if constexpr (!BT) wf[(i + 2) % 4] = i < 6 ? read_b(bcur, i + 2) : read_b(bnxt, i - 6);
+      else if (i % 2 == 0) read_two(i < 6 ? bcur : bnxt, i < 6 ? i + 2 : 0, wf[(i + 2) % 4], wf[(i + 3) % 4]);
       if (i < 2) load_a(abuf ^ 1, s + 1, i + 2);
       else if (i < 6) load_b(bnew, s + 2, i - 2);
       else load_a(abuf, s + 2, i - 6);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(half_of(wf[i % 3], 0), half_of(xf[j], 0), acc[i][j], 0, 0, 0);
+      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(half_of(wf[i % 4], 0), half_of(xf[j], 0), acc[i][j], 0, 0, 0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(half_of(wf[i % 3], 1), half_of(xf[j], 1), acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(half_of(wf[i % 4], 1), half_of(xf[j], 1), acc[i][j], 0, 0, 0);
         if (i == 7) xf[j] = frag_read(anxt + a_frag + j * 16 * 128, frag_lo, frag_hi);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    wf_n0 = wf[8 % 3];
-    wf_n1 = wf[9 % 3];
     abuf ^= 1;
     bbuf = bnext;
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);          // vmcnt(0): the last transfers write to this workgroup's LDS
-  finish_tile<EPI, 8, kTile>(p, q, acc, m0, n0, m0 + wm * 64 + l16 * 4, n0 + wn * 128, g, lds);
+}
+
+template <int EPI>
+__global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[5 * kSlabBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pid = blockIdx.x;
+  const int before = EPI == kGrads ? p.part[0].tiles * p.part[0].splits : 0;
+  const bool second = EPI == kGrads && pid >= before;
+  Product q = second ? p.part[1] : p.part[0];
+  int t = tile_of_workgroup(second ? pid - before : pid, q.tiles * q.splits), tm, tn;
+  if (EPI == kGrads && q.splits > 1) {
+    const int split = t / q.tiles, all = (q.K + kSlab - 1) / kSlab;
+    t -= split * q.tiles;
+    const int from = (int)((int64_t)all * split / q.splits), to = (int)((int64_t)all * (split + 1) / q.splits);
+    q.a += (int64_t)from * kSlab * 2;
+    q.b += (int64_t)from * kSlab * (q.b_by_k ? q.ldb : 2);
+    q.K = (to < all ? to * kSlab : q.K) - from * kSlab;
+    q.c = reinterpret_cast<float*>(q.c) + (int64_t)split * q.M * q.ldc;
+  }
+  tile_at(t, (q.M + kTile - 1) / kTile, (q.N + kTile - 1) / kTile, tm, tn);
+  const int m0 = tm * kTile, n0 = tn * kTile;
+  v4f acc[8][4];
+  if (EPI == kGrads && q.b_by_k) multiply<true>(q, m0, n0, lds, lane, wave, acc);
+  else multiply<false>(q, m0, n0, lds, lane, wave, acc);
+  finish_tile<EPI, 8, kTile>(p, q, acc, m0, n0, m0 + (wave >> 1) * 64 + (lane & 15) * 4, n0 + (wave & 1) * 128, lane >> 4, lds);
 }
 
 // Few rows: tiles of 64 x 256, a wave has all 64 rows and 32 columns.  What such a tile waits for is b, so LDS is four slabs of both operands
@@ -666,7 +701,7 @@ int hpfp8_linear_cross_entropy_reduce(const float* loss, const int64_t* target, 
 int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_t, const void* w, int64_t ld_w, const int64_t* target,
                                      int64_t tokens, int64_t hidden, int64_t vocab, int64_t first, int64_t width, int64_t ignore_index,
                                      float smoothing, const float* lse, const float* grad, int64_t grad_stride, const float* count, void* dl,
-                                     void* dl_t, void* w_t, float* dx, int splits, int dx_add, void* dw, int dw_type, int dw_add,
+                                     void* dl_t, float* dx, int splits, int dx_add, void* dw, int dw_type, int dw_add,
                                      hpfp8_stream_t stream) {
   const int bad = check(tokens, hidden, vocab, ld_x, ld_w);
   if (bad != HPFP8_OK) return bad;
@@ -675,10 +710,11 @@ int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_
   HPFP8_REQUIRE(!dx || (splits >= 1 && splits <= 16), HPFP8_ERR_ARG, "dx in %d parts", splits);
   const int64_t slabs = (width + kSlab - 1) / kSlab;
   HPFP8_REQUIRE(!dx || dx_add || splits <= slabs, HPFP8_ERR_ARG, "dx in %d parts of %lld slabs", splits, (long long)slabs);
+  HPFP8_REQUIRE(width * ld_w < (int64_t)1 << 30, HPFP8_ERR_SHAPE, "a piece of %lld rows of the weight spans 2 GiB or more", (long long)width);
   HPFP8_REQUIRE(!dw_add || dw_type == HPFP8_OUT_F32, HPFP8_ERR_ARG, "only fp32 is added onto");
   if (tokens == 0) return HPFP8_OK;
-  HPFP8_REQUIRE(x && w && target && lse && grad && dl && dl_t && (!dx == !w_t) && (!dw == !x_t), HPFP8_ERR_ARG, "null buffer");
-  HPFP8_REQUIRE(aligned16(x) && aligned16(w) && aligned16(dl) && aligned16(dl_t) && aligned16(w_t) && aligned16(x_t) && aligned16(dx) && aligned16(dw),
+  HPFP8_REQUIRE(x && w && target && lse && grad && dl && dl_t && (!dw == !x_t), HPFP8_ERR_ARG, "null buffer");
+  HPFP8_REQUIRE(aligned16(x) && aligned16(w) && aligned16(dl) && aligned16(dl_t) && aligned16(x_t) && aligned16(dx) && aligned16(dw),
                 HPFP8_ERR_ALIGN, "a buffer is not 16-byte aligned");
   const hipStream_t s = (hipStream_t)stream;
   const int64_t rows_padded = stride_of(tokens), cols_padded = stride_of(width);
@@ -704,11 +740,8 @@ int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_
   CeParams g = {};
   int n = 0;
   if (dx) {
-    ce_transpose_kernel<<<dim3((unsigned)((width + 63) / 64), (unsigned)((hidden + 63) / 64)), 256, 0, s>>>(piece, ld_w, width, hidden, nullptr, 0, (uint16_t*)w_t,
-                                                                                                       cols_padded);
-    rc = check_launch("linear_cross_entropy_piece (transpose)");
-    if (rc != HPFP8_OK) return rc;
-    g.part[n] = product(dl, cols_padded, w_t, cols_padded, tokens, hidden, up(width, kSlab), dx, hidden, dx_add ? kF32Add : kF32);
+    g.part[n] = product(dl, cols_padded, piece, ld_w, tokens, hidden, width, dx, hidden, dx_add ? kF32Add : kF32);
+    g.part[n].b_by_k = 1;
     g.part[n++].splits = (int)(splits < slabs ? splits : slabs);      // (a narrower piece adds onto fewer parts)
   }
   if (dw) {

@@ -83,7 +83,7 @@ SIGNATURES = {
     "hpfp8_activation_backward": [_vp, _vp, _i64, _vp, _vp, _int, _i64, _i64, _int, _vp, _vp],
     "hpfp8_linear_cross_entropy_forward": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _f32, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "hpfp8_linear_cross_entropy_piece": [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _i64, _vp, _vp,
-                                         _vp, _vp, _vp, _int, _int, _vp, _int, _int, _vp],
+                                         _vp, _vp, _int, _int, _vp, _int, _int, _vp],
     "hpfp8_linear_cross_entropy_reduce": [_vp, _vp, _i64, _i64, _int, _vp, _vp, _vp],
     "hpfp8_linear_cross_entropy_rows_t": [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp],
     "hpfp8_linear_cross_entropy_round": [_vp, _i64, _int, _vp, _vp],

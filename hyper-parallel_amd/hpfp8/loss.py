@@ -12,7 +12,8 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 _TILE = 256
 # The forward takes this many tokens at a time: its per-tile results (8 bytes for 256 columns of a row) stay at 64 MiB for 131072 columns
 _FORWARD_ROWS = 16384
-# What the backward's workspaces for a piece of the vocabulary may take: the gradient of its logits, twice, and its transposed weight
+# What a piece of the vocabulary may take of memory: the gradient of its logits, twice, and its rows of the weight (which the kernels address
+# with 32 bits)
 _PIECE_BYTES = 512 << 20
 
 
@@ -50,10 +51,11 @@ def _forward(x, weight, target, ignore_index, reduction, smoothing, want_lse):
     return (out if reduction else loss), lse, count
 
 
-def _pieces(tokens: int, hidden: int, vocab: int, budget: int):
-    """[(first, width)]: pieces of the vocabulary, of equal width but for the last, whole tiles wide, whose workspaces fit the budget."""
+def _pieces(tokens: int, stride: int, vocab: int, budget: int):
+    """[(first, width)]: pieces of the vocabulary, of equal width but for the last, whole tiles wide, that fit the budget.  stride: elements
+    between the weight's rows."""
     padded = (tokens + _TILE - 1) // _TILE * _TILE
-    most = max(_TILE, budget // (4 * padded + 2 * hidden) // _TILE * _TILE)
+    most = max(_TILE, budget // (4 * padded + 2 * stride) // _TILE * _TILE)
     count = (vocab + most - 1) // most
     width = ((vocab + count - 1) // count + _TILE - 1) // _TILE * _TILE
     return [(at, min(width, vocab - at)) for at in range(0, vocab, width)]
@@ -86,9 +88,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         device = x2.device
         bf16, f32 = dict(dtype=torch.bfloat16, device=device), dict(dtype=torch.float32, device=device)
         grad = grad_out.reshape(-1).contiguous()
-        dw = dx = x_t = w_t = None
+        dw = dx = x_t = None
         splits = 1
-        pieces = _pieces(tokens, hidden, vocab, _PIECE_BYTES)
+        pieces = _pieces(tokens, w.stride(0), vocab, _PIECE_BYTES)
         width = pieces[0][1]
         row_t, row = (_lib.load().hpfp8_cross_entropy_stride(n) for n in (tokens, width))
         dl = torch.empty(((tokens + _TILE - 1) // _TILE * _TILE, row), **bf16)
@@ -103,11 +105,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
         if need_dx:
             splits = _lib.load().hpfp8_cross_entropy_splits(tokens, hidden, pieces[0][1], int(need_dw))
             dx = torch.empty((splits, tokens, hidden), **f32)
-            w_t = torch.empty((hidden, row), **bf16)
         for first, n in pieces:
             _lib.call("hpfp8_linear_cross_entropy_piece", ops._ptr(x2), x2.stride(0), ops._ptr(x_t), ops._ptr(w), w.stride(0), ops._ptr(target),
                       tokens, hidden, vocab, first, n, ctx.ignore_index, ctx.smoothing, ops._ptr(lse), ops._ptr(grad),
-                      0 if ctx.reduction else 1, ops._ptr(count) if ctx.reduction == 1 else None, ops._ptr(dl), ops._ptr(dl_t), ops._ptr(w_t),
+                      0 if ctx.reduction else 1, ops._ptr(count) if ctx.reduction == 1 else None, ops._ptr(dl), ops._ptr(dl_t),
                       ops._ptr(dx), splits, int(first > 0), ops._ptr(dw), _lib.OUT_BF16 if param is None else _lib.OUT_F32, int(main_grad is not None),
                       ops._stream())
         if need_dx:

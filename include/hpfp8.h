@@ -556,14 +556,14 @@ int hpfp8_linear_cross_entropy_reduce(const float* loss, const int64_t* target, 
  * fp32 only).  Either may be NULL.  grad is the loss's gradient, one value with grad_stride 0 or one for each row; count as the
  * forward wrote it for reduction 1, otherwise NULL.  x_t is what hpfp8_linear_cross_entropy_rows_t makes of x, with row stride
  * S(tokens), S(n) = hpfp8_cross_entropy_stride(n) (needed for dw).  Workspaces, bf16, with R(n) = n rounded up to 256: dl [R(tokens), S(width)],
- * dl_t [R(width), S(tokens)], w_t [hidden, S(width)] (needed for dx).  splits: what hpfp8_cross_entropy_splits says for the widest piece, or another number from 1 to 16 up to its
+ * dl_t [R(width), S(tokens)].  The piece's rows of w span less than 2 GiB.  splits: what hpfp8_cross_entropy_splits says for the widest piece, or another number from 1 to 16 up to its
  * slabs of 64 columns. */
 int64_t hpfp8_cross_entropy_stride(int64_t n);
 int64_t hpfp8_cross_entropy_splits(int64_t tokens, int64_t hidden, int64_t width, int with_dw);
 int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_t, const void* w, int64_t ld_w, const int64_t* target,
                                      int64_t tokens, int64_t hidden, int64_t vocab, int64_t first, int64_t width, int64_t ignore_index,
                                      float smoothing, const float* lse, const float* grad, int64_t grad_stride, const float* count, void* dl,
-                                     void* dl_t, void* w_t, float* dx, int splits, int dx_add, void* dw, int dw_type, int dw_add,
+                                     void* dl_t, float* dx, int splits, int dx_add, void* dw, int dw_type, int dw_add,
                                      hpfp8_stream_t stream);
 /* x[rows, cols] -> x_t[cols, ld_t], bf16, zeros behind the rows up to a multiple of 64 and in place of rows whose target (may be NULL) is
  * ignore_index. */

@@ -73,11 +73,11 @@ def test_linear_cross_entropy(p):
     assert forward(x=p + 2) == -3 and forward(stats=None) == -1 and forward(target=None) == -1
     assert forward(tokens=0, x=None, target=None) == 0
 
-    def backward(first=0, width=10, dx=None, w_t=None, dw=None, x_t=None, dw_type=0, dw_add=0, dl=p, tokens=4, splits=1):
-        return c(piece, p, 64, x_t, p, 64, p, tokens, 64, 10, first, width, -100, 0.0, p, p, 0, None, dl, p, w_t, dx, splits, 0, dw, dw_type, dw_add, None)[0]
+    def backward(first=0, width=10, dx=None, dw=None, x_t=None, dw_type=0, dw_add=0, dl=p, tokens=4, splits=1):
+        return c(piece, p, 64, x_t, p, 64, p, tokens, 64, 10, first, width, -100, 0.0, p, p, 0, None, dl, p, dx, splits, 0, dw, dw_type, dw_add, None)[0]
     assert backward(first=5, width=6) == -2 and backward(width=0) == -2 and backward(first=-1) == -2
-    assert backward(dx=p) == -1 and backward(dw=p) == -1 and backward(dw_type=2) == -1 and backward(dw_add=1) == -1 and backward(dl=None) == -1
-    assert backward(dl=p + 8) == -3 and backward(dx=p, w_t=p, splits=0) == -1 and backward(dx=p, w_t=p, splits=17) == -1
+    assert backward(dw=p) == -1 and backward(dw_type=2) == -1 and backward(dw_add=1) == -1 and backward(dl=None) == -1
+    assert backward(dl=p + 8) == -3 and backward(dx=p, splits=0) == -1 and backward(dx=p, splits=17) == -1 and backward(dx=p, splits=2) == -1
     assert backward(tokens=0) == 0
     t = "hpfp8_linear_cross_entropy_rows_t"
     assert c(t, p, 10, 64, 64, None, 0, p, 56, None)[0] == -2 and c(t, p, 10, 60, 64, None, 0, p, 64, None)[0] == -2
