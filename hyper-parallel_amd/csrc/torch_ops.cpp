@@ -41,7 +41,8 @@ constexpr int64_t kBlock = 128;
   X(hpfp8_swiglu_quantize_1x128_pow2_bf16) X(hpfp8_swiglu_quantize_1x128_fast_bf16) X(hpfp8_gemm_grouped_blockwise) \
   X(hpfp8_bucket_pack_quantize_bf16) X(hpfp8_bucket_unpack_dequantize_bf16) \
   X(hpfp8_quantize_rows) X(hpfp8_dequantize_rows) X(hpfp8_activation_forward) X(hpfp8_activation_backward) X(hpfp8_layer_norm_forward) \
-  X(hpfp8_layer_norm_backward) X(hpfp8_layer_norm_partials)
+  X(hpfp8_layer_norm_backward) X(hpfp8_layer_norm_partials) X(hpfp8_cross_entropy_parts) X(hpfp8_cross_entropy_stride) X(hpfp8_cross_entropy_splits) \
+  X(hpfp8_linear_cross_entropy_forward) X(hpfp8_linear_cross_entropy_piece) X(hpfp8_linear_cross_entropy_rows_t) X(hpfp8_linear_cross_entropy_round)
 struct Library {
 #define HPFP8_POINTER(name) decltype(&::name) name = nullptr;
   HPFP8_FUNCTIONS(HPFP8_POINTER)
@@ -901,6 +902,7 @@ PyObject* bucket_unpack(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
 // ------------------------------------------------------------------------------------------------
 PyObject* norm_backward_function = nullptr;         // the Python backwards, for what the nodes below do not take
 PyObject* activation_backward_function = nullptr;
+PyObject* loss_backward_function = nullptr;
 
 int type_code(at::ScalarType t) { return t == at::kBFloat16 ? HPFP8_OUT_BF16 : t == at::kFloat ? HPFP8_OUT_F32 : t == at::kHalf ? HPFP8_TYPE_F16 : -1; }
 at::ScalarType type_of(int code) { return code == HPFP8_OUT_BF16 ? at::kBFloat16 : code == HPFP8_OUT_F32 ? at::kFloat : at::kHalf; }
@@ -1195,6 +1197,130 @@ PyObject* dequantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the loss over a vocabulary: x [.., hidden] and weight [vocab, hidden] bf16, contiguous; one forward's worth of tokens
+constexpr int64_t kLossTile = 256, kForwardRows = 16384;       // (hpfp8/loss.py has the reasons)
+int64_t whole_tiles(int64_t n) { return (n + kLossTile - 1) / kLossTile * kLossTile; }
+
+struct Loss {
+  at::Tensor loss, lse, count;
+  int64_t ignore_index, reduction, budget;
+  double smoothing;
+};
+
+struct LossNode : torch::autograd::Function<LossNode> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target,
+                            const Loss& made) {
+    ctx->save_for_backward({x, weight, target, made.lse, made.count});
+    ctx->saved_data["how"] = std::vector<int64_t>{made.ignore_index, made.reduction, made.budget};
+    ctx->saved_data["smoothing"] = made.smoothing;
+    return made.loss;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &weight = saved[1], &target = saved[2], &lse = saved[3], &count = saved[4], &grad = grads[0];
+    const std::vector<int64_t> how = ctx->saved_data["how"].toIntVector();
+    const int64_t ignore_index = how[0], reduction = how[1], budget = how[2];
+    const double smoothing = ctx->saved_data["smoothing"].toDouble();
+    const bool need_dx = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1);
+    const int64_t hidden = weight.size(-1), vocab = weight.numel() / hidden, tokens = x.numel() / hidden;
+    const bool as_made = no_modes() && grad.is_cuda() && grad.layout() == at::kStrided && !at::isTensorSubclassLike(grad) &&
+                         grad.scalar_type() == at::kFloat && again(x, grad, at::kBFloat16, tokens * hidden) &&
+                         again(weight, grad, at::kBFloat16, vocab * hidden) && again(target, grad, at::kLong, tokens) && again(lse, grad, at::kFloat, tokens) &&
+                         (!count.defined() || again(count, grad, at::kFloat, 1)) && (uintptr_t)x.data_ptr() % 16 == 0 && (uintptr_t)weight.data_ptr() % 16 == 0;
+    if (!as_made) {
+      pybind11::gil_scoped_acquire held;
+      return from_python(loss_backward_function, pybind11::make_tuple(grad, x, weight, target, lse, or_none(count), ignore_index, reduction, smoothing,
+                                                                     need_dx, need_dw), 4);
+    }
+    const at::Tensor go = grad.contiguous();
+    void* const stream = c10::hip::getCurrentHIPStream(go.get_device()).stream();
+    const at::TensorOptions bf16 = x.options().requires_grad(false), floats = bf16.dtype(at::kFloat);
+    const int64_t padded = whole_tiles(tokens);
+    const int64_t most = std::max(kLossTile, budget / (4 * padded + 2 * hidden) / kLossTile * kLossTile), pieces = (vocab + most - 1) / most;
+    const int64_t width = std::min(whole_tiles((vocab + pieces - 1) / pieces), vocab);
+    const int64_t row_t = lib.hpfp8_cross_entropy_stride(tokens), row = lib.hpfp8_cross_entropy_stride(width);
+    const at::Tensor dl = at::empty({padded, row}, bf16), dl_t = at::empty({whole_tiles(width), row_t}, bf16);
+    at::Tensor dw, x_t, sum, dx;
+    Call call;
+    if (need_dw) {
+      dw = at::empty(weight.sizes(), bf16);
+      x_t = at::empty({hidden, row_t}, bf16);
+      HPFP8_CALL(call, hpfp8_linear_cross_entropy_rows_t, x.data_ptr(), tokens, hidden, hidden, target.data_ptr<int64_t>(), ignore_index, x_t.data_ptr(),
+                 row_t, stream);
+    }
+    int splits = 1;
+    if (need_dx) {
+      splits = (int)lib.hpfp8_cross_entropy_splits(tokens, hidden, width, need_dw);
+      sum = at::empty({splits, tokens, hidden}, floats);
+    }
+    for (int64_t first = 0; first < vocab && call.ok(); first += width)
+      HPFP8_CALL(call, hpfp8_linear_cross_entropy_piece, x.data_ptr(), hidden, need_dw ? x_t.data_ptr() : nullptr, weight.data_ptr(), hidden,
+                 target.data_ptr<int64_t>(), tokens, hidden, vocab, first, std::min(width, vocab - first), ignore_index, (float)smoothing, f32(lse), f32(go),
+                 reduction ? 0 : 1, reduction == 1 ? f32(count) : nullptr, dl.data_ptr(), dl_t.data_ptr(), need_dx ? f32(sum) : nullptr, splits, first > 0,
+                 need_dw ? dw.data_ptr() : nullptr, HPFP8_OUT_BF16, 0, stream);
+    if (need_dx && call.ok()) {
+      dx = at::empty(x.sizes(), bf16);
+      HPFP8_CALL(call, hpfp8_linear_cross_entropy_round, f32(sum), tokens * hidden, splits, dx.data_ptr(), stream);
+    }
+    if (!call.ok()) raise(call);
+    return once({dx, dw, at::Tensor(), at::Tensor()}, grad);
+  }
+};
+
+// (x, weight, target, ignore_index, reduction, smoothing, bytes of a piece, device, stream) -> loss, with its place in the graph where it has one
+PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 9);
+  const Where at_ = where(args, n_args);
+  Loss made;
+  made.ignore_index = PyLong_AsLongLong(args[3]);
+  made.reduction = PyLong_AsLongLong(args[4]);
+  made.smoothing = PyFloat_AsDouble(args[5]);
+  made.budget = PyLong_AsLongLong(args[6]);
+  if (PyErr_Occurred()) throw python_error();
+  const at::Tensor *x, *weight, *target;
+  if (!rows_of_values(args[0], at_.device, x) || x->scalar_type() != at::kBFloat16 || x->numel() == 0 || !rows_of_values(args[1], at_.device, weight) ||
+      weight->scalar_type() != at::kBFloat16 || weight->dim() != 2 || !plain(args[2], at_.device, target) || target->scalar_type() != at::kLong ||
+      !target->is_contiguous())
+    Py_RETURN_NONE;
+  const int64_t hidden = x->size(-1), vocab = weight->size(0), tokens = x->numel() / hidden;
+  if (weight->size(1) != hidden || hidden % 8 || hidden >= 1 << 22 || vocab < 1 || vocab > 1 << 24 || tokens > kForwardRows ||
+      target->sizes() != x->sizes().slice(0, x->dim() - 1) || (uintptr_t)x->data_ptr() % 16 || (uintptr_t)weight->data_ptr() % 16 || !ordinary({x, weight}))
+    Py_RETURN_NONE;
+  const bool train = to_train({x, weight});
+  Call call;
+  {
+    pybind11::gil_scoped_release free;
+    at::NoGradGuard no_grad;
+    const at::TensorOptions floats = x->options().requires_grad(false).dtype(at::kFloat);
+    const int64_t parts = lib.hpfp8_cross_entropy_parts(vocab);
+    const at::Tensor stats = at::empty({tokens, parts, 2}, floats), own = at::empty({tokens}, floats);
+    at::Tensor sums, out, loss = at::empty(target->sizes(), floats);
+    if (made.smoothing != 0) sums = at::empty({tokens, parts}, floats);
+    if (train) made.lse = at::empty({tokens}, floats);
+    if (made.reduction) {
+      out = at::empty({}, floats);
+      made.count = at::empty({}, floats);
+    }
+    HPFP8_CALL(call, hpfp8_linear_cross_entropy_forward, x->data_ptr(), hidden, weight->data_ptr(), hidden, target->data_ptr<int64_t>(), tokens, hidden,
+               vocab, made.ignore_index, (float)made.smoothing, (int)made.reduction, f32(stats), sums.defined() ? f32(sums) : nullptr, f32(own),
+               train ? f32(made.lse) : nullptr, f32(loss), made.reduction ? f32(out) : nullptr, made.reduction ? f32(made.count) : nullptr, at_.stream);
+    made.loss = made.reduction ? out : loss;
+  }
+  if (!call.ok()) return failed(call);
+  return THPVariable_Wrap(train ? LossNode::apply(*x, *weight, *target, made) : made.loss);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* bind_loss_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 1);
+  Py_INCREF(args[0]);
+  loss_backward_function = args[0];
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // (the Python functions that NormNode's and ActivationNode's backwards call where they do not apply themselves)
 PyObject* bind_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -1251,6 +1377,7 @@ PyMethodDef methods[] = {HPFP8_METHOD(built_for), HPFP8_METHOD(bind), HPFP8_METH
                          HPFP8_METHOD(gemm_per_tensor), HPFP8_METHOD(trains), HPFP8_METHOD(linear_node), HPFP8_METHOD(linear_train), HPFP8_METHOD(linear_infer), HPFP8_METHOD(linear_backward),
                          HPFP8_METHOD(swiglu_mlp_infer), HPFP8_METHOD(grouped_infer), HPFP8_METHOD(bucket_pack), HPFP8_METHOD(bucket_unpack),
                          HPFP8_METHOD(layer_norm), HPFP8_METHOD(activation), HPFP8_METHOD(quantize_rows), HPFP8_METHOD(dequantize_rows),
+                         HPFP8_METHOD(linear_cross_entropy), HPFP8_METHOD(bind_loss_backward),
                          HPFP8_METHOD(bind_norm_backward), HPFP8_METHOD(bind_activation_backward),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

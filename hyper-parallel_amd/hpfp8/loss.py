@@ -73,53 +73,58 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        x, weight, target, lse, count = ctx.saved_tensors
-        target, lse = target.contiguous(), lse.contiguous()      # (hooks on saved tensors may have handed them back with other strides)
-        need_dx, need_dw = ctx.needs_input_grad[:2]
-        x2, w = _rows(x), _rows(weight)
-        tokens, hidden = x2.shape
-        vocab = w.shape[0]
-        param = ctx.main_grad_of
-        main_grad = None if param is None else getattr(param, "main_grad", None)
-        if tokens == 0:
-            if need_dw and param is not None and main_grad is None:
-                param.main_grad = torch.zeros(weight.shape, dtype=torch.float32, device=w.device)
-            return (torch.zeros_like(x) if need_dx else None, torch.zeros_like(weight) if need_dw and param is None else None) + (None,) * 5
-        device = x2.device
-        bf16, f32 = dict(dtype=torch.bfloat16, device=device), dict(dtype=torch.float32, device=device)
-        grad = grad_out.reshape(-1).contiguous()
-        dw = dx = x_t = None
-        splits = 1
-        pieces = _pieces(tokens, w.stride(0), vocab, _PIECE_BYTES)
-        width = pieces[0][1]
-        row_t, row = (_lib.load().hpfp8_cross_entropy_stride(n) for n in (tokens, width))
-        dl = torch.empty(((tokens + _TILE - 1) // _TILE * _TILE, row), **bf16)
-        dl_t = torch.empty(((width + _TILE - 1) // _TILE * _TILE, row_t), **bf16)
-        if need_dw:
-            dw = torch.empty((vocab, hidden), **bf16) if param is None else main_grad
-            if dw is None:
-                dw = torch.empty((vocab, hidden), **f32)
-            x_t = torch.empty((hidden, row_t), **bf16)
-            _lib.call("hpfp8_linear_cross_entropy_rows_t", ops._ptr(x2), tokens, hidden, x2.stride(0), ops._ptr(target), ctx.ignore_index,
-                      ops._ptr(x_t), row_t, ops._stream())
-        if need_dx:
-            splits = _lib.load().hpfp8_cross_entropy_splits(tokens, hidden, pieces[0][1], int(need_dw))
-            dx = torch.empty((splits, tokens, hidden), **f32)
-        for first, n in pieces:
-            _lib.call("hpfp8_linear_cross_entropy_piece", ops._ptr(x2), x2.stride(0), ops._ptr(x_t), ops._ptr(w), w.stride(0), ops._ptr(target),
-                      tokens, hidden, vocab, first, n, ctx.ignore_index, ctx.smoothing, ops._ptr(lse), ops._ptr(grad),
-                      0 if ctx.reduction else 1, ops._ptr(count) if ctx.reduction == 1 else None, ops._ptr(dl), ops._ptr(dl_t),
-                      ops._ptr(dx), splits, int(first > 0), ops._ptr(dw), _lib.OUT_BF16 if param is None else _lib.OUT_F32, int(main_grad is not None),
-                      ops._stream())
-        if need_dx:
-            rounded = torch.empty(x.shape, **bf16)
-            _lib.call("hpfp8_linear_cross_entropy_round", ops._ptr(dx), tokens * hidden, splits, ops._ptr(rounded), ops._stream())
-            dx = rounded
-        if need_dw and param is not None:
-            if main_grad is None:
-                param.main_grad = dw
-            dw = None
-        return dx, dw, None, None, None, None, None
+        return _backward(grad_out, *ctx.saved_tensors, ctx.ignore_index, ctx.reduction, ctx.smoothing, *ctx.needs_input_grad[:2],
+                         ctx.main_grad_of) + (None,) * 5
+
+
+def _backward(grad_out, x, weight, target, lse, count, ignore_index, reduction, smoothing, need_dx, need_dw, param=None):
+    """(dx, dw); with ``param`` the weight's gradient goes to param.main_grad."""
+    target, lse = target.contiguous(), lse.contiguous()      # (hooks on saved tensors may have handed them back with other strides)
+    x2, w = _rows(x), _rows(weight)
+    tokens, hidden = x2.shape
+    vocab = w.shape[0]
+    main_grad = None if param is None else getattr(param, "main_grad", None)
+    if tokens == 0:
+        if need_dw and param is not None and main_grad is None:
+            param.main_grad = torch.zeros(weight.shape, dtype=torch.float32, device=w.device)
+        return torch.zeros_like(x) if need_dx else None, torch.zeros_like(weight) if need_dw and param is None else None
+    bf16, f32 = dict(dtype=torch.bfloat16, device=x2.device), dict(dtype=torch.float32, device=x2.device)
+    grad = grad_out.reshape(-1).contiguous()
+    dw = dx = x_t = None
+    splits = 1
+    pieces = _pieces(tokens, w.stride(0), vocab, _PIECE_BYTES)
+    width = pieces[0][1]
+    row_t, row = (_lib.load().hpfp8_cross_entropy_stride(n) for n in (tokens, width))
+    dl = torch.empty(((tokens + _TILE - 1) // _TILE * _TILE, row), **bf16)
+    dl_t = torch.empty(((width + _TILE - 1) // _TILE * _TILE, row_t), **bf16)
+    if need_dw:
+        dw = torch.empty((vocab, hidden), **bf16) if param is None else main_grad
+        if dw is None:
+            dw = torch.empty((vocab, hidden), **f32)
+        x_t = torch.empty((hidden, row_t), **bf16)
+        _lib.call("hpfp8_linear_cross_entropy_rows_t", ops._ptr(x2), tokens, hidden, x2.stride(0), ops._ptr(target), ignore_index, ops._ptr(x_t),
+                  row_t, ops._stream())
+    if need_dx:
+        splits = _lib.load().hpfp8_cross_entropy_splits(tokens, hidden, width, int(need_dw))
+        dx = torch.empty((splits, tokens, hidden), **f32)
+    for first, n in pieces:
+        _lib.call("hpfp8_linear_cross_entropy_piece", ops._ptr(x2), x2.stride(0), ops._ptr(x_t), ops._ptr(w), w.stride(0), ops._ptr(target),
+                  tokens, hidden, vocab, first, n, ignore_index, smoothing, ops._ptr(lse), ops._ptr(grad), 0 if reduction else 1,
+                  ops._ptr(count) if reduction == 1 else None, ops._ptr(dl), ops._ptr(dl_t), ops._ptr(dx), splits, int(first > 0), ops._ptr(dw),
+                  _lib.OUT_BF16 if param is None else _lib.OUT_F32, int(main_grad is not None), ops._stream())
+    if need_dx:
+        rounded = torch.empty(x.shape, **bf16)
+        _lib.call("hpfp8_linear_cross_entropy_round", ops._ptr(dx), tokens * hidden, splits, ops._ptr(rounded), ops._stream())
+        dx = rounded
+    if need_dw and param is not None:
+        if main_grad is None:
+            param.main_grad = dw
+        dw = None
+    return dx, dw
+
+
+if ops._native is not None:
+    ops._native.bind_loss_backward(_backward)
 
 
 _DEFAULTS = dict(ignore_index=-100, reduction="mean", label_smoothing=0.0, apply_grad_on_fp32_main_grad=False)
@@ -146,6 +151,12 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
         raise ValueError(f"reduction must be one of {tuple(_REDUCTIONS)}, got {reduction!r}")
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
+    if not apply_grad_on_fp32_main_grad and ops._gpu(input):
+        device = ops._device()
+        loss = ops._native.linear_cross_entropy(input, weight, target, ignore_index, _REDUCTIONS[reduction], label_smoothing, _PIECE_BYTES,
+                                                device, ops._raw_stream(device))
+        if loss is not None:
+            return loss
     for name, t in (("input", input), ("weight", weight)):
         ops._check_bf16(t, name, contiguous=False)
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[0] > 1 << 24:

@@ -228,3 +228,36 @@ def test_gradient_against_differences(gpu):
             # the loss's third derivative along c is below 8 (a moment of weights below 2); bf16 rounds dl's 50 summands
             limit = 8 / 6 * 0.0625 ** 2 * 1.2 + 2.0 ** -7 * 2 * float(w.abs().max()) + 1e-4 + (step - 0.125).abs() * 8
             assert ((d - dx.double().cpu()[:, c]).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("reduction,smoothing", [("mean", 0.1), ("none", 0.0)])
+def test_the_python_form_and_other_ways_through_the_graph(gpu, reduction, smoothing, monkeypatch):
+    """Without the native host path, under a dispatch mode and with hooks on saved tensors, in one piece and in several: the same results."""
+    import hpfp8
+    from hpfp8 import loss as module, ops
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x, w, t = (v.to(gpu) for v in make(90, 64, 1500, 12))
+    x, t = x.reshape(3, 30, 64), t.reshape(3, 30)
+    go = torch.rand(t.shape if reduction == "none" else (), device=gpu)
+
+    def step(hooks=None, mode=None):
+        a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+        with hooks or torch.enable_grad():
+            loss = hpfp8.linear_cross_entropy(a, b, t, reduction=reduction, label_smoothing=smoothing)
+        with mode or torch.enable_grad():
+            return (loss.detach(),) + torch.autograd.grad(loss, (a, b), go)
+    for budget in (1 << 30, 1 << 19):
+        monkeypatch.setattr(module, "_PIECE_BYTES", budget)
+        want = step()
+        hooks = torch.autograd.graph.saved_tensors_hooks(lambda v: v.cpu(), lambda v: v.to(gpu))
+        strided = torch.autograd.graph.saved_tensors_hooks(lambda v: v, lambda v: torch.stack((v, v), -1)[..., 0])
+        for got in (step(hooks), step(strided), step(None, Mode()), step(Mode())):
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+        with monkeypatch.context() as m:
+            m.setattr(ops, "_native", None)
+            assert all(torch.equal(p, q) for p, q in zip(step(), want))
