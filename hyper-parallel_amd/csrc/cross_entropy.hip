@@ -29,6 +29,8 @@ constexpr int kSlab = 64;                     // values of k in a slab: 128 byte
 constexpr int kSlabBytes = kTile * 2 * kSlab;
 constexpr float kLog2e = 1.44269504f;
 
+constexpr int64_t kPieceElements = 0x3FFFF000;      // of a piece of the weight: its bytes are addressed with 31 bits
+
 enum Epilogue { kStats = 0, kDlogits = 1, kGrads = 2 };
 enum Store { kBf16 = 0, kF32 = 1, kF32Add = 2 };
 
@@ -409,67 +411,89 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
   finish_tile<EPI, 8, kTile>(p, q, acc, m0, n0, m0 + (wave >> 1) * 64 + (lane & 15) * 4, n0 + (wave & 1) * 128, lane >> 4, lds);
 }
 
-// Few rows: tiles of 64 x 256, a wave has all 64 rows and 32 columns.  What such a tile waits for is b, so LDS is four slabs of both operands
-// and three of them are on their way while the fourth is multiplied; one barrier per slab.
-constexpr int kNarrow = 64, kNarrowStages = 4, kNarrowStage = (kNarrow + kTile) * 128;
-template <int EPI>
-__global__ __launch_bounds__(512) void ce_gemm_narrow_kernel(CeParams p) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kNarrowStages * kNarrowStage];
+// All but this wave's last LEFT transfers have landed; then all waves'.
+template <int LEFT>
+__device__ __forceinline__ void wait_and_meet() {
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
+
+// Fewer rows: tiles of 64 WM x 256, eight waves of 64 rows and 32 or 64 columns.  LDS is a ring of slabs of both operands, all but one of them on
+// their way while that one is multiplied; one barrier per slab.
+constexpr int ring_stages(int wm) { return wm == 1 ? 4 : 3; }
+template <int EPI, int WM>
+__device__ __forceinline__ void ring_tile(const CeParams& p, uint8_t* lds) {
+  constexpr int kRows = 64 * WM, WN = 8 / WM, NS = kTile / (16 * WN), kStages = ring_stages(WM), kStage = (kRows + kTile) * 128;
+  constexpr int kLeft = (kStages - 2) * (WM + 4);       // transfers of the slabs behind the next one
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Product q = p.part[0];
   int tm, tn;
-  tile_at(tile_of_workgroup(blockIdx.x, q.tiles), (q.M + kNarrow - 1) / kNarrow, (q.N + kTile - 1) / kTile, tm, tn);
-  const int m0 = tm * kNarrow, n0 = tn * kTile, slabs = (q.K + kSlab - 1) / kSlab, whole = q.K / kSlab;
+  tile_at(tile_of_workgroup(blockIdx.x, q.tiles), (q.M + kRows - 1) / kRows, (q.N + kTile - 1) / kTile, tm, tn);
+  const int m0 = tm * kRows, n0 = tn * kTile, slabs = (q.K + kSlab - 1) / kSlab, whole = q.K / kSlab;
   const __amdgpu_buffer_rsrc_t rsrc_a = resource(q.a + (int64_t)m0 * q.lda, q.M - m0, q.lda, q.K);
   const __amdgpu_buffer_rsrc_t rsrc_b = resource(q.b + (int64_t)n0 * q.ldb, q.N - n0, q.ldb, q.K);
-  // a wave's transfers of a slab: one of a (rows 8 wave ...), four of b
-  uint32_t off[5], past[2];
+  // a wave's transfers of a slab: WM of a, four of b
+  uint32_t a_off[WM], b_off[4], past[2];
+  auto chunk_of = [&](int r) { return (lane & 7) ^ row_swizzle(r); };
 #pragma unroll
-  for (int i = 0; i < 5; ++i) {
-    const int r = (i == 0 ? wave : wave * 4 + i - 1) * 8 + (lane >> 3);
-    const int chunk = (lane & 7) ^ row_swizzle(r);
-    const int from = i == 0 ? (r & 15) * 4 + (r >> 4) : (r & ~31) + column_of((r >> 4) & 1, (r >> 2) & 3, r & 3);
-    off[i] = (uint32_t)from * (uint32_t)(i == 0 ? q.lda : q.ldb) + chunk * 16;
-    // (behind the end of k: from beyond the resource, as zeros; the swizzle has two patterns, by whether r / 8 is odd)
-    if (i == 1 || i == 2) past[i - 1] = chunk * 8 >= q.K % kSlab ? 0x80000000u : 0u;
+  for (int i = 0; i < WM; ++i) {
+    const int r = (wave * WM + i) * 8 + (lane >> 3);
+    a_off[i] = (uint32_t)((r & ~63) + (r & 15) * 4 + ((r >> 4) & 3)) * (uint32_t)q.lda + chunk_of(r) * 16;
   }
-  const uint32_t past_a = wave & 1 ? past[1] : past[0];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = (wave * 4 + i) * 8 + (lane >> 3);
+    b_off[i] = (uint32_t)((r & ~(16 * NS - 1)) + column_of((r >> 4) & (NS - 1), (r >> 2) & 3, r & 3)) * (uint32_t)q.ldb + chunk_of(r) * 16;
+    // (a chunk behind the end of k is read from beyond the resource, as zeros; the swizzle has two patterns, by whether r / 8 is odd)
+    if (i < 2) past[i] = chunk_of(r) * 8 >= q.K % kSlab ? 0x80000000u : 0u;
+  }
   auto load = [&](int slab) {
-    uint8_t* const to = lds + slab % kNarrowStages * kNarrowStage;
+    uint8_t* const to = lds + slab % kStages * kStage;
     const int s = slab < slabs ? slab : slabs - 1;        // (behind the last slab the last one again: those are never used)
     const bool cut = s >= whole;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_a, (lds_ptr_t)(to + wave * 1024), 16, off[0] + (cut ? past_a : 0u), s * 128, 0, 0);
+#pragma unroll
+    for (int i = 0; i < WM; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_a, (lds_ptr_t)(to + (wave * WM + i) * 1024), 16, a_off[i] + (cut ? past[(wave * WM + i) & 1] : 0u),
+                                               s * 128, 0, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_b, (lds_ptr_t)(to + kNarrow * 128 + (wave * 4 + i) * 1024), 16, off[1 + i] + (cut ? past[i & 1] : 0u),
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_b, (lds_ptr_t)(to + kRows * 128 + (wave * 4 + i) * 1024), 16, b_off[i] + (cut ? past[i & 1] : 0u),
                                                s * 128, 0, 0);
   };
-  const int l16 = lane & 15, g = lane >> 4;
+  const int wm = wave / WN, wn = wave % WN, l16 = lane & 15, g = lane >> 4;
   const int frag_lo = l16 * 128 + ((2 * g) ^ row_swizzle(l16)) * 16, frag_hi = frag_lo ^ 16;
   const v4f zero = {0.f, 0.f, 0.f, 0.f};
-  v4f acc[2][4] = {{zero, zero, zero, zero}, {zero, zero, zero, zero}};
-  load(0);
-  load(1);
-  load(2);
-  for (int s = 0; s < slabs; ++s) {
-    asm volatile("s_waitcnt vmcnt(10)\n\ts_barrier" ::: "memory");       // slab s is there, and the one before has been read by all
-    load(s + 3);
-    const uint8_t* const a = lds + s % kNarrowStages * kNarrowStage;
-    const uint8_t* const b = a + kNarrow * 128 + wave * 32 * 128;
-    v8i wf[2], xf[4];
+  v4f acc[NS][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) wf[i] = frag_read(b + i * 16 * 128, frag_lo, frag_hi);
+  for (int i = 0; i < NS; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = zero;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) load(s);
+  for (int s = 0; s < slabs; ++s) {
+    // slab s is there (those after it may be under way), and the one before has been read by all
+    wait_and_meet<kLeft>();
+    load(s + kStages - 1);
+    const uint8_t* const a = lds + s % kStages * kStage + wm * 64 * 128;
+    const uint8_t* const b = lds + s % kStages * kStage + kRows * 128 + wn * 16 * NS * 128;
+    v8i wf[NS], xf[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) xf[j] = frag_read(a + j * 16 * 128, frag_lo, frag_hi);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int i = 0; i < NS; ++i) wf[i] = frag_read(b + i * 16 * 128, frag_lo, frag_hi);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(half_of(wf[i], h), half_of(xf[j], h), acc[i][j], 0, 0, 0);
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);          // vmcnt(0): the last transfers write to this workgroup's LDS
-  finish_tile<EPI, 2, kNarrow>(p, q, acc, m0, n0, m0 + l16 * 4, n0 + wave * 32, g, lds);
+  finish_tile<EPI, NS, kRows>(p, q, acc, m0, n0, m0 + wm * 64 + l16 * 4, n0 + wn * 16 * NS, g, lds);
+}
+template <int EPI, int WM>
+__global__ __launch_bounds__(512) void ce_gemm_ring_kernel(CeParams p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[ring_stages(WM) * (64 * WM + kTile) * 128];
+  ring_tile<EPI, WM>(p, lds);
 }
 
 // ---- joins the forward's partial results, a wave for each row
@@ -598,7 +622,7 @@ int check(int64_t tokens, int64_t hidden, int64_t vocab, int64_t ld_x, int64_t l
   HPFP8_REQUIRE(tokens >= 0 && hidden > 0 && vocab > 0, HPFP8_ERR_SHAPE, "tokens=%lld hidden=%lld vocab=%lld", (long long)tokens, (long long)hidden, (long long)vocab);
   HPFP8_REQUIRE(hidden % 8 == 0 && ld_x % 8 == 0 && ld_w % 8 == 0, HPFP8_ERR_SHAPE, "hidden and the row strides must be multiples of 8");
   HPFP8_REQUIRE(ld_x >= hidden && ld_w >= hidden, HPFP8_ERR_SHAPE, "a row stride is below hidden");
-  HPFP8_REQUIRE(ld_x < (1 << 22) && ld_w < (1 << 22), HPFP8_ERR_SHAPE, "rows of 8 MiB and more");
+  HPFP8_REQUIRE(ld_x < (1 << 21) && ld_w < (1 << 21), HPFP8_ERR_SHAPE, "rows of 4 MiB and more");
   HPFP8_REQUIRE(tokens <= (1 << 22) && vocab <= (1 << 24), HPFP8_ERR_SHAPE, "tokens=%lld vocab=%lld: at most 2^22 and 2^24", (long long)tokens, (long long)vocab);
   return HPFP8_OK;
 }
@@ -620,17 +644,23 @@ Product product(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t 
   return q;
 }
 
-// Tiles of 64 rows up to 64 rows, and wherever the compute units' rounds of them are shorter: a slab takes at least 0.85 us in a tile of 256
-// rows and 0.42 in one of 64.  us of a forward, 256 / 64 rows: 5 tokens, 7168, 131072 375 / 312, 128, 2048, 32000 60 / 44, 256, 2048, 32000
-// 62 / 66, 512, 896, 5165 30 / 27, 512, 4096, 32000 120 / 212.
+// The tile whose rounds on the compute units are the shortest: a slab takes about 1.25, 0.9 and 0.7 us in a tile of 256, 128 and 64 rows, and a
+// tile's start and end 5, 4 and 4.  us of a forward with 256 / 128 / 64: 5 tokens, 7168, 131072 368 / 313 / 308, 65 384 / 317 / 385, 256
+// 438 / 541 / 744; 128, 2048, 32000 58 / 47 / 43, 256 61 / 47 / 67, 512 63 / 83 / 117; 300, 4096, 16000 96 / 66 / 92; 1000, 1024, 8000 32 / 25 / 31;
+// 512, 896, 5165 28 / 22 / 16; 1531, 2048, 50001 289 / 357 / 437.
 template <int EPI>
 void launch_logits(CeParams& p, hipStream_t s) {
   Product& q = p.part[0];
-  const int64_t slabs = (q.K + kSlab - 1) / kSlab, narrow = (int64_t)((q.M + kNarrow - 1) / kNarrow) * ((q.N + kTile - 1) / kTile);
-  const int64_t cost = (q.tiles + 255) / 256 * (85 * slabs + 500), narrow_cost = (narrow + 255) / 256 * (42 * slabs + 400);
-  if (q.M <= kNarrow || narrow_cost < cost) {
-    q.tiles = (int)narrow;
-    ce_gemm_narrow_kernel<EPI><<<q.tiles, 512, 0, s>>>(p);
+  const int64_t slabs = (q.K + kSlab - 1) / kSlab;
+  auto tiles = [&](int rows) { return (int64_t)((q.M + rows - 1) / rows) * ((q.N + kTile - 1) / kTile); };
+  auto cost = [&](int rows, int slab, int ends) { return (tiles(rows) + 255) / 256 * (slab * slabs + ends); };
+  const int64_t c256 = cost(256, 125, 500), c128 = cost(128, 90, 400), c64 = cost(64, 70, 400);
+  if (c64 < c128 && c64 < c256) {
+    q.tiles = (int)tiles(64);
+    ce_gemm_ring_kernel<EPI, 1><<<q.tiles, 512, 0, s>>>(p);
+  } else if (c128 < c256) {
+    q.tiles = (int)tiles(128);
+    ce_gemm_ring_kernel<EPI, 2><<<q.tiles, 512, 0, s>>>(p);
   } else {
     ce_gemm_kernel<EPI><<<q.tiles, 512, 0, s>>>(p);
   }
@@ -652,9 +682,9 @@ int64_t hpfp8_cross_entropy_splits(int64_t tokens, int64_t hidden, int64_t width
   if (tokens <= 0 || hidden <= 0 || width <= 0) return 1;
   const int64_t slabs_x = (width + kSlab - 1) / kSlab, slabs_w = (tokens + kSlab - 1) / kSlab;
   const int64_t all = tiles_of(tokens, hidden) * (slabs_x + 6) + (with_dw ? tiles_of(width, hidden) * (slabs_w + 6) : 0);
-  const int64_t half = all / 512 > 24 ? all / 512 : 24;
+  const int64_t half = all / 512 > 8 ? all / 512 : 8;
   const int64_t splits = (slabs_x + half - 1) / half;
-  return splits < 16 ? splits : 16;
+  return splits < 32 ? splits : 32;
 }
 int64_t hpfp8_cross_entropy_stride(int64_t n) { return n > 0 ? stride_of(n) : 0; }
 
@@ -707,10 +737,10 @@ int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_
   if (bad != HPFP8_OK) return bad;
   HPFP8_REQUIRE(first >= 0 && width > 0 && first + width <= vocab, HPFP8_ERR_SHAPE, "piece %lld + %lld of %lld", (long long)first, (long long)width, (long long)vocab);
   HPFP8_REQUIRE(dw_type == HPFP8_OUT_BF16 || dw_type == HPFP8_OUT_F32, HPFP8_ERR_ARG, "unknown output type %d", dw_type);
-  HPFP8_REQUIRE(!dx || (splits >= 1 && splits <= 16), HPFP8_ERR_ARG, "dx in %d parts", splits);
+  HPFP8_REQUIRE(!dx || (splits >= 1 && splits <= 32), HPFP8_ERR_ARG, "dx in %d parts", splits);
   const int64_t slabs = (width + kSlab - 1) / kSlab;
   HPFP8_REQUIRE(!dx || dx_add || splits <= slabs, HPFP8_ERR_ARG, "dx in %d parts of %lld slabs", splits, (long long)slabs);
-  HPFP8_REQUIRE(width * ld_w < (int64_t)1 << 30, HPFP8_ERR_SHAPE, "a piece of %lld rows of the weight spans 2 GiB or more", (long long)width);
+  HPFP8_REQUIRE(width * ld_w < kPieceElements, HPFP8_ERR_SHAPE, "a piece of %lld rows of the weight spans 2 GiB or more", (long long)width);
   HPFP8_REQUIRE(!dw_add || dw_type == HPFP8_OUT_F32, HPFP8_ERR_ARG, "only fp32 is added onto");
   if (tokens == 0) return HPFP8_OK;
   HPFP8_REQUIRE(x && w && target && lse && grad && dl && dl_t && (!dw == !x_t), HPFP8_ERR_ARG, "null buffer");

@@ -1198,7 +1198,7 @@ PyObject* dequantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
 }
 
 // ---- the loss over a vocabulary: x [.., hidden] and weight [vocab, hidden] bf16, contiguous; one forward's worth of tokens
-constexpr int64_t kLossTile = 256, kForwardRows = 16384;       // (hpfp8/loss.py has the reasons)
+constexpr int64_t kLossTile = 256, kForwardRows = 16384, kPieceElements = 0x3FFFF000;       // (hpfp8/loss.py has the reasons)
 int64_t whole_tiles(int64_t n) { return (n + kLossTile - 1) / kLossTile * kLossTile; }
 
 struct Loss {
@@ -1236,7 +1236,7 @@ struct LossNode : torch::autograd::Function<LossNode> {
     void* const stream = c10::hip::getCurrentHIPStream(go.get_device()).stream();
     const at::TensorOptions bf16 = x.options().requires_grad(false), floats = bf16.dtype(at::kFloat);
     const int64_t padded = whole_tiles(tokens);
-    const int64_t most = std::max(kLossTile, budget / (4 * padded + 2 * hidden) / kLossTile * kLossTile), pieces = (vocab + most - 1) / most;
+    const int64_t most = std::max(kLossTile, std::min(budget / (4 * padded), (kPieceElements - 1) / hidden) / kLossTile * kLossTile), pieces = (vocab + most - 1) / most;
     const int64_t width = std::min(whole_tiles((vocab + pieces - 1) / pieces), vocab);
     const int64_t row_t = lib.hpfp8_cross_entropy_stride(tokens), row = lib.hpfp8_cross_entropy_stride(width);
     const at::Tensor dl = at::empty({padded, row}, bf16), dl_t = at::empty({whole_tiles(width), row_t}, bf16);
@@ -1284,7 +1284,7 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n_ar
       !target->is_contiguous())
     Py_RETURN_NONE;
   const int64_t hidden = x->size(-1), vocab = weight->size(0), tokens = x->numel() / hidden;
-  if (weight->size(1) != hidden || hidden % 8 || hidden >= 1 << 22 || vocab < 1 || vocab > 1 << 24 || tokens > kForwardRows ||
+  if (weight->size(1) != hidden || hidden % 8 || hidden >= 1 << 21 || vocab < 1 || vocab > 1 << 24 || tokens > kForwardRows ||
       target->sizes() != x->sizes().slice(0, x->dim() - 1) || (uintptr_t)x->data_ptr() % 16 || (uintptr_t)weight->data_ptr() % 16 || !ordinary({x, weight}))
     Py_RETURN_NONE;
   const bool train = to_train({x, weight});

@@ -12,15 +12,16 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 _TILE = 256
 # The forward takes this many tokens at a time: its per-tile results (8 bytes for 256 columns of a row) stay at 64 MiB for 131072 columns
 _FORWARD_ROWS = 16384
-# What a piece of the vocabulary may take of memory: the gradient of its logits, twice, and its rows of the weight (which the kernels address
-# with 32 bits)
-_PIECE_BYTES = 512 << 20
+# What the gradient of a piece's logits may take of memory, which is there twice
+_PIECE_BYTES = 256 << 20
+# Elements that a piece's rows of the weight may span: the kernels address them with 31 bits
+_PIECE_ELEMENTS = 0x3FFFF000
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x[..., C] as [rows, C] the kernels can read: unit stride along a row, rows 16 bytes apart and aligned."""
     x = x.reshape(-1, x.shape[-1])
-    return x if x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.stride(0) >= x.shape[1] and x.data_ptr() % 16 == 0 else x.contiguous()
+    return x if x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.shape[1] <= x.stride(0) < 1 << 21 and x.data_ptr() % 16 == 0 else x.contiguous()
 
 
 def _forward(x, weight, target, ignore_index, reduction, smoothing, want_lse):
@@ -55,7 +56,7 @@ def _pieces(tokens: int, stride: int, vocab: int, budget: int):
     """[(first, width)]: pieces of the vocabulary, of equal width but for the last, whole tiles wide, that fit the budget.  stride: elements
     between the weight's rows."""
     padded = (tokens + _TILE - 1) // _TILE * _TILE
-    most = max(_TILE, budget // (4 * padded + 2 * stride) // _TILE * _TILE)
+    most = max(_TILE, min(budget // (4 * padded), (_PIECE_ELEMENTS - 1) // stride) // _TILE * _TILE)
     count = (vocab + most - 1) // most
     width = ((vocab + count - 1) // count + _TILE - 1) // _TILE * _TILE
     return [(at, min(width, vocab - at)) for at in range(0, vocab, width)]
@@ -164,8 +165,8 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
     hidden = weight.shape[1]
     if input.dim() < 1 or input.shape[-1] != hidden:
         raise ValueError(f"input {tuple(input.shape)} does not end with weight's hidden size {hidden}")
-    if hidden < 8 or hidden % 8 or hidden >= 1 << 22:
-        raise ValueError(f"hidden must be a multiple of 8 below 2^22, got {hidden}")
+    if hidden < 8 or hidden % 8 or hidden >= 1 << 21:
+        raise ValueError(f"hidden must be a multiple of 8 below 2^21, got {hidden}")
     if not isinstance(target, torch.Tensor) or target.dtype != torch.int64:
         raise TypeError("target must be an int64 tensor")
     ops._check_device(target, "target")
