@@ -3,7 +3,7 @@
 //   hat = (x - mean(x)) / sqrt(mean((x - mean)^2) + eps),   y = hat w + b
 //   u = dy w,   dx = (u - mean(u) - hat mean(u hat)) / sqrt(...),   dw = sum over rows of dy hat,   db = sum over rows of dy
 //
-// One pass over memory each way, bound by it: a row is in the registers of a team of 64, 256 or 512 threads, eight neighbouring
+// One pass over memory each way, bound by it: a row is in the registers of a team of 16 to 512 threads, eight neighbouring
 // values per thread and step, from its load to its results.  All sums are fp32; the variance is taken around the mean (each wave's
 // values around the wave's own mean, the waves joined by their counts), so an offset many times the spread costs nothing.
 // The workgroups stay for many rows: the weight's values are loaded once, the next row's loads are under way while a row is worked on,
@@ -19,8 +19,7 @@ namespace hpfp8 {
 namespace {
 
 constexpr int kMaxCols = 16384;
-constexpr int kBackwardThreads = 512;
-constexpr int kMaxPartials = 256;          // one workgroup of the backward per compute unit
+constexpr int kMaxPartials = 256;          // one workgroup of the backward per compute unit (two where rows are short)
 
 struct NormParams {
   const void* x;
@@ -66,33 +65,107 @@ __device__ __forceinline__ void load_vector8(const void* w, int type, int col, i
   }
 }
 
+// How a row's length and its chunks of eight values go together.
+enum Edge {
+  kWhole = 0,      // the length is a multiple of 128
+   kOverlap = 1,    // any length from 8 on.  The last chunk is the row's last eight values, of which the first `dup` are the chunk's before it: every
+                   // load is a whole vector, so no load has to be waited for before its turn (loads of single values of the last chunk, merged
+                   // with the others' vectors, waited in every row: forward of 65536 x 1030 217 us, where this takes 86)
+  kSingle = 2,     // shorter rows: value by value
+};
+// The chunk of eight values that a thread has in step j.
+struct Chunk {
+  int col;         // its first value's column
+  int dup;         // values before those that are its own
+  bool any;        // it has some
+};
+template <int EDGE>
+__device__ __forceinline__ Chunk chunk_at(int index, int cols) {
+  Chunk c;
+  const int left = cols - index * 8;
+  c.any = left > 0;
+  c.dup = EDGE == kOverlap && c.any && left < 8 ? 8 - left : 0;
+  c.col = c.any ? index * 8 - c.dup : 0;
+  return c;
+}
+// whether value i of the chunk is its own
+template <int EDGE>
+__device__ __forceinline__ bool own(const Chunk& c, int i, int cols) {
+  return EDGE == kWhole ? c.any : (EDGE == kOverlap ? c.any && i >= c.dup : c.any && c.col + i < cols);
+}
+template <typename E, int EDGE>
+__device__ __forceinline__ Pack8<E> load_chunk(const typename E::raw* row, const Chunk& c, int cols, bool in) {
+  return load_pack8<E, kStream<E>, EDGE == kSingle>(row + c.col, in && c.any ? (EDGE == kSingle ? cols - c.col : 8) : 0);
+}
+template <typename E, int EDGE>
+__device__ __forceinline__ void store_chunk(typename E::raw* row, const Chunk& c, int cols, const float v[8]) {
+  if (!c.any) return;
+  if (EDGE == kWhole || (EDGE == kOverlap && c.dup == 0)) {
+    store8<E, kStream<E>, false>(row + c.col, 8, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (own<EDGE>(c, i, cols)) row[c.col + i] = from_f32<E>(v[i]);
+}
+template <int EDGE>
+__device__ __forceinline__ void store_chunk_codes(uint8_t* row, const Chunk& c, int cols, uint2 codes) {
+  if (!c.any) return;
+  if (EDGE == kWhole || (EDGE == kOverlap && c.dup == 0)) {
+    store_codes8<false>(row + c.col, 8, codes);
+    return;
+  }
+  const uint64_t w = (uint64_t)codes.y << 32 | codes.x;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (own<EDGE>(c, i, cols)) row[c.col + i] = (uint8_t)(w >> (8 * i));
+}
+template <int EDGE>
+__device__ __forceinline__ void vector_chunk(const void* w, int type, const Chunk& c, int cols, float none, float v[8]) {
+  load_vector8(w, type, c.col, c.any ? (EDGE == kSingle ? cols - c.col : 8) : 0, none, v);
+}
+
+template <int TPR>
+__device__ __forceinline__ float team_sum(float v) {          // of a wave, or of the 16 lanes of a smaller team
+  if constexpr (TPR >= 64) return wave_sum(v);
+  v += __uint_as_float(dpp_u32<kDppQuadXor1>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_u32<kDppQuadXor2>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_u32<kDppRowHalfMirror>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_u32<kDppRowMirror>(__float_as_uint(v)));
+  return v;
+}
+template <int TPR>
+__device__ __forceinline__ int team_of() {                    // (the same in a whole wave where teams are that large: a row's address is a scalar then)
+  return TPR >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TPR) : threadIdx.x / TPR;
+}
+
 // A row per team of TPR threads; thread t has the chunks of eight values t, t + TPR, ...: 16 neighbouring threads have one group of 128.
-template <typename E, int TPR, int NV, bool KEEP, bool TAIL>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(NormParams p) {
+template <typename E, int TPR, int NV, bool KEEP, int EDGE>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV <= 2 && sizeof(typename E::raw) == 2 ? 4 : 2) void norm_forward_kernel(NormParams p) {
   using raw = typename E::raw;
-  constexpr int kTeams = (TPR < 256 ? 256 : TPR) / TPR, kWaves = TPR / 64, kAhead = 2;
+  constexpr int kTeams = (TPR < 256 ? 256 : TPR) / TPR, kWaves = TPR < 64 ? 1 : TPR / 64, kAhead = 2;
   __shared__ v4f parts[2][kTeams][kWaves];
-  // (the same in a whole wave, so a row's address is a scalar)
-  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, wave = __builtin_amdgcn_readfirstlane(t / 64);
+  const int team = team_of<TPR>(), t = threadIdx.x % TPR, wave = __builtin_amdgcn_readfirstlane(t / 64);
   const int C = p.cols, groups = (C + kBlock - 1) / kBlock;
-  int left[NV];
+  Chunk at[NV];
+  bool live[NV];         // whether this wave has any of the step's values: with none it does nothing (4104 values are one more than a step's)
   float w[NV][8], b[NV][8];
   int mine = 0;                                       // values of a row in this wave's hands
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    left[j] = C - (j * TPR + t) * 8;
-    const int first = (j * TPR + wave * 64) * 8;
-    mine += C - first < 0 ? 0 : (C - first < 512 ? C - first : 512);
-    load_vector8(p.w, p.wtype, (j * TPR + t) * 8, left[j], 1.f, w[j]);
-    load_vector8(p.b, p.wtype, (j * TPR + t) * 8, left[j], 0.f, b[j]);
+    at[j] = chunk_at<EDGE>(j * TPR + t, C);
+    live[j] = j == 0 && TPR <= 64 ? true : (j * TPR + wave * 64) * 8 < C;
+    const int left = C - (j * TPR + wave * 64) * 8, most = (TPR < 64 ? TPR : 64) * 8;
+    mine += left < 0 ? 0 : (left < most ? left : most);
+    vector_chunk<EDGE>(p.w, p.wtype, at[j], C, 1.f, w[j]);
+    vector_chunk<EDGE>(p.b, p.wtype, at[j], C, 0.f, b[j]);
   }
   const float n = (float)mine;
   const int64_t step = (int64_t)gridDim.x * kTeams;
   Pack8<E> next[kAhead][NV];
   auto fetch = [&](Pack8<E> (&to)[NV], int64_t r) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      to[j] = load_pack8<E, kStream<E>, TAIL>((const raw*)p.x + (r < p.rows ? r : 0) * p.ld + (j * TPR + t) * 8, r < p.rows ? left[j] : 0);
+    for (int j = 0; j < NV; ++j) to[j] = load_chunk<E, EDGE>((const raw*)p.x + (r < p.rows ? r : 0) * p.ld, at[j], C, r < p.rows);
   };
   auto work = [&](const Pack8<E> (&packed)[NV], int64_t row, int turn) {
     float v[NV][8];
@@ -101,18 +174,20 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(Nor
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
+      if (live[j])
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[j][i];
-    float mean = mine ? wave_sum(s) / n : 0.f;
+        for (int i = 0; i < 8; ++i) s += EDGE == kOverlap && i < 7 && i < at[j].dup ? 0.f : v[j][i];
+    float mean = mine ? team_sum<TPR>(s) / n : 0.f;
     float m2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
+      if (live[j])
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = i < left[j] ? v[j][i] - mean : 0.f;
-        m2 = __builtin_fmaf(d, d, m2);
-      }
-    m2 = wave_sum(m2);
+        for (int i = 0; i < 8; ++i) {
+          const float d = own<EDGE>(at[j], i, C) ? v[j][i] - mean : 0.f;
+          m2 = __builtin_fmaf(d, d, m2);
+        }
+    m2 = team_sum<TPR>(m2);
     if constexpr (kWaves > 1) {
       if ((t & 63) == 0) parts[turn][team][wave] = v4f{n, mean, m2, 0.f};
       __syncthreads();                                // (one barrier: the next turn writes the other half)
@@ -135,21 +210,21 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(Nor
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int col = (j * TPR + t) * 8;
+      if (!live[j]) continue;
       float out[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[j][i] = i < left[j] ? (v[j][i] - mean) * rstd : 0.f;
+        v[j][i] = (v[j][i] - mean) * rstd;
         out[i] = __builtin_fmaf(v[j][i], w[j][i], b[j][i]);
       }
-      if (left[j] > 0) store8<E, kStream<E>, TAIL>((raw*)p.y + row * C + col, left[j], out);
+      store_chunk<E, EDGE>((raw*)p.y + row * C, at[j], C, out);
       if constexpr (KEEP) {
-        float si;
-        const uint2 c = encode_group(v[j], si);
-        if (left[j] > 0) {
-          store_codes8<TAIL>(p.q + row * C + col, left[j], c);
-          if ((t & 15) == 0) p.scale_inv[row * groups + col / kBlock] = si;
-        }
+        float si, hat[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) hat[i] = own<EDGE>(at[j], i, C) ? v[j][i] : 0.f;     // (a group's maximum is that of its own values)
+        const uint2 c = encode_group(hat, si);
+        store_chunk_codes<EDGE>(p.q + row * C, at[j], C, c);
+        if (at[j].any && (t & 15) == 0) p.scale_inv[row * groups + (j * TPR + t) / 16] = si;
       }
     }
   };
@@ -157,10 +232,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(Nor
 #pragma unroll
   for (int u = 0; u < kAhead; ++u) fetch(next[u], first + team + u * step);
   int turn = 0;
-  for (int64_t at = first; at < p.rows; at += kAhead * step) {
+  for (int64_t at_row = first; at_row < p.rows; at_row += kAhead * step) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u, turn ^= 1) {
-      const int64_t from = at + u * step;             // (as many turns for every team)
+      const int64_t from = at_row + u * step;         // (as many turns for every team)
       if (from >= p.rows) break;
       Pack8<E> packed[NV];
 #pragma unroll
@@ -171,22 +246,31 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_forward_kernel(Nor
   }
 }
 
-template <typename E, int TPR, int NV, bool KEEP, bool TAIL>
+constexpr int kBackwardThreads = 512;
+template <typename E, int TPR, int NV, bool KEEP, int EDGE>
 __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(NormParams p) {
   using raw = typename E::raw;
-  constexpr int kTeams = kBackwardThreads / TPR, kWaves = TPR / 64, kChunks = TPR * NV, kAhead = NV <= 2 ? 3 : 1;
-  constexpr bool kHoldWeight = NV <= 2;      // (four steps' weights beside four steps' sums: over 256 registers)
+  constexpr int kTeams = kBackwardThreads / TPR, kWaves = TPR < 64 ? 1 : TPR / 64, kChunks = TPR * NV;
+  // (rows of over 8192 values: four steps' sums fill half of the registers, so one row is on its way instead of three and the weight is in LDS)
+  constexpr int kAhead = NV <= 2 ? 3 : 1;
+  constexpr bool kHoldWeight = NV <= 2;
   __shared__ v2f parts[2][kTeams][kWaves];
   __shared__ v4f joined[kTeams > 1 ? 2 * kChunks * 2 : 1];
-  // (the same in a whole wave, so a row's address is a scalar)
-  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR), t = threadIdx.x % TPR, wave = __builtin_amdgcn_readfirstlane(t / 64);
+  __shared__ v4f weight[kHoldWeight ? 1 : kChunks * 2];
+  const int team = team_of<TPR>(), t = threadIdx.x % TPR, wave = __builtin_amdgcn_readfirstlane(t / 64);
   const int C = p.cols, groups = (C + kBlock - 1) / kBlock;
-  int left[NV];
+  Chunk at[NV];
+  bool live[NV];         // whether this wave has any of the step's values: with none it does nothing (4104 values are one more than a step's)
   float w[kHoldWeight ? NV : 1][8], dw[NV][8], db[NV][8];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    left[j] = C - (j * TPR + t) * 8;
-    if (kHoldWeight) load_vector8(p.w, p.wtype, (j * TPR + t) * 8, left[j], 1.f, w[j]);
+    at[j] = chunk_at<EDGE>(j * TPR + t, C);
+    live[j] = j == 0 && TPR <= 64 ? true : (j * TPR + wave * 64) * 8 < C;
+    vector_chunk<EDGE>(p.w, p.wtype, at[j], C, 1.f, w[kHoldWeight ? j : 0]);
+    if (!kHoldWeight) {                                // (read by the thread that wrote it)
+      weight[(j * TPR + t) * 2] = v4f{w[0][0], w[0][1], w[0][2], w[0][3]};
+      weight[(j * TPR + t) * 2 + 1] = v4f{w[0][4], w[0][5], w[0][6], w[0][7]};
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[j][i] = db[j][i] = 0.f;
   }
@@ -199,50 +283,56 @@ __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(NormPar
   Row next[kAhead];
   auto fetch = [&](Row& to, int64_t r) {
     const bool in = r < p.rows;
-    const int64_t at = in ? r : 0;
+    const int64_t row = in ? r : 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int col = (j * TPR + t) * 8, n = in ? left[j] : 0;
-      to.dy[j] = load_pack8<E, kStream<E>, TAIL>((const raw*)p.dy + at * p.ld_dy + col, n);
+      to.dy[j] = load_chunk<E, EDGE>((const raw*)p.dy + row * p.ld_dy, at[j], C, in);
       if constexpr (KEEP) {
-        to.q[j] = load_codes8<TAIL>(p.q + at * C + col, n);
-        to.s[j] = n > 0 ? (p.scale_inv + at * groups)[col / kBlock] : 0.f;
+        to.q[j] = load_codes8<EDGE == kSingle>(p.q + row * C + at[j].col, in && at[j].any ? (EDGE == kSingle ? C - at[j].col : 8) : 0);
+        to.s[j] = in && at[j].any ? (p.scale_inv + row * groups)[(j * TPR + t) / 16] : 0.f;
       } else {
-        to.x[j] = load_pack8<E, kStream<E>, TAIL>((const raw*)p.x + at * p.ld + col, n);
+        to.x[j] = load_chunk<E, EDGE>((const raw*)p.x + row * p.ld, at[j], C, in);
       }
     }
-    to.mean = !KEEP && in ? p.mean[r] : 0.f;
-    to.rstd = in ? p.rstd[r] : 0.f;
+    to.mean = !KEEP && in ? p.mean[row] : 0.f;
+    to.rstd = in ? p.rstd[row] : 0.f;
   };
   auto work = [&](const Row& from, int64_t row, int turn) {
     float go[NV][8], hat[NV][8];
     const float rstd = from.rstd;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      if (!live[j]) continue;
       unpack8<E>(from.dy[j], go[j]);
       if constexpr (KEEP) {
-        decode8(from.q[j], from.s[j], hat[j]);
+        decode8(from.q[j], from.s[j], hat[j]);        // (the values before a chunk's own have another group's scale: they are not used)
       } else {
         unpack8<E>(from.x[j], hat[j]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) hat[j][i] = i < left[j] ? (hat[j][i] - from.mean) * rstd : 0.f;
+        for (int i = 0; i < 8; ++i) hat[j][i] = (hat[j][i] - from.mean) * rstd;
       }
     }
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (!kHoldWeight) load_vector8(p.w, p.wtype, (j * TPR + t) * 8, left[j], 1.f, w[0]);
+      if (!live[j]) continue;
+      if (!kHoldWeight) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[0][i] = weight[(j * TPR + t) * 2 + i / 4][i % 4];
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         dw[j][i] = __builtin_fmaf(go[j][i], hat[j][i], dw[j][i]);
         db[j][i] += go[j][i];
         go[j][i] *= w[kHoldWeight ? j : 0][i];        // from here on u
-        s1 += go[j][i];
-        s2 = __builtin_fmaf(go[j][i], hat[j][i], s2);
+        // (where there is nothing, go is 0, and x and mean with it or finite)
+        const float u = EDGE == kOverlap && i < 7 && i < at[j].dup ? 0.f : go[j][i];
+        s1 += u;
+        s2 = EDGE == kOverlap && i < 7 && i < at[j].dup ? s2 : __builtin_fmaf(u, hat[j][i], s2);
       }
     }
-    s1 = wave_sum(s1);
-    s2 = wave_sum(s2);
+    s1 = team_sum<TPR>(s1);
+    s2 = team_sum<TPR>(s2);
     if constexpr (kWaves > 1) {
       if ((t & 63) == 0) parts[turn][team][wave] = v2f{s1, s2};
       __syncthreads();
@@ -257,20 +347,21 @@ __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(NormPar
     const float m1 = s1 / (float)C, m2 = s2 / (float)C;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      if (!live[j]) continue;
       float out[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) out[i] = (go[j][i] - m1 - hat[j][i] * m2) * rstd;
-      if (left[j] > 0) store8<E, kStream<E>, TAIL>((raw*)p.dx + row * C + (j * TPR + t) * 8, left[j], out);
+      store_chunk<E, EDGE>((raw*)p.dx + row * C, at[j], C, out);
     }
   };
   const int64_t first = (int64_t)blockIdx.x * kTeams;
 #pragma unroll
   for (int u = 0; u < kAhead; ++u) fetch(next[u], first + team + u * step);
   int turn = 0;
-  for (int64_t at = first; at < p.rows; at += kAhead * step) {
+  for (int64_t at_row = first; at_row < p.rows; at_row += kAhead * step) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u, turn ^= 1) {
-      const int64_t from = at + u * step;             // (as many turns for every team)
+      const int64_t from = at_row + u * step;         // (as many turns for every team)
       if (from >= p.rows) break;
       const Row row = next[u];
       fetch(next[u], from + team + kAhead * step);
@@ -283,10 +374,9 @@ __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(NormPar
     if (team == k) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int chunk = j * TPR + t;
         if constexpr (kTeams > 1) {
-          v4f* const a = joined + chunk * 2;
-          v4f* const b = joined + (kChunks + chunk) * 2;
+          v4f* const a = joined + (j * TPR + t) * 2;
+          v4f* const b = joined + (kChunks + j * TPR + t) * 2;
           if (k > 0) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -302,9 +392,9 @@ __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(NormPar
             }
           }
         }
-        if (k == kTeams - 1 && left[j] > 0) {
-          store8<F32, false, TAIL>(to + chunk * 8, left[j], dw[j]);
-          store8<F32, false, TAIL>(to + C + chunk * 8, left[j], db[j]);
+        if (k == kTeams - 1) {
+          store_chunk<F32, EDGE>(to, at[j], C, dw[j]);
+          store_chunk<F32, EDGE>(to + C, at[j], C, db[j]);
         }
       }
     }
@@ -345,34 +435,42 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const float* __restrict
   }
 }
 
-// The smallest team that holds a row, and its steps.  f(E, threads per row, steps).
-template <typename E, typename F>
+// The smallest team that holds a row, and its steps.  f(E, threads per row, steps).  (From 1025 to 2048 values two waves of two steps are better in
+// the forward, where four of one step meet at twice as many barriers, 32768 x 2048 48 / 57 us, and four in the backward, 81 / 77.)
+template <typename E, bool BACKWARD, typename F>
 void by_width(int cols, F&& f) {
   const int chunks = (cols + 7) / 8;
-  if (chunks <= 64) f(E(), std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+  if (chunks <= 16) f(E(), std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
+  else if (chunks <= 32) f(E(), std::integral_constant<int, 16>(), std::integral_constant<int, 2>());
+  else if (chunks <= 64) f(E(), std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
   else if (chunks <= 128) f(E(), std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+  else if (chunks <= 256) f(E(), std::integral_constant<int, BACKWARD ? 256 : 128>(), std::integral_constant<int, BACKWARD ? 1 : 2>());
   else if (chunks <= 512) f(E(), std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
   else if (chunks <= 1024) f(E(), std::integral_constant<int, 512>(), std::integral_constant<int, 2>());
   else f(E(), std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
 }
-template <typename F>
+template <bool BACKWARD, typename F>
 void by_type_and_width(int dtype, int cols, F&& f) {
-  if (dtype == HPFP8_OUT_BF16) by_width<Bf16>(cols, f);
-  else if (dtype == HPFP8_TYPE_F16) by_width<F16>(cols, f);
-  else by_width<F32>(cols, f);
+  if (dtype == HPFP8_OUT_BF16) by_width<Bf16, BACKWARD>(cols, f);
+  else if (dtype == HPFP8_TYPE_F16) by_width<F16, BACKWARD>(cols, f);
+  else by_width<F32, BACKWARD>(cols, f);
+}
+template <int TPR, int NV, typename F>
+void by_form(bool keep, int cols, F&& f) {
+  auto with = [&](auto edge) {
+    if (keep) f(std::true_type(), edge);
+    else f(std::false_type(), edge);
+  };
+  if constexpr (TPR * NV == 16) {
+    if (cols < 8) return with(std::integral_constant<int, kSingle>());
+  }
+  if (cols % kBlock == 0) with(std::integral_constant<int, kWhole>());
+  else with(std::integral_constant<int, kOverlap>());
 }
 
-template <typename F>
-void by_form(bool keep, bool tail, F&& f) {
-  if (keep && tail) f(std::true_type(), std::true_type());
-  else if (keep) f(std::true_type(), std::false_type());
-  else if (tail) f(std::false_type(), std::true_type());
-  else f(std::false_type(), std::false_type());
-}
-
-int team_threads(int64_t cols) {
+int backward_teams(int64_t cols) {
   const int64_t chunks = (cols + 7) / 8;
-  return chunks <= 128 ? 64 : (chunks <= 512 ? 256 : 512);
+  return chunks <= 32 ? 32 : (chunks <= 128 ? 8 : (chunks <= 512 ? 2 : 1));
 }
 
 bool at_element(const void* p, int dtype) { return ((uintptr_t)p & (dtype == HPFP8_OUT_F32 ? 3 : 1)) == 0; }
@@ -393,8 +491,8 @@ extern "C" {
 
 int64_t hpfp8_layer_norm_partials(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0 || cols > kMaxCols) return 0;
-  const int64_t teams = kBackwardThreads / team_threads(cols), blocks = (rows + teams - 1) / teams;
-  return blocks < kMaxPartials ? blocks : kMaxPartials;
+  const int64_t teams = backward_teams(cols), blocks = (rows + teams - 1) / teams, most = cols <= 2048 ? 2 * kMaxPartials : kMaxPartials;
+  return blocks < most ? blocks : most;
 }
 
 int hpfp8_layer_norm_forward(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const void* w, const void* b, int wtype, float eps,
@@ -420,13 +518,13 @@ int hpfp8_layer_norm_forward(const void* x, int dtype, int64_t rows, int64_t col
   p.rstd = rstd;
   p.q = (uint8_t*)q;
   p.scale_inv = scale_inv;
-  by_type_and_width(dtype, (int)cols, [&](auto e, auto tpr, auto nv) {
+  by_type_and_width<false>(dtype, (int)cols, [&](auto e, auto tpr, auto nv) {
     using E = decltype(e);
     constexpr int kThreads = tpr < 256 ? 256 : tpr, kTeams = kThreads / tpr;
     const int64_t blocks = (rows + kTeams - 1) / kTeams, most = 256 * (1024 / kThreads);   // every compute unit full once
     const dim3 grid((unsigned)(blocks < most ? blocks : most));
-    auto launch = [&](auto keep, auto tail) { norm_forward_kernel<E, tpr, nv, keep, tail><<<grid, kThreads, 0, (hipStream_t)stream>>>(p); };
-    by_form(q != nullptr, cols % 8 != 0, launch);
+    by_form<tpr, nv>(q != nullptr, (int)cols,
+                     [&](auto keep, auto edge) { norm_forward_kernel<E, tpr, nv, keep, edge><<<grid, kThreads, 0, (hipStream_t)stream>>>(p); });
   });
   return check_launch("layer_norm_forward");
 }
@@ -458,10 +556,11 @@ int hpfp8_layer_norm_backward(const void* dy, int64_t ld_dy, const void* x, int6
     p.dx = dx;
     p.partial = partial;
     const dim3 grid((unsigned)hpfp8_layer_norm_partials(rows, cols));
-    by_type_and_width(dtype, (int)cols, [&](auto e, auto tpr, auto nv) {
+    by_type_and_width<true>(dtype, (int)cols, [&](auto e, auto tpr, auto nv) {
       using E = decltype(e);
-      by_form(q != nullptr, cols % 8 != 0,
-              [&](auto keep, auto tail) { norm_backward_kernel<E, tpr, nv, keep, tail><<<grid, kBackwardThreads, 0, (hipStream_t)stream>>>(p); });
+      by_form<tpr, nv>(q != nullptr, (int)cols, [&](auto keep, auto edge) {
+        norm_backward_kernel<E, tpr, nv, keep, edge><<<grid, kBackwardThreads, 0, (hipStream_t)stream>>>(p);
+      });
     });
     const int rc = check_launch("layer_norm_backward");
     if (rc != HPFP8_OK) return rc;

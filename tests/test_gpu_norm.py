@@ -62,7 +62,7 @@ def close(got, want, bound, dtype):
 
 CASES = [  # rows, cols
     (1, 1), (1, 8), (5, 3), (3, 64), (9, 127), (33, 512), (20, 513), (17, 1024), (16, 1025), (300, 1027), (7, 4096), (13, 4100), (31, 7168),
-    (5, 8192), (3, 8200), (9, 16384), (2, 16381), (1100, 40), (2500, 136)]
+    (5, 8192), (3, 8200), (9, 16384), (2, 16381), (1100, 40), (2500, 136), (40, 9), (70, 128), (33, 129), (21, 200), (65, 256), (12, 257), (11, 2047), (6, 2048), (5, 2055), (6, 8191), (3, 8193)]
 
 
 @pytest.mark.parametrize("rows,cols", CASES)
@@ -84,7 +84,7 @@ def test_forward_and_backward(gpu, rows, cols, dtype, wdtype):
         assert torch.equal(hpfp8.layer_norm(xg, (cols,), wg, bg, 1e-5), y)
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 1), (5, 3), (9, 127), (33, 512), (20, 513), (300, 1027), (7, 4100), (31, 7168), (9, 16384), (2, 16381)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (5, 3), (9, 127), (33, 512), (20, 513), (300, 1027), (7, 4100), (31, 7168), (9, 16384), (2, 16381), (40, 9), (33, 129), (21, 253), (5, 2055)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_kept_in_8_bits(gpu, rows, cols, dtype):
     import hpfp8
