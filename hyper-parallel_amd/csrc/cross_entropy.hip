@@ -15,6 +15,8 @@
 // by direct loads (rows past the end read as zeros) with 16-byte chunks swizzled by row, so that fragments are read without bank conflicts.
 // The rows of a slab are permuted on their way into LDS so that a lane's sums are four neighbouring rows by eight neighbouring
 // columns: results leave as 16 bytes of a row, transposed ones as 8 bytes of a column, without a pass through LDS.
+#include <utility>
+
 #include "gemm_tile.h"
 #include "hpfp8_host.h"
 
@@ -666,6 +668,34 @@ void launch_logits(CeParams& p, hipStream_t s) {
   }
 }
 
+// The gradients' launch: dx's product contracts over the whole piece and has few tiles, so with few tokens a few of its tiles would still be at
+// work long after dw's are done.  Its contraction is split, and the longer of the two kinds of work goes first.  This is the time that 256
+// compute units need for both, in slabs; a tile's start and end cost about six.  us of the launch unsplit / split: 512 tokens, 4096, 32000
+// 736 / 256, 1531, 2048, 50001 1112 / 541.
+constexpr int64_t kEnds = 6;
+int64_t dx_part(int64_t width, int64_t splits) { return ((width + kSlab - 1) / kSlab + splits - 1) / splits + kEnds; }
+int64_t dw_tile(int64_t tokens) { return (tokens + kSlab - 1) / kSlab + kEnds; }
+int64_t gradients_time(int64_t tokens, int64_t hidden, int64_t width, int64_t splits, int with_dw) {
+  int64_t n1 = tiles_of(tokens, hidden) * splits, each1 = dx_part(width, splits), n2 = with_dw ? tiles_of(width, hidden) : 0, each2 = dw_tile(tokens);
+  if (each2 > each1) {
+    std::swap(n1, n2);
+    std::swap(each1, each2);
+  }
+  const int64_t rounds = n1 / 256, rest = n1 % 256;
+  // compute units that have finished the longer kind, `rest` of them one round later, take the shorter one as it comes
+  auto holds = [&](int64_t t) {
+    const int64_t early = t - rounds * each1, late = early - each1;
+    return (256 - rest) * (early > 0 ? early / each2 : 0) + rest * (late > 0 ? late / each2 : 0) >= n2;
+  };
+  int64_t from = (rounds + (rest > 0)) * each1, to = from + (n2 + 255) / 256 * each2;
+  while (from < to) {
+    const int64_t t = (from + to) / 2;
+    if (holds(t)) to = t;
+    else from = t + 1;
+  }
+  return from;
+}
+
 }  // namespace
 }  // namespace hpfp8
 
@@ -674,17 +704,19 @@ using namespace hpfp8;
 extern "C" {
 
 int64_t hpfp8_cross_entropy_parts(int64_t vocab) { return vocab > 0 ? (vocab + kTile - 1) / kTile : 0; }
-// dx's product contracts over the whole piece and has few tiles, so with few tokens a few of its tiles would still be at work long after
-// dw's are done.  Its contraction is split until one part takes at most half of what all of the launch takes the 256 compute units
-// together (in slabs; a tile's start and end cost about six).  us of the launch unsplit / split: 512 tokens, 4096, 32000 736 / 256,
-// 1531, 2048, 50001 1112 / 541.
 int64_t hpfp8_cross_entropy_splits(int64_t tokens, int64_t hidden, int64_t width, int with_dw) {
   if (tokens <= 0 || hidden <= 0 || width <= 0) return 1;
-  const int64_t slabs_x = (width + kSlab - 1) / kSlab, slabs_w = (tokens + kSlab - 1) / kSlab;
-  const int64_t all = tiles_of(tokens, hidden) * (slabs_x + 6) + (with_dw ? tiles_of(width, hidden) * (slabs_w + 6) : 0);
-  const int64_t half = all / 512 > 8 ? all / 512 : 8;
-  const int64_t splits = (slabs_x + half - 1) / half;
-  return splits < 32 ? splits : 32;
+  const int64_t slabs = (width + kSlab - 1) / kSlab;
+  int64_t best = 1, least = INT64_MAX;
+  for (int64_t splits = 1; splits <= 32 && splits <= slabs; ++splits) {
+    // (the parts are written, and read by the sum: so many slabs' time at 4 TB/s)
+    const int64_t cost = gradients_time(tokens, hidden, width, splits, with_dw) + splits * tokens * hidden * 8 / 5000000;
+    if (cost < least) {
+      least = cost;
+      best = splits;
+    }
+  }
+  return best;
 }
 int64_t hpfp8_cross_entropy_stride(int64_t n) { return n > 0 ? stride_of(n) : 0; }
 
@@ -780,6 +812,7 @@ int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_
                           dw_type == HPFP8_OUT_BF16 ? kBf16 : (dw_add ? kF32Add : kF32));
   }
   if (n == 0) return HPFP8_OK;
+  if (n == 2 && dw_tile(tokens) > dx_part(width, splits)) std::swap(g.part[0], g.part[1]);
   g.grad = grad_stride ? nullptr : grad;
   g.count = count;
   ce_gemm_kernel<kGrads><<<g.part[0].tiles * g.part[0].splits + g.part[1].tiles * g.part[1].splits, 512, 0, s>>>(g);

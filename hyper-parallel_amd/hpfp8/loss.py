@@ -13,7 +13,7 @@ _TILE = 256
 # The forward takes this many tokens at a time: its per-tile results (8 bytes for 256 columns of a row) stay at 64 MiB for 131072 columns
 _FORWARD_ROWS = 16384
 # What the gradient of a piece's logits may take of memory, which is there twice
-_PIECE_BYTES = 256 << 20
+_PIECE_BYTES = 512 << 20
 # Elements that a piece's rows of the weight may span: the kernels address them with 31 bits
 _PIECE_ELEMENTS = 0x3FFFF000
 
