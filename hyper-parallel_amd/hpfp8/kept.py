@@ -58,10 +58,19 @@ class Fp8Activation(NamedTuple):
             x = ops._native.dequantize_rows(self.codes, self.scale_inv, _TYPES[dtype], device, ops._raw_stream(device))
             if x is not None:
                 return x
-        ops._check_device(self.codes, "codes")
-        x = torch.empty(self.codes.shape, dtype=dtype, device=self.codes.device)
-        cols = x.shape[-1]
-        _lib.call("hpfp8_dequantize_rows", ops._ptr(self.codes), ops._ptr(self.scale_inv), x.numel() // max(cols, 1), cols, ops._ptr(x),
+        codes, scale_inv = self.codes, self.scale_inv
+        if codes.dtype != ops.FP8 or scale_inv.dtype != torch.float32:
+            raise TypeError(f"codes and scale_inv must be float8_e4m3fn and float32, got {codes.dtype} and {scale_inv.dtype}")
+        ops._check_device(codes, "codes")
+        ops._check_device(scale_inv, "scale_inv")
+        if codes.dim() < 1:
+            raise ValueError("codes must have at least one dimension")
+        cols = codes.shape[-1]
+        if cols and scale_inv.numel() != codes.numel() // cols * _groups(cols):
+            raise ValueError(f"codes {tuple(codes.shape)} have a scale for each 128 values of a row, not {tuple(scale_inv.shape)}")
+        codes, scale_inv = codes.contiguous(), scale_inv.contiguous()         # (a slice of what was made, say)
+        x = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+        _lib.call("hpfp8_dequantize_rows", ops._ptr(codes), ops._ptr(scale_inv), x.numel() // max(cols, 1), cols, ops._ptr(x),
                   _TYPES[dtype], ops._stream())
         return x
 

@@ -287,3 +287,37 @@ def test_the_python_form_and_hooks_on_what_is_saved(gpu, keep, monkeypatch):
     assert all(torch.equal(p, q) for p, q in zip(step(), want))
     again = hpfp8.quantize_activation(x)
     assert torch.equal(again.codes.view(torch.uint8), kept.codes.view(torch.uint8)) and torch.equal(again.dequantize(), kept.dequantize())
+
+
+def test_codes_of_a_part_and_wrong_ones(gpu):
+    """Slices of what was made are read with their strides; scales that do not belong to the codes are refused."""
+    import hpfp8
+    from hpfp8.kept import Fp8Activation
+    made = hpfp8.quantize_activation(torch.randn(12, 5, 200, device=gpu).to(torch.bfloat16))
+    whole = made.dequantize()
+    for part in ((slice(None, None, 2),), (slice(None), 3), (slice(3, 7), slice(1, 4))):
+        assert torch.equal(Fp8Activation(made.codes[part], made.scale_inv[part], made.dtype).dequantize(), whole[part])
+    for codes, scale_inv in ((made.codes, made.scale_inv[:6]), (made.codes[..., :100], made.scale_inv), (made.codes[0, 0, 0], made.scale_inv)):
+        with pytest.raises(ValueError):
+            Fp8Activation(codes, scale_inv, torch.bfloat16).dequantize()
+    for codes, scale_inv in ((whole, made.scale_inv), (made.codes, made.scale_inv.half())):
+        with pytest.raises(TypeError):
+            Fp8Activation(codes, scale_inv, torch.bfloat16).dequantize()
+
+
+@pytest.mark.parametrize("kind,cols", [("silu", 8200), ("swiglu", 4100)])
+def test_more_than_2_31_values(gpu, kind, cols):
+    """The last rows of a tensor that large have the bits that they have alone."""
+    import hpfp8
+    width = 2 * cols if kind == "swiglu" else cols
+    rows = (1 << 31) // width + 100
+    x = torch.empty((rows, width), dtype=torch.bfloat16, device=gpu).normal_().requires_grad_()
+    y = hpfp8.activation(x, kind)
+    go = torch.empty_like(y).normal_()
+    dx, = torch.autograd.grad(y, x, go)
+    last = x.detach()[-150:].clone().requires_grad_()
+    y_last = hpfp8.activation(last, kind)
+    assert torch.equal(y[-150:], y_last) and torch.equal(dx[-150:], torch.autograd.grad(y_last, last, go[-150:])[0])
+    made, made_last = hpfp8.quantize_activation(x.detach()), hpfp8.quantize_activation(last.detach())
+    assert torch.equal(made.codes[-150:].view(torch.uint8), made_last.codes.view(torch.uint8)) and torch.equal(made.scale_inv[-150:], made_last.scale_inv)
+    assert torch.equal(made.dequantize()[-150:], made_last.dequantize())

@@ -278,3 +278,19 @@ def test_second_derivatives_are_refused_and_writes_in_between_noticed(gpu, nativ
     t.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("keep", [False, True])
+def test_more_than_2_31_values(gpu, keep):
+    """The last rows of a tensor that large have the bits that they have alone."""
+    import hpfp8
+    cols = 4100
+    rows = (1 << 31) // cols + 100
+    x = torch.empty((rows, cols), dtype=torch.bfloat16, device=gpu).normal_().requires_grad_()
+    w = torch.empty((cols,), dtype=torch.bfloat16, device=gpu).normal_()
+    y = hpfp8.layer_norm(x, cols, w, keep_8bit=keep)
+    go = torch.empty_like(y).normal_()
+    dx, = torch.autograd.grad(y, x, go)
+    last = x.detach()[-150:].clone().requires_grad_()
+    y_last = hpfp8.layer_norm(last, cols, w, keep_8bit=keep)
+    assert torch.equal(y[-150:], y_last) and torch.equal(dx[-150:], torch.autograd.grad(y_last, last, go[-150:])[0])
