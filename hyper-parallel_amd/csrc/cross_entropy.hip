@@ -221,7 +221,8 @@ __device__ __forceinline__ void finish_tile(const CeParams& p, const Product& q,
     if (p.grad) {
       // (one factor for all rows is applied here, so that what was rounded is a difference of probabilities: of c (p - 1) the most
       // frequent value by far, -c, would be rounded the same way in every row)
-      const float c = p.grad[0] / (p.count ? p.count[0] : 1.f);
+      // (the mean over no rows is NaN, but no row has a part in it: its gradient is 0)
+      const float rows = p.count ? p.count[0] : 1.f, c = rows > 0.f ? p.grad[0] / rows : 0.f;
 #pragma unroll
       for (int i = 0; i < NS; ++i)
 #pragma unroll
@@ -625,7 +626,8 @@ int check(int64_t tokens, int64_t hidden, int64_t vocab, int64_t ld_x, int64_t l
   HPFP8_REQUIRE(hidden % 8 == 0 && ld_x % 8 == 0 && ld_w % 8 == 0, HPFP8_ERR_SHAPE, "hidden and the row strides must be multiples of 8");
   HPFP8_REQUIRE(ld_x >= hidden && ld_w >= hidden, HPFP8_ERR_SHAPE, "a row stride is below hidden");
   HPFP8_REQUIRE(ld_x < (1 << 21) && ld_w < (1 << 21), HPFP8_ERR_SHAPE, "rows of 4 MiB and more");
-  HPFP8_REQUIRE(tokens <= (1 << 22) && vocab <= (1 << 24), HPFP8_ERR_SHAPE, "tokens=%lld vocab=%lld: at most 2^22 and 2^24", (long long)tokens, (long long)vocab);
+  // (256 rows of a workspace with a column for each token are addressed with 31 bits)
+  HPFP8_REQUIRE(tokens <= (1 << 21) && vocab <= (1 << 24), HPFP8_ERR_SHAPE, "tokens=%lld vocab=%lld: at most 2^21 and 2^24", (long long)tokens, (long long)vocab);
   return HPFP8_OK;
 }
 
@@ -772,6 +774,7 @@ int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_
   HPFP8_REQUIRE(!dx || (splits >= 1 && splits <= 32), HPFP8_ERR_ARG, "dx in %d parts", splits);
   const int64_t slabs = (width + kSlab - 1) / kSlab;
   HPFP8_REQUIRE(!dx || dx_add || splits <= slabs, HPFP8_ERR_ARG, "dx in %d parts of %lld slabs", splits, (long long)slabs);
+  HPFP8_REQUIRE(width <= (1 << 21), HPFP8_ERR_SHAPE, "a piece of %lld columns: at most 2^21", (long long)width);
   HPFP8_REQUIRE(width * ld_w < kPieceElements, HPFP8_ERR_SHAPE, "a piece of %lld rows of the weight spans 2 GiB or more", (long long)width);
   HPFP8_REQUIRE(!dw_add || dw_type == HPFP8_OUT_F32, HPFP8_ERR_ARG, "only fp32 is added onto");
   if (tokens == 0) return HPFP8_OK;

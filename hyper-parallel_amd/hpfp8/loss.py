@@ -138,7 +138,8 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
     (hidden a multiple of 8, any vocabulary up to 2^24), target int64 of input's leading shape.
 
     The logits are fp32 accumulators of the tensors' products and are not rounded; the loss is fp32: [...] with reduction "none" (0 where
-    target is ``ignore_index``), its sum, or its mean over the tokens that are not ignored (NaN if all are), summed in a fixed order.
+    target is ``ignore_index``), its sum, or its mean over the tokens that are not ignored (NaN if all are, with gradients of 0), summed in
+    a fixed order.  At most 2^21 tokens in a call.
     A target that is neither ``ignore_index`` nor in [0, vocab) makes its token's loss and gradients NaN.  In the backward the logits are
     computed again, a piece of the vocabulary at a time, their gradient rounded to bfloat16 for the products of both gradients.
 
@@ -172,8 +173,8 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
     ops._check_device(target, "target")
     if target.shape != input.shape[:-1]:
         raise ValueError(f"target must have input's leading shape {tuple(input.shape[:-1])}, got {tuple(target.shape)}")
-    if target.numel() > 1 << 22:
-        raise ValueError(f"at most 2^22 tokens in a call, got {target.numel()}")
+    if target.numel() > 1 << 21:
+        raise ValueError(f"at most 2^21 tokens in a call, got {target.numel()}")
     if apply_grad_on_fp32_main_grad:
         mg = getattr(weight, "main_grad", None)
         if mg is not None and (mg.dtype != torch.float32 or mg.shape != weight.shape or not mg.is_contiguous()):

@@ -539,7 +539,8 @@ int hpfp8_layer_norm_backward(const void* dy, int64_t ld_dy, const void* x, int6
 int64_t hpfp8_layer_norm_partials(int64_t rows, int64_t cols);
 
 /* Softmax cross entropy of the linear l = x w^T over a vocabulary, without the logits in memory.  x[tokens, hidden] and w[vocab, hidden] are
- * bf16, row strides ld_x and ld_w in elements, hidden and the strides multiples of 8 and below 2^21; target[tokens] is int64.
+ * bf16, row strides ld_x and ld_w in elements, hidden and the strides multiples of 8 and below 2^21, tokens at most 2^21, vocab at most 2^24;
+ * target[tokens] is int64.
  *   loss[t] = lse(l_t) - (1 - smoothing) l_t[target] - smoothing mean(l_t);  0 where target is ignore_index, NaN where it is neither that
  *   nor in [0, vocab).  reduction 0: nothing more; 1: out[0] = their mean over the count[0] rows that are not ignored; 2: their sum.
  * Workspaces, fp32: stats[tokens, hpfp8_cross_entropy_parts(vocab), 2], sums (with smoothing only) half of that, target_logit[tokens].  lse[tokens] (may be NULL) is what the backward needs; out and count may be NULL with reduction 0. */
@@ -556,7 +557,7 @@ int hpfp8_linear_cross_entropy_reduce(const float* loss, const int64_t* target, 
  * fp32 only).  Either may be NULL.  grad is the loss's gradient, one value with grad_stride 0 or one for each row; count as the
  * forward wrote it for reduction 1, otherwise NULL.  x_t is what hpfp8_linear_cross_entropy_rows_t makes of x, with row stride
  * S(tokens), S(n) = hpfp8_cross_entropy_stride(n) (needed for dw).  Workspaces, bf16, with R(n) = n rounded up to 256: dl [R(tokens), S(width)],
- * dl_t [R(width), S(tokens)].  The piece's rows of w span less than 2 GiB.  splits: what hpfp8_cross_entropy_splits says for the widest piece, or another number from 1 to 32 up to its
+ * dl_t [R(width), S(tokens)].  The piece's rows of w span less than 2 GiB and are at most 2^21.  splits: what hpfp8_cross_entropy_splits says for the widest piece, or another number from 1 to 32 up to its
  * slabs of 64 columns. */
 int64_t hpfp8_cross_entropy_stride(int64_t n);
 int64_t hpfp8_cross_entropy_splits(int64_t tokens, int64_t hidden, int64_t width, int with_dw);

@@ -261,3 +261,87 @@ def test_the_python_form_and_other_ways_through_the_graph(gpu, reduction, smooth
         with monkeypatch.context() as m:
             m.setattr(ops, "_native", None)
             assert all(torch.equal(p, q) for p, q in zip(step(), want))
+
+
+@pytest.mark.parametrize("main_grad", [False, True])
+def test_the_mean_over_no_rows_is_nan_and_its_gradients_are_zero(gpu, main_grad):
+    """A micro-batch of padding alone, as in torch."""
+    import hpfp8
+    x, w, _ = make(20, 64, 300, 8)
+    xg, wg = x.to(gpu).requires_grad_(), torch.nn.Parameter(w.to(gpu))
+    loss = hpfp8.linear_cross_entropy(xg, wg, torch.full((20,), IGNORE, device=gpu), apply_grad_on_fp32_main_grad=main_grad)
+    loss.backward()
+    dw = wg.main_grad if main_grad else wg.grad
+    assert loss.isnan() and (xg.grad == 0).all() and dw.shape == w.shape and (dw == 0).all()
+
+
+@pytest.mark.parametrize("tokens,hidden,vocab", [(2100, 1024, 20000), (1100, 520, 33000)])
+def test_several_rounds_of_the_largest_tiles(gpu, tokens, hidden, vocab):
+    """More tiles of 256 rows than compute units, the last of each side cut; the reference on the GPU, in 64 bits too."""
+    import hpfp8
+    x, w, t = (v.to(gpu) for v in make(tokens, hidden, vocab, 9))
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = hpfp8.linear_cross_entropy(xg, wg, t, label_smoothing=0.1)
+    dx, dw = torch.autograd.grad(loss, (xg, wg))
+    n = int((t != IGNORE).sum())
+    rows, rdx, rdw, b_rows, b_dx, b_dw = (v.cpu() for v in reference(x, w, t, 0.1, torch.full((tokens,), 1.0 / n, device=gpu, dtype=torch.float64)))
+    within(loss.detach(), rows.sum() / n, (b_rows * (t != IGNORE).cpu()).sum() / n + U * (rows.sum() / n).abs())
+    within(dx, rdx, b_dx, H)
+    within(dw, rdw, b_dw, H)
+
+
+def test_as_many_tokens_as_a_call_takes(gpu):
+    """2^21 rows: workspaces whose rows have a column for each of them."""
+    import hpfp8
+    tokens, hidden, vocab = 1 << 21, 8, 300
+    g = torch.Generator(device=gpu).manual_seed(10)
+    x = torch.randn((tokens, hidden), generator=g, device=gpu).to(torch.bfloat16)
+    w = torch.randn((vocab, hidden), generator=g, device=gpu).to(torch.bfloat16)
+    t = torch.randint(vocab, (tokens,), generator=g, device=gpu)
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = hpfp8.linear_cross_entropy(xg, wg, t, reduction="none")
+    go = torch.randn((tokens,), generator=g, device=gpu)
+    dx, dw = torch.autograd.grad(loss, (xg, wg), go)
+    rdw, b_dw = torch.zeros((vocab, hidden), dtype=torch.float64), torch.zeros((vocab, hidden), dtype=torch.float64)
+    for at in range(0, tokens, 1 << 18):
+        part = slice(at, at + (1 << 18))
+        rows, rdx, dw_part, b_rows, b_dx, b_part = (v.cpu() for v in reference(x[part], w, t[part], 0.0, go[part]))
+        within(loss[part].detach(), rows, b_rows)
+        within(dx[part], rdx, b_dx, H)
+        rdw += dw_part
+        b_dw += b_part * 8            # (the sum's roundings are bounded by the number of all tokens, here by that of a part's)
+    within(dw, rdw, b_dw, H)
+    with pytest.raises(ValueError, match="2\\^21 tokens"):
+        hpfp8.linear_cross_entropy(x.new_zeros(tokens + 1, hidden), w, t.new_zeros(tokens + 1))
+
+
+def test_a_weight_of_more_than_2_31_values(gpu):
+    import hpfp8
+    tokens, hidden, vocab = 70, 8192, 270000
+    g = torch.Generator(device=gpu).manual_seed(11)
+    x = torch.randn((tokens, hidden), generator=g, device=gpu).to(torch.bfloat16)
+    w = torch.empty((vocab, hidden), dtype=torch.bfloat16, device=gpu).normal_(0.0, 0.02, generator=g)
+    t = torch.randint(vocab, (tokens,), generator=g, device=gpu)
+    t[0] = vocab - 1
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = hpfp8.linear_cross_entropy(xg, wg, t, reduction="none")
+    dx, dw = torch.autograd.grad(loss.sum(), (xg, wg))
+    x64 = x.double()
+    l = torch.cat([x64 @ w[a:a + 30000].double().t() for a in range(0, vocab, 30000)], 1)
+    size = max(float((x64.abs() @ w[a:a + 30000].double().abs().t()).max()) for a in range(0, vocab, 30000))
+    off = (hidden / 32 + 32) * 2 * U * size             # a logit's error, as in `reference`
+    lse = torch.logsumexp(l, 1)
+    at = torch.arange(tokens, device=gpu)
+    within(loss.detach(), (lse - l[at, t]).cpu(), 2 * off + 64 * U + 8 * U * (lse.abs() + l.abs().amax(1)).cpu())
+    p = torch.exp(l - lse[:, None])
+    p[at, t] -= 1
+    b_p = H * p.abs() + (p.abs() + 2 * (torch.arange(vocab, device=gpu) == t[:, None])) * (4 * off + 64 * U + 4 * U * l.abs().amax())
+    for rows in (slice(0, 600), slice(vocab - 9000, vocab)):
+        want, bound = p[:, rows].t() @ x64, (b_p[:, rows].t() @ x64.abs()) * 1.01 + (tokens / 32 + 64) * 2 * U * (p[:, rows].abs().t() @ x64.abs())
+        within(dw[rows], want.cpu(), bound.cpu(), H)
+    want, bound = torch.zeros_like(x64), torch.zeros_like(x64)
+    for a in range(0, vocab, 30000):
+        part = w[a:a + 30000].double()
+        want += p[:, a:a + 30000] @ part
+        bound += b_p[:, a:a + 30000] @ part.abs() * 1.01 + (vocab / 32 + 64) * 2 * U * (p[:, a:a + 30000].abs() @ part.abs())
+    within(dx, want.cpu(), bound.cpu(), H)

@@ -132,3 +132,25 @@ def test_subclasses_are_handed_the_call():
     assert hpfp8.linear_cross_entropy(x, torch.zeros(3, 64), torch.zeros(4), reduction="sum") == "handed off"
     assert [f.__name__ for f, _, _ in Recorder.calls] == ["layer_norm", "activation", "linear_cross_entropy"]
     assert [k for _, _, k in Recorder.calls] == [{"keep_8bit": True}, {}, {"reduction": "sum"}]
+
+
+def test_sizes_that_31_bits_do_not_address(p):
+    """256 rows of a workspace that has a column for each token, or for each of a piece's, span less than 2 GiB."""
+    def forward(tokens):
+        return c("hpfp8_linear_cross_entropy_forward", None, 8, p, 8, p, tokens, 8, 10, -100, 0.0, 0, p, None, p, None, p, None, None, None)[0]
+    assert forward((1 << 21) + 1) == -2 and forward(1 << 21) == -1           # (the second for its null x)
+
+    def piece(width):
+        return c("hpfp8_linear_cross_entropy_piece", None, 8, None, p, 8, p, 4, 8, 1 << 24, 0, width, -100, 0.0, p, p, 0, None, p, p, None, 1, 0, None,
+                 0, 0, None)[0]
+    assert piece((1 << 21) + 1) == -2 and piece(1 << 21) == -1
+
+
+def test_codes_and_scales_of_other_types():
+    from hpfp8.kept import Fp8Activation
+    codes, scale_inv = torch.zeros(4, 64, dtype=torch.float8_e4m3fn), torch.ones(4, 1)
+    for wrong in ((codes.float(), scale_inv), (codes, scale_inv.double())):
+        with pytest.raises(TypeError):
+            Fp8Activation(*wrong, BF16).dequantize()
+    with pytest.raises(ValueError, match="must live on the GPU"):
+        Fp8Activation(codes, scale_inv, BF16).dequantize()
