@@ -4,17 +4,27 @@
 //   lse = log sum_v exp(l_v),  loss = lse - (1 - s) l_target - s mean_v(l_v)                 (s: label smoothing)
 //   dl  = c (exp(l - lse) - s / V - (1 - s) [v = target]),  dx = dl W,  dW = dl^T x          (c: the row's share of the loss's gradient)
 //
-// Forward: one product whose tiles leave, for each row and 128 columns, the largest logit and the sum of exp(l - largest) in fp32; a second
-// launch joins them.  Backward, a piece of the vocabulary at a time: the same product again, whose tiles leave dl rounded to bf16 (8
-// bits of a value that is a difference of probabilities: an error of 2^-9 relative in each of dx's and dW's summands, and half of that of the
-// result's own rounding in their sum), row-major and transposed, then both gradients in one launch.  Recomputing the logits is a quarter of the
+// Forward: one product whose tiles leave, for each row and 256 columns, the largest logit and the sum of exp(l - largest) in fp32; a second
+// launch joins them.  Backward, a piece of the vocabulary at a time: the same product again, whose tiles leave dl rounded to bf16 (at most
+// 2^-8 relative in each of dx's and dW's summands, with signs that differ: their sum is off by 1.9e-3 in the norm, of which the result's own
+// rounding is 1.7e-3), row-major and transposed, then both gradients in one launch.  Recomputing the logits is a quarter of the
 // step's products; keeping them would be tokens x vocab.
 //
-// All three are one kernel: c[m, n] = sum_k a[m, k] b[n, k] in bf16 with both operands contiguous along k, 256 x 256 tiles, 8 waves
-// of 64 x 128, v_mfma_f32_16x16x32_bf16.  64 values of k are 128 bytes of a row: LDS holds two such slabs of a and three of b, written
-// by direct loads (rows past the end read as zeros) with 16-byte chunks swizzled by row, so that fragments are read without bank conflicts.
-// The rows of a slab are permuted on their way into LDS so that a lane's sums are four neighbouring rows by eight neighbouring
-// columns: results leave as 16 bytes of a row, transposed ones as 8 bytes of a column, without a pass through LDS.
+// The products are c[m, n] = sum_k a[m, k] b[n, k] in bf16, v_mfma_f32_16x16x32_bf16, eight waves a workgroup.  64 values of k are 128
+// bytes of a row: such slabs go to LDS by direct loads (rows past the end read as zeros), their 16-byte chunks swizzled by row, so that fragments
+// are read without bank conflicts.  The rows of a slab are permuted on their way so that a lane's sums are four neighbouring rows by
+// eight neighbouring columns: results leave as 16 bytes of a row, transposed ones as 8 bytes of a column, without a pass through LDS.
+// x's gradient contracts over the weight's rows; it takes the weight as it lies, slabs of 64 rows of k, by transposing reads of LDS.
+//
+//   256 x 256 tiles (`ce_gemm_kernel`): 64 x 128 a wave; two slabs of a and three of b, one barrier per slab in the middle of its products.
+//   64 or 128 x 256 (`ce_gemm_ring_kernel`): few tokens, or few tiles; four or three slabs of both in a ring.
+//
+// Bound by the matrix units where there are many tokens, and there by the board's power: 4096 tokens, 7168, 131072: forward 5.54 ms, 1.39
+// PFLOP/s (hipBLASLt's product alone 1.46), backward 17.3 ms for three such products.  With few tokens by the weight's way from memory: 5 tokens
+// 300 us, 6.2 TB/s.  In between by tiles' starts and ends: 512 tokens, 4096, 32000: 112 us, 1.20 PFLOP/s, and 406 us for the backward.
+// One workgroup per compute unit with a list of tiles, whose first slabs arrive during the last ones of the tile before, was no
+// faster (1531 tokens, 2048, 50001: 288 / 284 us forward, 535 / 540 the gradients) and slower where there is much work (gradients of a piece of
+// 4096, 7168, 16384: 3072 / 2840 us): the next tile's first wait includes the results' stores, and fixed lists do not even out.
 #include <utility>
 
 #include "gemm_tile.h"

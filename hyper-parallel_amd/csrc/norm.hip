@@ -8,8 +8,11 @@
 // values around the wave's own mean, the waves joined by their counts), so an offset many times the spread costs nothing.
 // The workgroups stay for many rows: the weight's values are loaded once, the next row's loads are under way while a row is worked on,
 // and in the backward the two vectors' gradients grow in registers.  At the end a workgroup's teams are joined in LDS in their order and
-// its sums leave as one row of partial sums, at most 256 of them, which a second launch adds up in a fixed order: the same
-// bits every time, and for 4096 rows of 7168 14 MB of sums beside 176 MB of values.
+// its sums leave as one row of partial sums, at most 256 of them (512 where rows are short), which a second launch adds up in a fixed
+// order: the same bits every time, and for 4096 rows of 7168 14 MB of sums beside 176 MB of values.
+//
+// bf16: 4096 x 7168 forward 24 us, 4.9 TB/s, backward 36 + 4 us, 4.9 TB/s; 16384 x 7168 kept in 8 bits 114 us, 5.2 TB/s, and 112 + 4; 8 x 7168 4.4 us,
+// a launch's latency with one row's.
 #include <type_traits>
 
 #include "hpfp8_host.h"
@@ -68,7 +71,7 @@ __device__ __forceinline__ void load_vector8(const void* w, int type, int col, i
 // How a row's length and its chunks of eight values go together.
 enum Edge {
   kWhole = 0,      // the length is a multiple of 128
-   kOverlap = 1,    // any length from 8 on.  The last chunk is the row's last eight values, of which the first `dup` are the chunk's before it: every
+  kOverlap = 1,    // any length from 8 on.  The last chunk is the row's last eight values, of which the first `dup` are the chunk's before it: every
                    // load is a whole vector, so no load has to be waited for before its turn (loads of single values of the last chunk, merged
                    // with the others' vectors, waited in every row: forward of 65536 x 1030 217 us, where this takes 86)
   kSingle = 2,     // shorter rows: value by value

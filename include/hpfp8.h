@@ -543,7 +543,8 @@ int64_t hpfp8_layer_norm_partials(int64_t rows, int64_t cols);
  * target[tokens] is int64.
  *   loss[t] = lse(l_t) - (1 - smoothing) l_t[target] - smoothing mean(l_t);  0 where target is ignore_index, NaN where it is neither that
  *   nor in [0, vocab).  reduction 0: nothing more; 1: out[0] = their mean over the count[0] rows that are not ignored; 2: their sum.
- * Workspaces, fp32: stats[tokens, hpfp8_cross_entropy_parts(vocab), 2], sums (with smoothing only) half of that, target_logit[tokens].  lse[tokens] (may be NULL) is what the backward needs; out and count may be NULL with reduction 0. */
+ * Workspaces, fp32: stats[tokens, hpfp8_cross_entropy_parts(vocab), 2], sums (with smoothing only) half of that, target_logit[tokens].
+ * lse[tokens] (may be NULL) is what the backward needs; out and count may be NULL with reduction 0. */
 int64_t hpfp8_cross_entropy_parts(int64_t vocab);
 int hpfp8_linear_cross_entropy_forward(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t tokens,
                                        int64_t hidden, int64_t vocab, int64_t ignore_index, float smoothing, int reduction, float* stats,
@@ -553,12 +554,12 @@ int hpfp8_linear_cross_entropy_forward(const void* x, int64_t ld_x, const void* 
 int hpfp8_linear_cross_entropy_reduce(const float* loss, const int64_t* target, int64_t tokens, int64_t ignore_index, int reduction, float* out,
                                       float* count, hpfp8_stream_t stream);
 /* The backward's part of the vocabulary's columns [first, first + width): the gradient of the logits, rounded to bf16, and with it
- * dx (fp32 [splits, tokens, hidden], the parts of a sum; dx_add: added onto) and rows [first, first + width) of dw ([vocab, hidden], dw_type HPFP8_OUT_*; dw_add: added onto,
- * fp32 only).  Either may be NULL.  grad is the loss's gradient, one value with grad_stride 0 or one for each row; count as the
- * forward wrote it for reduction 1, otherwise NULL.  x_t is what hpfp8_linear_cross_entropy_rows_t makes of x, with row stride
+ * dx (fp32 [splits, tokens, hidden], the parts of a sum; dx_add: added onto) and rows [first, first + width) of dw ([vocab, hidden],
+ * dw_type HPFP8_OUT_*; dw_add: added onto, fp32 only).  Either may be NULL.  grad is the loss's gradient, one value
+ * with grad_stride 0 or one for each row; count as the forward wrote it for reduction 1, otherwise NULL.  x_t is what hpfp8_linear_cross_entropy_rows_t makes of x, with row stride
  * S(tokens), S(n) = hpfp8_cross_entropy_stride(n) (needed for dw).  Workspaces, bf16, with R(n) = n rounded up to 256: dl [R(tokens), S(width)],
- * dl_t [R(width), S(tokens)].  The piece's rows of w span less than 2 GiB and are at most 2^21.  splits: what hpfp8_cross_entropy_splits says for the widest piece, or another number from 1 to 32 up to its
- * slabs of 64 columns. */
+ * dl_t [R(width), S(tokens)].  The piece's rows of w span less than 2 GiB and are at most 2^21.  splits: what
+ * hpfp8_cross_entropy_splits says for the widest piece, or another number from 1 to 32 up to its slabs of 64 columns. */
 int64_t hpfp8_cross_entropy_stride(int64_t n);
 int64_t hpfp8_cross_entropy_splits(int64_t tokens, int64_t hidden, int64_t width, int with_dw);
 int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_t, const void* w, int64_t ld_w, const int64_t* target,
