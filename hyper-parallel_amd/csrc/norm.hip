@@ -146,7 +146,10 @@ __device__ __forceinline__ int team_of() {                    // (the same in a 
 template <typename E, int TPR, int NV, bool KEEP, int EDGE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV <= 2 && sizeof(typename E::raw) == 2 ? 4 : 2) void norm_forward_kernel(NormParams p) {
   using raw = typename E::raw;
-  constexpr int kTeams = (TPR < 256 ? 256 : TPR) / TPR, kWaves = TPR < 64 ? 1 : TPR / 64, kAhead = 2;
+  constexpr int kTeams = (TPR < 256 ? 256 : TPR) / TPR, kWaves = TPR < 64 ? 1 : TPR / 64;
+  // (four rows on their way where they fit the registers of two workgroups a compute unit: 16384 x 5120 70.6 / 65.9 us, x 7168 90.8 / 87.7, x 8192
+  // 93.5 / 91.9; with codes they do not, 118 us with two and 158 with four, nor with the masks of rows that are no multiple of 128)
+  constexpr int kAhead = TPR == 512 && NV == 2 && !KEEP && EDGE == kWhole && sizeof(raw) == 2 ? 4 : 2;
   __shared__ v4f parts[2][kTeams][kWaves];
   const int team = team_of<TPR>(), t = threadIdx.x % TPR, wave = __builtin_amdgcn_readfirstlane(t / 64);
   const int C = p.cols, groups = (C + kBlock - 1) / kBlock;
@@ -254,8 +257,9 @@ template <typename E, int TPR, int NV, bool KEEP, int EDGE>
 __global__ __launch_bounds__(kBackwardThreads) void norm_backward_kernel(NormParams p) {
   using raw = typename E::raw;
   constexpr int kTeams = kBackwardThreads / TPR, kWaves = TPR < 64 ? 1 : TPR / 64, kChunks = TPR * NV;
-  // (rows of over 8192 values: four steps' sums fill half of the registers, so one row is on its way instead of three and the weight is in LDS)
-  constexpr int kAhead = NV <= 2 ? 3 : 1;
+  // (rows on their way: teams of a wave and less have several anyway, 65536 x 1024 79 us with three and 80 with four; a wider row is in more hands, 16384 x
+  // 5120 99 / 95, x 7168 kept in 8 bits 120 / 115; of over 8192 values four steps' sums fill half of the registers: one row, the weight in LDS)
+  constexpr int kAhead = NV > 2 ? 1 : (TPR >= 256 && sizeof(raw) == 2 ? 4 : 3);
   constexpr bool kHoldWeight = NV <= 2;
   __shared__ v2f parts[2][kTeams][kWaves];
   __shared__ v4f joined[kTeams > 1 ? 2 * kChunks * 2 : 1];
