@@ -4,7 +4,7 @@
 //   lse = log sum_v exp(l_v),  loss = lse - (1 - s) l_target - s mean_v(l_v)                 (s: label smoothing)
 //   dl  = c (exp(l - lse) - s / V - (1 - s) [v = target]),  dx = dl W,  dW = dl^T x          (c: the row's share of the loss's gradient)
 //
-// Forward: one product whose tiles leave, for each row and 256 columns, the largest logit and the sum of exp(l - largest) in fp32; a second
+// Forward: one product whose tiles leave, for each row and their columns, the largest logit and the sum of exp(l - largest) in fp32; a second
 // launch joins them.  Backward, a piece of the vocabulary at a time: the same product again, whose tiles leave dl rounded to bf16 (at most
 // 2^-8 relative in each of dx's and dW's summands, with signs that differ: their sum is off by 1.9e-3 in the norm, of which the result's own
 // rounding is 1.7e-3), row-major and transposed, then both gradients in one launch.  Recomputing the logits is a quarter of the
@@ -17,7 +17,7 @@
 // x's gradient contracts over the weight's rows; it takes the weight as it lies, slabs of 64 rows of k, by transposing reads of LDS.
 //
 //   256 x 256 tiles (`ce_gemm_kernel`): 64 x 128 a wave; two slabs of a and three of b, one barrier per slab in the middle of its products.
-//   64 or 128 x 256 (`ce_gemm_ring_kernel`): few tokens, or few tiles; four or three slabs of both in a ring.
+//   64 or 128 x 256, 64 x 64 (`ce_gemm_ring_kernel`): few tokens, or few tiles; four, three or eight slabs of both in a ring.
 //
 // Bound by the matrix units where there are many tokens, and there by the board's power: 4096 tokens, 7168, 131072: forward 5.54 ms, 1.39
 // PFLOP/s (hipBLASLt's product alone 1.46), backward 17.3 ms for three such products.  With few tokens by the weight's way from memory: 5 tokens
@@ -117,8 +117,8 @@ __device__ __forceinline__ bf16x8 half_of(const v8i& f, int h) {
   return __builtin_bit_cast(bf16x8, v4i{f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]});
 }
 
-// The end of a tile of TM rows: lane (l16, g) of a wave has the sums of rows m + j and columns n + column_of(i, g, r).
-template <int EPI, int NS, int TM>
+// The end of a tile of TM x TN: lane (l16, g) of a wave has the sums of rows m + j and columns n + column_of(i, g, r).
+template <int EPI, int NS, int TM, int TN>
 __device__ __forceinline__ void finish_tile(const CeParams& p, const Product& q, v4f (&acc)[NS][4], int m0, int n0, int m, int n, int g, uint8_t* lds) {
   const bool cut = n + 16 * NS > q.N;          // columns behind the end (their sums are zeros)
   if constexpr (EPI == kStats) {
@@ -172,15 +172,15 @@ __device__ __forceinline__ void finish_tile(const CeParams& p, const Product& q,
     if ((int)threadIdx.x < TM && row < q.M) {
       float top = -INFINITY, sum = 0.f, all = 0.f;
 #pragma unroll
-      for (int k = 0; k < kTile / (16 * NS); ++k) top = fmaxf(top, each[k * TM + threadIdx.x].x);
+      for (int k = 0; k < TN / (16 * NS); ++k) top = fmaxf(top, each[k * TM + threadIdx.x].x);
       const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
-      for (int k = 0; k < kTile / (16 * NS); ++k) {
+      for (int k = 0; k < TN / (16 * NS); ++k) {
         const float4 v = each[k * TM + threadIdx.x];
         sum += v.y * __builtin_amdgcn_exp2f((v.x - from) * kLog2e);
         all += v.z;
       }
-      const int64_t at = (int64_t)row * p.parts + n0 / kTile;
+      const int64_t at = (int64_t)row * p.parts + n0 / TN;
       p.stats[at] = make_float2(top, sum);
       if (p.sums) p.sums[at] = all;
     }
@@ -421,7 +421,7 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
   v4f acc[8][4];
   if (EPI == kGrads && q.b_by_k) multiply<true>(q, m0, n0, lds, lane, wave, acc);
   else multiply<false>(q, m0, n0, lds, lane, wave, acc);
-  finish_tile<EPI, 8, kTile>(p, q, acc, m0, n0, m0 + (wave >> 1) * 64 + (lane & 15) * 4, n0 + (wave & 1) * 128, lane >> 4, lds);
+  finish_tile<EPI, 8, kTile, kTile>(p, q, acc, m0, n0, m0 + (wave >> 1) * 64 + (lane & 15) * 4, n0 + (wave & 1) * 128, lane >> 4, lds);
 }
 
 // All but this wave's last LEFT transfers have landed; then all waves'.
@@ -430,31 +430,35 @@ __device__ __forceinline__ void wait_and_meet() {
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
-// Fewer rows: tiles of 64 WM x 256, eight waves of 64 rows and 32 or 64 columns.  LDS is a ring of slabs of both operands, all but one of them on
-// their way while that one is multiplied; one barrier per slab.
-constexpr int ring_stages(int wm) { return wm == 1 ? 4 : 3; }
-template <int EPI, int WM>
+// Fewer rows: tiles of 64 WM rows and 256 columns, eight waves, or of 64 x 64, two waves (few columns too: more compute units have a tile).  A wave
+// has 64 rows and 32 or 64 columns.  LDS is a ring of slabs of both operands, on their way while another one is multiplied; one barrier per slab.
+constexpr int ring_stages(int wm, int wn) { return wn == 2 ? 8 : (wm == 1 ? 4 : 3); }
+constexpr int ring_columns(int wm, int wn) { return wn == 2 ? 64 : kTile; }
+template <int EPI, int WM, int WN>
 __device__ __forceinline__ void ring_tile(const CeParams& p, uint8_t* lds) {
-  constexpr int kRows = 64 * WM, WN = 8 / WM, NS = kTile / (16 * WN), kStages = ring_stages(WM), kStage = (kRows + kTile) * 128;
-  constexpr int kLeft = (kStages - 2) * (WM + 4);       // transfers of the slabs behind the next one
+  constexpr int kRows = 64 * WM, kCols = ring_columns(WM, WN), NS = kCols / (16 * WN), kStages = ring_stages(WM, WN), kStage = (kRows + kCols) * 128;
+  constexpr int kLoadsA = 8 / WN, kLoadsB = kCols / (8 * WM * WN);      // a wave's transfers of a slab
+  constexpr int kLeft = (kStages - 2) * (kLoadsA + kLoadsB);            // transfers of the slabs behind the next one
+  // a slab's fragments are read while the one before is multiplied, at the price of one slab fewer on its way (64 x 64 tiles, 16 tokens, 6592,
+  // 2859 41 / 35 us; 64 x 256 ones, 506, 6328, 5743 120 / 115)
+  constexpr bool kReadAhead = kStages > 3;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Product q = p.part[0];
   int tm, tn;
-  tile_at(tile_of_workgroup(blockIdx.x, q.tiles), (q.M + kRows - 1) / kRows, (q.N + kTile - 1) / kTile, tm, tn);
-  const int m0 = tm * kRows, n0 = tn * kTile, slabs = (q.K + kSlab - 1) / kSlab, whole = q.K / kSlab;
+  tile_at(tile_of_workgroup(blockIdx.x, q.tiles), (q.M + kRows - 1) / kRows, (q.N + kCols - 1) / kCols, tm, tn);
+  const int m0 = tm * kRows, n0 = tn * kCols, slabs = (q.K + kSlab - 1) / kSlab, whole = q.K / kSlab;
   const __amdgpu_buffer_rsrc_t rsrc_a = resource(q.a + (int64_t)m0 * q.lda, q.M - m0, q.lda, q.K);
   const __amdgpu_buffer_rsrc_t rsrc_b = resource(q.b + (int64_t)n0 * q.ldb, q.N - n0, q.ldb, q.K);
-  // a wave's transfers of a slab: WM of a, four of b
-  uint32_t a_off[WM], b_off[4], past[2];
+  uint32_t a_off[kLoadsA], b_off[kLoadsB], past[2];
   auto chunk_of = [&](int r) { return (lane & 7) ^ row_swizzle(r); };
 #pragma unroll
-  for (int i = 0; i < WM; ++i) {
-    const int r = (wave * WM + i) * 8 + (lane >> 3);
+  for (int i = 0; i < kLoadsA; ++i) {
+    const int r = (wave * kLoadsA + i) * 8 + (lane >> 3);
     a_off[i] = (uint32_t)((r & ~63) + (r & 15) * 4 + ((r >> 4) & 3)) * (uint32_t)q.lda + chunk_of(r) * 16;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = (wave * 4 + i) * 8 + (lane >> 3);
+  for (int i = 0; i < kLoadsB; ++i) {
+    const int r = (wave * kLoadsB + i) * 8 + (lane >> 3);
     b_off[i] = (uint32_t)((r & ~(16 * NS - 1)) + column_of((r >> 4) & (NS - 1), (r >> 2) & 3, r & 3)) * (uint32_t)q.ldb + chunk_of(r) * 16;
     // (a chunk behind the end of k is read from beyond the resource, as zeros; the swizzle has two patterns, by whether r / 8 is odd)
     if (i < 2) past[i] = chunk_of(r) * 8 >= q.K % kSlab ? 0x80000000u : 0u;
@@ -464,12 +468,12 @@ __device__ __forceinline__ void ring_tile(const CeParams& p, uint8_t* lds) {
     const int s = slab < slabs ? slab : slabs - 1;        // (behind the last slab the last one again: those are never used)
     const bool cut = s >= whole;
 #pragma unroll
-    for (int i = 0; i < WM; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_a, (lds_ptr_t)(to + (wave * WM + i) * 1024), 16, a_off[i] + (cut ? past[(wave * WM + i) & 1] : 0u),
+    for (int i = 0; i < kLoadsA; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_a, (lds_ptr_t)(to + (wave * kLoadsA + i) * 1024), 16, a_off[i] + (cut ? past[(wave * kLoadsA + i) & 1] : 0u),
                                                s * 128, 0, 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_b, (lds_ptr_t)(to + kRows * 128 + (wave * 4 + i) * 1024), 16, b_off[i] + (cut ? past[i & 1] : 0u),
+    for (int i = 0; i < kLoadsB; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_b, (lds_ptr_t)(to + kRows * 128 + (wave * kLoadsB + i) * 1024), 16, b_off[i] + (cut ? past[i & 1] : 0u),
                                                s * 128, 0, 0);
   };
   const int wm = wave / WN, wn = wave % WN, l16 = lane & 15, g = lane >> 4;
@@ -482,31 +486,53 @@ __device__ __forceinline__ void ring_tile(const CeParams& p, uint8_t* lds) {
     for (int j = 0; j < 4; ++j) acc[i][j] = zero;
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) load(s);
-  for (int s = 0; s < slabs; ++s) {
-    // slab s is there (those after it may be under way), and the one before has been read by all
-    wait_and_meet<kLeft>();
-    load(s + kStages - 1);
+  v8i wf[kReadAhead ? 2 : 1][NS], xf[kReadAhead ? 2 : 1][4];
+  auto read = [&](v8i (&w)[NS], v8i (&x)[4], int s) {
     const uint8_t* const a = lds + s % kStages * kStage + wm * 64 * 128;
     const uint8_t* const b = lds + s % kStages * kStage + kRows * 128 + wn * 16 * NS * 128;
-    v8i wf[NS], xf[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) xf[j] = frag_read(a + j * 16 * 128, frag_lo, frag_hi);
+    for (int j = 0; j < 4; ++j) x[j] = frag_read(a + j * 16 * 128, frag_lo, frag_hi);
 #pragma unroll
-    for (int i = 0; i < NS; ++i) wf[i] = frag_read(b + i * 16 * 128, frag_lo, frag_hi);
+    for (int i = 0; i < NS; ++i) w[i] = frag_read(b + i * 16 * 128, frag_lo, frag_hi);
+  };
+  auto multiply_slab = [&](const v8i (&w)[NS], const v8i (&x)[4]) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(half_of(wf[i], h), half_of(xf[j], h), acc[i][j], 0, 0, 0);
+        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(half_of(w[i], h), half_of(x[j], h), acc[i][j], 0, 0, 0);
+  };
+  if constexpr (kReadAhead) {
+    wait_and_meet<kLeft>();
+    read(wf[0], xf[0], 0);
+    auto step = [&](int s, int u) {
+      // slab s + 1 is there, and slab s - 1 has been multiplied by all: its place takes the next transfers
+      wait_and_meet<kLeft - kLoadsA - kLoadsB>();
+      load(s + kStages - 1);
+      read(wf[u ^ 1], xf[u ^ 1], s + 1);
+      multiply_slab(wf[u], xf[u]);
+    };
+    for (int s = 0; s < slabs; s += 2) {
+      step(s, 0);
+      if (s + 1 < slabs) step(s + 1, 1);
+    }
+  } else {
+    for (int s = 0; s < slabs; ++s) {
+      // slab s is there (those after it may be under way), and the one before has been read by all
+      wait_and_meet<kLeft>();
+      load(s + kStages - 1);
+      read(wf[0], xf[0], s);
+      multiply_slab(wf[0], xf[0]);
+    }
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);          // vmcnt(0): the last transfers write to this workgroup's LDS
-  finish_tile<EPI, NS, kRows>(p, q, acc, m0, n0, m0 + wm * 64 + l16 * 4, n0 + wn * 16 * NS, g, lds);
+  finish_tile<EPI, NS, kRows, kCols>(p, q, acc, m0, n0, m0 + wm * 64 + l16 * 4, n0 + wn * 16 * NS, g, lds);
 }
-template <int EPI, int WM>
-__global__ __launch_bounds__(512) void ce_gemm_ring_kernel(CeParams p) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[ring_stages(WM) * (64 * WM + kTile) * 128];
-  ring_tile<EPI, WM>(p, lds);
+template <int EPI, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void ce_gemm_ring_kernel(CeParams p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[ring_stages(WM, WN) * (64 * WM + ring_columns(WM, WN)) * 128];
+  ring_tile<EPI, WM, WN>(p, lds);
 }
 
 // ---- joins the forward's partial results, a wave for each row
@@ -629,7 +655,7 @@ __global__ __launch_bounds__(256) void ce_round_kernel(const float* __restrict__
 int64_t up(int64_t n, int64_t to);
 int64_t stride_of(int64_t n) { return up(n, kTile) + kSlab; }
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
-int tiles_of(int64_t m, int64_t n) { return (int)((m + kTile - 1) / kTile * ((n + kTile - 1) / kTile)); }
+int64_t tiles_of(int64_t m, int64_t n, int rows = kTile, int cols = kTile) { return (m + rows - 1) / rows * ((n + cols - 1) / cols); }
 
 int check(int64_t tokens, int64_t hidden, int64_t vocab, int64_t ld_x, int64_t ld_w) {
   HPFP8_REQUIRE(tokens >= 0 && hidden > 0 && vocab > 0, HPFP8_ERR_SHAPE, "tokens=%lld hidden=%lld vocab=%lld", (long long)tokens, (long long)hidden, (long long)vocab);
@@ -653,31 +679,37 @@ Product product(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t 
   q.c = c;
   q.ldc = ldc;
   q.store = store;
-  q.tiles = tiles_of(M, N);
+  q.tiles = (int)tiles_of(M, N);
   q.splits = 1;
   return q;
 }
 
-// The tile whose rounds on the compute units are the shortest: a slab takes about 1.25, 0.9 and 0.7 us in a tile of 256, 128 and 64 rows, and a
-// tile's start and end 5, 4 and 4.  us of a forward with 256 / 128 / 64: 5 tokens, 7168, 131072 368 / 313 / 308, 65 384 / 317 / 385, 256
-// 438 / 541 / 744; 128, 2048, 32000 58 / 47 / 43, 256 61 / 47 / 67, 512 63 / 83 / 117; 300, 4096, 16000 96 / 66 / 92; 1000, 1024, 8000 32 / 25 / 31;
-// 512, 896, 5165 28 / 22 / 16; 1531, 2048, 50001 289 / 357 / 437.
+// The tile whose rounds on the compute units are the shortest: a slab takes about 1.25, 0.9, 0.7 and 0.35 us in a tile of 256, 128 and
+// 64 rows and in one of 64 x 64, and a tile's start and end 5, 4, 4 and 3.  us of a forward with 256 x 256 / 128 x 256 / 64 x 256 / 64 x 64:
+//   16 tokens, 6592, 2859    132 /  90 /  73 /  35        5, 7168, 131072     358 / 312 / 309 / 335
+//   20, 5176, 13482          121 / 104 / 102 /  41        506, 6328, 5743     172 / 136 / 115 / 149
+//   1000, 7000, 1000         136 / 107 /  86 /  42        1014, 6784, 5994    137 / 100 / 135 / 198
+//   64, 7168, 16384          149 / 104 /  99 /  52        153, 1744, 87170    110 / 119 / 145 / 189
+struct Form {
+  int rows, cols;        // of a tile
+};
+Form form_of(int64_t tokens, int64_t hidden, int64_t vocab) {
+  const int64_t slabs = (hidden + kSlab - 1) / kSlab;
+  auto cost = [&](int rows, int cols, int slab, int ends) { return (tiles_of(tokens, vocab, rows, cols) + 255) / 256 * (slab * slabs + ends); };
+  const int64_t c256 = cost(256, 256, 125, 500), c128 = cost(128, 256, 90, 400), c64 = cost(64, 256, 70, 400);
+  const int64_t narrow = cost(64, 64, 35, 300);
+  if (narrow < c64 && narrow < c128 && narrow < c256) return {64, 64};
+  if (c64 < c128 && c64 < c256) return {64, kTile};
+  return {c128 < c256 ? 128 : 256, kTile};
+}
 template <int EPI>
-void launch_logits(CeParams& p, hipStream_t s) {
+void launch_logits(CeParams& p, const Form& form, hipStream_t s) {
   Product& q = p.part[0];
-  const int64_t slabs = (q.K + kSlab - 1) / kSlab;
-  auto tiles = [&](int rows) { return (int64_t)((q.M + rows - 1) / rows) * ((q.N + kTile - 1) / kTile); };
-  auto cost = [&](int rows, int slab, int ends) { return (tiles(rows) + 255) / 256 * (slab * slabs + ends); };
-  const int64_t c256 = cost(256, 125, 500), c128 = cost(128, 90, 400), c64 = cost(64, 70, 400);
-  if (c64 < c128 && c64 < c256) {
-    q.tiles = (int)tiles(64);
-    ce_gemm_ring_kernel<EPI, 1><<<q.tiles, 512, 0, s>>>(p);
-  } else if (c128 < c256) {
-    q.tiles = (int)tiles(128);
-    ce_gemm_ring_kernel<EPI, 2><<<q.tiles, 512, 0, s>>>(p);
-  } else {
-    ce_gemm_kernel<EPI><<<q.tiles, 512, 0, s>>>(p);
-  }
+  q.tiles = (int)tiles_of(q.M, q.N, form.rows, form.cols);
+  if (form.cols == 64) ce_gemm_ring_kernel<EPI, 1, 2><<<q.tiles, 128, 0, s>>>(p);
+  else if (form.rows == 64) ce_gemm_ring_kernel<EPI, 1, 8><<<q.tiles, 512, 0, s>>>(p);
+  else if (form.rows == 128) ce_gemm_ring_kernel<EPI, 2, 4><<<q.tiles, 512, 0, s>>>(p);
+  else ce_gemm_kernel<EPI><<<q.tiles, 512, 0, s>>>(p);
 }
 
 // The gradients' launch: dx's product contracts over the whole piece and has few tiles, so with few tokens a few of its tiles would still be at
@@ -715,7 +747,11 @@ using namespace hpfp8;
 
 extern "C" {
 
-int64_t hpfp8_cross_entropy_parts(int64_t vocab) { return vocab > 0 ? (vocab + kTile - 1) / kTile : 0; }
+int64_t hpfp8_cross_entropy_parts(int64_t tokens, int64_t hidden, int64_t vocab) {
+  if (tokens <= 0 || hidden <= 0 || vocab <= 0) return 0;
+  const int cols = form_of(tokens, hidden, vocab).cols;
+  return (vocab + cols - 1) / cols;
+}
 int64_t hpfp8_cross_entropy_splits(int64_t tokens, int64_t hidden, int64_t width, int with_dw) {
   if (tokens <= 0 || hidden <= 0 || width <= 0) return 1;
   const int64_t slabs = (width + kSlab - 1) / kSlab;
@@ -751,8 +787,9 @@ int hpfp8_linear_cross_entropy_forward(const void* x, int64_t ld_x, const void* 
     p.sums = smoothing != 0.f ? sums : nullptr;
     p.target_logit = target_logit;
     p.target = target;
-    p.parts = (int)hpfp8_cross_entropy_parts(vocab);
-    launch_logits<kStats>(p, s);
+    const Form form = form_of(tokens, hidden, vocab);
+    p.parts = (int)((vocab + form.cols - 1) / form.cols);
+    launch_logits<kStats>(p, form, s);
     int rc = check_launch("linear_cross_entropy_forward");
     if (rc != HPFP8_OK) return rc;
     ce_join_kernel<<<(unsigned)((tokens + 3) / 4), 256, 0, s>>>(p.stats, p.sums, target_logit, target, p.parts, tokens, ignore_index, vocab, smoothing,
@@ -809,7 +846,7 @@ int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_
   p.dl = (uint16_t*)dl;
   p.ld_dl = cols_padded;
   p.dl_t = (uint16_t*)dl_t;
-  launch_logits<kDlogits>(p, s);
+  launch_logits<kDlogits>(p, form_of(tokens, hidden, width), s);
   int rc = check_launch("linear_cross_entropy_piece");
   if (rc != HPFP8_OK) return rc;
   CeParams g = {};

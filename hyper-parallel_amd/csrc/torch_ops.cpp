@@ -1293,7 +1293,7 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n_ar
     pybind11::gil_scoped_release free;
     at::NoGradGuard no_grad;
     const at::TensorOptions floats = x->options().requires_grad(false).dtype(at::kFloat);
-    const int64_t parts = lib.hpfp8_cross_entropy_parts(vocab);
+    const int64_t parts = lib.hpfp8_cross_entropy_parts(tokens, hidden, vocab);
     const at::Tensor stats = at::empty({tokens, parts, 2}, floats), own = at::empty({tokens}, floats);
     at::Tensor sums, out, loss = at::empty(target->sizes(), floats);
     if (made.smoothing != 0) sums = at::empty({tokens, parts}, floats);

@@ -97,7 +97,7 @@ SIZE_FUNCTIONS = {
     "hpfp8_gemm_few_rows": [_i64],
     "hpfp8_linear_few_rows": [_i64, _i64],
     "hpfp8_layer_norm_partials": [_i64, _i64],
-    "hpfp8_cross_entropy_parts": [_i64],
+    "hpfp8_cross_entropy_parts": [_i64, _i64, _i64],
     "hpfp8_cross_entropy_splits": [_i64, _i64, _i64, _int],
     "hpfp8_cross_entropy_stride": [_i64],
 }

@@ -30,9 +30,10 @@ def _forward(x, weight, target, ignore_index, reduction, smoothing, want_lse):
     tokens, vocab = x.shape[0], weight.shape[0]
     f32 = dict(dtype=torch.float32, device=x.device)
     most = min(tokens, _FORWARD_ROWS)
-    parts = lib.hpfp8_cross_entropy_parts(vocab)
-    stats = torch.empty((most, parts, 2), **f32)
-    sums = torch.empty((most, parts), **f32) if smoothing else None
+    # (the last tokens may take other tiles than the others)
+    parts = max((n * lib.hpfp8_cross_entropy_parts(n, x.shape[1], vocab) for n in (most, tokens % _FORWARD_ROWS)))
+    stats = torch.empty((parts, 2), **f32)
+    sums = torch.empty((parts,), **f32) if smoothing else None
     own = torch.empty((most,), **f32)
     loss = torch.empty((tokens,), **f32)
     lse = torch.empty((tokens,), **f32) if want_lse else None

@@ -543,9 +543,9 @@ int64_t hpfp8_layer_norm_partials(int64_t rows, int64_t cols);
  * target[tokens] is int64.
  *   loss[t] = lse(l_t) - (1 - smoothing) l_t[target] - smoothing mean(l_t);  0 where target is ignore_index, NaN where it is neither that
  *   nor in [0, vocab).  reduction 0: nothing more; 1: out[0] = their mean over the count[0] rows that are not ignored; 2: their sum.
- * Workspaces, fp32: stats[tokens, hpfp8_cross_entropy_parts(vocab), 2], sums (with smoothing only) half of that, target_logit[tokens].
+ * Workspaces, fp32: stats[tokens, hpfp8_cross_entropy_parts(tokens, hidden, vocab), 2], sums (with smoothing only) half of that, target_logit[tokens].
  * lse[tokens] (may be NULL) is what the backward needs; out and count may be NULL with reduction 0. */
-int64_t hpfp8_cross_entropy_parts(int64_t vocab);
+int64_t hpfp8_cross_entropy_parts(int64_t tokens, int64_t hidden, int64_t vocab);
 int hpfp8_linear_cross_entropy_forward(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t tokens,
                                        int64_t hidden, int64_t vocab, int64_t ignore_index, float smoothing, int reduction, float* stats,
                                        float* sums, float* target_logit, float* lse, float* loss, float* out, float* count,

@@ -345,3 +345,41 @@ def test_a_weight_of_more_than_2_31_values(gpu):
         want += p[:, a:a + 30000] @ part
         bound += b_p[:, a:a + 30000] @ part.abs() * 1.01 + (vocab / 32 + 64) * 2 * U * (p[:, a:a + 30000].abs() @ part.abs())
     within(dx, want.cpu(), bound.cpu(), H)
+
+
+@pytest.mark.parametrize("tokens,hidden,vocab", [(300, 520, 10000), (1000, 1024, 8010), (16, 1000, 2859), (200, 328, 3000)])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+def test_every_shape_of_tiles(gpu, tokens, hidden, vocab, smoothing):
+    """64 x 256, 128 x 256 and, the last two, 64 x 64; the largest are above.  Each row's loss, and both gradients."""
+    import hpfp8
+    from hpfp8 import _lib
+    cols = -(-vocab // _lib.load().hpfp8_cross_entropy_parts(tokens, hidden, vocab))
+    assert (cols <= 64) == (vocab < 8000)
+    x, w, t = (v.to(gpu) for v in make(tokens, hidden, vocab, 12))
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = hpfp8.linear_cross_entropy(xg, wg, t, label_smoothing=smoothing, reduction="none")
+    go = torch.randn((tokens,), generator=torch.Generator().manual_seed(13)).to(gpu)
+    dx, dw = torch.autograd.grad(loss, (xg, wg), go)
+    rows, rdx, rdw, b_rows, b_dx, b_dw = (v.cpu() for v in reference(x, w, t, smoothing, go))
+    within(loss.detach(), rows, b_rows)
+    within(dx, rdx, b_dx, H)
+    within(dw, rdw, b_dw, H)
+
+
+def test_the_last_tokens_may_take_other_tiles(gpu, monkeypatch):
+    """A forward in several launches, whose last one writes more parts for fewer rows."""
+    import hpfp8
+    from hpfp8 import _lib
+    from hpfp8 import loss as module
+    parts = _lib.load().hpfp8_cross_entropy_parts
+    assert parts(512, 512, 8000) < parts(68, 512, 8000)
+    x, w, t = (v.to(gpu) for v in make(580, 512, 8000, 14))
+    want = hpfp8.linear_cross_entropy(x, w, t, reduction="none", label_smoothing=0.1).cpu().double()
+    monkeypatch.setattr(module, "_FORWARD_ROWS", 512)
+    hook = []
+    monkeypatch.setattr(module.ops, "_gpu", lambda x: hook.append(x) or False)        # (the Python form, which is the one that takes several)
+    got = hpfp8.linear_cross_entropy(x, w, t, reduction="none", label_smoothing=0.1)
+    rows, b_rows = (v.cpu() for v in (lambda r: (r[0], r[3]))(reference(x, w, t, 0.1, torch.ones(580, device=gpu))))
+    assert hook
+    within(got, rows, b_rows)
+    within(want, rows, b_rows)

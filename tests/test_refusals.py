@@ -154,3 +154,13 @@ def test_codes_and_scales_of_other_types():
             Fp8Activation(*wrong, BF16).dequantize()
     with pytest.raises(ValueError, match="must live on the GPU"):
         Fp8Activation(codes, scale_inv, BF16).dequantize()
+
+
+def test_parts_of_the_forward():
+    from hpfp8 import _lib
+    parts = _lib.load().hpfp8_cross_entropy_parts
+    assert parts(0, 64, 100) == 0 and parts(4, 64, 0) == 0
+    assert parts(4, 64, 100) == 2 and parts(4096, 7168, 131072) == 512
+    for tokens in (1, 64, 65, 300, 5000):
+        for vocab in (1, 64, 257, 5000, 131072):
+            assert parts(tokens, 512, vocab) in (-(-vocab // 64), -(-vocab // 256))
