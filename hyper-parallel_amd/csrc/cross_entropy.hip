@@ -17,14 +17,14 @@
 // x's gradient contracts over the weight's rows; it takes the weight as it lies, slabs of 64 rows of k, by transposing reads of LDS.
 //
 //   256 x 256 tiles (`ce_gemm_kernel`): 64 x 128 a wave; two slabs of a and three of b, one barrier per slab in the middle of its products.
-//   64 or 128 x 256, 64 x 64 (`ce_gemm_ring_kernel`): few tokens, or few tiles; four, three or eight slabs of both in a ring.
+//   64 or 128 x 64, 128 or 256 (`ce_gemm_ring_kernel`): few tokens, or few tiles; three to eight slabs of both in a ring.
 //
 // Bound by the matrix units where there are many tokens, and there by the board's power: 4096 tokens, 7168, 131072: forward 5.54 ms, 1.39
 // PFLOP/s (hipBLASLt's product alone 1.46), backward 17.3 ms for three such products.  With few tokens by the weight's way from memory: 5 tokens
 // 300 us, 6.2 TB/s.  In between by tiles' starts and ends: 512 tokens, 4096, 32000: 112 us, 1.20 PFLOP/s, and 406 us for the backward.
 // One workgroup per compute unit with a list of tiles, whose first slabs arrive during the last ones of the tile before, was no
 // faster (1531 tokens, 2048, 50001: 288 / 284 us forward, 535 / 540 the gradients) and slower where there is much work (gradients of a piece of
-// 4096, 7168, 16384: 3072 / 2840 us): the next tile's first wait includes the results' stores, and fixed lists do not even out.
+// 4096, 7168, 16384: 3.07 / 2.84 ms): the next tile's first wait includes the results' stores, and fixed lists do not even out.
 #include <utility>
 
 #include "gemm_tile.h"
@@ -430,13 +430,12 @@ __device__ __forceinline__ void wait_and_meet() {
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
-// Fewer rows: tiles of 64 WM rows and 256 columns, eight waves, or of 64 x 64, two waves (few columns too: more compute units have a tile).  A wave
-// has 64 rows and 32 or 64 columns.  LDS is a ring of slabs of both operands, on their way while another one is multiplied; one barrier per slab.
-constexpr int ring_stages(int wm, int wn) { return wn == 2 ? 8 : (wm == 1 ? 4 : 3); }
-constexpr int ring_columns(int wm, int wn) { return wn == 2 ? 64 : kTile; }
-template <int EPI, int WM, int WN>
+// Smaller tiles: 64 WM rows and COLS columns in WM x WN waves, each with 64 rows and 32 or 64 columns, so that few tokens or a small vocabulary
+// give more compute units a tile.  LDS is a ring of slabs of both operands, on their way while another one is multiplied; one barrier per slab.
+constexpr int ring_stages(int rows, int cols) { return cols == 64 ? 8 : cols == 128 ? (rows == 64 ? 6 : 5) : (rows == 64 ? 4 : 3); }
+template <int EPI, int WM, int WN, int COLS>
 __device__ __forceinline__ void ring_tile(const CeParams& p, uint8_t* lds) {
-  constexpr int kRows = 64 * WM, kCols = ring_columns(WM, WN), NS = kCols / (16 * WN), kStages = ring_stages(WM, WN), kStage = (kRows + kCols) * 128;
+  constexpr int kRows = 64 * WM, kCols = COLS, NS = kCols / (16 * WN), kStages = ring_stages(kRows, kCols), kStage = (kRows + kCols) * 128;
   constexpr int kLoadsA = 8 / WN, kLoadsB = kCols / (8 * WM * WN);      // a wave's transfers of a slab
   constexpr int kLeft = (kStages - 2) * (kLoadsA + kLoadsB);            // transfers of the slabs behind the next one
   // a slab's fragments are read while the one before is multiplied, at the price of one slab fewer on its way (64 x 64 tiles, 16 tokens, 6592,
@@ -529,10 +528,10 @@ __device__ __forceinline__ void ring_tile(const CeParams& p, uint8_t* lds) {
   __builtin_amdgcn_s_waitcnt(0x0F70);          // vmcnt(0): the last transfers write to this workgroup's LDS
   finish_tile<EPI, NS, kRows, kCols>(p, q, acc, m0, n0, m0 + wm * 64 + l16 * 4, n0 + wn * 16 * NS, g, lds);
 }
-template <int EPI, int WM, int WN>
+template <int EPI, int WM, int WN, int COLS>
 __global__ __launch_bounds__(64 * WM * WN) void ce_gemm_ring_kernel(CeParams p) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[ring_stages(WM, WN) * (64 * WM + ring_columns(WM, WN)) * 128];
-  ring_tile<EPI, WM, WN>(p, lds);
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[ring_stages(64 * WM, COLS) * (64 * WM + COLS) * 128];
+  ring_tile<EPI, WM, WN, COLS>(p, lds);
 }
 
 // ---- joins the forward's partial results, a wave for each row
@@ -684,31 +683,39 @@ Product product(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t 
   return q;
 }
 
-// The tile whose rounds on the compute units are the shortest: a slab takes about 1.25, 0.9, 0.7 and 0.35 us in a tile of 256, 128 and
-// 64 rows and in one of 64 x 64, and a tile's start and end 5, 4, 4 and 3.  us of a forward with 256 x 256 / 128 x 256 / 64 x 256 / 64 x 64:
-//   16 tokens, 6592, 2859    132 /  90 /  73 /  35        5, 7168, 131072     358 / 312 / 309 / 335
-//   20, 5176, 13482          121 / 104 / 102 /  41        506, 6328, 5743     172 / 136 / 115 / 149
-//   1000, 7000, 1000         136 / 107 /  86 /  42        1014, 6784, 5994    137 / 100 / 135 / 198
-//   64, 7168, 16384          149 / 104 /  99 /  52        153, 1744, 87170    110 / 119 / 145 / 189
+// The tile whose rounds on the compute units are the shortest, from what a slab of it takes and its start and end.  us of a forward with
+//                          256 x 256 / 128 x 256 / 64 x 256 / 128 x 128 / 64 x 128 / 64 x 64
+//   16 tokens, 6592, 2859    133 /  89 /  74 /  50 /  45 /  35        506, 6328, 5743     173 / 136 / 115 /  98 / 130 / 151
+//   24, 1472, 33651           44 /  31 /  29 /  39 /  38 /  39        1014, 6784, 5994    138 / 100 / 132 / 118 / 134 / 200
+//   100, 2048, 16000          53 /  39 /  34 /  29 /  26 /  35        3715, 1616, 4098     53 /  67 /  97 /  85 / 126 / 184
+//   128, 4096, 32000         101 /  80 /  73 /  67 /  81 / 107        96, 4096, 131072    223 / 187 / 226 / 197 / 260 / 354
 struct Form {
   int rows, cols;        // of a tile
+  int slab, ends;        // 10 ns
 };
+constexpr Form kForms[] = {{256, 256, 125, 500}, {128, 256, 90, 400}, {64, 256, 70, 400}, {128, 128, 55, 350}, {64, 128, 38, 350}, {64, 64, 30, 300}};
 Form form_of(int64_t tokens, int64_t hidden, int64_t vocab) {
   const int64_t slabs = (hidden + kSlab - 1) / kSlab;
-  auto cost = [&](int rows, int cols, int slab, int ends) { return (tiles_of(tokens, vocab, rows, cols) + 255) / 256 * (slab * slabs + ends); };
-  const int64_t c256 = cost(256, 256, 125, 500), c128 = cost(128, 256, 90, 400), c64 = cost(64, 256, 70, 400);
-  const int64_t narrow = cost(64, 64, 35, 300);
-  if (narrow < c64 && narrow < c128 && narrow < c256) return {64, 64};
-  if (c64 < c128 && c64 < c256) return {64, kTile};
-  return {c128 < c256 ? 128 : 256, kTile};
+  Form best = kForms[0];
+  int64_t least = INT64_MAX;
+  for (const Form& f : kForms) {
+    const int64_t cost = (tiles_of(tokens, vocab, f.rows, f.cols) + 255) / 256 * (f.slab * slabs + f.ends);
+    if (cost < least) {
+      least = cost;
+      best = f;
+    }
+  }
+  return best;
 }
 template <int EPI>
 void launch_logits(CeParams& p, const Form& form, hipStream_t s) {
   Product& q = p.part[0];
   q.tiles = (int)tiles_of(q.M, q.N, form.rows, form.cols);
-  if (form.cols == 64) ce_gemm_ring_kernel<EPI, 1, 2><<<q.tiles, 128, 0, s>>>(p);
-  else if (form.rows == 64) ce_gemm_ring_kernel<EPI, 1, 8><<<q.tiles, 512, 0, s>>>(p);
-  else if (form.rows == 128) ce_gemm_ring_kernel<EPI, 2, 4><<<q.tiles, 512, 0, s>>>(p);
+  if (form.cols == 64) ce_gemm_ring_kernel<EPI, 1, 2, 64><<<q.tiles, 128, 0, s>>>(p);
+  else if (form.cols == 128 && form.rows == 64) ce_gemm_ring_kernel<EPI, 1, 4, 128><<<q.tiles, 256, 0, s>>>(p);
+  else if (form.cols == 128) ce_gemm_ring_kernel<EPI, 2, 4, 128><<<q.tiles, 512, 0, s>>>(p);
+  else if (form.rows == 64) ce_gemm_ring_kernel<EPI, 1, 8, 256><<<q.tiles, 512, 0, s>>>(p);
+  else if (form.rows == 128) ce_gemm_ring_kernel<EPI, 2, 4, 256><<<q.tiles, 512, 0, s>>>(p);
   else ce_gemm_kernel<EPI><<<q.tiles, 512, 0, s>>>(p);
 }
 

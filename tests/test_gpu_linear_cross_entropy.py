@@ -347,10 +347,10 @@ def test_a_weight_of_more_than_2_31_values(gpu):
     within(dx, want.cpu(), bound.cpu(), H)
 
 
-@pytest.mark.parametrize("tokens,hidden,vocab", [(300, 520, 10000), (1000, 1024, 8010), (16, 1000, 2859), (200, 328, 3000)])
+@pytest.mark.parametrize("tokens,hidden,vocab", [(300, 520, 10000), (1000, 1024, 8010), (24, 1472, 33651), (100, 1032, 15900), (16, 1000, 2859), (200, 328, 3000)])
 @pytest.mark.parametrize("smoothing", [0.0, 0.1])
 def test_every_shape_of_tiles(gpu, tokens, hidden, vocab, smoothing):
-    """64 x 256, 128 x 256 and, the last two, 64 x 64; the largest are above.  Each row's loss, and both gradients."""
+    """128 x 128, 128 x 256, 64 x 256, 64 x 128 and, the last two, 64 x 64; the largest are above.  Each row's loss, and both gradients."""
     import hpfp8
     from hpfp8 import _lib
     cols = -(-vocab // _lib.load().hpfp8_cross_entropy_parts(tokens, hidden, vocab))

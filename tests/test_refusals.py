@@ -163,4 +163,4 @@ def test_parts_of_the_forward():
     assert parts(4, 64, 100) == 2 and parts(4096, 7168, 131072) == 512
     for tokens in (1, 64, 65, 300, 5000):
         for vocab in (1, 64, 257, 5000, 131072):
-            assert parts(tokens, 512, vocab) in (-(-vocab // 64), -(-vocab // 256))
+            assert parts(tokens, 512, vocab) in [-(-vocab // cols) for cols in (64, 128, 256)]
