@@ -19,7 +19,7 @@
 //   256 x 256 tiles (`ce_gemm_kernel`): 64 x 128 a wave; two slabs of a and three of b, one barrier per slab in the middle of its products.
 //   64 or 128 x 64, 128 or 256 (`ce_gemm_ring_kernel`): few tokens, or few tiles; three to eight slabs of both in a ring.
 //
-// Bound by the matrix units where there are many tokens, and there by the board's power: 4096 tokens, 7168, 131072: forward 5.54 ms, 1.39
+// Bound by the matrix units where there are many tokens, and there by the board's power: 4096 tokens, 7168, 131072: forward 5.35 to 5.54 ms, 1.39 to 1.44
 // PFLOP/s (hipBLASLt's product alone 1.46), backward 17.3 ms for three such products.  With few tokens by the weight's way from memory: 5 tokens
 // 300 us, 6.2 TB/s.  In between by tiles' starts and ends: 512 tokens, 4096, 32000: 112 us, 1.20 PFLOP/s, and 406 us for the backward.
 // One workgroup per compute unit with a list of tiles, whose first slabs arrive during the last ones of the tile before, was no
