@@ -424,10 +424,11 @@ __global__ __launch_bounds__(512) void ce_gemm_kernel(CeParams p) {
   finish_tile<EPI, 8, kTile, kTile>(p, q, acc, m0, n0, m0 + (wave >> 1) * 64 + (lane & 15) * 4, n0 + (wave & 1) * 128, lane >> 4, lds);
 }
 
-// All but this wave's last LEFT transfers have landed; then all waves'.
+// All but this wave's last LEFT transfers have landed, and what it has read of LDS is in its registers (behind the barrier a transfer of any wave may
+// take the place of what was read); then all waves'.
 template <int LEFT>
 __device__ __forceinline__ void wait_and_meet() {
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
 // Smaller tiles: 64 WM rows and COLS columns in WM x WN waves, each with 64 rows and 32 or 64 columns, so that few tokens or a small vocabulary
