@@ -63,6 +63,20 @@ def _pieces(tokens: int, stride: int, vocab: int, budget: int):
     return [(at, min(width, vocab - at)) for at in range(0, vocab, width)]
 
 
+def _main_grad_of(param):
+    """param.main_grad (None: there is none yet), which the kernels are about to add onto.  Looked at by the call and again by its backward:
+    what is there then may be another tensor."""
+    main_grad = getattr(param, "main_grad", None)
+    if main_grad is not None:
+        if main_grad.dtype != torch.float32 or main_grad.shape != param.shape or not main_grad.is_contiguous():
+            raise ValueError("weight.main_grad must be a contiguous float32 tensor of the weight's shape")
+        if main_grad.device != param.device:
+            raise ValueError(f"weight.main_grad lives on {main_grad.device}, the weight on {param.device}")
+        if main_grad.data_ptr() % 16:
+            raise ValueError("weight.main_grad must start at a multiple of 16 bytes")
+    return main_grad
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction, smoothing, main_grad_of):
@@ -85,7 +99,7 @@ def _backward(grad_out, x, weight, target, lse, count, ignore_index, reduction, 
     x2, w = _rows(x), _rows(weight)
     tokens, hidden = x2.shape
     vocab = w.shape[0]
-    main_grad = None if param is None else getattr(param, "main_grad", None)
+    main_grad = None if param is None else _main_grad_of(param)
     if tokens == 0:
         if need_dw and param is not None and main_grad is None:
             param.main_grad = torch.zeros(weight.shape, dtype=torch.float32, device=w.device)
@@ -144,8 +158,8 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
     A target that is neither ``ignore_index`` nor in [0, vocab) makes its token's loss and gradients NaN.  In the backward the logits are
     computed again, a piece of the vocabulary at a time, their gradient rounded to bfloat16 for the products of both gradients.
 
-    ``apply_grad_on_fp32_main_grad`` as in `fp8_linear`: the weight's gradient goes to ``weight.main_grad`` (fp32), created by the first
-    backward and added onto by every later one."""
+    ``apply_grad_on_fp32_main_grad`` as in `fp8_linear`: the weight's gradient goes to ``weight.main_grad`` (fp32, on the weight's
+    device, 16-byte aligned), created by the first backward and added onto by every later one."""
     if torch.overrides.has_torch_function((input, weight, target)):
         return _hand_off(linear_cross_entropy, (input, weight, target), (input, weight, target),
                          dict(ignore_index=ignore_index, reduction=reduction, label_smoothing=label_smoothing,
@@ -177,9 +191,7 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
     if target.numel() > 1 << 21:
         raise ValueError(f"at most 2^21 tokens in a call, got {target.numel()}")
     if apply_grad_on_fp32_main_grad:
-        mg = getattr(weight, "main_grad", None)
-        if mg is not None and (mg.dtype != torch.float32 or mg.shape != weight.shape or not mg.is_contiguous()):
-            raise ValueError("weight.main_grad must be a contiguous float32 tensor of the weight's shape")
+        _main_grad_of(weight)
     flat = target.reshape(-1).contiguous()
     r = _REDUCTIONS[reduction]
     if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad):

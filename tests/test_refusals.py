@@ -164,3 +164,23 @@ def test_parts_of_the_forward():
     for tokens in (1, 64, 65, 300, 5000):
         for vocab in (1, 64, 257, 5000, 131072):
             assert parts(tokens, 512, vocab) in [-(-vocab // cols) for cols in (64, 128, 256)]
+
+
+@pytest.mark.parametrize("wrong", ["device", "start", "shape", "type", "strides"])
+def test_a_main_grad_that_the_kernels_cannot_add_onto(wrong, monkeypatch):
+    """Refused by the call, and by the backward if it was put there in between: before anything is launched."""
+    import hpfp8
+    from hpfp8 import _lib, loss, ops
+    launched = []
+    monkeypatch.setattr(_lib, "call", lambda name, *args: launched.append(name))
+    monkeypatch.setattr(ops, "_check_device", lambda *args: None)
+    monkeypatch.setattr(ops, "_stream", lambda: None)
+    w = torch.nn.Parameter(torch.zeros(10, 64, dtype=BF16))
+    w.main_grad = {"device": torch.zeros(10, 64, device="meta"), "start": torch.zeros(643)[3:].view(10, 64), "shape": torch.zeros(64, 10),
+                   "type": torch.zeros(10, 64, dtype=BF16), "strides": torch.zeros(64, 10).t()}[wrong]
+    x, t = torch.zeros(4, 64, dtype=BF16, requires_grad=True), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(ValueError, match="main_grad"):
+        hpfp8.linear_cross_entropy(x, w, t, apply_grad_on_fp32_main_grad=True)
+    with pytest.raises(ValueError, match="main_grad"):
+        loss._backward(torch.ones(()), x.detach(), w.detach(), t, torch.zeros(4), torch.ones(()), -100, 1, 0.0, True, True, w)
+    assert not launched
