@@ -38,6 +38,15 @@ def _as_rows(x: torch.Tensor, cols: int) -> torch.Tensor:
     return x if cols == 1 or x.stride(1) == 1 else x.contiguous()
 
 
+def _check_saved(*saved) -> None:
+    """(tensor, dtype, number of elements) of what a backward is about to give to its kernels.  It is what the forward saved unless a hook on
+    saved tensors handed back something else; that is refused, as the kernels would read beyond it, or memory that is not the GPU's."""
+    for t, dtype, numel in saved:
+        if t.dtype != dtype or t.numel() != numel:
+            raise ValueError(f"a saved tensor of {numel} values of {dtype} came back as {tuple(t.shape)} of {t.dtype}")
+        ops._check_device(t, "a saved tensor")
+
+
 def _groups(cols: int) -> int:
     return (cols + ops.BLOCK - 1) // ops.BLOCK
 
@@ -165,11 +174,15 @@ class _Activation(torch.autograd.Function):
 
 def _backward(grad_out, kept, scale_inv, keep, kind, shape):
     """dx.  kept: x, or its codes with their scales."""
-    cols = shape[-1] // (2 if kind == 3 else 1)
+    shape = torch.Size(shape)
+    halves = 2 if kind == 3 else 1
+    cols = shape[-1] // halves
     x2 = None
-    if keep:                # (hooks on saved tensors may have handed them back with other strides)
-        kept, scale_inv = kept.contiguous(), scale_inv.contiguous()
+    if keep:
+        _check_saved((kept, ops.FP8, shape.numel()), (scale_inv, torch.float32, shape[:-1].numel() * halves * _groups(cols)))
+        kept, scale_inv = kept.contiguous(), scale_inv.contiguous()      # (with other strides, which hooks on saved tensors may give them)
     else:
+        _check_saved((kept, grad_out.dtype, shape.numel()))
         x2 = _as_rows(kept, shape[-1])
     go = grad_out.contiguous()
     dx = torch.empty(shape, dtype=go.dtype, device=go.device)

@@ -6,6 +6,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
+from .kept import _check_saved
 from .linear import _hand_off
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -95,10 +96,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
 def _backward(grad_out, x, weight, target, lse, count, ignore_index, reduction, smoothing, need_dx, need_dw, param=None):
     """(dx, dw); with ``param`` the weight's gradient goes to param.main_grad."""
+    tokens, (vocab, hidden) = grad_out.numel() if reduction == 0 else target.numel(), weight.shape
+    _check_saved((x, torch.bfloat16, tokens * hidden), (weight, torch.bfloat16, vocab * hidden), (target, torch.int64, tokens),
+                 (lse, torch.float32, tokens), *(((count, torch.float32, 1),) if count is not None else ()))
     target, lse = target.contiguous(), lse.contiguous()      # (hooks on saved tensors may have handed them back with other strides)
     x2, w = _rows(x), _rows(weight)
-    tokens, hidden = x2.shape
-    vocab = w.shape[0]
     main_grad = None if param is None else _main_grad_of(param)
     if tokens == 0:
         if need_dw and param is not None and main_grad is None:

@@ -8,7 +8,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .kept import _TYPES, _as_rows, _check_rows, _groups
+from .kept import _TYPES, _as_rows, _check_rows, _check_saved, _groups
 from .linear import _hand_off
 
 MAX_WIDTH = 16384
@@ -62,6 +62,9 @@ def _backward(grad_out, kept, other, rstd, weight, keep, cols, shape, dtype, vec
     """(dx, dw, db).  kept, other: x and its mean, or the codes and scales of its normalised values; vector: the shape of weight and bias."""
     go = _as_rows(grad_out, cols)
     rows = go.shape[0]
+    f32 = torch.float32
+    _check_saved(*(((kept, ops.FP8, rows * cols), (other, f32, rows * _groups(cols))) if keep else ((kept, _OF_CODE[dtype], rows * cols), (other, f32, rows))),
+                 (rstd, f32, rows), *(((weight, _OF_CODE[vector_dtype], cols),) if weight is not None else ()))
     # (hooks on saved tensors may have handed them back with other strides)
     kept, other, rstd = kept.contiguous() if keep else kept, other.contiguous(), rstd.contiguous()
     dx = torch.empty(shape, dtype=_OF_CODE[dtype], device=go.device)

@@ -184,3 +184,34 @@ def test_a_main_grad_that_the_kernels_cannot_add_onto(wrong, monkeypatch):
     with pytest.raises(ValueError, match="main_grad"):
         loss._backward(torch.ones(()), x.detach(), w.detach(), t, torch.zeros(4), torch.ones(()), -100, 1, 0.0, True, True, w)
     assert not launched
+
+
+def test_saved_tensors_that_a_hook_handed_back_as_something_else(monkeypatch):
+    """Left on the CPU, shortened or of another type: refused before anything is launched."""
+    from hpfp8 import _lib, kept, loss, norm, ops
+    launched = []
+    monkeypatch.setattr(_lib, "call", lambda name, *args: launched.append(name))
+    monkeypatch.setattr(ops, "_stream", lambda: None)
+    x, go, codes, one = torch.zeros(4, 64, dtype=BF16), torch.zeros(4, 64, dtype=BF16), torch.zeros(4, 64, dtype=torch.float8_e4m3fn), torch.zeros(4, 1)
+    t, row = torch.zeros(4, dtype=torch.int64), torch.zeros(4)
+    code = kept._TYPES[BF16]
+    calls = {kept._backward: [(go, x, None, False, 0, x.shape), (go, codes, one, True, 0, x.shape)],
+             norm._backward: [(go, x, row, row, x[0], False, 64, x.shape, code, (64,), code, True, True),
+                              (go, codes, one, row, x[0], True, 64, x.shape, code, (64,), code, True, True)],
+             loss._backward: [(torch.ones(()), x, x, t, row, torch.ones(()), -100, 1, 0.0, True, True)]}
+    for function, each in calls.items():
+        for args in each:
+            with pytest.raises(ValueError, match="must live on the GPU"):
+                function(*args)
+    monkeypatch.setattr(ops, "_check_device", lambda *args: None)
+    for function, each in calls.items():
+        for args in each:
+            saved = [i for i, a in enumerate(args) if i > 0 and isinstance(a, torch.Tensor)]
+            for i in saved:
+                wrongs = [args[i].to(torch.float64)]
+                if not (function is loss._backward and i == 2):              # (the vocabulary is the weight's own)
+                    wrongs.append(args[i][:-1] if args[i].dim() else args[i].expand(2))
+                for wrong in wrongs:
+                    with pytest.raises(ValueError, match="came back as"):
+                        function(*args[:i], wrong, *args[i + 1:])
+    assert not launched
