@@ -22,7 +22,9 @@ _PIECE_ELEMENTS = 0x3FFFF000
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x[..., C] as [rows, C] the kernels can read: unit stride along a row, rows 16 bytes apart and aligned."""
     x = x.reshape(-1, x.shape[-1])
-    return x if x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.shape[1] <= x.stride(0) < 1 << 21 and x.data_ptr() % 16 == 0 else x.contiguous()
+    if x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.shape[1] <= x.stride(0) < 1 << 21 and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)     # (contiguous() gives back a contiguous one that starts between two vectors)
 
 
 def _forward(x, weight, target, ignore_index, reduction, smoothing, want_lse):

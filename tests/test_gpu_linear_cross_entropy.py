@@ -383,3 +383,26 @@ def test_the_last_tokens_may_take_other_tiles(gpu, monkeypatch):
     assert hook
     within(got, rows, b_rows)
     within(want, rows, b_rows)
+
+
+@pytest.mark.parametrize("at", [1, 3, 4])
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_contiguous_tensors_that_start_between_two_vectors(gpu, at, tokens):
+    """Views in a flat buffer: input and weight, and what hooks on saved tensors hand back."""
+    import hpfp8
+    x, w, t = (v.to(gpu) for v in make(tokens, 64, 300, 15))
+
+    def view(v):
+        out = torch.empty(v.numel() + at, dtype=v.dtype, device=gpu)[at:].view(v.shape).copy_(v)
+        assert out.is_contiguous() and out.data_ptr() % 16
+        return out
+
+    def step(x, w, hooks=None):
+        a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+        with hooks or torch.enable_grad():
+            loss = hpfp8.linear_cross_entropy(a, b, t)
+        return (loss.detach(),) + torch.autograd.grad(loss, (a, b))
+    want = step(x, w)
+    hooks = torch.autograd.graph.saved_tensors_hooks(lambda v: v, lambda v: view(v) if v.dtype == torch.bfloat16 else v)
+    for got in (step(view(x), w), step(x, view(w)), step(view(x), view(w)), step(x, w, hooks)):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))

@@ -215,3 +215,14 @@ def test_saved_tensors_that_a_hook_handed_back_as_something_else(monkeypatch):
                     with pytest.raises(ValueError, match="came back as"):
                         function(*args[:i], wrong, *args[i + 1:])
     assert not launched
+
+
+def test_rows_that_start_between_two_vectors_or_have_odd_strides_are_copied():
+    """Contiguous tensors among them: views in a flat buffer, a single row cut out of columns."""
+    from hpfp8.loss import _rows
+    flat = torch.arange(1 + 5 * 64).to(BF16)
+    for x in (flat[1:].view(5, 64), flat[1:65].view(1, 64), flat[:64].view(64, 1).t(), flat[:320].view(64, 5).t(), flat[:64].expand(5, 64),
+              flat[:63 * 5].view(5, 63)[:, 3:59]):
+        rows = _rows(x)
+        assert torch.equal(rows, x) and rows.data_ptr() % 16 == 0 and rows.stride(1) == 1 and rows.stride(0) % 8 == 0 and rows.stride(0) >= rows.shape[1]
+    assert _rows(flat[:320].view(5, 64)).data_ptr() == flat.data_ptr()
