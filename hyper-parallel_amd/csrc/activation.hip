@@ -103,8 +103,8 @@ __device__ __forceinline__ Place place(const Grid& g) {
   return p;
 }
 
-// ---- quantize and read back
-template <typename E>
+// ---- quantize and read back.  SPECIAL: infinities and NaN come back as they were and leave their group's other values alone
+template <typename E, bool SPECIAL>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename E::raw* __restrict__ x, int64_t ld, Grid g, uint8_t* __restrict__ q,
                                                             float* __restrict__ scale_inv) {
   const Place p = place(g);
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename E::ra
       const int64_t r = first + u * p.step;
       float f[8], s;
       unpack8<E>(v[u], f);
-      const uint2 c = encode_group(f, s);
+      const uint2 c = encode_group<SPECIAL>(f, s);
       if (r < g.rows && p.left > 0) {
         store_codes8(q + r * g.cols + p.col, p.left, c);
         if ((threadIdx.x & 15) == 0) scale_inv[r * g.groups + p.group] = s;
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename E::ra
   }
 }
 
-template <typename E>
+template <typename E, bool SPECIAL>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scale_inv, Grid g,
                                                               typename E::raw* __restrict__ x) {
   const Place p = place(g);
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(const uint8_t* __r
       const int64_t r = first + u * p.step;
       if (r >= g.rows || p.left <= 0) break;
       float f[8];
-      decode8(c[u], s[u], f);
+      decode8<SPECIAL>(c[u], s[u], f);
       store8<E>(x + r * g.cols + p.col, p.left, f);
     }
   }
@@ -298,14 +298,8 @@ void by_kind(int kind, F&& f) {
 
 bool at_element(const void* p, int dtype) { return ((uintptr_t)p & (dtype == HPFP8_OUT_F32 ? 3 : 1)) == 0; }
 
-}  // namespace
-}  // namespace hpfp8
-
-using namespace hpfp8;
-
-extern "C" {
-
-int hpfp8_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, void* q, float* scale_inv, hpfp8_stream_t stream) {
+template <bool SPECIAL>
+int quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, void* q, float* scale_inv, hpfp8_stream_t stream) {
   HPFP8_REQUIRE(dtype >= 0 && dtype <= 2, HPFP8_ERR_ARG, "unknown element type %d", dtype);
   HPFP8_REQUIRE(rows >= 0 && cols >= 0 && ld >= 0, HPFP8_ERR_SHAPE, "negative size (rows=%lld cols=%lld ld=%lld)", (long long)rows, (long long)cols, (long long)ld);
   if (rows == 0 || cols == 0) return HPFP8_OK;
@@ -316,12 +310,13 @@ int hpfp8_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, in
   HPFP8_REQUIRE(shape(rows, cols, g, grid), HPFP8_ERR_SHAPE, "a row of %lld values is too long", (long long)cols);
   const int rc = by_type(dtype, [&](auto e) {
     using E = decltype(e);
-    quantize_rows_kernel<E><<<grid, 256, 0, (hipStream_t)stream>>>((const typename E::raw*)x, ld, g, (uint8_t*)q, scale_inv);
+    quantize_rows_kernel<E, SPECIAL><<<grid, 256, 0, (hipStream_t)stream>>>((const typename E::raw*)x, ld, g, (uint8_t*)q, scale_inv);
   });
   return rc != HPFP8_OK ? rc : check_launch("quantize_rows");
 }
 
-int hpfp8_dequantize_rows(const void* q, const float* scale_inv, int64_t rows, int64_t cols, void* x, int dtype, hpfp8_stream_t stream) {
+template <bool SPECIAL>
+int dequantize_rows(const void* q, const float* scale_inv, int64_t rows, int64_t cols, void* x, int dtype, hpfp8_stream_t stream) {
   HPFP8_REQUIRE(dtype >= 0 && dtype <= 2, HPFP8_ERR_ARG, "unknown element type %d", dtype);
   HPFP8_REQUIRE(rows >= 0 && cols >= 0, HPFP8_ERR_SHAPE, "negative size (rows=%lld cols=%lld)", (long long)rows, (long long)cols);
   if (rows == 0 || cols == 0) return HPFP8_OK;
@@ -332,9 +327,29 @@ int hpfp8_dequantize_rows(const void* q, const float* scale_inv, int64_t rows, i
   HPFP8_REQUIRE(shape(rows, cols, g, grid), HPFP8_ERR_SHAPE, "a row of %lld values is too long", (long long)cols);
   const int rc = by_type(dtype, [&](auto e) {
     using E = decltype(e);
-    dequantize_rows_kernel<E><<<grid, 256, 0, (hipStream_t)stream>>>((const uint8_t*)q, scale_inv, g, (typename E::raw*)x);
+    dequantize_rows_kernel<E, SPECIAL><<<grid, 256, 0, (hipStream_t)stream>>>((const uint8_t*)q, scale_inv, g, (typename E::raw*)x);
   });
   return rc != HPFP8_OK ? rc : check_launch("dequantize_rows");
+}
+
+}  // namespace
+}  // namespace hpfp8
+
+using namespace hpfp8;
+
+extern "C" {
+
+int hpfp8_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, void* q, float* scale_inv, hpfp8_stream_t stream) {
+  return quantize_rows<false>(x, dtype, rows, cols, ld, q, scale_inv, stream);
+}
+int hpfp8_quantize_saved_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, void* q, float* scale_inv, hpfp8_stream_t stream) {
+  return quantize_rows<true>(x, dtype, rows, cols, ld, q, scale_inv, stream);
+}
+int hpfp8_dequantize_rows(const void* q, const float* scale_inv, int64_t rows, int64_t cols, void* x, int dtype, hpfp8_stream_t stream) {
+  return dequantize_rows<false>(q, scale_inv, rows, cols, x, dtype, stream);
+}
+int hpfp8_dequantize_saved_rows(const void* q, const float* scale_inv, int64_t rows, int64_t cols, void* x, int dtype, hpfp8_stream_t stream) {
+  return dequantize_rows<true>(q, scale_inv, rows, cols, x, dtype, stream);
 }
 
 int hpfp8_activation_forward(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, int kind, void* y, void* q, float* scale_inv,

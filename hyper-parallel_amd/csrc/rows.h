@@ -164,13 +164,28 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, int n, uint2 c) {
     if (i < n) p[i] = (uint8_t)(w >> (8 * i));
 }
 
+// E4M3 has one code of each sign for what is no number.  Where infinities have to come back as they were, those two are +inf and -inf,
+// and NaN is the code of -0 (a value that rounds to -0 gets the code of 0).
+constexpr uint32_t kCodeInf = 0x7F, kCodeNan = 0x80;
+__device__ __forceinline__ uint32_t no_negative_zero(uint32_t w) {         // (a byte's upper bit stays where its others are not all 0)
+  return w & (0x7F7F7F7Fu | ((w & 0x7F7F7F7Fu) + 0x7F7F7F7Fu));
+}
+
 // The group's 16 lanes' eight values each -> their codes; scale_inv is the same in all 16.  |v| orders like its bits, and a NaN
 // above everything: the group's scale and codes are NaN then.  (No clamp: |v * (448 / amax)| <= 448 (1 + 2^-23), which rounds to 448.)
+// SPECIAL: infinities and NaN have codes of their own, and the scale is that of the finite values.
+template <bool SPECIAL = false>
 __device__ __forceinline__ uint2 encode_group(const float v[8], float& scale_inv) {
   // (the maximum that keeps NaN: one instruction for two values more)
   float top = __builtin_elementwise_maximum(__builtin_fabsf(v[0]), __builtin_fabsf(v[1]));
 #pragma unroll
   for (int i = 2; i < 8; i += 2) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, __builtin_fabsf(v[i])), __builtin_fabsf(v[i + 1]));
+  const bool special = SPECIAL && !(top < INFINITY);                        // (few lanes take this way)
+  if (special) {
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = __builtin_fabsf(v[i]) < INFINITY ? fmaxf(top, __builtin_fabsf(v[i])) : top;
+  }
   const uint32_t m = row16_max_u32(__float_as_uint(top) & 0x7FFFFFFFu);
   float scale;
   scales_from_amax(__uint_as_float(m), scale, scale_inv);
@@ -181,8 +196,22 @@ __device__ __forceinline__ uint2 encode_group(const float v[8], float& scale_inv
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * scale, v[7] * scale, hi, true);
   c.x = (uint32_t)lo;
   c.y = (uint32_t)hi;
+  if constexpr (SPECIAL) {
+    c.x = no_negative_zero(c.x);
+    c.y = no_negative_zero(c.y);
+    if (special) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (__builtin_fabsf(v[i]) < INFINITY) continue;
+        const uint32_t code = v[i] != v[i] ? kCodeNan : (v[i] < 0.f ? kCodeInf | 0x80u : kCodeInf);
+        uint32_t& w = i < 4 ? c.x : c.y;
+        w = (w & ~(0xFFu << 8 * (i % 4))) | code << 8 * (i % 4);
+      }
+    }
+  }
   return c;
 }
+template <bool SPECIAL = false>
 __device__ __forceinline__ void decode8(uint2 c, float scale_inv, float v[8]) {
   const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, true);
   const v2f d = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.y, false), e = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.y, true);
@@ -194,6 +223,18 @@ __device__ __forceinline__ void decode8(uint2 c, float scale_inv, float v[8]) {
   v[5] = d.y * scale_inv;
   v[6] = e.x * scale_inv;
   v[7] = e.y * scale_inv;
+  if constexpr (SPECIAL) {
+    // a byte whose low seven bits are all 1 is an infinity; one that no_negative_zero changes is a NaN
+    const uint32_t inf = (((c.x & 0x7F7F7F7Fu) + 0x01010101u) | ((c.y & 0x7F7F7F7Fu) + 0x01010101u)) & 0x80808080u;
+    if (inf || no_negative_zero(c.x) != c.x || no_negative_zero(c.y) != c.y) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t code = (i < 4 ? c.x : c.y) >> 8 * (i % 4) & 0xFFu;
+        if ((code & 0x7Fu) == kCodeInf) v[i] = code & 0x80u ? -INFINITY : INFINITY;
+        if (code == kCodeNan) v[i] = NAN;
+      }
+    }
+  }
 }
 
 }  // namespace hpfp8

@@ -40,7 +40,7 @@ constexpr int64_t kBlock = 128;
   X(hpfp8_quantize_per_tensor_sync_bf16) X(hpfp8_gemm_few_rows) X(hpfp8_linear_few_rows) X(hpfp8_linear_few_rows_bf16) X(hpfp8_linear_backward) X(hpfp8_quantize_two_per_tensor_t_bf16) X(hpfp8_gemm_blockwise_swiglu_quantize) X(hpfp8_swiglu_quantize_1x128_bf16) \
   X(hpfp8_swiglu_quantize_1x128_pow2_bf16) X(hpfp8_swiglu_quantize_1x128_fast_bf16) X(hpfp8_gemm_grouped_blockwise) \
   X(hpfp8_bucket_pack_quantize_bf16) X(hpfp8_bucket_unpack_dequantize_bf16) \
-  X(hpfp8_quantize_rows) X(hpfp8_dequantize_rows) X(hpfp8_activation_forward) X(hpfp8_activation_backward) X(hpfp8_layer_norm_forward) \
+  X(hpfp8_quantize_rows) X(hpfp8_dequantize_rows) X(hpfp8_quantize_saved_rows) X(hpfp8_dequantize_saved_rows) X(hpfp8_activation_forward) X(hpfp8_activation_backward) X(hpfp8_layer_norm_forward) \
   X(hpfp8_layer_norm_backward) X(hpfp8_layer_norm_partials) X(hpfp8_cross_entropy_parts) X(hpfp8_cross_entropy_stride) X(hpfp8_cross_entropy_splits) \
   X(hpfp8_linear_cross_entropy_forward) X(hpfp8_linear_cross_entropy_piece) X(hpfp8_linear_cross_entropy_rows_t) X(hpfp8_linear_cross_entropy_round)
 struct Library {
@@ -1147,11 +1147,12 @@ PyObject* activation(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// (x, device, stream) -> (codes, scale_inv)
+// (x, saved, device, stream) -> (codes, scale_inv); saved: with codes for infinities and NaN
 PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  expect(n_args, 3);
+  expect(n_args, 4);
   const Where at_ = where(args, n_args);
+  const bool saved = truth(args[1]);
   const at::Tensor* x;
   if (!rows_of_values(args[0], at_.device, x) || x->numel() == 0 || !no_modes()) Py_RETURN_NONE;
   at::Tensor codes, scales;
@@ -1165,18 +1166,20 @@ PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     codes = at::empty(shape, options.dtype(at::kFloat8_e4m3fn));
     shape.back() = groups_of(cols);
     scales = at::empty(shape, options.dtype(at::kFloat));
-    HPFP8_CALL(call, hpfp8_quantize_rows, x->data_ptr(), type_code(x->scalar_type()), x->numel() / cols, cols, cols, codes.data_ptr(), f32(scales),
-               at_.stream);
+    const int type = type_code(x->scalar_type());
+    if (saved) HPFP8_CALL(call, hpfp8_quantize_saved_rows, x->data_ptr(), type, x->numel() / cols, cols, cols, codes.data_ptr(), f32(scales), at_.stream);
+    else HPFP8_CALL(call, hpfp8_quantize_rows, x->data_ptr(), type, x->numel() / cols, cols, cols, codes.data_ptr(), f32(scales), at_.stream);
   }
   return call.ok() ? tuple_of(std::move(codes), std::move(scales)) : failed(call);
   END_HANDLE_TH_ERRORS
 }
 
-// (codes, scale_inv, element type, device, stream) -> x
+// (codes, scale_inv, element type, saved, device, stream) -> x
 PyObject* dequantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  expect(n_args, 5);
+  expect(n_args, 6);
   const Where at_ = where(args, n_args);
+  const bool saved = truth(args[3]);
   const int type = (int)PyLong_AsLongLong(args[2]);
   if (PyErr_Occurred()) throw python_error();
   const at::Tensor *codes, *scales;
@@ -1191,7 +1194,8 @@ PyObject* dequantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     at::NoGradGuard no_grad;
     x = at::empty(codes->sizes(), codes->options().dtype(type_of(type)));
     const int64_t cols = codes->size(-1);
-    HPFP8_CALL(call, hpfp8_dequantize_rows, codes->data_ptr(), f32(*scales), codes->numel() / cols, cols, x.data_ptr(), type, at_.stream);
+    if (saved) HPFP8_CALL(call, hpfp8_dequantize_saved_rows, codes->data_ptr(), f32(*scales), codes->numel() / cols, cols, x.data_ptr(), type, at_.stream);
+    else HPFP8_CALL(call, hpfp8_dequantize_rows, codes->data_ptr(), f32(*scales), codes->numel() / cols, cols, x.data_ptr(), type, at_.stream);
   }
   return call.ok() ? THPVariable_Wrap(std::move(x)) : failed(call);
   END_HANDLE_TH_ERRORS

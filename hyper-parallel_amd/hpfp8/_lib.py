@@ -79,6 +79,8 @@ SIGNATURES = {
     "hpfp8_grouped_zero_unrouted_rows_bf16": [_vp, _i64, _vp, _int, _i64, _i64, _vp],
     "hpfp8_quantize_rows": [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp],
     "hpfp8_dequantize_rows": [_vp, _vp, _i64, _i64, _vp, _int, _vp],
+    "hpfp8_quantize_saved_rows": [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp],
+    "hpfp8_dequantize_saved_rows": [_vp, _vp, _i64, _i64, _vp, _int, _vp],
     "hpfp8_activation_forward": [_vp, _int, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp],
     "hpfp8_activation_backward": [_vp, _vp, _i64, _vp, _vp, _int, _i64, _i64, _int, _vp, _vp],
     "hpfp8_linear_cross_entropy_forward": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _f32, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],

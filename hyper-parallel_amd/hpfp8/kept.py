@@ -51,6 +51,47 @@ def _groups(cols: int) -> int:
     return (cols + ops.BLOCK - 1) // ops.BLOCK
 
 
+def _dequantize(codes, scale_inv, dtype, saved: bool):
+    if ops._gpu(codes):
+        device = ops._device()
+        x = ops._native.dequantize_rows(codes, scale_inv, _TYPES[dtype], saved, device, ops._raw_stream(device))
+        if x is not None:
+            return x
+    if codes.dtype != ops.FP8 or scale_inv.dtype != torch.float32:
+        raise TypeError(f"codes and scale_inv must be float8_e4m3fn and float32, got {codes.dtype} and {scale_inv.dtype}")
+    ops._check_device(codes, "codes")
+    ops._check_device(scale_inv, "scale_inv")
+    if codes.dim() < 1:
+        raise ValueError("codes must have at least one dimension")
+    cols = codes.shape[-1]
+    if cols and scale_inv.numel() != codes.numel() // cols * _groups(cols):
+        raise ValueError(f"codes {tuple(codes.shape)} have a scale for each 128 values of a row, not {tuple(scale_inv.shape)}")
+    codes, scale_inv = codes.contiguous(), scale_inv.contiguous()         # (a slice of what was made, say)
+    x = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    _lib.call("hpfp8_dequantize_saved_rows" if saved else "hpfp8_dequantize_rows", ops._ptr(codes), ops._ptr(scale_inv),
+              x.numel() // max(cols, 1), cols, ops._ptr(x), _TYPES[dtype], ops._stream())
+    return x
+
+
+def _quantize(x, saved: bool):
+    """(codes, scale_inv) of x; ``saved``: with codes for infinities and NaN, for `_dequantize` with the same."""
+    if ops._gpu(x):
+        device = ops._device()
+        made = ops._native.quantize_rows(x, saved, device, ops._raw_stream(device))
+        if made is not None:
+            return made
+    _check_rows(x, "x")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    cols = x.shape[-1]
+    x2 = _as_rows(x, cols)
+    codes = torch.empty(x.shape, dtype=ops.FP8, device=x.device)
+    scale_inv = torch.empty(x.shape[:-1] + (_groups(cols),), dtype=torch.float32, device=x.device)
+    _lib.call("hpfp8_quantize_saved_rows" if saved else "hpfp8_quantize_rows", ops._ptr(x2), _TYPES[x.dtype], x2.shape[0], cols, x2.stride(0),
+              ops._ptr(codes), ops._ptr(scale_inv), ops._stream())
+    return codes, scale_inv
+
+
 class Fp8Activation(NamedTuple):
     """A tensor in 8 bits: what `quantize_activation` makes."""
     codes: torch.Tensor                 # e4m3, the tensor's shape
@@ -62,26 +103,7 @@ class Fp8Activation(NamedTuple):
         dtype = self.dtype if dtype is None else dtype
         if dtype not in _TYPES:
             raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
-        if ops._gpu(self.codes):
-            device = ops._device()
-            x = ops._native.dequantize_rows(self.codes, self.scale_inv, _TYPES[dtype], device, ops._raw_stream(device))
-            if x is not None:
-                return x
-        codes, scale_inv = self.codes, self.scale_inv
-        if codes.dtype != ops.FP8 or scale_inv.dtype != torch.float32:
-            raise TypeError(f"codes and scale_inv must be float8_e4m3fn and float32, got {codes.dtype} and {scale_inv.dtype}")
-        ops._check_device(codes, "codes")
-        ops._check_device(scale_inv, "scale_inv")
-        if codes.dim() < 1:
-            raise ValueError("codes must have at least one dimension")
-        cols = codes.shape[-1]
-        if cols and scale_inv.numel() != codes.numel() // cols * _groups(cols):
-            raise ValueError(f"codes {tuple(codes.shape)} have a scale for each 128 values of a row, not {tuple(scale_inv.shape)}")
-        codes, scale_inv = codes.contiguous(), scale_inv.contiguous()         # (a slice of what was made, say)
-        x = torch.empty(codes.shape, dtype=dtype, device=codes.device)
-        _lib.call("hpfp8_dequantize_rows", ops._ptr(codes), ops._ptr(scale_inv), x.numel() // max(cols, 1), cols, ops._ptr(x),
-                  _TYPES[dtype], ops._stream())
-        return x
+        return _dequantize(self.codes, self.scale_inv, dtype, False)
 
     def __repr__(self) -> str:          # (shapes, never values: see Fp8Weight)
         return f"Fp8Activation({tuple(self.codes.shape)}@{self.codes.data_ptr():#x}, {self.dtype})"
@@ -90,22 +112,15 @@ class Fp8Activation(NamedTuple):
 def quantize_activation(x: torch.Tensor) -> Fp8Activation:
     """x[..., C] (bfloat16, float16 or float32; any C, any strides) in 8 bits: E4M3 codes, one scale for each 128 values of the last
     dimension, the last group of a row being what is left.  For bf16 rows of a multiple of 128 values the codes and scales of
-    `quantize_1x128`."""
-    if ops._gpu(x):
-        device = ops._device()
-        made = ops._native.quantize_rows(x, device, ops._raw_stream(device))
-        if made is not None:
-            return Fp8Activation(*made, x.dtype)
-    _check_rows(x, "x")
-    if x.dim() < 1:
-        raise ValueError("x must have at least one dimension")
-    cols = x.shape[-1]
-    x2 = _as_rows(x, cols)
-    codes = torch.empty(x.shape, dtype=ops.FP8, device=x.device)
-    scale_inv = torch.empty(x.shape[:-1] + (_groups(cols),), dtype=torch.float32, device=x.device)
-    _lib.call("hpfp8_quantize_rows", ops._ptr(x2), _TYPES[x.dtype], x2.shape[0], cols, x2.stride(0), ops._ptr(codes), ops._ptr(scale_inv),
-              ops._stream())
-    return Fp8Activation(codes, scale_inv, x.dtype)
+    `quantize_1x128`.  An infinity or a NaN makes its whole group NaN."""
+    return Fp8Activation(*_quantize(x, False), x.dtype)
+
+
+class _Saved(NamedTuple):
+    """What `keep_activations_8bit` puts in a tensor's place."""
+    codes: torch.Tensor
+    scale_inv: torch.Tensor
+    dtype: torch.dtype
 
 
 def _is_parameter(t: torch.Tensor) -> bool:
@@ -120,7 +135,10 @@ def keep_activations_8bit(min_elements: int = 1 << 16, dtypes: Sequence[torch.dt
 
     Kept so are GPU tensors of ``min_elements`` values and more in one of ``dtypes`` (by default the 16-bit types: an fp32 tensor is
     more often a statistic or a scale than an activation), unless they are parameters or views of one (leaves that require a gradient) or
-    ``select(tensor)`` says no.  Everything else is kept as it is.  The backward may run after the context has ended."""
+    ``select(tensor)`` says no.  Everything else is kept as it is.  The backward may run after the context has ended.
+
+    What the backward reads is off by 2^-4 of a value at most, or by 2^-10 of 1 / 448 of the largest finite value among its group's 128 where that is
+    more; infinities and NaN (a mask's -inf, say) come back as they were."""
     for d in dtypes:
         if d not in _TYPES:
             raise TypeError(f"dtypes must be bfloat16, float16 or float32, got {d}")
@@ -130,13 +148,13 @@ def keep_activations_8bit(min_elements: int = 1 << 16, dtypes: Sequence[torch.dt
                 or _is_parameter(t) or (select is not None and not select(t))):
             return t
         with torch.cuda.device(t.device):
-            return quantize_activation(t.detach())
+            return _Saved(*_quantize(t.detach(), True), t.dtype)
 
     def unpack(kept):
-        if not isinstance(kept, Fp8Activation):
+        if not isinstance(kept, _Saved):
             return kept
         with torch.cuda.device(kept.codes.device):
-            return kept.dequantize()
+            return _dequantize(kept.codes, kept.scale_inv, kept.dtype, True)
 
     with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
         yield

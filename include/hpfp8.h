@@ -516,6 +516,10 @@ int hpfp8_grouped_zero_unrouted_rows_bf16(void* out, int64_t ld, const int32_t* 
 int hpfp8_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, void* q, float* scale_inv, hpfp8_stream_t stream);
 /* x[r, c] = code * scale_inv, rounded once to dtype. */
 int hpfp8_dequantize_rows(const void* q, const float* scale_inv, int64_t rows, int64_t cols, void* x, int dtype, hpfp8_stream_t stream);
+/* The same for any tensor that a backward reads again: infinities and NaN come back as they were, by codes of their own (+-inf the two codes
+ * that are no number, NaN that of -0), and a group's scale is that of its finite values. */
+int hpfp8_quantize_saved_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, void* q, float* scale_inv, hpfp8_stream_t stream);
+int hpfp8_dequantize_saved_rows(const void* q, const float* scale_inv, int64_t rows, int64_t cols, void* x, int dtype, hpfp8_stream_t stream);
 
 /* y = f(x), in fp32, rounded once; kind 0 silu, 1 gelu, 2 gelu (tanh form), 3 SwiGLU: x[rows, 2 cols] = gate | up, y = silu(gate) up.
  * cols is y's width.  q and scale_inv (both or neither NULL) receive x in 8 bits: [rows, cols] as above, for SwiGLU [rows, 2, cols] and

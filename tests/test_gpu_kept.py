@@ -321,3 +321,48 @@ def test_more_than_2_31_values(gpu, kind, cols):
     made, made_last = hpfp8.quantize_activation(x.detach()), hpfp8.quantize_activation(last.detach())
     assert torch.equal(made.codes[-150:].view(torch.uint8), made_last.codes.view(torch.uint8)) and torch.equal(made.scale_inv[-150:], made_last.scale_inv)
     assert torch.equal(made.dequantize()[-150:], made_last.dequantize())
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [1, 7, 128, 300])
+def test_what_a_backward_saved_comes_back_with_its_infinities(gpu, dtype, cols, native, monkeypatch):
+    """Infinities and NaN as they were; every other value as if 0 stood in their places."""
+    from hpfp8 import kept, ops
+    if not native:
+        monkeypatch.setattr(ops, "_native", None)
+    x = randn((50, cols), 17, dtype, 2.0)
+    x[1], x[2], x[3] = math.inf, -math.inf, math.nan
+    pick = torch.rand((50, cols), generator=torch.Generator().manual_seed(18))
+    x[4:] = torch.where(pick[4:] < 0.1, -math.inf, torch.where(pick[4:] < 0.15, math.inf, torch.where(pick[4:] < 0.2, math.nan, x[4:].float()))).to(dtype)
+    x[40:44] = torch.where(pick[40:44] < 0.5, -math.inf, 0.0).to(dtype)
+    x[44:46] = torch.where(pick[44:46] < 0.5, torch.finfo(dtype).min, 0.0).to(dtype)             # (a mask of the type's lowest value)
+    x[46] = torch.where(pick[46] < 0.5, -1e-30, 3.0).to(dtype)                                   # (values that round to -0)
+    finite = torch.where(x.isfinite(), x, 0.0)
+    codes, scale_inv = quantized(finite)
+    want = (codes.float() * scale_inv.repeat_interleave(128, -1)[:, :cols]).to(dtype)
+    want = torch.where(x.isfinite(), want, x)
+    made = kept._quantize(x.to(gpu), True)
+    assert torch.equal(made[1].cpu(), scale_inv)
+    got = kept._dequantize(*made, dtype, True).cpu()
+    assert torch.equal(got.isnan(), x.isnan()) and torch.equal(got.nan_to_num(0.0, math.inf, -math.inf), want.nan_to_num(0.0, math.inf, -math.inf))
+
+
+def test_saved_tensors_with_infinities_have_finite_gradients(gpu):
+    """log_softmax of masked scores saves its result, -inf where the mask is; the gradient is that of the result as it is kept."""
+    import hpfp8
+    from hpfp8 import kept
+    x = randn((300, 500), 19, torch.bfloat16, 2.0)
+    mask = torch.rand((300, 500), generator=torch.Generator().manual_seed(20)) < 0.3
+    x = x.masked_fill(mask, -math.inf).to(gpu).requires_grad_()
+    go = randn((300, 500), 21, torch.bfloat16).masked_fill(mask, 0.0).to(gpu)
+    with hpfp8.keep_activations_8bit(min_elements=1000):
+        y = torch.log_softmax(x, -1)
+    dx, = torch.autograd.grad(y, x, go)
+    at = kept._dequantize(*kept._quantize(y.detach(), True), torch.bfloat16, True).double()
+    p = torch.exp(at)
+    want = go.double() - p * go.double().sum(1, keepdim=True)
+    assert dx.isfinite().all() and (dx[mask.to(gpu)] == 0).all()
+    # bf16's rounding of the result; fp32 sums of 500 summands, an exponential of an argument below 128
+    size = go.double().abs() + p * go.double().abs().sum(1, keepdim=True)
+    assert ((dx.double() - want).abs() <= 2.0 ** -8 * want.abs() + U * (500 + 256) * size).all()

@@ -226,3 +226,11 @@ def test_rows_that_start_between_two_vectors_or_have_odd_strides_are_copied():
         rows = _rows(x)
         assert torch.equal(rows, x) and rows.data_ptr() % 16 == 0 and rows.stride(1) == 1 and rows.stride(0) % 8 == 0 and rows.stride(0) >= rows.shape[1]
     assert _rows(flat[:320].view(5, 64)).data_ptr() == flat.data_ptr()
+
+
+def test_saved_rows_in_8_bits(p):
+    q, d = "hpfp8_quantize_saved_rows", "hpfp8_dequantize_saved_rows"
+    assert c(q, p, 3, 4, 8, 8, p, p, None)[0] == -1 and c(q, p, 0, -1, 8, 8, p, p, None)[0] == -2 and c(q, p + 1, 0, 4, 8, 8, p, p, None)[0] == -3
+    assert c(q, p, 0, 4, 8, 8, p, None, None)[0] == -1 and c(q, p, 0, 1, 1 << 40, 8, p, p, None)[0] == -2 and c(q, None, 0, 0, 8, 8, None, None, None)[0] == 0
+    assert c(d, p, p, 4, 8, p, 7, None)[0] == -1 and c(d, p, p, 4, 8, p + 1, 2, None)[0] == -3 and c(d, None, p, 4, 8, p, 2, None)[0] == -1
+    assert c(d, None, None, 0, 8, None, 2, None)[0] == 0
