@@ -445,6 +445,15 @@ struct Made {
   bool per_tensor, pow2, has_bias, w_transposed;
 };
 
+// What keep_activations_8bit leaves as it is of the tensors that a node below is saving: ops._saving.
+thread_local int saving_level = 0;
+struct Saving {
+  const int before = saving_level;
+  explicit Saving(int level) { saving_level = level; }
+  ~Saving() { saving_level = before; }
+};
+PyObject* saving(PyObject*, PyObject* const*, Py_ssize_t) { return PyLong_FromLong(saving_level); }
+
 // The graph's node.  A step of a small layer, forward and backward, with the Python function's backward 175 us, 114 with this one: on
 // the autograd engine's own thread the interpreter runs cold.  (An empty Python node's step takes 55.)
 struct LinearNode : torch::autograd::Function<LinearNode> {
@@ -565,6 +574,7 @@ PyObject* linear_node(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor* t[5];
   for (int i = 0; i < 5; ++i) TORCH_CHECK_TYPE(plain(args[3 + i], x.get_device(), t[i]), "tensors on ", x.device(), " expected");
   const Made made{*t[0], *t[1], *t[2], *t[3], *t[4], truth(args[8]), truth(args[9]), bias != nullptr, truth(args[10])};
+  const Saving level(1);
   return THPVariable_Wrap(LinearNode::apply(x, weight, bias ? std::optional<at::Tensor>(*bias) : std::nullopt, made));
   END_HANDLE_TH_ERRORS
 }
@@ -697,6 +707,7 @@ PyObject* linear_train(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     }
   }
   if (!call.ok()) return failed(call);
+  const Saving level(1);
   return THPVariable_Wrap(LinearNode::apply(*x, *weight, bias ? std::optional<at::Tensor>(*bias) : std::nullopt, made));
   END_HANDLE_TH_ERRORS
 }
@@ -1065,6 +1076,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   }
   if (!call.ok()) return failed(call);
   if (!train) return THPVariable_Wrap(made.y);
+  const Saving level(2);
   return THPVariable_Wrap(NormNode::apply(*x, v[0] ? std::optional<at::Tensor>(*v[0]) : std::nullopt,
                                           v[1] ? std::optional<at::Tensor>(*v[1]) : std::nullopt, made));
   END_HANDLE_TH_ERRORS
@@ -1143,6 +1155,7 @@ PyObject* activation(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
                made.keep ? made.codes.data_ptr() : nullptr, made.keep ? f32(made.scales) : nullptr, at_.stream);
   }
   if (!call.ok()) return failed(call);
+  const Saving level(made.keep);
   return THPVariable_Wrap(train ? ActivationNode::apply(*x, made) : made.y);
   END_HANDLE_TH_ERRORS
 }
@@ -1312,6 +1325,7 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n_ar
     made.loss = made.reduction ? out : loss;
   }
   if (!call.ok()) return failed(call);
+  const Saving level(2);
   return THPVariable_Wrap(train ? LossNode::apply(*x, *weight, *target, made) : made.loss);
   END_HANDLE_TH_ERRORS
 }
@@ -1376,7 +1390,7 @@ PyObject* bind_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 #define HPFP8_METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {HPFP8_METHOD(built_for), HPFP8_METHOD(bind), HPFP8_METHOD(bind_backward), HPFP8_METHOD(quantize_1x128), HPFP8_METHOD(both_forms),
+PyMethodDef methods[] = {HPFP8_METHOD(built_for), HPFP8_METHOD(bind), HPFP8_METHOD(bind_backward), HPFP8_METHOD(saving), HPFP8_METHOD(quantize_1x128), HPFP8_METHOD(both_forms),
                          HPFP8_METHOD(quantize_128x128), HPFP8_METHOD(quantize_per_tensor_t), HPFP8_METHOD(gemm_blockwise),
                          HPFP8_METHOD(gemm_per_tensor), HPFP8_METHOD(trains), HPFP8_METHOD(linear_node), HPFP8_METHOD(linear_train), HPFP8_METHOD(linear_infer), HPFP8_METHOD(linear_backward),
                          HPFP8_METHOD(swiglu_mlp_infer), HPFP8_METHOD(grouped_infer), HPFP8_METHOD(bucket_pack), HPFP8_METHOD(bucket_unpack),

@@ -128,6 +128,14 @@ def _is_parameter(t: torch.Tensor) -> bool:
     return base.is_leaf and base.requires_grad
 
 
+def _own(t: torch.Tensor) -> bool:
+    """Whether t, just being saved, is a scale of codes or a statistic of this package's own operators, or belongs to a statistic: the
+    softmax of logits that are computed again from 8 bits does not sum to 1 with the exact ones' sum, nor are values normalised by the mean
+    and deviation of others."""
+    level = max(ops._saving.level, ops._native.saving() if ops._native is not None else 0)
+    return level == 2 or (level == 1 and t.dtype == torch.float32)
+
+
 @contextlib.contextmanager
 def keep_activations_8bit(min_elements: int = 1 << 16, dtypes: Sequence[torch.dtype] = (torch.bfloat16, torch.float16),
                           select: Optional[Callable[[torch.Tensor], bool]] = None):
@@ -135,7 +143,8 @@ def keep_activations_8bit(min_elements: int = 1 << 16, dtypes: Sequence[torch.dt
 
     Kept so are GPU tensors of ``min_elements`` values and more in one of ``dtypes`` (by default the 16-bit types: an fp32 tensor is
     more often a statistic or a scale than an activation), unless they are parameters or views of one (leaves that require a gradient) or
-    ``select(tensor)`` says no.  Everything else is kept as it is.  The backward may run after the context has ended.
+    ``select(tensor)`` says no.  This package's own operators keep their scales and statistics as they are, and `layer_norm` and
+    `linear_cross_entropy`, whose statistics are those of the exact input, their input too.  Everything else is kept as it is.  The backward may run after the context has ended.
 
     What the backward reads is off by 2^-4 of a value at most, or by 2^-10 of 1 / 448 of the largest finite value among its group's 128 where that is
     more; infinities and NaN (a mask's -inf, say) come back as they were."""
@@ -145,7 +154,7 @@ def keep_activations_8bit(min_elements: int = 1 << 16, dtypes: Sequence[torch.dt
 
     def pack(t):
         if (type(t) is not torch.Tensor or not t.is_cuda or t.dtype not in dtypes or t.dim() < 1 or t.numel() < min_elements
-                or _is_parameter(t) or (select is not None and not select(t))):
+                or _own(t) or _is_parameter(t) or (select is not None and not select(t))):
             return t
         with torch.cuda.device(t.device):
             return _Saved(*_quantize(t.detach(), True), t.dtype)
@@ -239,6 +248,6 @@ def activation(input: torch.Tensor, kind: str, *, keep_8bit: bool = True) -> tor
         raise ValueError(f"swiglu takes gate | up in the last dimension, which is {input.shape[-1]}")
     k = KINDS[kind]
     if torch.is_grad_enabled() and input.requires_grad:
-        return _Activation.apply(input, k, bool(keep_8bit))
+        return ops._apply(_Activation, int(bool(keep_8bit)), input, k, bool(keep_8bit))
     cols = input.shape[-1] // (2 if kind == "swiglu" else 1)
     return _forward(_as_rows(input.detach(), input.shape[-1]), k, cols, False)[0].reshape(input.shape[:-1] + (cols,))

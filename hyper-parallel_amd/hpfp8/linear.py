@@ -347,8 +347,8 @@ def fp8_linear(input: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
         if y is not None:
             return y
     if recipe == "per_tensor":
-        return _Fp8LinearPerTensor.apply(input, weight, bias, wq, sw, torch.is_grad_enabled())
-    return _Fp8LinearBlockwise.apply(input, weight, bias, wq, sw, wqt, apply_grad_on_fp32_main_grad, pow2, torch.is_grad_enabled())
+        return ops._apply(_Fp8LinearPerTensor, 1, input, weight, bias, wq, sw, torch.is_grad_enabled())
+    return ops._apply(_Fp8LinearBlockwise, 1, input, weight, bias, wq, sw, wqt, apply_grad_on_fp32_main_grad, pow2, torch.is_grad_enabled())
 
 
 _FP8_LINEAR_DEFAULTS = dict(recipe="blockwise", weight_fp8=None, apply_grad_on_fp32_main_grad=False)
@@ -560,9 +560,9 @@ def fp8_grouped_linear(input: torch.Tensor, weight: torch.Tensor, offs: torch.Te
             y = ops._native.grouped_infer(input, weight, offs, weight_fp8.codes, weight_fp8.scale_inv, device, ops._raw_stream(device))
             if y is not None:
                 return y
-        return _Fp8GroupedLinear.apply(input, weight, offs, weight_fp8.codes, weight_fp8.scale_inv, weight_fp8.codes_t,
-                                       torch.is_grad_enabled())
-    return _Fp8GroupedLinear.apply(input, weight, offs, None, None, None, torch.is_grad_enabled())
+        return ops._apply(_Fp8GroupedLinear, 1, input, weight, offs, weight_fp8.codes, weight_fp8.scale_inv, weight_fp8.codes_t,
+                          torch.is_grad_enabled())
+    return ops._apply(_Fp8GroupedLinear, 1, input, weight, offs, None, None, None, torch.is_grad_enabled())
 
 
 def _keep(h, in_8_bits: bool):
@@ -717,9 +717,9 @@ def fp8_swiglu_mlp(input: torch.Tensor, w_gate_up, w_down, *, fast: bool = True,
         rows = input.numel() // max(input.shape[-1], 1)
         if (w_gate_up.requires_grad and w_down.requires_grad and rows > 0
                 and input.dtype == torch.bfloat16 and w_gate_up.dtype == torch.bfloat16 and w_down.dtype == torch.bfloat16):
-            return _Fp8SwiGLUMLPBlock.apply(input, w_gate_up, w_down, fast, gate_up_fp8, d8, keep_8bit)
+            return ops._apply(_Fp8SwiGLUMLPBlock, 1, input, w_gate_up, w_down, fast, gate_up_fp8, d8, keep_8bit)
         h = fp8_linear(input, w_gate_up, weight_fp8=gate_up_fp8)
-        return _Fp8SwiGLUDown.apply(h, w_down, fast, *((d8.codes, d8.scale_inv, d8.codes_t) if d8 is not None else (None, None, None)), keep_8bit)
+        return ops._apply(_Fp8SwiGLUDown, 1, h, w_down, fast, *((d8.codes, d8.scale_inv, d8.codes_t) if d8 is not None else (None, None, None)), keep_8bit)
     gu = w_gate_up if isinstance(w_gate_up, Fp8Weight) else (gate_up_fp8 or quantize_weight(w_gate_up.detach(), with_transpose=False))
     dn = w_down if isinstance(w_down, Fp8Weight) else (down_fp8 or quantize_weight(w_down.detach(), with_transpose=False))
     inter = gu.codes.shape[0] // 2

@@ -199,7 +199,7 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
     flat = target.reshape(-1).contiguous()
     r = _REDUCTIONS[reduction]
     if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad):
-        loss = _LinearCrossEntropy.apply(input, weight, flat, int(ignore_index), r, float(label_smoothing),
+        loss = ops._apply(_LinearCrossEntropy, 2, input, weight, flat, int(ignore_index), r, float(label_smoothing),
                                          weight if apply_grad_on_fp32_main_grad else None)
     else:
         loss = _forward(_rows(input.detach()), _rows(weight.detach()), flat, int(ignore_index), r, float(label_smoothing), False)[0]

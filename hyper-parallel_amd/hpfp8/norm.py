@@ -118,7 +118,7 @@ def layer_norm(input: torch.Tensor, normalized_shape: Union[int, Sequence[int]],
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"weight and bias must be of one type, got {weight.dtype} and {bias.dtype}")
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        return _LayerNorm.apply(input, weight, bias, cols, float(eps), bool(keep_8bit))
+        return ops._apply(_LayerNorm, 2, input, weight, bias, cols, float(eps), bool(keep_8bit))
     w = None if weight is None else weight.detach().reshape(-1).contiguous()
     b = None if bias is None else bias.detach().reshape(-1).contiguous()
     return _forward(_as_rows(input.detach(), cols), w, b, float(eps), False, False)[0].reshape(input.shape)

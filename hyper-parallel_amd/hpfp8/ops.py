@@ -11,6 +11,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import ctypes
+import threading
 
 import torch
 
@@ -28,6 +29,25 @@ _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_devic
 
 
 _native = _lib.load_native()
+
+# What `keep_activations_8bit` leaves as it is of the tensors that an operator of this package is saving for its backward: 1, those in fp32, which are
+# scales of codes and statistics; 2, all of them, where a statistic belongs to the others.  (The native nodes have a level of their own.)
+class _Saving(threading.local):
+    level = 0
+
+
+_saving = _Saving()
+
+
+def _apply(function, level: int, *args):
+    """function.apply(*args) for an autograd function whose saved tensors are left as they are by ``level``."""
+    before, _saving.level = _saving.level, level
+    try:
+        return function.apply(*args)
+    finally:
+        _saving.level = before
+
+
 _PLAIN = frozenset((torch.Tensor, torch.nn.Parameter))
 
 

@@ -366,3 +366,66 @@ def test_saved_tensors_with_infinities_have_finite_gradients(gpu):
     # bf16's rounding of the result; fp32 sums of 500 summands, an exponential of an argument below 128
     size = go.double().abs() + p * go.double().abs().sum(1, keepdim=True)
     assert ((dx.double() - want).abs() <= 2.0 ** -8 * want.abs() + U * (500 + 256) * size).all()
+
+
+def inside(f, leaves, go, **context):
+    """(result, gradients) of f(*leaves), inside keep_activations_8bit(**context) if there is one."""
+    import contextlib
+    import hpfp8
+    leaves = [v.clone().requires_grad_() for v in leaves]
+    with hpfp8.keep_activations_8bit(**context) if context else contextlib.nullcontext():
+        y = f(*leaves)
+    return (y.detach(),) + torch.autograd.grad(y, leaves, go)
+
+
+ALL = dict(min_elements=1, dtypes=(torch.bfloat16, torch.float16, torch.float32))
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("context", [dict(min_elements=1), ALL])
+def test_statistics_and_what_belongs_to_them_stay_exact(gpu, context, native, monkeypatch):
+    """A loss whose targets have almost all of the probability, a norm of rows far from zero: as outside the context, bit for bit."""
+    import hpfp8
+    from hpfp8 import ops
+    if not native:
+        monkeypatch.setattr(ops, "_native", None)
+    w = randn((1000, 256), 22, torch.bfloat16, 0.1)
+    t = torch.randint(1000, (200,), generator=torch.Generator().manual_seed(23))
+    x = (w[t].float() * 8 + randn((200, 256), 24, torch.float32, 0.1)).to(torch.bfloat16)            # (losses around 1e-3)
+
+    def loss(x, w):
+        return hpfp8.linear_cross_entropy(x * 1, w, t.to(gpu))          # (no leaf: an activation)
+    leaves, go = (x.to(gpu), w.to(gpu)), torch.ones((), device=gpu)
+    want, got = inside(loss, leaves, go), inside(loss, leaves, go, **context)
+    assert want[0] < 0.1 and all(torch.equal(p, q) for p, q in zip(got, want))
+    for dtype in DTYPES:
+        x, v = (randn((64, 384), 25, torch.float32) + 100).to(dtype).to(gpu), randn((384,), 26, dtype).to(gpu)
+        go = randn((64, 384), 27, dtype).to(gpu)
+        for keep in (False, True):
+            def norm(x, w, b):
+                return hpfp8.layer_norm(x * 1, 384, w, b, keep_8bit=keep)
+            want, got = inside(norm, (x, v, v), go), inside(norm, (x, v, v), go, **context)
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_scales_of_codes_stay_exact(gpu, native, monkeypatch):
+    """Linears, experts and activations keep codes: with fp32 tensors in 8 bits too their results are those outside the context."""
+    import hpfp8
+    from hpfp8 import ops
+    if not native:
+        monkeypatch.setattr(ops, "_native", None)
+    x, w, go = randn((200, 256), 28, torch.bfloat16).to(gpu), randn((384, 256), 29, torch.bfloat16, 0.1).to(gpu), randn((200, 384), 30, torch.bfloat16).to(gpu)
+    experts, offs = randn((3, 384, 256), 31, torch.bfloat16, 0.1).to(gpu), torch.tensor([50, 128, 200], dtype=torch.int32, device=gpu)
+    cases = [(lambda x, w: hpfp8.fp8_linear(x * 1, w), (x, w), go), (lambda x, w: hpfp8.fp8_linear(x * 1, w, recipe="per_tensor"), (x, w), go),
+             (lambda x, w: hpfp8.fp8_grouped_linear(x * 1, w, offs), (x, experts), go),
+             (lambda x: hpfp8.activation(x * 1, "gelu"), (x,), x)]
+    for f, leaves, g in cases:
+        want, got = inside(f, leaves, g), inside(f, leaves, g, **ALL)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    # the MLP's gate/up output is no statistic's: it is kept in 8 bits, as keep_8bit does
+    wgu, wd = randn((512, 256), 33, torch.bfloat16, 0.1).to(gpu), randn((256, 256), 34, torch.bfloat16, 0.1).to(gpu)
+    want = inside(lambda *t: hpfp8.fp8_swiglu_mlp(*t, keep_8bit=True), (x, wgu, wd), x)
+    got = inside(lambda *t: hpfp8.fp8_swiglu_mlp(*t), (x, wgu, wd), x, **ALL)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    assert not torch.equal(want[1], inside(lambda *t: hpfp8.fp8_swiglu_mlp(*t), (x, wgu, wd), x)[1])
