@@ -124,8 +124,9 @@ class _Saved(NamedTuple):
 
 
 def _is_parameter(t: torch.Tensor) -> bool:
+    """Whether t is a parameter (frozen ones too), another leaf that requires a gradient, or a view of one: what is there anyway."""
     base = t if t._base is None else t._base
-    return base.is_leaf and base.requires_grad
+    return isinstance(base, torch.nn.Parameter) or (base.is_leaf and base.requires_grad)
 
 
 def _own(t: torch.Tensor) -> bool:
@@ -142,8 +143,8 @@ def keep_activations_8bit(min_elements: int = 1 << 16, dtypes: Sequence[torch.dt
     """Inside this context the tensors that backward nodes save are kept in 8 bits until the backward reads them.
 
     Kept so are GPU tensors of ``min_elements`` values and more in one of ``dtypes`` (by default the 16-bit types: an fp32 tensor is
-    more often a statistic or a scale than an activation), unless they are parameters or views of one (leaves that require a gradient) or
-    ``select(tensor)`` says no.  This package's own operators keep their scales and statistics as they are, and `layer_norm` and
+    more often a statistic or a scale than an activation), unless they are parameters, other leaves that require a gradient, or views of
+    one (a copy, such as a parameter cast to 16 bits, is none), or ``select(tensor)`` says no.  This package's own operators keep their scales and statistics as they are, and `layer_norm` and
     `linear_cross_entropy`, whose statistics are those of the exact input, their input too.  Everything else is kept as it is.  The backward may run after the context has ended.
 
     What the backward reads is off by 2^-4 of a value at most, or by 2^-10 of 1 / 448 of the largest finite value among its group's 128 where that is

@@ -429,3 +429,18 @@ def test_scales_of_codes_stay_exact(gpu, native, monkeypatch):
     got = inside(lambda *t: hpfp8.fp8_swiglu_mlp(*t), (x, wgu, wd), x, **ALL)
     assert all(torch.equal(p, q) for p, q in zip(got, want))
     assert not torch.equal(want[1], inside(lambda *t: hpfp8.fp8_swiglu_mlp(*t), (x, wgu, wd), x)[1])
+
+
+def test_frozen_parameters_are_parameters(gpu):
+    """Neither they nor views of them are kept in 8 bits: the gradient of the input is that outside the context."""
+    import hpfp8
+    lin = torch.nn.Linear(512, 768, bias=False, device=gpu, dtype=torch.bfloat16).requires_grad_(False)
+    x, go = randn((300, 512), 35, torch.bfloat16).to(gpu), randn((300, 768), 36, torch.bfloat16).to(gpu)
+    scale = torch.nn.Parameter(randn((300, 1536), 37, torch.bfloat16).to(gpu), requires_grad=False)
+    seen = []
+
+    def f(x):
+        return lin(x) * scale[:, ::2]
+    want = inside(f, (x,), go)
+    got = inside(f, (x,), go, min_elements=1000, select=lambda t: seen.append(t) or True)
+    assert not seen and all(torch.equal(p, q) for p, q in zip(got, want))
