@@ -129,6 +129,14 @@ def _is_parameter(t: torch.Tensor) -> bool:
     return isinstance(base, torch.nn.Parameter) or (base.is_leaf and base.requires_grad)
 
 
+def _takes_less(t: torch.Tensor) -> bool:
+    """Whether codes and scales are less than what t holds: not for an expanded tensor, whose values are there once, nor for rows of a few values."""
+    if t.layout != torch.strided or any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        return False
+    cols = t.shape[-1]
+    return cols + 4 * _groups(cols) < t.element_size() * cols
+
+
 def _own(t: torch.Tensor) -> bool:
     """Whether t, just being saved, is a scale of codes or a statistic of this package's own operators, or belongs to a statistic: the
     softmax of logits that are computed again from 8 bits does not sum to 1 with the exact ones' sum, nor are values normalised by the mean
@@ -147,6 +155,9 @@ def keep_activations_8bit(min_elements: int = 1 << 16, dtypes: Sequence[torch.dt
     one (a copy, such as a parameter cast to 16 bits, is none), or ``select(tensor)`` says no.  This package's own operators keep their scales and statistics as they are, and `layer_norm` and
     `linear_cross_entropy`, whose statistics are those of the exact input, their input too.  Everything else is kept as it is.  The backward may run after the context has ended.
 
+    An expanded tensor stays as it is too, and one whose last dimension is so short (4 values of 16 bits) that the scales take what the codes save.  Each
+    node that saves a tensor has codes of its own: a 16-bit tensor that two nodes save takes 2.06 bytes a value, where both share one of 2 outside.
+
     What the backward reads is off by 2^-4 of a value at most, or by 2^-10 of 1 / 448 of the largest finite value among its group's 128 where that is
     more; infinities and NaN (a mask's -inf, say) come back as they were."""
     for d in dtypes:
@@ -155,7 +166,7 @@ def keep_activations_8bit(min_elements: int = 1 << 16, dtypes: Sequence[torch.dt
 
     def pack(t):
         if (type(t) is not torch.Tensor or not t.is_cuda or t.dtype not in dtypes or t.dim() < 1 or t.numel() < min_elements
-                or _own(t) or _is_parameter(t) or (select is not None and not select(t))):
+                or not _takes_less(t) or _own(t) or _is_parameter(t) or (select is not None and not select(t))):
             return t
         with torch.cuda.device(t.device):
             return _Saved(*_quantize(t.detach(), True), t.dtype)

@@ -444,3 +444,39 @@ def test_frozen_parameters_are_parameters(gpu):
     want = inside(f, (x,), go)
     got = inside(f, (x,), go, min_elements=1000, select=lambda t: seen.append(t) or True)
     assert not seen and all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_tensors_that_would_take_more_in_8_bits_stay_as_they_are(gpu):
+    """Expanded ones, rows of a few values, sparse ones; of all others the context holds the codes and scales instead."""
+    import hpfp8
+    seen = []
+    context = dict(ALL, select=lambda t: seen.append(tuple(t.shape)) or True)
+    v, x = randn((512,), 38, torch.bfloat16).to(gpu), randn((300, 512), 39, torch.bfloat16).to(gpu)
+    cases = [(lambda x: x * v.expand(300, 512), x)]
+    for cols, dtype in ((1, torch.bfloat16), (4, torch.bfloat16), (4, torch.float16), (1, torch.float32)):
+        u = randn((700, cols), 40, dtype).to(gpu)
+        cases.append((lambda x, u=u: x * (u * 1), u))
+    sparse = torch.eye(300, device=gpu).to_sparse()
+    cases.append((lambda x: torch.sparse.mm(sparse, x), x.float()))
+    for f, leaf in cases:
+        want, got = inside(f, (leaf,), torch.ones_like(leaf)), inside(f, (leaf,), torch.ones_like(leaf), **context)
+        assert not seen and all(torch.equal(p, q) for p, q in zip(got, want))
+    for cols, dtype in ((5, torch.bfloat16), (5, torch.float16), (2, torch.float32)):
+        u = randn((700, cols), 41, dtype).to(gpu)
+        inside(lambda x: x * (u * 1), (u,), u, **context)
+        assert seen.pop() == (700, cols) and not seen
+
+
+def test_what_the_context_holds(gpu):
+    """A chain of nodes that each save one tensor: its codes and scales, to the byte."""
+    import hpfp8
+    x = randn((1024, 2048), 42, torch.bfloat16).to(gpu).requires_grad_()
+
+    def held(context):
+        with context:
+            before = torch.cuda.memory_stats()["requested_bytes.all.current"]
+            y = torch.nn.functional.silu(torch.nn.functional.silu(x * 2) * 2)       # (saves the products, not the results)
+            return torch.cuda.memory_stats()["requested_bytes.all.current"] - before, y
+    n = 1024 * 2048
+    held(torch.enable_grad()), held(hpfp8.keep_activations_8bit())
+    assert held(torch.enable_grad())[0] - held(hpfp8.keep_activations_8bit())[0] == 2 * (2 * n - n - n // 128 * 4)
