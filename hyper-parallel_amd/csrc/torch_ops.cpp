@@ -1249,7 +1249,10 @@ struct LossNode : torch::autograd::Function<LossNode> {
       return from_python(loss_backward_function, pybind11::make_tuple(grad, x, weight, target, lse, or_none(count), ignore_index, reduction, smoothing,
                                                                      need_dx, need_dw), 4);
     }
-    const at::Tensor go = grad.contiguous();
+    // (the same for every row, as behind a sum or a mean of the losses: one factor of the sums, which the logits' gradient is not rounded with)
+    bool same = true;
+    for (int64_t d = 0; d < grad.dim(); ++d) same = same && (grad.size(d) == 1 || grad.stride(d) == 0);
+    const at::Tensor go = same ? grad : grad.contiguous();
     void* const stream = c10::hip::getCurrentHIPStream(go.get_device()).stream();
     const at::TensorOptions bf16 = x.options().requires_grad(false), floats = bf16.dtype(at::kFloat);
     const int64_t padded = whole_tiles(tokens);
@@ -1273,7 +1276,7 @@ struct LossNode : torch::autograd::Function<LossNode> {
     for (int64_t first = 0; first < vocab && call.ok(); first += width)
       HPFP8_CALL(call, hpfp8_linear_cross_entropy_piece, x.data_ptr(), hidden, need_dw ? x_t.data_ptr() : nullptr, weight.data_ptr(), hidden,
                  target.data_ptr<int64_t>(), tokens, hidden, vocab, first, std::min(width, vocab - first), ignore_index, (float)smoothing, f32(lse), f32(go),
-                 reduction ? 0 : 1, reduction == 1 ? f32(count) : nullptr, dl.data_ptr(), dl_t.data_ptr(), need_dx ? f32(sum) : nullptr, splits, first > 0,
+                 same ? 0 : 1, reduction == 1 ? f32(count) : nullptr, dl.data_ptr(), dl_t.data_ptr(), need_dx ? f32(sum) : nullptr, splits, first > 0,
                  need_dw ? dw.data_ptr() : nullptr, HPFP8_OUT_BF16, 0, stream);
     if (need_dx && call.ok()) {
       dx = at::empty(x.sizes(), bf16);

@@ -109,7 +109,9 @@ def _backward(grad_out, x, weight, target, lse, count, ignore_index, reduction, 
             param.main_grad = torch.zeros(weight.shape, dtype=torch.float32, device=w.device)
         return torch.zeros_like(x) if need_dx else None, torch.zeros_like(weight) if need_dw and param is None else None
     bf16, f32 = dict(dtype=torch.bfloat16, device=x2.device), dict(dtype=torch.float32, device=x2.device)
-    grad = grad_out.reshape(-1).contiguous()
+    # (the same for every row, as behind a sum or a mean of the losses: one factor of the sums, which the logits' gradient is not rounded with)
+    same = reduction != 0 or all(n == 1 or s == 0 for n, s in zip(grad_out.shape, grad_out.stride()))
+    grad = grad_out if same else grad_out.reshape(-1).contiguous()
     dw = dx = x_t = None
     splits = 1
     pieces = _pieces(tokens, w.stride(0), vocab, _PIECE_BYTES)
@@ -129,7 +131,7 @@ def _backward(grad_out, x, weight, target, lse, count, ignore_index, reduction, 
         dx = torch.empty((splits, tokens, hidden), **f32)
     for first, n in pieces:
         _lib.call("hpfp8_linear_cross_entropy_piece", ops._ptr(x2), x2.stride(0), ops._ptr(x_t), ops._ptr(w), w.stride(0), ops._ptr(target),
-                  tokens, hidden, vocab, first, n, ignore_index, smoothing, ops._ptr(lse), ops._ptr(grad), 0 if reduction else 1,
+                  tokens, hidden, vocab, first, n, ignore_index, smoothing, ops._ptr(lse), ops._ptr(grad), 0 if same else 1,
                   ops._ptr(count) if reduction == 1 else None, ops._ptr(dl), ops._ptr(dl_t), ops._ptr(dx), splits, int(first > 0), ops._ptr(dw),
                   _lib.OUT_BF16 if param is None else _lib.OUT_F32, int(main_grad is not None), ops._stream())
     if need_dx:

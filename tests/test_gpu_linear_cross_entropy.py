@@ -406,3 +406,32 @@ def test_contiguous_tensors_that_start_between_two_vectors(gpu, at, tokens):
     hooks = torch.autograd.graph.saved_tensors_hooks(lambda v: v, lambda v: view(v) if v.dtype == torch.bfloat16 else v)
     for got in (step(view(x), w), step(x, view(w)), step(view(x), view(w)), step(x, w, hooks)):
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("shape", [(300,), (3, 100), (1, 1)])
+def test_a_gradient_that_all_rows_share_is_one_factor(gpu, shape, native, monkeypatch):
+    """Losses one by one, summed or averaged by torch: the gradients are those of the sum with that factor, bit for bit, and the logits'
+    gradient is not rounded with the factor in it."""
+    import hpfp8
+    from hpfp8 import ops
+    if not native:
+        monkeypatch.setattr(ops, "_native", None)
+    tokens = math.prod(shape)
+    x, w, t = (v.to(gpu) for v in make(tokens, 256, 1100, 16))
+    x, t = x.reshape(shape + (256,)), t.reshape(shape)
+
+    def gradients(reduction, after, go):
+        a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = after(hpfp8.linear_cross_entropy(a, b, t, reduction=reduction))
+        return torch.autograd.grad(loss, (a, b), go)
+    go = torch.tensor(0.7, device=gpu)
+    want = gradients("sum", lambda v: v, go)
+    for got in (gradients("none", lambda v: v.sum(), go), gradients("none", lambda v: v, go.expand(shape))):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    # one value for each row is another matter, also where the values agree
+    rows = gradients("none", lambda v: v, go.expand(shape).clone())
+    _, rdx, rdw, _, b_dx, b_dw = reference(x.reshape(tokens, 256).cpu(), w.cpu(), t.reshape(-1).cpu(), 0.0, go.cpu().expand(tokens))
+    for dx, dw in (want, rows):
+        within(dx.reshape(tokens, 256), rdx, b_dx, H)
+        within(dw, rdw, b_dw, H)
