@@ -1215,12 +1215,13 @@ PyObject* dequantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
 }
 
 // ---- the loss over a vocabulary: x [.., hidden] and weight [vocab, hidden] bf16, contiguous; one forward's worth of tokens
-constexpr int64_t kLossTile = 256, kForwardRows = 16384, kPieceElements = 0x3FFFF000;       // (hpfp8/loss.py has the reasons)
+constexpr int64_t kLossTile = 256;
 int64_t whole_tiles(int64_t n) { return (n + kLossTile - 1) / kLossTile * kLossTile; }
 
 struct Loss {
   at::Tensor loss, lse, count;
-  int64_t ignore_index, reduction, budget;
+  int64_t ignore_index, reduction;
+  int64_t budget, elements;              // of a piece: loss.py's _PIECE_BYTES and _PIECE_ELEMENTS
   double smoothing;
 };
 
@@ -1228,7 +1229,7 @@ struct LossNode : torch::autograd::Function<LossNode> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target,
                             const Loss& made) {
     ctx->save_for_backward({x, weight, target, made.lse, made.count});
-    ctx->saved_data["how"] = std::vector<int64_t>{made.ignore_index, made.reduction, made.budget};
+    ctx->saved_data["how"] = std::vector<int64_t>{made.ignore_index, made.reduction, made.budget, made.elements};
     ctx->saved_data["smoothing"] = made.smoothing;
     return made.loss;
   }
@@ -1236,7 +1237,7 @@ struct LossNode : torch::autograd::Function<LossNode> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &weight = saved[1], &target = saved[2], &lse = saved[3], &count = saved[4], &grad = grads[0];
     const std::vector<int64_t> how = ctx->saved_data["how"].toIntVector();
-    const int64_t ignore_index = how[0], reduction = how[1], budget = how[2];
+    const int64_t ignore_index = how[0], reduction = how[1], budget = how[2], elements = how[3];
     const double smoothing = ctx->saved_data["smoothing"].toDouble();
     const bool need_dx = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1);
     const int64_t hidden = weight.size(-1), vocab = weight.numel() / hidden, tokens = x.numel() / hidden;
@@ -1256,7 +1257,7 @@ struct LossNode : torch::autograd::Function<LossNode> {
     void* const stream = c10::hip::getCurrentHIPStream(go.get_device()).stream();
     const at::TensorOptions bf16 = x.options().requires_grad(false), floats = bf16.dtype(at::kFloat);
     const int64_t padded = whole_tiles(tokens);
-    const int64_t most = std::max(kLossTile, std::min(budget / (4 * padded), (kPieceElements - 1) / hidden) / kLossTile * kLossTile), pieces = (vocab + most - 1) / most;
+    const int64_t most = std::max(kLossTile, std::min(budget / (4 * padded), (elements - 1) / hidden) / kLossTile * kLossTile), pieces = (vocab + most - 1) / most;
     const int64_t width = std::min(whole_tiles((vocab + pieces - 1) / pieces), vocab);
     const int64_t row_t = lib.hpfp8_cross_entropy_stride(tokens), row = lib.hpfp8_cross_entropy_stride(width);
     const at::Tensor dl = at::empty({padded, row}, bf16), dl_t = at::empty({whole_tiles(width), row_t}, bf16);
@@ -1287,16 +1288,18 @@ struct LossNode : torch::autograd::Function<LossNode> {
   }
 };
 
-// (x, weight, target, ignore_index, reduction, smoothing, bytes of a piece, device, stream) -> loss, with its place in the graph where it has one
+// (x, weight, target, ignore_index, reduction, smoothing, tokens of a forward, bytes of a piece, elements of a piece, device, stream) -> loss, with its place in the graph where it has one
 PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  expect(n_args, 9);
+  expect(n_args, 11);
   const Where at_ = where(args, n_args);
   Loss made;
   made.ignore_index = PyLong_AsLongLong(args[3]);
   made.reduction = PyLong_AsLongLong(args[4]);
   made.smoothing = PyFloat_AsDouble(args[5]);
-  made.budget = PyLong_AsLongLong(args[6]);
+  const int64_t forward_rows = PyLong_AsLongLong(args[6]);
+  made.budget = PyLong_AsLongLong(args[7]);
+  made.elements = PyLong_AsLongLong(args[8]);
   if (PyErr_Occurred()) throw python_error();
   const at::Tensor *x, *weight, *target;
   if (!rows_of_values(args[0], at_.device, x) || x->scalar_type() != at::kBFloat16 || x->numel() == 0 || !rows_of_values(args[1], at_.device, weight) ||
@@ -1304,7 +1307,7 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n_ar
       !target->is_contiguous())
     Py_RETURN_NONE;
   const int64_t hidden = x->size(-1), vocab = weight->size(0), tokens = x->numel() / hidden;
-  if (weight->size(1) != hidden || hidden % 8 || hidden >= 1 << 21 || vocab < 1 || vocab > 1 << 24 || tokens > kForwardRows ||
+  if (weight->size(1) != hidden || hidden % 8 || hidden >= 1 << 21 || vocab < 1 || vocab > 1 << 24 || tokens > forward_rows ||
       target->sizes() != x->sizes().slice(0, x->dim() - 1) || (uintptr_t)x->data_ptr() % 16 || (uintptr_t)weight->data_ptr() % 16 || !ordinary({x, weight}))
     Py_RETURN_NONE;
   const bool train = to_train({x, weight});

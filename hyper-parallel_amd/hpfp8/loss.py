@@ -176,8 +176,8 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
         raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
     if not apply_grad_on_fp32_main_grad and ops._gpu(input):
         device = ops._device()
-        loss = ops._native.linear_cross_entropy(input, weight, target, ignore_index, _REDUCTIONS[reduction], label_smoothing, _PIECE_BYTES,
-                                                device, ops._raw_stream(device))
+        loss = ops._native.linear_cross_entropy(input, weight, target, ignore_index, _REDUCTIONS[reduction], label_smoothing, _FORWARD_ROWS,
+                                                _PIECE_BYTES, _PIECE_ELEMENTS, device, ops._raw_stream(device))
         if loss is not None:
             return loss
     for name, t in (("input", input), ("weight", weight)):

@@ -435,3 +435,76 @@ def test_a_gradient_that_all_rows_share_is_one_factor(gpu, shape, native, monkey
     for dx, dw in (want, rows):
         within(dx.reshape(tokens, 256), rdx, b_dx, H)
         within(dw, rdw, b_dw, H)
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+@pytest.mark.parametrize("tokens,rows,smoothing", [(600, 256, 0.1), (513, 256, 0.0), (257, 256, 0.1), (256, 256, 0.0)])
+def test_a_forward_in_several_launches_and_its_backward(gpu, tokens, rows, smoothing, reduction, monkeypatch):
+    """A last launch of one row, one whose rows are all ignored: the losses are reduced once, over all of them."""
+    import hpfp8
+    from hpfp8 import _lib
+    from hpfp8 import loss as module
+    x, w, t = make(tokens, 64, 500, 17)
+    t[256:512] = IGNORE
+    if tokens == 513:
+        t[512] = 3
+    names, call = [], _lib.call
+    monkeypatch.setattr(_lib, "call", lambda name, *args: names.append(name) or call(name, *args))
+    monkeypatch.setattr(module, "_FORWARD_ROWS", rows)
+    xg, wg = x.to(gpu).requires_grad_(), w.to(gpu).requires_grad_()
+    loss = hpfp8.linear_cross_entropy(xg, wg, t.to(gpu), reduction=reduction, label_smoothing=smoothing)
+    launches = -(-tokens // rows)
+    if launches > 1:
+        assert names.count("hpfp8_linear_cross_entropy_forward") == launches
+        assert names.count("hpfp8_linear_cross_entropy_reduce") == (reduction != "none")
+    counted = t != IGNORE
+    n = counted.sum() if reduction == "mean" else 1
+    go = torch.randn((tokens,), generator=torch.Generator().manual_seed(18)) if reduction == "none" else torch.tensor(0.7)
+    dx, dw = torch.autograd.grad(loss, (xg, wg), go.to(gpu))
+    each, rdx, rdw, b_rows, b_dx, b_dw = reference(x, w, t, smoothing, (go / n).expand(tokens))
+    if reduction == "none":
+        within(loss.detach(), each, b_rows)
+    else:
+        within(loss.detach(), each.sum() / n, (b_rows * counted).sum() / n + U * (each.sum() / n).abs())
+    within(dx, rdx, b_dx, H)
+    within(dw, rdw, b_dw, H)
+    with torch.no_grad():
+        assert torch.equal(hpfp8.linear_cross_entropy(xg, wg, t.to(gpu), reduction=reduction, label_smoothing=smoothing), loss)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_more_tokens_than_a_forward_takes(gpu, reduction):
+    import hpfp8
+    from hpfp8 import loss as module
+    tokens = module._FORWARD_ROWS + 3001
+    x, w, t = (v.to(gpu) for v in make(tokens, 64, 300, 19))
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = hpfp8.linear_cross_entropy(xg, wg, t, reduction=reduction, label_smoothing=0.1)
+    dx, dw = torch.autograd.grad(loss, (xg, wg))
+    counted = t != IGNORE
+    n = counted.sum() if reduction == "mean" else torch.ones((), device=gpu)
+    each, rdx, rdw, b_rows, b_dx, b_dw = reference(x, w, t, 0.1, (1 / n.double()).expand(tokens))
+    within(loss.detach(), (each.sum() / n).cpu(), ((b_rows * counted).sum() / n + U * (each.sum() / n).abs()).cpu())
+    within(dx, rdx.cpu(), b_dx.cpu(), H)
+    within(dw, rdw.cpu(), b_dw.cpu(), H)
+
+
+def test_both_host_paths_cut_the_vocabulary_alike(gpu, monkeypatch):
+    """By bytes and by elements: the pieces' bits in dx, which is summed over them, are those of the same pieces."""
+    import hpfp8
+    from hpfp8 import loss as module, ops
+    x, w, t = (v.to(gpu) for v in make(90, 64, 3000, 20))
+
+    def step():
+        a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+        return torch.autograd.grad(hpfp8.linear_cross_entropy(a, b, t), (a, b))
+    whole = step()
+    for name, value, pieces in (("_PIECE_BYTES", 4 * 256 * 1024, 3), ("_PIECE_ELEMENTS", 512 * 64 + 1, 6)):
+        with monkeypatch.context() as m:
+            m.setattr(module, name, value)
+            assert len(module._pieces(90, 64, 3000, module._PIECE_BYTES)) == pieces
+            native = step()
+            m.setattr(ops, "_native", None)
+            python = step()
+        assert all(torch.equal(p, q) for p, q in zip(native, python)) and torch.equal(native[1], whole[1])
+        assert not torch.equal(native[0], whole[0])
