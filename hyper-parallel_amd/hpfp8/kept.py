@@ -181,10 +181,11 @@ def keep_activations_8bit(min_elements: int = 1 << 16, dtypes: Sequence[torch.dt
         yield
 
 
-def _forward(x2, kind: int, cols: int, keep: bool):
-    """(y[rows, cols], codes, scale_inv): the last two None unless x is kept."""
-    rows, halves = x2.shape[0], 2 if kind == 3 else 1
-    y = torch.empty((rows, cols), dtype=x2.dtype, device=x2.device)
+def _forward(x2, kind: int, shape, keep: bool):
+    """(y of that shape, codes, scale_inv): the last two None unless x is kept."""
+    rows, cols, halves = x2.shape[0], shape[-1], 2 if kind == 3 else 1
+    # (not made as rows and returned as a view of them: an autograd function's result that is a view can't be written to)
+    y = torch.empty(shape, dtype=x2.dtype, device=x2.device)
     codes = scale_inv = None
     if keep:
         codes = torch.empty((rows, halves * cols), dtype=ops.FP8, device=x2.device)
@@ -198,12 +199,11 @@ class _Activation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, kind, keep):
         cols = x.shape[-1] // (2 if kind == 3 else 1)
-        x2 = _as_rows(x, x.shape[-1])
-        y, codes, scale_inv = _forward(x2, kind, cols, keep)
+        y, codes, scale_inv = _forward(_as_rows(x, x.shape[-1]), kind, x.shape[:-1] + (cols,), keep)
         # (as it was: x itself, so that a write to it in between is noticed)
         ctx.save_for_backward(*((codes, scale_inv) if keep else (x,)))
-        ctx.kind, ctx.keep, ctx.cols, ctx.shape = kind, keep, cols, x.shape
-        return y.reshape(x.shape[:-1] + (cols,))
+        ctx.kind, ctx.keep, ctx.shape = kind, keep, x.shape
+        return y
 
     @staticmethod
     @once_differentiable
@@ -262,4 +262,4 @@ def activation(input: torch.Tensor, kind: str, *, keep_8bit: bool = True) -> tor
     if torch.is_grad_enabled() and input.requires_grad:
         return ops._apply(_Activation, int(bool(keep_8bit)), input, k, bool(keep_8bit))
     cols = input.shape[-1] // (2 if kind == "swiglu" else 1)
-    return _forward(_as_rows(input.detach(), input.shape[-1]), k, cols, False)[0].reshape(input.shape[:-1] + (cols,))
+    return _forward(_as_rows(input.detach(), input.shape[-1]), k, input.shape[:-1] + (cols,), False)[0]

@@ -15,10 +15,11 @@ MAX_WIDTH = 16384
 _OF_CODE = {code: dtype for dtype, code in _TYPES.items()}
 
 
-def _forward(x2, weight, bias, eps, stats: bool, keep: bool):
-    """(y, mean, rstd, codes, scale_inv); without ``stats`` the middle two are None, without ``keep`` the last two, with it the mean."""
+def _forward(x2, weight, bias, eps, stats: bool, keep: bool, shape=None):
+    """(y of that shape, mean, rstd, codes, scale_inv); without ``stats`` the middle two are None, without ``keep`` the last two, with it the mean."""
     rows, cols = x2.shape
-    y = torch.empty((rows, cols), dtype=x2.dtype, device=x2.device)
+    # (not made as rows and returned as a view of them: an autograd function's result that is a view can't be written to)
+    y = torch.empty(x2.shape if shape is None else shape, dtype=x2.dtype, device=x2.device)
     mean = rstd = codes = scale_inv = None
     if stats:
         rstd = torch.empty((rows,), dtype=torch.float32, device=x2.device)
@@ -40,7 +41,7 @@ class _LayerNorm(torch.autograd.Function):
         x2 = _as_rows(x, cols)
         w = None if weight is None else weight.reshape(-1).contiguous()
         b = None if bias is None else bias.reshape(-1).contiguous()
-        y, mean, rstd, codes, scale_inv = _forward(x2, w, b, eps, True, keep)
+        y, mean, rstd, codes, scale_inv = _forward(x2, w, b, eps, True, keep, x.shape)
         if keep:
             ctx.save_for_backward(codes, scale_inv, rstd, weight)
         else:
@@ -48,7 +49,7 @@ class _LayerNorm(torch.autograd.Function):
         ctx.keep, ctx.cols, ctx.shape, ctx.dtype = keep, cols, x.shape, x.dtype
         vector = weight if weight is not None else bias
         ctx.vector = None if vector is None else (vector.shape, vector.dtype)
-        return y.reshape(x.shape)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -121,7 +122,7 @@ def layer_norm(input: torch.Tensor, normalized_shape: Union[int, Sequence[int]],
         return ops._apply(_LayerNorm, 2, input, weight, bias, cols, float(eps), bool(keep_8bit))
     w = None if weight is None else weight.detach().reshape(-1).contiguous()
     b = None if bias is None else bias.detach().reshape(-1).contiguous()
-    return _forward(_as_rows(input.detach(), cols), w, b, float(eps), False, False)[0].reshape(input.shape)
+    return _forward(_as_rows(input.detach(), cols), w, b, float(eps), False, False, input.shape)[0]
 
 
 class LayerNorm(nn.LayerNorm):
