@@ -6,7 +6,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-WAYS = ["mode", "vmap", "grad", "forward_ad", "trace", "batched_backward", "create_graph", "checkpoint", "reentrant", "dispatching_grad",
+WAYS = ["mode", "vmap", "grad", "forward_ad", "trace", "trace_inference", "batched_backward", "create_graph", "checkpoint", "reentrant", "dispatching_grad",
         "sparse_grad", "detect_anomaly", "in_place", "twice", "retained", "other_stream", "hooks"]
 
 
