@@ -167,7 +167,7 @@ def keep_activations_8bit(min_elements: int = 1 << 16, dtypes: Sequence[torch.dt
     def pack(t):
         if (type(t) is not torch.Tensor or not t.is_cuda or t.dtype not in dtypes or t.dim() < 1 or t.numel() < min_elements
                 or not _takes_less(t) or _own(t) or _is_parameter(t) or (select is not None and not select(t))):
-            return t
+            return t.detach()            # (a node that saves its own result would own itself through t)
         with torch.cuda.device(t.device):
             return _Saved(*_quantize(t.detach(), True), t.dtype)
 
