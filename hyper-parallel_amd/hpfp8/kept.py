@@ -117,10 +117,15 @@ def quantize_activation(x: torch.Tensor) -> Fp8Activation:
 
 
 class _Saved(NamedTuple):
-    """What `keep_activations_8bit` puts in a tensor's place."""
+    """What `keep_activations_8bit` puts in a tensor's place; `_AsItIs` for those that stay."""
     codes: torch.Tensor
     scale_inv: torch.Tensor
     dtype: torch.dtype
+
+
+class _AsItIs(NamedTuple):
+    tensor: torch.Tensor
+    version: int
 
 
 def _is_parameter(t: torch.Tensor) -> bool:
@@ -167,13 +172,16 @@ def keep_activations_8bit(min_elements: int = 1 << 16, dtypes: Sequence[torch.dt
     def pack(t):
         if (type(t) is not torch.Tensor or not t.is_cuda or t.dtype not in dtypes or t.dim() < 1 or t.numel() < min_elements
                 or not _takes_less(t) or _own(t) or _is_parameter(t) or (select is not None and not select(t))):
-            return t.detach()            # (a node that saves its own result would own itself through t)
+            return _AsItIs(t.detach(), t._version)         # (detached: a node that saves its own result would own itself through t)
         with torch.cuda.device(t.device):
             return _Saved(*_quantize(t.detach(), True), t.dtype)
 
     def unpack(kept):
-        if not isinstance(kept, _Saved):
-            return kept
+        if isinstance(kept, _AsItIs):
+            if kept.tensor._version != kept.version:       # (torch looks at this itself where there are no hooks)
+                raise RuntimeError(f"one of the variables needed for gradient computation has been modified by an inplace operation: "
+                                   f"{tuple(kept.tensor.shape)} of {kept.tensor.dtype} is at version {kept.tensor._version}; expected version {kept.version}")
+            return kept.tensor
         with torch.cuda.device(kept.codes.device):
             return _dequantize(kept.codes, kept.scale_inv, kept.dtype, True)
 
