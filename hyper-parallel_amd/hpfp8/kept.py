@@ -267,8 +267,7 @@ def activation(input: torch.Tensor, kind: str, *, keep_8bit: bool = True) -> tor
     if kind == "swiglu" and input.shape[-1] % 2:
         raise ValueError(f"swiglu takes gate | up in the last dimension, which is {input.shape[-1]}")
     k = KINDS[kind]
-    # (a trace keeps the autograd function; of kernels launched outside of one it would keep nothing but their empty results)
-    if torch.jit.is_tracing() or (torch.is_grad_enabled() and input.requires_grad):
+    if ops._in_graph(input):
         return ops._apply(_Activation, int(bool(keep_8bit)), input, k, bool(keep_8bit))
     cols = input.shape[-1] // (2 if kind == "swiglu" else 1)
     return _forward(_as_rows(input.detach(), input.shape[-1]), k, input.shape[:-1] + (cols,), False)[0]

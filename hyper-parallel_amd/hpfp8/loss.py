@@ -200,8 +200,7 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
         _main_grad_of(weight)
     flat = target.reshape(-1).contiguous()
     r = _REDUCTIONS[reduction]
-    # (a trace keeps the autograd function; of kernels launched outside of one it would keep nothing but their empty results)
-    if torch.jit.is_tracing() or (torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad)):
+    if ops._in_graph(input, weight):
         loss = ops._apply(_LinearCrossEntropy, 2, input, weight, flat, int(ignore_index), r, float(label_smoothing),
                                          weight if apply_grad_on_fp32_main_grad else None)
     else:

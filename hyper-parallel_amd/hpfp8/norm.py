@@ -118,8 +118,7 @@ def layer_norm(input: torch.Tensor, normalized_shape: Union[int, Sequence[int]],
                 raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"weight and bias must be of one type, got {weight.dtype} and {bias.dtype}")
-    # (a trace keeps the autograd function; of kernels launched outside of one it would keep nothing but their empty results)
-    if torch.jit.is_tracing() or (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)):
+    if ops._in_graph(*tensors):
         return ops._apply(_LayerNorm, 2, input, weight, bias, cols, float(eps), bool(keep_8bit))
     w = None if weight is None else weight.detach().reshape(-1).contiguous()
     b = None if bias is None else bias.detach().reshape(-1).contiguous()

@@ -14,6 +14,7 @@ import ctypes
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -37,6 +38,14 @@ class _Saving(threading.local):
 
 
 _saving = _Saving()
+
+
+def _in_graph(*tensors) -> bool:
+    """Whether a call on these tensors goes through its autograd function: with gradients to come; under a dual level, where the function raises
+    for a tangent that a kernel by itself would drop; while tracing, as a trace keeps the function, and of kernels launched outside of one nothing
+    but their empty results."""
+    return ((torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or getattr(forward_ad, "_current_level", 0) >= 0
+            or torch.jit.is_tracing())
 
 
 def _apply(function, level: int, *args):

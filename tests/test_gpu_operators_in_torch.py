@@ -148,3 +148,18 @@ def test_results_of_strided_inputs_can_be_written_to(gpu):
         want = torch.autograd.grad(f(x).sum(), x)[0]
         y += 1
         assert torch.equal(y, f(x) + 1) and torch.equal(torch.autograd.grad(y.sum(), x)[0], want)
+
+
+@pytest.mark.parametrize("name", ["norm", "norm_kept", "activation", "activation_kept", "loss_mean", "loss_none"])
+@pytest.mark.parametrize("grad", [True, False])
+def test_a_tangent_is_refused_and_not_dropped(gpu, name, grad):
+    """Forward mode with tensors that require no gradient; without a tangent the level changes nothing."""
+    import torch.autograd.forward_ad as fwAD
+    f, tensors, _ = operator(name)
+    with torch.set_grad_enabled(grad), fwAD.dual_level():
+        for i in range(len(tensors)):
+            dual = [fwAD.make_dual(t, torch.ones_like(t)) if k == i else t for k, t in enumerate(tensors)]
+            with pytest.raises((RuntimeError, NotImplementedError), match="jvp|forward mode"):
+                f(*dual)
+        inside = f(*tensors)
+    assert torch.equal(inside, f(*tensors))
