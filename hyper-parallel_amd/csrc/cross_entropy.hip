@@ -650,6 +650,11 @@ __global__ __launch_bounds__(256) void ce_round_kernel(const float* __restrict__
   reinterpret_cast<u32x4_st*>(out)[i] = u32x4_st{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])};
 }
 
+// ---- the weight's gradient of no tokens
+__global__ __launch_bounds__(256) void ce_zero_kernel(u32x4_st* __restrict__ out, int64_t n16) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n16; i += (int64_t)gridDim.x * 256) out[i] = u32x4_st{0, 0, 0, 0};
+}
+
 // Elements between the rows of the workspaces: whole tiles, and an odd number of 128-byte lines, so that the rows of a tile do not all lie
 // in the same few memory channels (the gradients' launch of 4096 tokens, 7168, 16384 columns: 1480 us with strides of 2^13 and 2^15 bytes).
 int64_t up(int64_t n, int64_t to);
@@ -832,7 +837,13 @@ int hpfp8_linear_cross_entropy_piece(const void* x, int64_t ld_x, const void* x_
   HPFP8_REQUIRE(width <= (1 << 21), HPFP8_ERR_SHAPE, "a piece of %lld columns: at most 2^21", (long long)width);
   HPFP8_REQUIRE(width * ld_w < kPieceElements, HPFP8_ERR_SHAPE, "a piece of %lld rows of the weight spans 2 GiB or more", (long long)width);
   HPFP8_REQUIRE(!dw_add || dw_type == HPFP8_OUT_F32, HPFP8_ERR_ARG, "only fp32 is added onto");
-  if (tokens == 0) return HPFP8_OK;
+  if (tokens == 0) {
+    if (!dw || dw_add) return HPFP8_OK;
+    HPFP8_REQUIRE(aligned16(dw), HPFP8_ERR_ALIGN, "a buffer is not 16-byte aligned");
+    const int64_t size = dw_type == HPFP8_OUT_F32 ? 4 : 2, n16 = width * hidden * size / 16, blocks = (n16 + 255) / 256;
+    ce_zero_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, (hipStream_t)stream>>>((u32x4_st*)((uint8_t*)dw + first * hidden * size), n16);
+    return check_launch("linear_cross_entropy_piece (no tokens)");
+  }
   HPFP8_REQUIRE(x && w && target && lse && grad && dl && dl_t && (!dw == !x_t), HPFP8_ERR_ARG, "null buffer");
   HPFP8_REQUIRE(aligned16(x) && aligned16(w) && aligned16(dl) && aligned16(dl_t) && aligned16(x_t) && aligned16(dx) && aligned16(dw),
                 HPFP8_ERR_ALIGN, "a buffer is not 16-byte aligned");

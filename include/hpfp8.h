@@ -559,7 +559,8 @@ int hpfp8_linear_cross_entropy_reduce(const float* loss, const int64_t* target, 
                                       float* count, hpfp8_stream_t stream);
 /* The backward's part of the vocabulary's columns [first, first + width): the gradient of the logits, rounded to bf16, and with it
  * dx (fp32 [splits, tokens, hidden], the parts of a sum; dx_add: added onto) and rows [first, first + width) of dw ([vocab, hidden],
- * dw_type HPFP8_OUT_*; dw_add: added onto, fp32 only).  Either may be NULL.  grad is the loss's gradient, one value
+ * dw_type HPFP8_OUT_*; dw_add: added onto, fp32 only).  Either may be NULL.  With no tokens
+ * (x, target and the workspaces may be NULL then) those rows of dw are zeros.  grad is the loss's gradient, one value
  * with grad_stride 0 or one for each row; count as the forward wrote it for reduction 1, otherwise NULL.  x_t is what hpfp8_linear_cross_entropy_rows_t makes of x, with row stride
  * S(tokens), S(n) = hpfp8_cross_entropy_stride(n) (needed for dw).  Workspaces, bf16, with R(n) = n rounded up to 256: dl [R(tokens), S(width)],
  * dl_t [R(width), S(tokens)].  The piece's rows of w span less than 2 GiB and are at most 2^21.  splits: what

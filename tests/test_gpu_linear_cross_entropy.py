@@ -508,3 +508,13 @@ def test_both_host_paths_cut_the_vocabulary_alike(gpu, monkeypatch):
             python = step()
         assert all(torch.equal(p, q) for p, q in zip(native, python)) and torch.equal(native[1], whole[1])
         assert not torch.equal(native[0], whole[0])
+
+
+@pytest.mark.parametrize("dtype,add", [(torch.bfloat16, 0), (torch.float32, 0), (torch.float32, 1)])
+def test_a_piece_of_no_tokens(gpu, dtype, add):
+    """Through the C entry: its rows of the weight's gradient are zeros, or as they were if they are added onto, all others untouched."""
+    from hpfp8 import _lib, ops
+    dw = torch.full((2500, 72), 3.0, dtype=dtype, device=gpu)
+    _lib.call("hpfp8_linear_cross_entropy_piece", None, 72, None, None, 72, None, 0, 72, 2500, 256, 2000, -100, 0.0, None, None, 0, None, None, None, None, 1, 0,
+              ops._ptr(dw), _lib.OUT_F32 if dtype == torch.float32 else _lib.OUT_BF16, add, ops._stream())
+    assert (dw[:256] == 3).all() and (dw[2256:] == 3).all() and (dw[256:2256] == (3 if add else 0)).all()

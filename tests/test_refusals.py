@@ -234,3 +234,10 @@ def test_saved_rows_in_8_bits(p):
     assert c(q, p, 0, 4, 8, 8, p, None, None)[0] == -1 and c(q, p, 0, 1, 1 << 40, 8, p, p, None)[0] == -2 and c(q, None, 0, 0, 8, 8, None, None, None)[0] == 0
     assert c(d, p, p, 4, 8, p, 7, None)[0] == -1 and c(d, p, p, 4, 8, p + 1, 2, None)[0] == -3 and c(d, None, p, 4, 8, p, 2, None)[0] == -1
     assert c(d, None, None, 0, 8, None, 2, None)[0] == 0
+
+
+def test_a_weight_gradient_of_no_tokens_is_checked_too(p):
+    def piece(dw, dw_add=0, dw_type=0):
+        return c("hpfp8_linear_cross_entropy_piece", None, 64, None, None, 64, None, 0, 64, 10, 0, 10, -100, 0.0, None, None, 0, None, None, None, None, 1, 0,
+                 dw, dw_type, dw_add, None)[0]
+    assert piece(p + 8) == -3 and piece(p, 1, 1) == 0 and piece(None) == 0
