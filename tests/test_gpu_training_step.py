@@ -165,3 +165,35 @@ def test_operators_on_another_stream_and_two_at_once(gpu):
         torch.cuda.synchronize()
         for g, r in zip(got, want):
             assert all(torch.equal(p, q) for p, q in zip(g, r))
+
+
+def test_a_step_inside_the_context_in_a_graph(gpu):
+    """What torch code saves is kept in 8 bits and read back within the capture; replayed with other inputs and eager work in between."""
+    import hpfp8
+    w, head, nw = randn((512, 256), 50, 0.05).requires_grad_(), randn((700, 256), 51, 0.05).requires_grad_(), randn((256,), 52).requires_grad_()
+    batches = [(randn((90, 256), 53 + i), torch.randint(700, (90,), generator=torch.Generator().manual_seed(60 + i)).cuda()) for i in range(3)]
+
+    def step(x, target):
+        x = x.detach().requires_grad_()
+        with hpfp8.keep_activations_8bit(min_elements=1000):
+            h = torch.nn.functional.linear(hpfp8.layer_norm(x, 256, nw), w)
+            gate, up = h.chunk(2, -1)
+            y = torch.nn.functional.silu(gate.masked_fill(gate > 2, -math.inf).clamp(min=-9)) * up
+            each = hpfp8.linear_cross_entropy(y, head, target, reduction="none")
+        return (each.detach(),) + torch.autograd.grad(each.mean(), (x, w, head, nw))
+    x, target = batches[0][0].clone(), batches[0][1].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, target)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outputs = step(x, target)
+    for a, b in batches + batches:
+        want = [t.clone() for t in step(a, b)]
+        x.copy_(a)
+        target.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(outputs, want)) and all(t.isfinite().all() for t in want)
