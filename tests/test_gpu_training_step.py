@@ -197,3 +197,40 @@ def test_a_step_inside_the_context_in_a_graph(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(outputs, want)) and all(t.isfinite().all() for t in want)
+
+
+def test_threads_side_by_side(gpu):
+    """Each on a stream of its own, half of them inside the context, which is a thread's own: results as one after the other."""
+    import contextlib
+    import threading
+    import hpfp8
+    head, nw, w = randn((1500, 256), 70, 0.05), randn((256,), 71), randn((256, 256), 72, 0.1)
+    inputs = [(randn((200 + 50 * i, 256), 73 + i), torch.randint(1500, (200 + 50 * i,), generator=torch.Generator().manual_seed(i)).cuda()) for i in range(4)]
+
+    def step(i):
+        x, t = inputs[i]
+        leaves = [v.clone().requires_grad_() for v in (x, head, nw, w)]
+        with hpfp8.keep_activations_8bit(min_elements=1000) if i % 2 else contextlib.nullcontext():
+            y = torch.nn.functional.silu(hpfp8.fp8_linear(hpfp8.layer_norm(leaves[0], 256, leaves[2]), leaves[3]))
+            loss = hpfp8.linear_cross_entropy(hpfp8.activation(y, "gelu"), leaves[1], t)
+        return torch.autograd.grad(loss, leaves)
+    want = [step(i) for i in range(4)]
+    torch.cuda.synchronize()
+    got, errors = [[None] * 5 for _ in range(4)], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for k in range(5):
+                    got[i][k] = step(i)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for i in range(4):
+        assert all(torch.equal(p, q) for k in range(5) for p, q in zip(got[i][k], want[i]))
