@@ -250,8 +250,8 @@ def activation(input: torch.Tensor, kind: str, *, keep_8bit: bool = True) -> tor
 
     kind: "silu", "gelu", "gelu_tanh" (the tanh form), or "swiglu": input [..., 2C] = gate | up, result silu(gate) * up [..., C].
     bfloat16, float16 or float32, any width; computed in fp32 and rounded once.  The result is that of the input as it is; the
-    gradient is taken where the codes are (each half of a SwiGLU input has scaling groups of its own).  ``keep_8bit=False`` keeps the
-    input itself."""
+    gradient is taken where the codes are (each half of a SwiGLU input has scaling groups of its own; an infinity or a NaN in the input makes the
+    gradient of its group of 128 NaN).  ``keep_8bit=False`` keeps the input itself."""
     if torch.overrides.has_torch_function((input,)):
         return _hand_off(activation, (input,), (input, kind), dict(keep_8bit=keep_8bit), _ACTIVATION_DEFAULTS)
     if kind not in KINDS:
