@@ -40,3 +40,21 @@ def test_a_write_to_a_saved_tensor_is_noticed():
         y.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(y, x, go)
+
+
+@pytest.mark.parametrize("second", [False, True])
+def test_gradients_of_what_stays_are_those_outside(second):
+    """Operations in place, nodes that save their result, views; first and second derivatives."""
+    import contextlib
+    import hpfp8
+    x, w = torch.randn(30, 40, generator=torch.Generator().manual_seed(0)), torch.randn(30, 40, generator=torch.Generator().manual_seed(1))
+    for f in (lambda x, w: ((x * 1).relu_() * w).sigmoid_() * w, lambda x, w: ((x * 0.1) ** 3).cumsum(0).exp() * w, lambda x, w: torch.linalg.norm(x @ w.t(), dim=1),
+              lambda x, w: x.t().contiguous().view(-1)[::3] ** 2 * w.view(-1)[::3]):
+        results = []
+        for context in (contextlib.nullcontext(), hpfp8.keep_activations_8bit(min_elements=1)):
+            leaves = [t.clone().requires_grad_() for t in (x, w)]
+            with context:
+                y = f(*leaves)
+                grads = torch.autograd.grad((y * y).sum(), leaves, create_graph=second)
+            results.append(torch.autograd.grad(sum(g.sum() for g in grads), leaves) if second else grads)
+        assert all(torch.equal(p, q) for p, q in zip(*results))
