@@ -5,25 +5,28 @@ Usage: python build.py [--force]
 """
 from __future__ import annotations
 
+import concurrent.futures
 import importlib.util
 import os
 import subprocess
 import sys
 import sysconfig
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "hpfp8", "libhpfp8.so")
 NATIVE = os.path.join(HERE, "hpfp8", "_native.so")
 NATIVE_SOURCE = os.path.join(CSRC, "torch_ops.cpp")
-SOURCES = ["capi.hip", "quantize.hip", "bucket.hip", "grouped.hip", "gemm.hip", "gemm_skinny.hip", "activation.hip", "norm.hip", "cross_entropy.hip"]
-HEADERS = ["rows.h", "gemm_skinny.h", "gemm_tile.h", "hpfp8_device.h", "hpfp8_host.h", os.path.join("..", "..", "include", "hpfp8.h")]
+SOURCES = ["capi.hip", "quantize.hip", "bucket.hip", "grouped.hip", "gemm.hip", "gemm_skinny.hip", "activation.hip", "norm.hip", "rms_norm.hip",
+           "rms_norm_backward.hip", "quantize_int8.hip", "grad_norm.hip", "cross_entropy.hip"]
+HEADERS = ["rows.h", "norm_rows.h", "gemm_skinny.h", "gemm_tile.h", "hpfp8_device.h", "hpfp8_host.h", os.path.join("..", "..", "include", "hpfp8.h")]
 
 
 def _flags():
     # full IEEE division/sqrt, denormals kept, no packed fp32 arithmetic
     return [
-        "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+        "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
         "-fno-fast-math", "-ffp-contract=off", "-fno-gpu-flush-denormals-to-zero",
         "-fhip-fp32-correctly-rounded-divide-sqrt",
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -89,7 +92,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
     """Each of the two where it is stale (``force``: both); the library first, which the package can do with alone."""
     if force or library_stale():
         hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-        _run([hipcc] + _flags() + [os.path.join(CSRC, s) for s in SOURCES] + ["-o", OUT], verbose)
+        with tempfile.TemporaryDirectory() as made, concurrent.futures.ThreadPoolExecutor(min(len(SOURCES), 8, os.cpu_count() or 1)) as pool:
+            objects = [os.path.join(made, s + ".o") for s in SOURCES]
+            list(pool.map(lambda s, o: _run([hipcc] + _flags() + ["-c", os.path.join(CSRC, s), "-o", o], verbose), SOURCES, objects))
+            _run([hipcc] + _flags() + ["-shared"] + objects + ["-o", OUT], verbose)
     if force or native_stale():
         _run(_native_command(), verbose)
     return OUT

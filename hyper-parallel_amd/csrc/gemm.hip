@@ -59,7 +59,9 @@ constexpr int kRectTiles = 32;              // tiles of the rectangle one XCD (3
 // applies them itself (its E8M0 block-scale operands) and accumulates across k-blocks, so there is no
 // promotion arithmetic at all.
 // kScalePow2Row: the same with the scales laid out as for kScaleRow.
-enum ScaleMode { kScaleTensor = 0, kScaleBlock = 1, kScaleRow = 2, kScalePow2 = 3, kScalePow2Row = 4 };
+// kInt8: codes are int8, sums int32 (exact), one scale for each row of a and one for each row of b, applied to the finished sums.
+enum ScaleMode { kScaleTensor = 0, kScaleBlock = 1, kScaleRow = 2, kScalePow2 = 3, kScalePow2Row = 4, kInt8 = 5 };
+__host__ __device__ constexpr bool end_scales(int mode) { return mode == kScaleTensor || mode == kInt8; }     // no scales of k-blocks
 
 enum Grouping { kDense = 0, kGroupedRows = 1, kGroupedK = 2 };
 
@@ -90,6 +92,7 @@ struct GemmParams {
   int pow2_out;
   float* q_scale;
   float* q_scale_inv;
+  int value_type;         // int8: element type of c and of bias
   int choose_cus;         // grouped by rows, tile chosen on the device: the compute units there are (test hook: minus the rows asked for)
 };
 
@@ -267,7 +270,7 @@ constexpr int kScaleSlot = 2048;
 // reads, those to other buffers included: the transfers' latency would be paid in every round.)
 __host__ __device__ constexpr int tile_lds(int mode, int wm, int tn) {
   const int stages = tile_stages(mode, wm, tn);
-  const int scales = fetchers(wm) ? (mode == kScaleTensor ? 0 : (stages + 1) * kScaleSlot) : (mode == kScalePow2Row ? 3 * 256 * 4 : 0);
+  const int scales = fetchers(wm) ? (end_scales(mode) ? 0 : (stages + 1) * kScaleSlot) : (mode == kScalePow2Row ? 3 * 256 * 4 : 0);
   return (fetchers(wm) ? stages : 2) * 64 * wm * BK + stages * tn * BK + scales;
 }
 
@@ -315,7 +318,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmParams& p, uint8_t* const l
   static_assert(EPI == 0 || TN == 256, "SwiGLU epilogue: 128 gate and 128 up columns per tile");
   static_assert(EPI == 0 || ((MODE == kScaleBlock || MODE == kScalePow2) && GROUPED == kDense && !OUT_F32 && !ACC),
                 "SwiGLU epilogue: dense block-scaled forward");
-  static_assert(!ACC || (OUT_F32 && MODE != kScaleTensor), "accumulating onto c: fp32 output, sums that start from c's values");
+  static_assert(!ACC || (OUT_F32 && !end_scales(MODE)), "accumulating onto c: fp32 output, sums that start from c's values");
   static_assert(GROUPED != kGroupedK || (!ACC && (MODE == kScaleRow || MODE == kScalePow2Row)),
                 "grouped along the contraction: the wgrad form");
   static_assert(!kFetchers || GROUPED != kGroupedK, "the fetching waves count k-blocks from 0");
@@ -327,7 +330,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmParams& p, uint8_t* const l
   constexpr bool kPromote = MODE == kScaleBlock || MODE == kScaleRow;       // partial sums scaled by FMAs
   constexpr bool kHwScale = MODE == kScalePow2 || MODE == kScalePow2Row;    // scales applied by the MFMA
   constexpr int kBAhead = kBStages - 1;     // k-blocks between issuing a b transfer and using it
-  constexpr int kScaleOps = MODE == kScaleTensor ? 0 : 2, kScaleSlots = kBStages + 1;
+  constexpr int kScaleOps = end_scales(MODE) ? 0 : 2, kScaleSlots = kBStages + 1;
   // per-row scales of the b operand for one k-block (wgrad form, powers of two), three stages of 256 floats: the
   // stage of k-block kb+1 is filled while slower waves may still read that of kb-1
   uint8_t* const scale_lds = lds + kAStages * kATile + kBStages * kBTile;
@@ -529,7 +532,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmParams& p, uint8_t* const l
   // that they span less than 2 GiB): the row part of an offset is per tile, the k-block part a
   // scalar, so a round spends no vector arithmetic on addresses.
   const __amdgpu_buffer_rsrc_t rsrc_sa = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)p.sa, 0, MODE == kScaleTensor ? 4 : (int)((((int64_t)p.M - 1) * p.sa_sm + ((int64_t)kblocks - 1) * p.sa_sk + 1) * 4),
+      (void*)p.sa, 0, end_scales(MODE) ? 4 : (int)((((int64_t)p.M - 1) * p.sa_sm + ((int64_t)kblocks - 1) * p.sa_sk + 1) * 4),
       0x00020000);
   const __amdgpu_buffer_rsrc_t rsrc_sbb = __builtin_amdgcn_make_buffer_rsrc((void*)p.sb, 0, p.sb_bytes, 0x00020000);
   uint32_t sa_voff[4];         // byte offset of this lane's four rows in sa (SA4: [0] covers all four)
@@ -558,7 +561,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmParams& p, uint8_t* const l
     }
     if (MODE == kScaleBlock || MODE == kScalePow2)
       raw[4] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc_sbb, 0, sb_soff + kb * sb_kstep, 0));
-    if (MODE != kScaleTensor) {
+    if (!end_scales(MODE)) {
       if (SA4) {
         const v4f four = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rsrc_sa, sa_voff[0], kb * sa_kstep, 0));
 #pragma unroll
@@ -655,7 +658,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmParams& p, uint8_t* const l
     }
   }
   auto read_scales = [&](int slot, float raw[6]) {      // (kFetchers)
-    if (MODE == kScaleTensor) return;
+    if (end_scales(MODE)) return;
     const uint8_t* const src = scale_lds + slot * kScaleSlot + (wm * 2 + wn * 2 / WN) * 256;
     if (MODE == kScaleRow) {
 #pragma unroll
@@ -960,6 +963,8 @@ __device__ __forceinline__ void gemm_tiles(const GemmParams& p, uint8_t* const l
           if (kHwScale)
             acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[i % 3], xf[j], acc[i][j], 0, 0, 0,
                                                                         MODE == kScalePow2 ? e_b : e_bi[i & 1], 0, e_a[j]);
+          else if (MODE == kInt8)
+            acc[i][j] = multiply_int8(wf[i % 3], xf[j], acc[i][j]);
           else
             acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[i % 3], xf[j], acc[i][j], 0, 0, 0, 0, 0, 0);
           if (!kTwoX && i == NS - 1) xn[j] = frag_read(anxt + a_frag + j * 16 * BK, frag_lo, frag_hi);
@@ -1043,6 +1048,41 @@ __device__ __forceinline__ void gemm_tiles(const GemmParams& p, uint8_t* const l
       cols_ok && rows_valid > 0 ? (int)((((int64_t)rows_valid - 1) * p.ldc + WC) * kEsize) : 0, 0x00020000);
   const uint32_t st_lane = (uint32_t)(((wm * 64 + ge * 4) * (int)p.ldc) * kEsize + l16e * 16);
   const int st_row = (int)p.ldc * kEsize;        // bytes from one row of c to the next
+  if constexpr (MODE == kInt8) {
+    // The sums become values where they are: times both scales, plus the bias.  The scales come from memory here (loaded in the passes below
+    // they would be waited for 32 times a tile, behind the transfers under way).
+    if (cols_ok) {
+      float sa_row[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = row0 + wm * 64 + l16e * 4 + j;
+        sa_row[j] = p.sa[r < p.M ? r : p.M - 1];
+      }
+      constexpr int kPart = 2;                       // (256 x 256 tiles have no registers for more)
+#pragma unroll
+      for (int i0 = 0; i0 < NS; i0 += kPart) {
+        v4f by[kPart];
+#pragma unroll
+        for (int i = 0; i < kPart; ++i) by[i] = p.sb ? *reinterpret_cast<const v4f*>(p.sb + ncol + (i0 + i) * 16 + ge * 4) : v4f{1.f, 1.f, 1.f, 1.f};
+#pragma unroll
+        for (int i = 0; i < kPart; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const v4i sums = __builtin_bit_cast(v4i, acc[i0 + i][j]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i0 + i][j][r] = (float)sums[r] * sa_row[j] * by[i][r];
+          }
+        if (p.bias) {
+#pragma unroll
+          for (int i = 0; i < kPart; ++i) by[i] = load_bias4(p.bias, p.value_type, ncol + (i0 + i) * 16 + ge * 4);
+#pragma unroll
+          for (int i = 0; i < kPart; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i0 + i][j] += by[i];
+        }
+      }
+    }
+  }
   auto store_tile = [&](auto with_bias) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -1068,8 +1108,13 @@ __device__ __forceinline__ void gemm_tiles(const GemmParams& p, uint8_t* const l
             asm volatile("ds_write_b128 %0, %1" ::"v"(stg_w + (((ii * 4 + ge) ^ l16e) * 16)), "v"(o) : "memory");
           } else {
             u32x2 o;
-            o[0] = pack_bf16x2(v[0], v[1]);
-            o[1] = pack_bf16x2(v[2], v[3]);
+            if (MODE == kInt8 && p.value_type == HPFP8_TYPE_F16) {
+              o[0] = pack_f16x2(v[0], v[1]);
+              o[1] = pack_f16x2(v[2], v[3]);
+            } else {
+              o[0] = pack_bf16x2(v[0], v[1]);
+              o[1] = pack_bf16x2(v[2], v[3]);
+            }
             asm volatile("ds_write_b64 %0, %1" ::"v"(stg_w + (((ii * 2 + (ge >> 1)) ^ l16e) * 16) + (ge & 1) * 8), "v"(o)
                          : "memory");
           }
@@ -1164,7 +1209,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmParams& p, uint8_t* const l
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
   } else if (cols_ok) {
-    if (!p.bias) store_tile(std::false_type{});
+    if (MODE == kInt8 || !p.bias) store_tile(std::false_type{});
     else store_tile(std::true_type{});
   } else {
 #pragma unroll
@@ -1459,7 +1504,7 @@ static bool try_skinny(const GemmParams& p, SkinnyMode mode, int out_type, hipSt
   SkinnyParams q{};
   q.a = p.a; q.b = p.b; q.sa = p.sa; q.sb = p.sb; q.lda = p.lda; q.ldb = p.ldb;
   q.sa_sm = p.sa_sm; q.sa_sk = p.sa_sk; q.sb_sn = p.sb_sn; q.sb_sk = p.sb_sk; q.sb_bytes = p.sb_bytes;
-  q.bias = p.bias; q.c = p.c; q.ldc = p.ldc; q.M = p.M; q.N = p.N; q.K = p.K; q.out_f32 = out_type == HPFP8_OUT_F32;
+  q.bias = p.bias; q.c = p.c; q.ldc = p.ldc; q.M = p.M; q.N = p.N; q.K = p.K; q.out_f32 = out_type == HPFP8_OUT_F32; q.value_type = p.value_type;
   rc = launch_skinny(q, mode, persistent_grid((int64_t)1 << 40), stream);
   return true;
 }
@@ -1468,7 +1513,7 @@ template <int MODE, int GROUPED, bool SA4, int WM, int NS, int WN>
 static int launch_sa(const GemmParams& p, int out_type, int64_t tiles, hipStream_t stream) {
   dim3 grid((unsigned)persistent_grid(tiles)), block(tile_threads(WM, WN));
   if (out_type == HPFP8_OUT_F32) {
-    if constexpr (MODE != kScaleTensor && GROUPED == kDense) {   // (the per-tensor and grouped entry points have no accumulate)
+    if constexpr (!end_scales(MODE) && GROUPED == kDense) {   // (the per-tensor and grouped entry points have no accumulate)
       if (p.accumulate) {
         gemm_kernel<MODE, GROUPED, true, true, SA4, 0, WM, NS, WN><<<grid, block, 0, stream>>>(p);
         return check_launch("gemm");
@@ -1484,7 +1529,7 @@ static int launch_sa(const GemmParams& p, int out_type, int64_t tiles, hipStream
 template <int MODE, int GROUPED, int WM, int NS, int WN>
 static int launch_shape(const GemmParams& p, int out_type, int64_t tiles, hipStream_t stream) {
   if constexpr (GROUPED == kGroupedK) return launch_sa<MODE, GROUPED, true, WM, NS, WN>(p, out_type, tiles, stream);   // (sa_sm = 1)
-  if constexpr (MODE != kScaleTensor && !fetchers(WM)) {      // (fetched to LDS, sa may have any strides)
+  if constexpr (!end_scales(MODE) && !fetchers(WM)) {      // (fetched to LDS, sa may have any strides)
     if (p.sa_sm == 1) return launch_sa<MODE, GROUPED, true, WM, NS, WN>(p, out_type, tiles, stream);
   }
   if constexpr (GROUPED != kGroupedK) return launch_sa<MODE, GROUPED, false, WM, NS, WN>(p, out_type, tiles, stream);
@@ -1748,6 +1793,24 @@ int hpfp8_gemm_per_tensor(const void* a, int64_t lda, const float* sa_inv, const
   GemmParams p{};
   const int rc = per_tensor_params(a, lda, sa_inv, b, ldb, sb_inv, M, N, K, bias, c, ldc, out_type, p);
   return rc <= 0 ? rc : launch_per_tensor(p, out_type, (hipStream_t)stream);
+}
+
+int hpfp8_gemm_int8(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t M, int64_t N, int64_t K,
+                    const void* bias, void* c, int64_t ldc, int out_type, hpfp8_stream_t stream) {
+  const char* what = "gemm_int8";
+  HPFP8_REQUIRE(out_type >= 0 && out_type <= 2, HPFP8_ERR_ARG, "%s: bad out_type", what);
+  // (rows of c are written in 16-byte pieces: as bf16 where fp16 is written)
+  const int rc = check_common(what, a, lda, b, ldb, sa, sb ? sb : sa, M, N, K, bias, c, ldc, out_type == HPFP8_OUT_F32 ? HPFP8_OUT_F32 : HPFP8_OUT_BF16, 0);
+  if (rc <= 0) return rc;
+  HPFP8_REQUIRE(K <= 130944, HPFP8_ERR_SHAPE, "%s: the sums of K=%lld products of codes do not fit 32 bits", what, (long long)K);
+  HPFP8_REQUIRE(aligned16(sb) && ((uintptr_t)sa & 3) == 0, HPFP8_ERR_ALIGN, "%s: scales are not aligned", what);
+  GemmParams p{};
+  p.a = (const uint8_t*)a; p.b = (const uint8_t*)b; p.sa = sa; p.sb = sb; p.lda = lda; p.ldb = ldb;
+  p.c = c; p.ldc = ldc; p.bias = (const uint16_t*)bias; p.value_type = out_type;
+  p.M = (int)M; p.N = (int)N; p.K = (int)K;
+  int status;
+  if (try_skinny(p, kSkinnyInt8, out_type, (hipStream_t)stream, status)) return status;
+  return launch<kInt8, kDense>(p, out_type, pick_shape(p.M, p.N), (hipStream_t)stream);
 }
 
 int hpfp8_linear_backward(const hpfp8_operand* go, const hpfp8_operand* wt, const hpfp8_operand* go_t, const hpfp8_operand* xt, int64_t M,

@@ -6,8 +6,8 @@
 namespace hpfp8 {
 
 // c[m, n] = sum_kb sa(m, kb) * sb(n / 128, kb) * (A_kb . B_kb^T) (+ bias); kSkinnyPow2: power-of-two scales, applied by the
-// matrix instruction; kSkinnyTensor: one scale each (sa[0], sb[0]).
-enum SkinnyMode { kSkinnyBlock, kSkinnyPow2, kSkinnyTensor };
+// matrix instruction; kSkinnyTensor: one scale each (sa[0], sb[0]); kSkinnyInt8: int8 codes, scales sa[m] and sb[n].
+enum SkinnyMode { kSkinnyBlock, kSkinnyPow2, kSkinnyTensor, kSkinnyInt8 };
 
 struct SkinnyParams {
   const uint8_t* a;
@@ -23,6 +23,7 @@ struct SkinnyParams {
   int64_t ldc;
   int M, N, K;
   int out_f32;
+  int value_type;         // int8: element type of c and of bias
 };
 
 constexpr int kSkinnyMaxRows = 64;        // four fragments of 16 rows; one row more takes tiles (64 rows of [7168, 16384]: 27 us here,

@@ -93,7 +93,8 @@ __device__ __forceinline__ void quantize_k_block(uint8_t* rows, float* scales, i
 // row of a alone, and rows past M are not stored.)
 template <int MODE, int ME, int F, bool QUANT = false>
 __global__ __launch_bounds__(skinny_threads(F, QUANT)) void gemm_skinny_kernel(const SkinnyParams p, int units) {
-  static_assert(!QUANT || (ME == 2 && MODE != kSkinnyTensor), "eight rows of bf16, scales of their own");
+  constexpr bool kBlockScales = MODE != kSkinnyTensor && MODE != kSkinnyInt8;      // scales that travel with the k-blocks
+  static_assert(!QUANT || (ME == 2 && kBlockScales), "eight rows of bf16, scales of their own");
   constexpr int MF = (ME + 1) / 2;                              // 16-row fragments of a
   constexpr int KS = skinny_kstep(ME, F, QUANT), U = skinny_stages(ME, F, QUANT);
   constexpr int kBlockBytes = skinny_block_bytes(ME, F), kStage = skinny_stage_bytes(ME, F, QUANT);
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(skinny_threads(F, QUANT)) void gemm_skinny_kernel(c
     constexpr int KW = KS > kSkinnyWaves ? KS / kSkinnyWaves : 1;       // k-blocks a wave fetches per stage
     constexpr int W = KS < kSkinnyWaves ? kSkinnyWaves / KS : 1;        // waves that fetch one k-block together
     constexpr int NBP = (2 * F + W - 1) / W, NAP = (ME + W - 1) / W;    // a wave's transfers of b and of a per k-block
-    constexpr int kScaleOps = MODE == kSkinnyTensor ? 0 : (W == 1 && !QUANT ? 2 : 1);
+    constexpr int kScaleOps = !kBlockScales ? 0 : (W == 1 && !QUANT ? 2 : 1);
     constexpr int kStageOps = KW * (NBP + NAP + kScaleOps);
     constexpr int kLeft = (U - (QUANT ? 3 : 2)) * kStageOps;            // in flight behind the oldest stage that has to be there
     static_assert(U >= 3 && kLeft <= 63 && (U - 2) * kStageOps <= 63, "the wait counter holds 63");
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(skinny_threads(F, QUANT)) void gemm_skinny_kernel(c
     }
     const uint32_t sa_off = (uint32_t)(lane < p.M ? lane : p.M - 1) * (uint32_t)p.sa_sm * 4u;
     const int a_bytes = (int)((p.M - 1) * p.lda + (QUANT ? 2 * p.K : p.K));
-    const int sa_bytes = MODE == kSkinnyTensor || QUANT ? 0 : (int)(((p.M - 1) * p.sa_sm + (kblocks - 1) * p.sa_sk + 1) * 4);
+    const int sa_bytes = !kBlockScales || QUANT ? 0 : (int)(((p.M - 1) * p.sa_sm + (kblocks - 1) * p.sa_sk + 1) * 4);
     const int sa_step = (int)p.sa_sk * 4, sb_step = (int)p.sb_sk * 4;
     int unit = first, kb = kb0, slot = 0;                       // the next stage to fetch
     const uint8_t* b0;
@@ -168,7 +169,7 @@ __global__ __launch_bounds__(skinny_threads(F, QUANT)) void gemm_skinny_kernel(c
           const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)p.a, 0, ok && in ? a_bytes : 0, 0x00020000);
           transfer_1k<false>(ra, in ? dst + kA + (i * W + h) * 1024 : lds + U * kStage, a_off[i], in ? (QUANT ? 2 * off : off) : 0);
         }
-        if (MODE != kSkinnyTensor) {
+        if (kBlockScales) {
           const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc((void*)p.sa, 0, ok ? sa_bytes : 0, 0x00020000);
           const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc((void*)p.sb, 0, ok ? p.sb_bytes : 0, 0x00020000);
           if (h == 0 && !QUANT) transfer_256(rsa, dst + kScales, sa_off, ok ? (kb + j) * sa_step : 0);
@@ -249,12 +250,12 @@ __global__ __launch_bounds__(skinny_threads(F, QUANT)) void gemm_skinny_kernel(c
 #pragma unroll
     for (int q = 0; q < FW; ++q) {
       w[q] = frag_read(src + frag[q] * 2048 + l16 * BK, pc0);
-      if (MODE != kSkinnyTensor) sb[q] = *reinterpret_cast<const float*>(src + kScales + 256 + frag[q] * 4);
+      if (kBlockScales) sb[q] = *reinterpret_cast<const float*>(src + kScales + 256 + frag[q] * 4);
     }
 #pragma unroll
     for (int r = 0; r < JW; ++r) {
       x[r] = frag_read(src + kA + rows16[r] * 2048 + l16 * BK, pc0);
-      if (MODE != kSkinnyTensor) sa[r] = *reinterpret_cast<const float*>(src + kScales + (rows16[r] * 16 + l16) * 4);
+      if (kBlockScales) sa[r] = *reinterpret_cast<const float*>(src + kScales + (rows16[r] * 16 + l16) * 4);
     }
 #pragma unroll
     for (int q = 0; q < FW; ++q)
@@ -262,6 +263,8 @@ __global__ __launch_bounds__(skinny_threads(F, QUANT)) void gemm_skinny_kernel(c
       for (int r = 0; r < JW; ++r) {
         if (MODE == kSkinnyTensor) {
           acc[q][r] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[q], x[r], acc[q][r], 0, 0, 0, 0, 0, 0);
+        } else if (MODE == kSkinnyInt8) {
+          acc[q][r] = multiply_int8(w[q], x[r], acc[q][r]);
         } else if (MODE == kSkinnyPow2) {
           acc[q][r] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[q], x[r], acc[q][r], 0, 0, 0,
                                                                       (int)(__builtin_bit_cast(uint32_t, sb[q]) >> 23), 0,
@@ -297,19 +300,35 @@ __global__ __launch_bounds__(skinny_threads(F, QUANT)) void gemm_skinny_kernel(c
       const int col = unit * kCols + (wf + WF * q) * 16 + g * 4;
       const bool col_ok = wf + WF * q < F && col < p.N;
       uint2 braw = make_uint2(0, 0);
-      if (p.bias && col_ok) braw = *reinterpret_cast<const uint2*>(p.bias + col);
+      v4f bias = zero, sb_col = zero;
+      if (MODE == kSkinnyInt8) {
+        if (col_ok) sb_col = p.sb ? *reinterpret_cast<const v4f*>(p.sb + col) : v4f{1.f, 1.f, 1.f, 1.f};
+        if (p.bias && col_ok) bias = load_bias4(p.bias, p.value_type, col);
+      } else if (p.bias && col_ok) {
+        braw = *reinterpret_cast<const uint2*>(p.bias + col);
+      }
 #pragma unroll
       for (int r = 0; r < JW; ++r) {
         v4f s = acc[q][r];
         acc[q][r] = zero;
         const int row = (wj + WJ * r) * 16 + l16;
         if (MODE == kSkinnyTensor) s *= tensor_scale;
-        if (p.bias) {
+        if (MODE == kSkinnyInt8) {                       // (as in the tile kernels, operation for operation)
+          const float sa_row = p.sa[row < p.M ? row : p.M - 1];
+          const v4i sums = __builtin_bit_cast(v4i, s);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[e] = (float)sums[e] * sa_row * sb_col[e];
+            if (p.bias) s[e] += bias[e];
+          }
+        } else if (p.bias) {
           s[0] += bf16lo(braw.x); s[1] += bf16hi(braw.x); s[2] += bf16lo(braw.y); s[3] += bf16hi(braw.y);
         }
         if (col_ok && row < p.M) {
           const int64_t o = (int64_t)row * p.ldc + col;
           if (p.out_f32) *reinterpret_cast<v4f*>(reinterpret_cast<float*>(p.c) + o) = s;
+          else if (MODE == kSkinnyInt8 && p.value_type == HPFP8_TYPE_F16)
+            *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.c) + o) = u32x2{pack_f16x2(s[0], s[1]), pack_f16x2(s[2], s[3])};
           else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.c) + o) = u32x2{pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])};
         }
       }
@@ -380,6 +399,7 @@ static void launch_skinny_rows(const SkinnyParams& p, int cus, hipStream_t strea
 int launch_skinny(const SkinnyParams& p, SkinnyMode mode, int cus, hipStream_t stream) {
   if (mode == kSkinnyTensor) launch_skinny_rows<kSkinnyTensor>(p, cus, stream);
   else if (mode == kSkinnyPow2) launch_skinny_rows<kSkinnyPow2>(p, cus, stream);
+  else if (mode == kSkinnyInt8) launch_skinny_rows<kSkinnyInt8>(p, cus, stream);
   else launch_skinny_rows<kSkinnyBlock>(p, cus, stream);
   return check_launch("gemm (few rows)");
 }

@@ -2,6 +2,7 @@
 // XOR-swizzled by row), fragment reads from it, bf16 packing.
 #pragma once
 #include "hpfp8_device.h"
+#include "../../include/hpfp8.h"
 
 namespace hpfp8 {
 
@@ -39,6 +40,32 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+}
+
+// One k-block of int8 codes onto int32 sums (which travel in the registers of fp32 ones).  A lane's 32 bytes are two operands of the 64-wide
+// instruction: each takes 16 of every lane, the same ones of both sides, so all 128 products of a row and a column are there once.
+__device__ __forceinline__ v4f multiply_int8(const v8i& w, const v8i& x, const v4f& sum) {
+  const v4i w0 = {w[0], w[1], w[2], w[3]}, w1 = {w[4], w[5], w[6], w[7]};
+  const v4i x0 = {x[0], x[1], x[2], x[3]}, x1 = {x[4], x[5], x[6], x[7]};
+  v4i s = __builtin_amdgcn_mfma_i32_16x16x64_i8(w0, x0, __builtin_bit_cast(v4i, sum), 0, 0, 0);
+  s = __builtin_amdgcn_mfma_i32_16x16x64_i8(w1, x1, s, 0, 0, 0);
+  return __builtin_bit_cast(v4f, s);
+}
+
+// four neighbouring values of a bias of element type HPFP8_OUT_BF16, HPFP8_OUT_F32 or HPFP8_TYPE_F16; at: a multiple of 4
+__device__ __forceinline__ v4f load_bias4(const void* bias, int type, int at) {
+  if (type == HPFP8_OUT_F32) return *reinterpret_cast<const v4f*>((const float*)bias + at);
+  const uint2 raw = *reinterpret_cast<const uint2*>((const uint16_t*)bias + at);
+  if (type == HPFP8_OUT_BF16) return v4f{bf16lo(raw.x), bf16hi(raw.x), bf16lo(raw.y), bf16hi(raw.y)};
+  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+  const f16x4 h = __builtin_bit_cast(f16x4, raw);
+  return v4f{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
 }
 
 }  // namespace hpfp8

@@ -175,7 +175,7 @@ __device__ __forceinline__ uint32_t no_negative_zero(uint32_t w) {         // (a
 // above everything: the group's scale and codes are NaN then.  (No clamp: |v * (448 / amax)| <= 448 (1 + 2^-23), which rounds to 448.)
 // SPECIAL: infinities and NaN have codes of their own, and the scale is that of the finite values.
 template <bool SPECIAL = false>
-__device__ __forceinline__ uint2 encode_group(const float v[8], float& scale_inv) {
+__device__ __forceinline__ uint2 encode_group(const float v[8], float& scale_inv, int pow2 = 0) {
   // (the maximum that keeps NaN: one instruction for two values more)
   float top = __builtin_elementwise_maximum(__builtin_fabsf(v[0]), __builtin_fabsf(v[1]));
 #pragma unroll
@@ -188,7 +188,7 @@ __device__ __forceinline__ uint2 encode_group(const float v[8], float& scale_inv
   }
   const uint32_t m = row16_max_u32(__float_as_uint(top) & 0x7FFFFFFFu);
   float scale;
-  scales_from_amax(__uint_as_float(m), scale, scale_inv);
+  scales_from_amax(__uint_as_float(m), scale, scale_inv, pow2);
   uint2 c;
   int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * scale, v[1] * scale, 0, false);
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * scale, v[3] * scale, lo, true);
@@ -211,6 +211,38 @@ __device__ __forceinline__ uint2 encode_group(const float v[8], float& scale_inv
   }
   return c;
 }
+// ---- int8, one scale for a row: code = rint(v * (127 / amax)), amax the row's largest magnitude (no clamp: as above).  A row with an infinity
+// or a NaN has codes of 0 and that as its scale: what the codes stand for is NaN.
+constexpr float kInt8Max = 127.0f;
+__device__ __forceinline__ void int8_scales(float amax, float& scale, float& scale_inv) {
+  const float amc = amax < kAmaxEps ? kAmaxEps : amax;
+  scale = amax < INFINITY ? kInt8Max / amc : 0.f;
+  scale_inv = amc / kInt8Max;
+}
+// (1.5 * 2^23 added rounds to the nearest integer, ties to even, whose low byte the sum's is.  finite: amax is, the same for a whole row)
+__device__ __forceinline__ uint2 int8_codes(const float v[8], float scale, bool finite) {
+  if (!finite) return make_uint2(0, 0);
+  uint32_t b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(v[i] * scale + 12582912.0f) & 0xFFu;
+  return make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24, b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
+}
+// the largest magnitude of eight values; NaN if one is (|v| orders like its bits, and a NaN above everything)
+__device__ __forceinline__ float magnitude8(const float v[8]) {
+  float top = __builtin_elementwise_maximum(__builtin_fabsf(v[0]), __builtin_fabsf(v[1]));
+#pragma unroll
+  for (int i = 2; i < 8; i += 2) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, __builtin_fabsf(v[i])), __builtin_fabsf(v[i + 1]));
+  return __uint_as_float(__float_as_uint(top) & 0x7FFFFFFFu);
+}
+// its maximum over the 16 lanes of a row of lanes, or over a wave's four
+template <bool WAVE>
+__device__ __forceinline__ float magnitude_over(float top) {
+  const uint32_t m = row16_max_u32(__float_as_uint(top));
+  if (!WAVE) return __uint_as_float(m);
+  auto at = [&](int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)m, lane); };
+  return __uint_as_float(umax(umax(at(0), at(16)), umax(at(32), at(48))));
+}
+
 template <bool SPECIAL = false>
 __device__ __forceinline__ void decode8(uint2 c, float scale_inv, float v[8]) {
   const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, true);

@@ -41,7 +41,9 @@ constexpr int64_t kBlock = 128;
   X(hpfp8_swiglu_quantize_1x128_pow2_bf16) X(hpfp8_swiglu_quantize_1x128_fast_bf16) X(hpfp8_gemm_grouped_blockwise) \
   X(hpfp8_bucket_pack_quantize_bf16) X(hpfp8_bucket_unpack_dequantize_bf16) \
   X(hpfp8_quantize_rows) X(hpfp8_dequantize_rows) X(hpfp8_quantize_saved_rows) X(hpfp8_dequantize_saved_rows) X(hpfp8_activation_forward) X(hpfp8_activation_backward) X(hpfp8_layer_norm_forward) \
-  X(hpfp8_layer_norm_backward) X(hpfp8_layer_norm_partials) X(hpfp8_cross_entropy_parts) X(hpfp8_cross_entropy_stride) X(hpfp8_cross_entropy_splits) \
+  X(hpfp8_layer_norm_backward) X(hpfp8_layer_norm_partials) X(hpfp8_rms_norm_forward) X(hpfp8_rms_norm_backward) X(hpfp8_rms_norm_partials) \
+  X(hpfp8_rms_norm_quantize_1x128_kmajor) X(hpfp8_rms_norm_quantize_int8) X(hpfp8_quantize_int8) X(hpfp8_gemm_int8) X(hpfp8_grad_norm) \
+  X(hpfp8_grad_norm_partials) X(hpfp8_grad_clip) X(hpfp8_cross_entropy_parts) X(hpfp8_cross_entropy_stride) X(hpfp8_cross_entropy_splits) \
   X(hpfp8_linear_cross_entropy_forward) X(hpfp8_linear_cross_entropy_piece) X(hpfp8_linear_cross_entropy_rows_t) X(hpfp8_linear_cross_entropy_round)
 struct Library {
 #define HPFP8_POINTER(name) decltype(&::name) name = nullptr;
@@ -912,6 +914,7 @@ PyObject* bucket_unpack(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
 // layer norm and activations, and tensors in 8 bits
 // ------------------------------------------------------------------------------------------------
 PyObject* norm_backward_function = nullptr;         // the Python backwards, for what the nodes below do not take
+PyObject* rms_norm_backward_function = nullptr;
 PyObject* activation_backward_function = nullptr;
 PyObject* loss_backward_function = nullptr;
 
@@ -1079,6 +1082,335 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   const Saving level(2);
   return THPVariable_Wrap(NormNode::apply(*x, v[0] ? std::optional<at::Tensor>(*v[0]) : std::nullopt,
                                           v[1] ? std::optional<at::Tensor>(*v[1]) : std::nullopt, made));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- root-mean-square norm
+struct RmsNorm {
+  at::Tensor y, sum, rstd;               // sum: of x and the residual, where there is one
+  int64_t cols;
+};
+
+struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& residual,
+                                                const std::optional<at::Tensor>& weight, const RmsNorm& made) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({residual ? made.sum : x, made.rstd, weight ? *weight : at::Tensor()});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    if (weight) ctx->saved_data["vector"] = weight->sizes().vec();
+    ctx->saved_data["flags"] = (int64_t)(type_code(x.scalar_type()) | (weight ? type_code(weight->scalar_type()) : 1) << 2 | weight.has_value() << 4 |
+                                            residual.has_value() << 5);
+    ctx->saved_data["cols"] = made.cols;
+    return residual ? torch::autograd::variable_list{made.y, made.sum} : torch::autograd::variable_list{made.y};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &kept = saved[0], &rstd = saved[1], &weight = saved[2];
+    const int64_t flags = ctx->saved_data["flags"].toInt(), cols = ctx->saved_data["cols"].toInt();
+    const int type = flags & 3, vtype = flags >> 2 & 3;
+    const bool has_w = flags >> 4 & 1, has_r = flags >> 5 & 1;       // (an input that is not there has no edge)
+    const bool need_dw = has_w && ctx->needs_input_grad(has_r ? 2 : 1);
+    const at::Tensor& grad = grads[0];
+    const at::Tensor onto = has_r ? grads[1] : at::Tensor();
+    if (!grad.defined() && !onto.defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    const at::Tensor& any = grad.defined() ? grad : onto;
+    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+    auto given = [&](const at::Tensor& g) { return g.is_cuda() && g.layout() == at::kStrided && !at::isTensorSubclassLike(g); };
+    const int64_t n = any.numel(), rows = n / cols;
+    const bool as_made = no_modes() && grad.defined() && given(grad) && (!onto.defined() || given(onto)) && again(kept, grad, type_of(type), n) &&
+                         again(rstd, grad, at::kFloat, rows) && (!weight.defined() || again(weight, grad, type_of(vtype), cols));
+    torch::autograd::variable_list out;
+    if (!as_made) {
+      pybind11::gil_scoped_acquire held;
+      const bool vector = ctx->saved_data.count("vector");
+      out = from_python(rms_norm_backward_function,
+                        pybind11::make_tuple(or_none(grad), or_none(onto), kept, rstd, or_none(weight), cols, as_tuple(shape), type,
+                                             vector ? pybind11::object(as_tuple(ctx->saved_data["vector"].toIntVector())) : pybind11::object(pybind11::none()),
+                                             vtype, need_dw), 2);
+    } else {
+      const at::Tensor go = grad.contiguous(), gs = onto.defined() ? onto.contiguous() : onto;
+      const at::TensorOptions plain_options = go.options().requires_grad(false);
+      out = {at::empty(shape, plain_options), need_dw ? at::empty(ctx->saved_data["vector"].toIntVector(), plain_options.dtype(type_of(vtype))) : at::Tensor()};
+      const at::Tensor partial = at::empty({lib.hpfp8_rms_norm_partials(rows, cols), cols}, plain_options.dtype(at::kFloat));
+      Call call;
+      HPFP8_CALL(call, hpfp8_rms_norm_backward, go.data_ptr(), cols, kept.data_ptr(), cols, gs.defined() ? gs.data_ptr() : nullptr, cols, f32(rstd), type,
+                 rows, cols, weight.defined() ? weight.data_ptr() : nullptr, vtype, out[0].data_ptr(), need_dw ? out[1].data_ptr() : nullptr, f32(partial),
+                 c10::hip::getCurrentHIPStream(go.get_device()).stream());
+      if (!call.ok()) raise(call);
+    }
+    // (a gradient handed on as it is keeps its own place in a graph: it needs no error)
+    if (grad.defined()) out = once(std::move(out), grad.requires_grad() || !onto.defined() ? grad : onto);
+    return {out[0], has_r ? out[0] : at::Tensor(), out[1], at::Tensor()};
+  }
+};
+
+// What the forms of the norm share: rows of x, a residual of the same shape and type, a weight of `dims` last dimensions; false: the Python
+// form's to copy or refuse.
+bool rms_operands(PyObject* const* args, int64_t device, const at::Tensor*& x, const at::Tensor*& weight, const at::Tensor*& residual) {
+  weight = residual = nullptr;
+  if (!rows_of_values(args[0], device, x) || x->numel() == 0) return false;
+  if (args[1] != Py_None && !rows_of_values(args[1], device, weight)) return false;
+  if (args[2] != Py_None && (!rows_of_values(args[2], device, residual) || residual->scalar_type() != x->scalar_type() || residual->sizes() != x->sizes()))
+    return false;
+  return ordinary({x, weight, residual});
+}
+
+// (x, normalized_shape, weight or None, residual or None, eps, device, stream) -> y, or (y, sum), with their place in the graph where they have one
+PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 7);
+  const Where at_ = where(args, n_args);
+  const double eps = PyFloat_AsDouble(args[4]);
+  if (PyErr_Occurred()) throw python_error();
+  const at::Tensor *x, *weight, *residual;
+  PyObject* const operands[] = {args[0], args[2], args[3]};
+  if (!rms_operands(operands, at_.device, x, weight, residual) || !PyTuple_Check(args[1])) Py_RETURN_NONE;
+  const Py_ssize_t dims = PyTuple_GET_SIZE(args[1]);
+  if (dims < 1 || dims > x->dim()) Py_RETURN_NONE;
+  int64_t cols = 1;
+  for (Py_ssize_t i = 0; i < dims; ++i) {
+    const int64_t size = PyLong_AsLongLong(PyTuple_GET_ITEM(args[1], i));
+    if (PyErr_Occurred()) throw python_error();
+    if (size != x->size(x->dim() - dims + i)) Py_RETURN_NONE;
+    cols *= size;
+  }
+  if (lib.hpfp8_rms_norm_partials(1, cols) == 0 || (weight && weight->sizes() != x->sizes().slice(x->dim() - dims))) Py_RETURN_NONE;
+  const bool train = to_train({x, weight, residual});
+  RmsNorm made;
+  Call call;
+  {
+    pybind11::gil_scoped_release free;
+    at::NoGradGuard no_grad;
+    const int64_t rows = x->numel() / cols;
+    const at::TensorOptions options = x->options().requires_grad(false);
+    made.cols = cols;
+    made.y = at::empty(x->sizes(), options);
+    if (residual) made.sum = at::empty(x->sizes(), options);
+    if (train) made.rstd = at::empty({rows}, options.dtype(at::kFloat));
+    HPFP8_CALL(call, hpfp8_rms_norm_forward, x->data_ptr(), cols, residual ? residual->data_ptr() : nullptr, cols, type_code(x->scalar_type()), rows, cols,
+               weight ? weight->data_ptr() : nullptr, weight ? type_code(weight->scalar_type()) : HPFP8_OUT_BF16, (float)eps,
+               residual ? made.sum.data_ptr() : nullptr, made.y.data_ptr(), train ? f32(made.rstd) : nullptr, at_.stream);
+  }
+  if (!call.ok()) return failed(call);
+  if (!train) return residual ? tuple_of(made.y, made.sum) : THPVariable_Wrap(made.y);
+  const Saving level(2);
+  const auto out = RmsNormNode::apply(*x, residual ? std::optional<at::Tensor>(*residual) : std::nullopt,
+                                      weight ? std::optional<at::Tensor>(*weight) : std::nullopt, made);
+  return residual ? tuple_of(out[0], out[1]) : THPVariable_Wrap(out[0]);
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, weight or None, residual or None, eps, form: 0 E4M3, 1 with powers of two, 2 int8, device, stream) -> (codes, scale_inv[, sum])
+PyObject* rms_norm_quantize(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 7);
+  const Where at_ = where(args, n_args);
+  const double eps = PyFloat_AsDouble(args[3]);
+  const int64_t form = PyLong_AsLongLong(args[4]);
+  if (PyErr_Occurred()) throw python_error();
+  const at::Tensor *x, *weight, *residual;
+  if (!rms_operands(args, at_.device, x, weight, residual) || to_train({x, weight, residual})) Py_RETURN_NONE;
+  const int64_t cols = x->size(-1), rows = x->numel() / cols;
+  if (cols % kBlock || lib.hpfp8_rms_norm_partials(1, cols) == 0 || (weight && (weight->dim() != 1 || weight->size(0) != cols))) Py_RETURN_NONE;
+  at::Tensor q, s, sum;
+  Call call;
+  {
+    pybind11::gil_scoped_release free;
+    at::NoGradGuard no_grad;
+    const at::TensorOptions options = x->options().requires_grad(false);
+    const int type = type_code(x->scalar_type()), wtype = weight ? type_code(weight->scalar_type()) : HPFP8_OUT_BF16;
+    const void* const w = weight ? weight->data_ptr() : nullptr;
+    const void* const r = residual ? residual->data_ptr() : nullptr;
+    if (residual) sum = at::empty(x->sizes(), options);
+    q = at::empty(x->sizes(), options.dtype(form == 2 ? at::kChar : at::kFloat8_e4m3fn));
+    s = form == 2 ? at::empty(x->sizes().slice(0, x->dim() - 1), options.dtype(at::kFloat)) : at::empty({cols / kBlock, rows}, options.dtype(at::kFloat));
+    void* const to = residual ? sum.data_ptr() : nullptr;
+    if (form == 2) {
+      HPFP8_CALL(call, hpfp8_rms_norm_quantize_int8, x->data_ptr(), cols, r, cols, type, rows, cols, w, wtype, (float)eps, to, q.data_ptr(), f32(s), at_.stream);
+    } else {
+      HPFP8_CALL(call, hpfp8_rms_norm_quantize_1x128_kmajor, x->data_ptr(), cols, r, cols, type, rows, cols, w, wtype, (float)eps, (int)form, to,
+                 q.data_ptr(), f32(s), at_.stream);
+      s = s.t();
+      if (x->dim() != 2) {
+        std::vector<int64_t> sizes = x->sizes().vec();
+        sizes.back() = cols / kBlock;
+        s = s.reshape(sizes);
+      }
+    }
+  }
+  if (!call.ok()) return failed(call);
+  return residual ? tuple_of(q, s, sum) : tuple_of(q, s);
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- linear in 8-bit integers
+struct Int8Rows {
+  at::Tensor codes, scale_inv;
+};
+void quantize_rows_int8(const at::Tensor& x, const at::Tensor* by, void* stream, Int8Rows& to, Call& call) {
+  const at::TensorOptions options = x.options().requires_grad(false);
+  const int64_t cols = x.size(-1);
+  to.codes = at::empty(x.sizes(), options.dtype(at::kChar));
+  to.scale_inv = at::empty(x.sizes().slice(0, x.dim() - 1), options.dtype(at::kFloat));
+  HPFP8_CALL(call, hpfp8_quantize_int8, x.data_ptr(), type_code(x.scalar_type()), x.numel() / cols, cols, cols, by ? f32(*by) : nullptr, to.codes.data_ptr(),
+             f32(to.scale_inv), stream);
+}
+constexpr int64_t kInt8MostFeatures = 130944;
+bool int8_source(PyObject* o, int64_t device, const at::Tensor*& x) {
+  return rows_of_values(o, device, x) && x->numel() > 0 && x->size(-1) % kBlock == 0 && x->size(-1) <= kInt8MostFeatures;
+}
+bool int8_codes(PyObject* o, int64_t device, const at::Tensor*& t) {
+  return plain(o, device, t) && t->scalar_type() == at::kChar && t->numel() > 0 && ((uintptr_t)t->data_ptr() & 15) == 0;
+}
+bool int8_weight(PyObject* o, int64_t device, int64_t k, const at::Tensor*& t) {
+  return int8_codes(o, device, t) && t->dim() == 2 && t->size(1) == k && t->stride(1) == 1 && t->stride(0) % 16 == 0 && t->stride(0) >= k &&
+         t->size(0) % kBlock == 0 && k % kBlock == 0 && k <= kInt8MostFeatures;
+}
+bool int8_vector(PyObject* o, int64_t device, int64_t n, at::ScalarType type, const at::Tensor*& t) {
+  return plain(o, device, t) && t->scalar_type() == type && t->dim() == 1 && t->size(0) == n && t->is_contiguous() && ((uintptr_t)t->data_ptr() & 15) == 0;
+}
+
+// (x, column_scale or None, device, stream) -> (codes, scale_inv)
+PyObject* quantize_int8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 4);
+  const Where at_ = where(args, n_args);
+  const at::Tensor *x, *by = nullptr;
+  if (!int8_source(args[0], at_.device, x) || (args[1] != Py_None && !int8_vector(args[1], at_.device, x->size(-1), at::kFloat, by)) || !ordinary({x, by}))
+    Py_RETURN_NONE;
+  Int8Rows made;
+  Call call;
+  {
+    pybind11::gil_scoped_release free;
+    at::NoGradGuard no_grad;
+    quantize_rows_int8(*x, by, at_.stream, made, call);
+  }
+  return call.ok() ? tuple_of(made.codes, made.scale_inv) : failed(call);
+  END_HANDLE_TH_ERRORS
+}
+
+// (a, sa, b, sb or None, bias or None, element type of the result, device, stream) -> c
+PyObject* gemm_int8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 8);
+  const Where at_ = where(args, n_args);
+  const int64_t type = PyLong_AsLongLong(args[5]);
+  if (PyErr_Occurred()) throw python_error();
+  const at::Tensor *a, *sa, *b, *sb = nullptr, *bias = nullptr;
+  if (!int8_codes(args[0], at_.device, a) || a->dim() < 1 || !a->is_contiguous() || !int8_weight(args[2], at_.device, a->size(-1), b)) Py_RETURN_NONE;
+  const int64_t k = a->size(-1), m = a->numel() / k, n = b->size(0);
+  if (!floats(args[1], at_.device, sa) || sa->numel() != m || !sa->is_contiguous() || (args[3] != Py_None && !int8_vector(args[3], at_.device, n, at::kFloat, sb)) ||
+      (args[4] != Py_None && !int8_vector(args[4], at_.device, n, type_of((int)type), bias)) || !ordinary({a, sa, b, sb, bias}))
+    Py_RETURN_NONE;
+  at::Tensor c;
+  Call call;
+  {
+    pybind11::gil_scoped_release free;
+    at::NoGradGuard no_grad;
+    std::vector<int64_t> sizes = a->sizes().vec();
+    sizes.back() = n;
+    c = at::empty(sizes, a->options().requires_grad(false).dtype(type_of((int)type)));
+    HPFP8_CALL(call, hpfp8_gemm_int8, a->data_ptr(), k, f32(*sa), b->data_ptr(), b->stride(0), sb ? f32(*sb) : nullptr, m, n, k,
+               bias ? bias->data_ptr() : nullptr, c.data_ptr(), n, (int)type, at_.stream);
+  }
+  return call.ok() ? THPVariable_Wrap(c) : failed(call);
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, codes, scale_inv, bias or None, device, stream) -> y, where there is no graph
+PyObject* int8_linear(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 6);
+  const Where at_ = where(args, n_args);
+  const at::Tensor *x, *w, *sw, *bias = nullptr;
+  if (!int8_source(args[0], at_.device, x) || !int8_weight(args[1], at_.device, x->size(-1), w)) Py_RETURN_NONE;
+  const int64_t k = x->size(-1), m = x->numel() / k, n = w->size(0);
+  if (n > kInt8MostFeatures || !int8_vector(args[2], at_.device, n, at::kFloat, sw) ||
+      (args[3] != Py_None && !int8_vector(args[3], at_.device, n, x->scalar_type(), bias)) || to_train({x, bias}) || !ordinary({x, w, sw, bias}))
+    Py_RETURN_NONE;
+  at::Tensor y;
+  Call call;
+  {
+    pybind11::gil_scoped_release free;
+    at::NoGradGuard no_grad;
+    Int8Rows rows;
+    quantize_rows_int8(*x, nullptr, at_.stream, rows, call);
+    if (call.ok()) {
+      std::vector<int64_t> sizes = x->sizes().vec();
+      sizes.back() = n;
+      y = at::empty(sizes, x->options().requires_grad(false));
+      HPFP8_CALL(call, hpfp8_gemm_int8, rows.codes.data_ptr(), k, f32(rows.scale_inv), w->data_ptr(), w->stride(0), f32(*sw), m, n, k,
+                 bias ? bias->data_ptr() : nullptr, y.data_ptr(), n, type_code(x->scalar_type()), at_.stream);
+    }
+  }
+  return call.ok() ? THPVariable_Wrap(y) : failed(call);
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- the norm of many gradients, and their clipping
+struct Gradients {
+  std::vector<const at::Tensor*> tensors;
+  std::vector<void*> ptrs;
+  std::vector<int64_t> numels;
+  std::vector<int> types;
+  // of a list of dense, contiguous tensors of the three types; false where one is anything else
+  bool take(PyObject* list, int64_t device) {
+    if (!PyList_CheckExact(list)) return false;
+    const Py_ssize_t n = PyList_GET_SIZE(list);
+    tensors.resize(n);
+    ptrs.resize(n);
+    numels.resize(n);
+    types.resize(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      const at::Tensor* t;
+      if (!plain(PyList_GET_ITEM(list, i), device, t) || type_code(t->scalar_type()) < 0 || !t->is_contiguous()) return false;
+      tensors[i] = t;
+      ptrs[i] = t->data_ptr();
+      numels[i] = t->numel();
+      types[i] = type_code(t->scalar_type());
+    }
+    return n > 0;
+  }
+};
+
+// (tensors, power, device, stream) -> norm
+PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 4);
+  const Where at_ = where(args, n_args);
+  const int64_t power = PyLong_AsLongLong(args[1]);
+  if (PyErr_Occurred()) throw python_error();
+  Gradients g;
+  if (!no_modes() || !g.take(args[0], at_.device)) Py_RETURN_NONE;
+  at::Tensor norm;
+  Call call;
+  {
+    at::NoGradGuard no_grad;
+    const int64_t count = (int64_t)g.ptrs.size();
+    const at::TensorOptions options = g.tensors[0]->options().requires_grad(false);
+    norm = at::empty({}, options.dtype(at::kFloat));
+    const at::Tensor partial = at::empty({lib.hpfp8_grad_norm_partials(g.numels.data(), g.types.data(), count)}, options.dtype(at::kDouble));
+    HPFP8_CALL(call, hpfp8_grad_norm, g.ptrs.data(), g.numels.data(), g.types.data(), count, (int)power, partial.data_ptr<double>(), f32(norm), at_.stream);
+  }
+  return call.ok() ? THPVariable_Wrap(norm) : failed(call);
+  END_HANDLE_TH_ERRORS
+}
+
+// (tensors, norm, max_norm, device, stream) -> whether it was done
+PyObject* grad_clip(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 5);
+  const Where at_ = where(args, n_args);
+  const double max_norm = PyFloat_AsDouble(args[2]);
+  if (PyErr_Occurred()) throw python_error();
+  Gradients g;
+  const at::Tensor* norm;
+  if (!no_modes() || !g.take(args[0], at_.device) || !floats(args[1], at_.device, norm) || norm->numel() != 1) Py_RETURN_FALSE;
+  for (const at::Tensor* t : g.tensors) t->unsafeGetTensorImpl()->bump_version();
+  Call call;
+  HPFP8_CALL(call, hpfp8_grad_clip, g.ptrs.data(), g.numels.data(), g.types.data(), (int64_t)g.ptrs.size(), f32(*norm), (float)max_norm, at_.stream);
+  if (!call.ok()) return failed(call);
+  Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
 
@@ -1354,6 +1686,14 @@ PyObject* bind_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
+PyObject* bind_rms_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 1);
+  Py_INCREF(args[0]);
+  rms_norm_backward_function = args[0];
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
 PyObject* bind_activation_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   expect(n, 1);
@@ -1402,7 +1742,9 @@ PyMethodDef methods[] = {HPFP8_METHOD(built_for), HPFP8_METHOD(bind), HPFP8_METH
                          HPFP8_METHOD(swiglu_mlp_infer), HPFP8_METHOD(grouped_infer), HPFP8_METHOD(bucket_pack), HPFP8_METHOD(bucket_unpack),
                          HPFP8_METHOD(layer_norm), HPFP8_METHOD(activation), HPFP8_METHOD(quantize_rows), HPFP8_METHOD(dequantize_rows),
                          HPFP8_METHOD(linear_cross_entropy), HPFP8_METHOD(bind_loss_backward),
-                         HPFP8_METHOD(bind_norm_backward), HPFP8_METHOD(bind_activation_backward),
+                         HPFP8_METHOD(bind_norm_backward), HPFP8_METHOD(bind_activation_backward), HPFP8_METHOD(bind_rms_norm_backward),
+                         HPFP8_METHOD(rms_norm), HPFP8_METHOD(rms_norm_quantize), HPFP8_METHOD(quantize_int8), HPFP8_METHOD(gemm_int8), HPFP8_METHOD(int8_linear),
+                         HPFP8_METHOD(grad_norm), HPFP8_METHOD(grad_clip),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -15,7 +15,9 @@ from .linear import (fp8_linear, Fp8Linear, fp8_grouped_linear, fp8_swiglu_mlp, 
 from . import fsdp, checkpoint  # noqa: E402
 from .bucket import quantize_bucket, dequantize_bucket, Fp8GradBucket  # noqa: E402
 from .kept import Fp8Activation, activation, keep_activations_8bit, quantize_activation  # noqa: E402
-from .norm import LayerNorm, layer_norm  # noqa: E402
+from .norm import LayerNorm, RMSNorm, layer_norm, rms_norm, rms_norm_quantize_1x128, rms_norm_quantize_int8  # noqa: E402
+from .int8 import Int8Linear, Int8Weight, gemm_int8, int8_linear, quantize_int8, quantize_weight_int8  # noqa: E402
+from .grads import clip_grad_norm_, clip_grads_with_norm_, get_total_norm  # noqa: E402
 from .loss import linear_cross_entropy  # noqa: E402
 from .policy import Fp8MixedPrecisionPolicy, Fp8Tensor, cast_fp_tensor, tensor_type_cast  # noqa: E402
 
@@ -28,4 +30,7 @@ __all__ = [
     "gemm_grouped_blockwise", "fp8_linear", "Fp8Linear", "fp8_grouped_linear", "fp8_swiglu_mlp", "Fp8SwiGLUMLP",
     "quantize_bucket", "dequantize_bucket", "Fp8GradBucket",
     "layer_norm", "LayerNorm", "quantize_activation", "Fp8Activation", "keep_activations_8bit", "activation", "linear_cross_entropy",
+    "rms_norm", "RMSNorm", "rms_norm_quantize_1x128", "rms_norm_quantize_int8",
+    "quantize_int8", "quantize_weight_int8", "Int8Weight", "gemm_int8", "int8_linear", "Int8Linear",
+    "get_total_norm", "clip_grads_with_norm_", "clip_grad_norm_",
 ]

@@ -91,6 +91,14 @@ SIGNATURES = {
     "hpfp8_linear_cross_entropy_round": [_vp, _i64, _int, _vp, _vp],
     "hpfp8_layer_norm_forward": [_vp, _int, _i64, _i64, _i64, _vp, _vp, _int, _f32, _vp, _vp, _vp, _vp, _vp, _vp],
     "hpfp8_layer_norm_backward": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _int, _i64, _i64, _vp, _int, _vp, _vp, _vp, _vp, _vp],
+    "hpfp8_rms_norm_forward": [_vp, _i64, _vp, _i64, _int, _i64, _i64, _vp, _int, _f32, _vp, _vp, _vp, _vp],
+    "hpfp8_rms_norm_quantize_1x128_kmajor": [_vp, _i64, _vp, _i64, _int, _i64, _i64, _vp, _int, _f32, _int, _vp, _vp, _vp, _vp],
+    "hpfp8_rms_norm_quantize_int8": [_vp, _i64, _vp, _i64, _int, _i64, _i64, _vp, _int, _f32, _vp, _vp, _vp, _vp],
+    "hpfp8_rms_norm_backward": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _vp, _int, _vp, _vp, _vp, _vp],
+    "hpfp8_quantize_int8": [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp],
+    "hpfp8_gemm_int8": [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _int, _vp],
+    "hpfp8_grad_norm": [_vp, _vp, _vp, _i64, _int, _vp, _vp, _vp],
+    "hpfp8_grad_clip": [_vp, _vp, _vp, _i64, _vp, _f32, _vp],
 }
 # functions that return a size, not a status
 SIZE_FUNCTIONS = {
@@ -99,6 +107,8 @@ SIZE_FUNCTIONS = {
     "hpfp8_gemm_few_rows": [_i64],
     "hpfp8_linear_few_rows": [_i64, _i64],
     "hpfp8_layer_norm_partials": [_i64, _i64],
+    "hpfp8_rms_norm_partials": [_i64, _i64],
+    "hpfp8_grad_norm_partials": [_vp, _vp, _i64],
     "hpfp8_cross_entropy_parts": [_i64, _i64, _i64],
     "hpfp8_cross_entropy_splits": [_i64, _i64, _i64, _int],
     "hpfp8_cross_entropy_stride": [_i64],

@@ -542,6 +542,44 @@ int hpfp8_layer_norm_backward(const void* dy, int64_t ld_dy, const void* x, int6
                               float* partial, hpfp8_stream_t stream);
 int64_t hpfp8_layer_norm_partials(int64_t rows, int64_t cols);
 
+/* Root-mean-square norm of rows of up to 16384 values, of s = x + residual where there is a residual (s rounded to dtype and written to sum;
+ * residual and sum both or neither NULL): y = s rstd w, rstd = 1 / sqrt(mean(s^2) + eps).  w [cols] of element type wtype, may be NULL; rstd
+ * (fp32 [rows], may be NULL) is what the backward needs.  Row strides in elements; sum and y contiguous. */
+int hpfp8_rms_norm_forward(const void* x, int64_t ld, const void* residual, int64_t ld_residual, int dtype, int64_t rows, int64_t cols, const void* w,
+                           int wtype, float eps, void* sum, void* y, float* rstd, hpfp8_stream_t stream);
+/* The same with y quantized from its fp32 values, cols a multiple of 128: E4M3 codes q[rows, cols] with scale_inv[cols / 128, rows] (the groups and
+ * scales of hpfp8_quantize_1x128_kmajor_bf16; pow2: powers of two), or int8 codes with scale_inv[rows] (as hpfp8_quantize_int8). */
+int hpfp8_rms_norm_quantize_1x128_kmajor(const void* x, int64_t ld, const void* residual, int64_t ld_residual, int dtype, int64_t rows, int64_t cols,
+                                         const void* w, int wtype, float eps, int pow2, void* sum, void* q, float* scale_inv, hpfp8_stream_t stream);
+int hpfp8_rms_norm_quantize_int8(const void* x, int64_t ld, const void* residual, int64_t ld_residual, int dtype, int64_t rows, int64_t cols,
+                                 const void* w, int wtype, float eps, void* sum, void* q, float* scale_inv, hpfp8_stream_t stream);
+/* ds (contiguous), the gradient of s: dy's through the norm plus ds_in (may be NULL); and dw (element type wtype, may be NULL) summed over the rows
+ * in a fixed order.  partial: fp32 [hpfp8_rms_norm_partials(rows, cols), cols], written and read by the call. */
+int hpfp8_rms_norm_backward(const void* dy, int64_t ld_dy, const void* s, int64_t ld, const void* ds_in, int64_t ld_ds, const float* rstd, int dtype,
+                            int64_t rows, int64_t cols, const void* w, int wtype, void* ds, void* dw, float* partial, hpfp8_stream_t stream);
+int64_t hpfp8_rms_norm_partials(int64_t rows, int64_t cols);
+
+/* Rows of x[rows, cols] (any of the three element types; cols a multiple of 128, at most 130944; row stride ld in elements) -> int8 codes q[rows, cols]
+ * and scale_inv[rows]: v = x, or x * column_scale[c] rounded to fp32 (column_scale fp32 [cols], may be NULL); amax = max |v| of the row, at least 1e-12;
+ * code = rint(v * (127 / amax)), scale_inv = amax / 127.  A row with an infinity or a NaN: codes 0 and that for its scale. */
+int hpfp8_quantize_int8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const float* column_scale, void* q, float* scale_inv,
+                        hpfp8_stream_t stream);
+/* c[m, n] = (sum_k a[m, k] b[n, k]) sa[m] sb[n] + bias[n] of int8 codes, the sum exact; c and bias of element type out_type; bias may be NULL,
+ * and sb (scales of 1).  Limits as hpfp8_gemm_per_tensor's; K at most 130944, sb on a 16-byte boundary. */
+int hpfp8_gemm_int8(const void* a, int64_t lda, const float* sa, const void* b, int64_t ldb, const float* sb, int64_t M, int64_t N, int64_t K,
+                    const void* bias, void* c, int64_t ldc, int out_type, hpfp8_stream_t stream);
+
+/* The norm of all elements of count tensors taken together: power 1, 2, or 0 for the largest magnitude.  Each tensor is numels[e] elements of type
+ * types[e] one behind the other from ptrs[e]; the tables are host memory, read before the call returns.  partial: fp64
+ * [hpfp8_grad_norm_partials(numels, types, count)], written and read by the call; norm: one fp32. */
+int64_t hpfp8_grad_norm_partials(const int64_t* numels, const int* types, int64_t count);
+int hpfp8_grad_norm(const void* const* ptrs, const int64_t* numels, const int* types, int64_t count, int power, double* partial, float* norm,
+                    hpfp8_stream_t stream);
+/* Every element times min(1, max_norm / (*norm + 1e-6)), in place, rounded once; nothing is written where that is 1.  Two tensors that share memory
+ * are refused. */
+int hpfp8_grad_clip(void* const* ptrs, const int64_t* numels, const int* types, int64_t count, const float* norm, float max_norm,
+                    hpfp8_stream_t stream);
+
 /* Softmax cross entropy of the linear l = x w^T over a vocabulary, without the logits in memory.  x[tokens, hidden] and w[vocab, hidden] are
  * bf16, row strides ld_x and ld_w in elements, hidden and the strides multiples of 8 and below 2^21, tokens at most 2^21, vocab at most 2^24;
  * target[tokens] is int64.

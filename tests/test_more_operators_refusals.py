@@ -1,0 +1,182 @@
+"""What the root-mean-square norm, the linear in 8-bit integers and the gradients' norm refuse, without a GPU: arguments are looked at before
+anything is launched."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture()
+def p():
+    buf = (ctypes.c_char * 8192)()
+    yield (ctypes.cast(buf, ctypes.c_void_p).value + 255) & ~255
+
+
+def c(name, *args):
+    from hpfp8 import _lib
+    lib = _lib.load()
+    return getattr(lib, name)(*args), lib.hpfp8_last_error().decode()
+
+
+def test_rms_norm(p):
+    f, b = "hpfp8_rms_norm_forward", "hpfp8_rms_norm_backward"
+    assert c(f, p, 8, None, 0, 0, 4, 16385, None, 0, 1e-5, None, p, None, None)[0] == -2
+    assert c(f, p, 8, None, 0, 0, 4, 1 << 40, None, 0, 1e-5, None, p, None, None)[0] == -2
+    assert c(f, p, 8, None, 0, 0, 4, 0, None, 0, 1e-5, None, p, None, None)[0] == -2
+    assert c(f, p, 8, None, 0, 0, -1, 8, None, 0, 1e-5, None, p, None, None)[0] == -2
+    assert c(f, p, -8, None, 0, 0, 4, 8, None, 0, 1e-5, None, p, None, None)[0] == -2
+    assert c(f, p, 8, p, -8, 0, 4, 8, None, 0, 1e-5, p, p, None, None)[0] == -2
+    assert c(f, p, 8, None, 0, 3, 4, 8, None, 0, 1e-5, None, p, None, None)[0] == -1
+    assert c(f, p, 8, None, 0, 0, 4, 8, p, -1, 1e-5, None, p, None, None)[0] == -1
+    assert c(f, p, 8, p, 8, 0, 4, 8, None, 0, 1e-5, None, p, None, None)[0] == -1          # a residual without a sum
+    assert c(f, p, 8, None, 0, 0, 4, 8, None, 0, 1e-5, p, p, None, None)[0] == -1
+    assert c(f, None, 8, None, 0, 0, 4, 8, None, 0, 1e-5, None, p, None, None)[0] == -1
+    assert c(f, p + 1, 8, None, 0, 0, 4, 8, None, 0, 1e-5, None, p, None, None)[0] == -3
+    assert c(f, p, 8, p + 2, 8, 1, 4, 8, None, 0, 1e-5, p, p, None, None)[0] == -3
+    assert c(f, p, 8, None, 0, 0, 4, 8, p + 2, 1, 1e-5, None, p, None, None)[0] == -3
+    assert c(f, None, 8, None, 0, 0, 0, 8, None, 0, 1e-5, None, None, None, None)[0] == 0
+    for q, more in (("hpfp8_rms_norm_quantize_1x128_kmajor", (0,)), ("hpfp8_rms_norm_quantize_int8", ())):
+        assert c(q, p, 8, None, 0, 0, 4, 100, None, 0, 1e-5, *more, None, p, p, None)[0] == -2
+        assert c(q, p, 8, None, 0, 0, 4, 16512, None, 0, 1e-5, *more, None, p, p, None)[0] == -2
+        assert c(q, p, 128, None, 0, 0, 4, 128, None, 0, 1e-5, *more, None, p, None, None)[0] == -1
+        assert c(q, None, 128, None, 0, 0, 0, 128, None, 0, 1e-5, *more, None, None, None, None)[0] == 0
+    assert c(b, p, 8, p, 8, None, 0, p, 0, 4, 16385, None, 0, p, p, p, None)[0] == -2
+    assert c(b, p, 8, p, 8, None, 0, None, 0, 4, 8, None, 0, p, p, p, None)[0] == -1
+    assert c(b, p, 8, p, 8, None, 0, p, 0, 4, 8, None, 0, p, p, None, None)[0] == -1       # no workspace
+    assert c(b, p, -8, p, 8, None, 0, p, 0, 4, 8, None, 0, p, p, p, None)[0] == -2
+    assert c(b, p, 8, p, 8, p + 1, 8, p, 0, 4, 8, None, 0, p, p, p, None)[0] == -3
+    assert c(b, p, 8, p, 8, None, 0, p, 0, 4, 8, None, 1, p, p + 2, p, None)[0] == -3
+    assert c(b, None, 8, None, 8, None, 0, None, 0, 0, 8, None, 0, None, None, None, None)[0] == 0
+    assert c("hpfp8_rms_norm_partials", 0, 8)[0] == 0 and c("hpfp8_rms_norm_partials", 1, 16385)[0] == 0
+    assert c("hpfp8_rms_norm_partials", 1 << 40, 4096)[0] == 256 and c("hpfp8_rms_norm_partials", 1 << 40, 2048)[0] == 512
+
+
+def test_int8(p):
+    q, g = "hpfp8_quantize_int8", "hpfp8_gemm_int8"
+    assert c(q, p, 3, 4, 128, 128, None, p, p, None)[0] == -1
+    assert c(q, p, 0, 4, 100, 128, None, p, p, None)[0] == -2
+    assert c(q, p, 0, 4, 131072, 131072, None, p, p, None)[0] == -2
+    assert c(q, p, 0, -4, 128, 128, None, p, p, None)[0] == -2
+    assert c(q, p, 0, 4, 128, -128, None, p, p, None)[0] == -2
+    assert c(q, p, 0, 4, 128, 128, None, p, None, None)[0] == -1
+    assert c(q, p + 1, 0, 4, 128, 128, None, p, p, None)[0] == -3
+    assert c(q, p, 0, 4, 128, 128, p + 2, p, p, None)[0] == -3
+    assert c(q, None, 0, 0, 128, 128, None, None, None, None)[0] == 0
+    assert c(g, p, 128, p, p, 128, p, 4, 100, 128, None, p, 128, 0, None)[0] == -2
+    assert c(g, p, 128, p, p, 128, p, 4, 128, 100, None, p, 128, 0, None)[0] == -2
+    assert c(g, p, 131072, p, p, 131072, p, 4, 128, 131072, None, p, 128, 0, None)[0] == -2       # sums past 32 bits
+    assert c(g, p, 120, p, p, 128, p, 4, 128, 128, None, p, 128, 0, None)[0] == -2
+    assert c(g, p, 128, p, p, 136, p, 4, 128, 128, None, p, 128, 0, None)[0] == -2
+    assert c(g, p, 128, p, p, 128, p, 4, 128, 128, None, p, 64, 0, None)[0] == -2
+    assert c(g, p, 128, p, p, 128, p, 4, 128, 128, None, p, 130, 2, None)[0] == -3
+    assert c(g, p, 128, p, p, 128, p, 4, 128, 128, None, p, 128, 3, None)[0] == -1
+    assert c(g, p, 128, None, p, 128, p, 4, 128, 128, None, p, 128, 0, None)[0] == -1
+    assert c(g, p + 1, 128, p, p, 128, p, 4, 128, 128, None, p, 128, 0, None)[0] == -3
+    assert c(g, p, 128, p, p, 128, p + 4, 4, 128, 128, None, p, 128, 0, None)[0] == -3
+    assert c(g, p, 128, p + 2, p, 128, p, 4, 128, 128, None, p, 128, 0, None)[0] == -3
+    assert c(g, p, 128, p, p, 128, p, 4, 128, 128, p + 8, p, 128, 0, None)[0] == -3
+    assert c(g, None, 128, None, None, 128, None, 0, 128, 128, None, None, 128, 0, None)[0] == 0
+
+
+def table(ptrs, numels, types):
+    n = max(len(ptrs), 1)
+    return (ctypes.c_void_p * n)(*ptrs), (ctypes.c_int64 * n)(*numels), (ctypes.c_int * n)(*types), len(ptrs)
+
+
+def test_gradients(p):
+    f, clip, size = "hpfp8_grad_norm", "hpfp8_grad_clip", "hpfp8_grad_norm_partials"
+    one = table([p], [8], [0])
+    assert c(f, *one, 3, p, p, None)[0] == -1
+    assert c(f, *one, 2, None, p, None)[0] == -1
+    assert c(f, *one, 2, p, None, None)[0] == -1
+    assert c(f, *table([p], [8], [3]), 2, p, p, None)[0] == -1
+    assert c(f, *table([p], [-8], [0]), 2, p, p, None)[0] == -2
+    assert c(f, *table([p], [1 << 50], [0]), 2, p, p, None)[0] == -2
+    assert c(f, *table([None], [8], [0]), 2, p, p, None)[0] == -1
+    assert c(f, *table([p + 1], [8], [0]), 2, p, p, None)[0] == -3
+    assert c(f, *table([p + 2], [8], [1]), 2, p, p, None)[0] == -3
+    assert c(f, None, None, None, 1, 2, p, p, None)[0] == -1
+    assert c(f, *one[:3], -1, 2, p, p, None)[0] == -2
+    assert c(clip, *one, None, 1.0, None)[0] == -1
+    assert c(clip, *table([p, p], [8, 8], [0, 0]), p, 1.0, None)[0] == -1
+    assert c(clip, *table([p, p + 14], [8, 8], [0, 0]), p, 1.0, None)[0] == -1
+    assert c(clip, *table([p + 64, p], [8, 20], [0, 1]), p, 1.0, None)[0] == -1
+    assert "share memory" in c(clip, *table([p + 64, p], [8, 20], [0, 1]), p, 1.0, None)[1]
+    assert c(clip, *table([], [], []), None, 1.0, None)[0] == 0
+    assert c(clip, *table([p, p], [0, 0], [0, 1]), p, 1.0, None)[0] == 0
+    assert c(size, *table([], [], [])[1:])[0] == 0 and c(size, *one[1:])[0] == 1
+    _, numels, types, n = table([p] * 3, [1 << 40, 1, 0], [1, 0, 0])
+    assert c(size, numels, types, n)[0] in range(2000, 2052)             # (work is dealt out by bytes)
+
+
+def test_tensors_that_are_not_on_the_gpu_and_wrong_arguments():
+    import hpfp8
+    x, w = torch.zeros(4, 256, dtype=BF16), torch.ones(256, dtype=BF16)
+    for f, error in ((lambda: hpfp8.rms_norm(x, 256, w), ValueError), (lambda: hpfp8.rms_norm(3, 256), TypeError),
+                     (lambda: hpfp8.rms_norm(x.double(), 256), TypeError), (lambda: hpfp8.rms_norm_quantize_1x128(x, w), ValueError),
+                     (lambda: hpfp8.rms_norm_quantize_int8(x), ValueError), (lambda: hpfp8.quantize_int8(x), ValueError),
+                     (lambda: hpfp8.quantize_weight_int8(x[:3]), ValueError), (lambda: hpfp8.quantize_weight_int8(w), ValueError),
+                     (lambda: hpfp8.gemm_int8(x, x, x, x), TypeError), (lambda: hpfp8.int8_linear(x, w), TypeError),
+                     (lambda: hpfp8.int8_linear(x, hpfp8.Int8Weight(torch.zeros(128, 256, dtype=torch.int8), torch.ones(128))), ValueError),
+                     (lambda: hpfp8.get_total_norm([x], 5), ValueError), (lambda: hpfp8.get_total_norm([x], math.nan), ValueError),
+                     (lambda: hpfp8.Int8Linear(256, 100), ValueError), (lambda: hpfp8.Int8Linear(0, 128), ValueError)):
+        with pytest.raises(error):
+            f()
+
+
+@pytest.fixture()
+def as_if_on_the_gpu(monkeypatch):
+    from hpfp8 import ops
+    monkeypatch.setattr(ops, "_check_device", lambda *a: None)
+
+
+def test_operands_that_do_not_go_together(as_if_on_the_gpu):
+    import hpfp8
+    x, w = torch.zeros(4, 256, dtype=BF16), torch.ones(256, dtype=BF16)
+    for f, error in ((lambda: hpfp8.rms_norm(x, 128), ValueError), (lambda: hpfp8.rms_norm(x, (4, 4, 256)), ValueError),
+                     (lambda: hpfp8.rms_norm(x, 256, w[:128]), ValueError), (lambda: hpfp8.rms_norm(x, 256, w.double()), TypeError),
+                     (lambda: hpfp8.rms_norm(x, 256, residual=x.float()), TypeError), (lambda: hpfp8.rms_norm(x, 256, residual=x[:1]), ValueError),
+                     (lambda: hpfp8.rms_norm(torch.zeros(1, 16385, dtype=BF16), 16385), ValueError),
+                     (lambda: hpfp8.rms_norm_quantize_int8(x[:, :100]), ValueError), (lambda: hpfp8.rms_norm_quantize_1x128(x, w, residual=x[0]), ValueError),
+                     (lambda: hpfp8.rms_norm_quantize_int8(x.clone().requires_grad_()), RuntimeError),
+                     (lambda: hpfp8.rms_norm_quantize_1x128(x, w.clone().requires_grad_(), residual=x), RuntimeError)):
+        with pytest.raises(error):
+            f()
+
+
+def test_subclasses_are_handed_the_call():
+    import hpfp8
+    seen = []
+
+    class Recording(torch.Tensor):
+        @classmethod
+        def __torch_function__(cls, func, types, args=(), kwargs=None):
+            seen.append((func, len(args), kwargs))
+            return "handed"
+    x = torch.zeros(4, 256).as_subclass(Recording)
+    y = torch.zeros(4, 256)
+    w8 = hpfp8.Int8Weight(torch.zeros(128, 256, dtype=torch.int8), torch.ones(128))
+    assert hpfp8.rms_norm(x, 256) == "handed" and seen[-1] == (hpfp8.rms_norm, 2, {})
+    assert hpfp8.rms_norm(y, 256, eps=1e-3, residual=x) == "handed" and seen[-1] == (hpfp8.rms_norm, 2, dict(eps=1e-3, residual=x))
+    assert hpfp8.int8_linear(x, w8) == "handed" and seen[-1] == (hpfp8.int8_linear, 3, {})
+    assert hpfp8.get_total_norm([y, x]) == "handed" and seen[-1][0].__name__ == "get_total_norm"
+    p = torch.nn.Parameter(torch.zeros(4, 256))
+    p.main_grad = x
+    with pytest.raises(TypeError, match="local tensors"):
+        hpfp8.clip_grads_with_norm_(p, 1.0, torch.ones(()))
+
+
+def test_saved_tensors_that_a_hook_handed_back_as_something_else(as_if_on_the_gpu):
+    from hpfp8 import norm
+    from hpfp8.int8 import _int8_backward
+    go, s, rstd = torch.zeros(4, 256, dtype=BF16), torch.zeros(4, 256, dtype=BF16), torch.ones(4)
+    for kept, other, weight in ((s[:3], rstd, None), (s.float(), rstd, None), (s, rstd[:2], None), (s, rstd.double(), None), (s, rstd, torch.ones(5, dtype=BF16))):
+        with pytest.raises(ValueError, match="came back"):
+            norm._rms_backward(go, None, kept, other, weight, 256, (4, 256), 0, None if weight is None else (256,), 0, False)
+    codes, scale = torch.zeros(128, 256, dtype=torch.int8), torch.ones(128)
+    for q, sc in ((codes[:64], scale), (codes.float(), scale), (codes, scale[:5]), (codes, scale.double())):
+        with pytest.raises(ValueError, match="came back"):
+            _int8_backward(torch.zeros(4, 128, dtype=BF16), q, sc, False, (4, 256))
