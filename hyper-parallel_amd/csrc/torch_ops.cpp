@@ -24,6 +24,7 @@
 
 #include <map>
 #include <mutex>
+#include <unordered_set>
 
 #include "../../include/hpfp8.h"
 
@@ -43,7 +44,7 @@ constexpr int64_t kBlock = 128;
   X(hpfp8_quantize_rows) X(hpfp8_dequantize_rows) X(hpfp8_quantize_saved_rows) X(hpfp8_dequantize_saved_rows) X(hpfp8_activation_forward) X(hpfp8_activation_backward) X(hpfp8_layer_norm_forward) \
   X(hpfp8_layer_norm_backward) X(hpfp8_layer_norm_partials) X(hpfp8_rms_norm_forward) X(hpfp8_rms_norm_backward) X(hpfp8_rms_norm_partials) \
   X(hpfp8_rms_norm_quantize_1x128_kmajor) X(hpfp8_rms_norm_quantize_int8) X(hpfp8_quantize_int8) X(hpfp8_gemm_int8) X(hpfp8_grad_norm) \
-  X(hpfp8_grad_norm_partials) X(hpfp8_grad_clip) X(hpfp8_cross_entropy_parts) X(hpfp8_cross_entropy_stride) X(hpfp8_cross_entropy_splits) \
+  X(hpfp8_grad_norm_partials) X(hpfp8_grad_clip) X(hpfp8_grad_norm_and_clip) X(hpfp8_cross_entropy_parts) X(hpfp8_cross_entropy_stride) X(hpfp8_cross_entropy_splits) \
   X(hpfp8_linear_cross_entropy_forward) X(hpfp8_linear_cross_entropy_piece) X(hpfp8_linear_cross_entropy_rows_t) X(hpfp8_linear_cross_entropy_round)
 struct Library {
 #define HPFP8_POINTER(name) decltype(&::name) name = nullptr;
@@ -1371,6 +1372,32 @@ struct Gradients {
     }
     return n > 0;
   }
+  // of a list of parameters, each gradient once: what grads._gradients finds of them
+  bool of_parameters(PyObject* list, int64_t device) {
+    if (!PyList_CheckExact(list)) return false;
+    std::unordered_set<const c10::TensorImpl*> seen;
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+      const at::Tensor *p, *g;
+      PyObject* const o = PyList_GET_ITEM(list, i);
+      if (!plain(o, device, p)) return false;
+      PyObject** const dict = _PyObject_GetDictPtr(o);
+      PyObject* const main_grad = dict && *dict ? PyDict_GetItemString(*dict, "main_grad") : nullptr;       // (borrowed; no error set where there is none)
+      if (main_grad && main_grad != Py_None) {
+        if (!plain(main_grad, device, g) || (p->grad().defined() && p->grad().unsafeGetTensorImpl() != g->unsafeGetTensorImpl())) return false;
+      } else {
+        g = &p->grad();
+        if (!g->defined()) continue;
+        if (!g->is_cuda() || g->get_device() != device || g->layout() != at::kStrided || at::isTensorSubclassLike(*g)) return false;
+      }
+      if (type_code(g->scalar_type()) < 0 || !g->is_contiguous()) return false;
+      if (!seen.insert(g->unsafeGetTensorImpl()).second) continue;
+      tensors.push_back(g);
+      ptrs.push_back(g->data_ptr());
+      numels.push_back(g->numel());
+      types.push_back(type_code(g->scalar_type()));
+    }
+    return !tensors.empty();
+  }
 };
 
 // (tensors, power, device, stream) -> norm
@@ -1391,6 +1418,32 @@ PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     norm = at::empty({}, options.dtype(at::kFloat));
     const at::Tensor partial = at::empty({lib.hpfp8_grad_norm_partials(g.numels.data(), g.types.data(), count)}, options.dtype(at::kDouble));
     HPFP8_CALL(call, hpfp8_grad_norm, g.ptrs.data(), g.numels.data(), g.types.data(), count, (int)power, partial.data_ptr<double>(), f32(norm), at_.stream);
+  }
+  return call.ok() ? THPVariable_Wrap(norm) : failed(call);
+  END_HANDLE_TH_ERRORS
+}
+
+// (parameters, max_norm, power, device, stream) -> norm
+PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  expect(n_args, 5);
+  const Where at_ = where(args, n_args);
+  const double max_norm = PyFloat_AsDouble(args[1]);
+  const int64_t power = PyLong_AsLongLong(args[2]);
+  if (PyErr_Occurred()) throw python_error();
+  Gradients g;
+  if (!no_modes() || !g.of_parameters(args[0], at_.device)) Py_RETURN_NONE;
+  at::Tensor norm;
+  Call call;
+  {
+    at::NoGradGuard no_grad;
+    const int64_t count = (int64_t)g.ptrs.size();
+    const at::TensorOptions options = g.tensors[0]->options().requires_grad(false);
+    norm = at::empty({}, options.dtype(at::kFloat));
+    const at::Tensor partial = at::empty({lib.hpfp8_grad_norm_partials(g.numels.data(), g.types.data(), count)}, options.dtype(at::kDouble));
+    for (const at::Tensor* t : g.tensors) t->unsafeGetTensorImpl()->bump_version();
+    HPFP8_CALL(call, hpfp8_grad_norm_and_clip, g.ptrs.data(), g.numels.data(), g.types.data(), count, (int)power, (float)max_norm,
+               partial.data_ptr<double>(), f32(norm), at_.stream);
   }
   return call.ok() ? THPVariable_Wrap(norm) : failed(call);
   END_HANDLE_TH_ERRORS
@@ -1744,7 +1797,7 @@ PyMethodDef methods[] = {HPFP8_METHOD(built_for), HPFP8_METHOD(bind), HPFP8_METH
                          HPFP8_METHOD(linear_cross_entropy), HPFP8_METHOD(bind_loss_backward),
                          HPFP8_METHOD(bind_norm_backward), HPFP8_METHOD(bind_activation_backward), HPFP8_METHOD(bind_rms_norm_backward),
                          HPFP8_METHOD(rms_norm), HPFP8_METHOD(rms_norm_quantize), HPFP8_METHOD(quantize_int8), HPFP8_METHOD(gemm_int8), HPFP8_METHOD(int8_linear),
-                         HPFP8_METHOD(grad_norm), HPFP8_METHOD(grad_clip),
+                         HPFP8_METHOD(grad_norm), HPFP8_METHOD(grad_clip), HPFP8_METHOD(clip_grad_norm),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

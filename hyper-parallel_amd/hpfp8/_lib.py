@@ -99,6 +99,7 @@ SIGNATURES = {
     "hpfp8_gemm_int8": [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _int, _vp],
     "hpfp8_grad_norm": [_vp, _vp, _vp, _i64, _int, _vp, _vp, _vp],
     "hpfp8_grad_clip": [_vp, _vp, _vp, _i64, _vp, _f32, _vp],
+    "hpfp8_grad_norm_and_clip": [_vp, _vp, _vp, _i64, _int, _f32, _vp, _vp, _vp],
 }
 # functions that return a size, not a status
 SIZE_FUNCTIONS = {

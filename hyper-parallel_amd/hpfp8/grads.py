@@ -91,10 +91,14 @@ def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_ty
     return norm
 
 
-def _clip(grads, max_norm, total_norm) -> None:
+def _bound(max_norm) -> float:
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    return max_norm
+
+
+def _clip(grads, max_norm, total_norm) -> None:
     if torch.overrides.has_torch_function(grads):
         raise TypeError("clip_grads_with_norm_ takes local tensors: call it on the shards, with the norm over all of them")
     if not grads:
@@ -122,7 +126,7 @@ def _clip(grads, max_norm, total_norm) -> None:
 def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor) -> None:
     """torch.nn.utils.clip_grads_with_norm_: every gradient times min(1, max_norm / (total_norm + 1e-6)) in place, rounded once.  Where that is 1
     nothing is read or written.  Gradients must not share memory."""
-    _clip(_gradients(parameters), max_norm, total_norm)
+    _clip(_gradients(parameters), _bound(max_norm), total_norm)
 
 
 @torch.no_grad()
@@ -130,6 +134,12 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_ for gradients in ``grad`` and in ``main_grad``: their total norm (a 0-dim float32 tensor), and the gradients
     scaled in place so that it is at most ``max_norm``."""
+    parameters, power, max_norm = _list_of(parameters), _power(norm_type), _bound(max_norm)
+    if ops._native is not None and parameters and not error_if_nonfinite:
+        device = ops._device()
+        norm = ops._native.clip_grad_norm(parameters, max_norm, power, device, ops._raw_stream(device))
+        if norm is not None:
+            return norm
     grads = _gradients(parameters)
     norm = get_total_norm(grads, norm_type, error_if_nonfinite)
     _clip(grads, max_norm, norm)

@@ -579,6 +579,9 @@ int hpfp8_grad_norm(const void* const* ptrs, const int64_t* numels, const int* t
  * are refused. */
 int hpfp8_grad_clip(void* const* ptrs, const int64_t* numels, const int* types, int64_t count, const float* norm, float max_norm,
                     hpfp8_stream_t stream);
+/* Both, with one launch fewer. */
+int hpfp8_grad_norm_and_clip(void* const* ptrs, const int64_t* numels, const int* types, int64_t count, int power, float max_norm, double* partial,
+                             float* norm, hpfp8_stream_t stream);
 
 /* Softmax cross entropy of the linear l = x w^T over a vocabulary, without the logits in memory.  x[tokens, hidden] and w[vocab, hidden] are
  * bf16, row strides ld_x and ld_w in elements, hidden and the strides multiples of 8 and below 2^21, tokens at most 2^21, vocab at most 2^24;
