@@ -30,11 +30,15 @@ struct RmsParams {
   int pow2;              // E4M3: scales that are powers of two
 };
 
+// Rows on their way while one is worked on.  us with two / one, 16384 x 7168 bf16, 4096 x 16384: own type 78.5 / 87, 49.1 / 46.7; E4M3 75.2 / 76.8,
+// 50.5 / 45.1; int8 70.1 / 65.2, 44.8 / 35.1.  With a residual a row is two streams and (launch_forward) a workgroup has mostly one.
+constexpr int rows_ahead(int out, bool residual, int steps) { return residual || steps > 2 || out == kInt8 ? 1 : 2; }
+
 template <typename E, int TPR, int NV, int OUT, bool RES, int EDGE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV <= 2 && sizeof(typename E::raw) == 2 ? 4 : 2) void rms_forward_kernel(RmsParams p) {
   using raw = typename E::raw;
   constexpr int kTeams = (TPR < 256 ? 256 : TPR) / TPR, kWaves = TPR < 64 ? 1 : TPR / 64;
-  constexpr int kAhead = NV > 2 && sizeof(raw) == 4 && RES ? 1 : 2;      // rows under way (two of both fp32 streams of over 8192 values do not fit the registers)
+  constexpr int kAhead = rows_ahead(OUT, RES, NV);
   static_assert(OUT == kOwnType || EDGE == kWhole, "codes are of whole groups");
   __shared__ float sums[2][kTeams][kWaves], tops[2][kTeams][kWaves];
   const int team = team_of<TPR>(), t = threadIdx.x % TPR, wave = __builtin_amdgcn_readfirstlane(t / 64);
@@ -158,8 +162,13 @@ int launch_forward(const RmsParams& p, int dtype, hipStream_t stream) {
   by_type_and_width<false>(dtype, p.cols, [&](auto e, auto tpr, auto nv) {
     using E = decltype(e);
     constexpr int kThreads = tpr < 256 ? 256 : tpr, kTeams = kThreads / tpr;
-    const int64_t blocks = (p.rows + kTeams - 1) / kTeams, most = 256 * (1024 / kThreads);   // every compute unit full once
-    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    const int64_t blocks = (p.rows + kTeams - 1) / kTeams, full = 256 * (1024 / kThreads);   // every compute unit full once
+    // Workgroups that stay for many rows load the weight once; with a residual, and so two streams written beside two read, ones that leave after
+    // one row sweep memory in a tighter order, which is worth more from a few rounds on.  us, staying / leaving, own type, E4M3, int8:
+    //   16384 x 7168 bf16  162 / 154, 164 / 141, 147 / 133      65536 x 256  26.2 / 24.3, 24.6 / 22.7, 23.5 / 21.8      fp32 4096 x 7168  92 / 86, 80 / 72, 72 / 69
+    //   1024 x 7168        12.1 / 14.1, 13.6 / 13.3, 12.8 / 12.6     4096 x 16384  97 / 90, 94 / 100, 81 / 79;   without a residual 78 / 80, 75 / 79, 65 / 67
+    const bool leave = p.residual && blocks > 2 * full && !(OUT == kE4m3 && nv > 2) && blocks < ((int64_t)1 << 31);
+    const dim3 grid((unsigned)(leave || blocks < full ? blocks : full));
     auto with = [&](auto edge) {
       if (p.residual) rms_forward_kernel<E, tpr, nv, OUT, true, edge><<<grid, kThreads, 0, stream>>>(p);
       else rms_forward_kernel<E, tpr, nv, OUT, false, edge><<<grid, kThreads, 0, stream>>>(p);
