@@ -34,8 +34,10 @@ template <typename E, int TPR, int NV, bool DS, int EDGE>
 __global__ __launch_bounds__(kThreads) void rms_backward_kernel(RmsBackwardParams p) {
   using raw = typename E::raw;
   constexpr int kTeams = kThreads / TPR, kWaves = TPR < 64 ? 1 : TPR / 64, kChunks = TPR * NV;
-  constexpr int kAhead = NV > 2 ? 1 : (sizeof(raw) == 2 ? 3 : 2);
-  constexpr bool kEarlyDs = DS && (NV <= 2 || sizeof(raw) == 2);         // (of over 8192 fp32 values the third stream does not fit the registers)
+  // Rows on their way while one is worked on, us with two / three / four, with ds': 16384 x 7168 bf16 166 / 163 / 162, x 2048 52 / 55 / 55, 65536 x 256
+  // 41 / 44 / 44; 4096 x 16384 with one / two 110 / 107 (without ds' 89 / 80).
+  constexpr int kAhead = sizeof(raw) == 4 ? (NV > 2 ? 1 : 2) : (TPR == 512 && NV == 2 ? 4 : (TPR == 256 && NV == 2 ? 3 : 2));
+  constexpr bool kEarlyDs = DS && NV <= 2;   // (of over 8192 values the third stream does not fit the registers)
   constexpr bool kHoldWeight = NV <= 2;      // (four steps' sums and rows fill the registers: the weight in LDS then)
   __shared__ float parts[2][kTeams][kWaves];
   __shared__ v4f joined[kTeams > 1 ? kChunks * 2 : 1];
@@ -133,9 +135,19 @@ __global__ __launch_bounds__(kThreads) void rms_backward_kernel(RmsBackwardParam
       work(row, from + team, turn);
     }
   }
-  // the teams' sums, one after the other
+  // the teams' sums: a wave's four first, then one after the other
+  constexpr int kJoint = TPR < 64 ? 4 : 1;
+  if constexpr (kJoint > 1) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        dw[j][i] += __shfl_xor(dw[j][i], 16);
+        dw[j][i] += __shfl_xor(dw[j][i], 32);
+      }
+  }
   float* const to = p.partial + (int64_t)blockIdx.x * C;
-  for (int k = 0; k < kTeams; ++k) {
+  for (int k = 0; k < kTeams; k += kJoint) {
     if (team == k) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -145,41 +157,41 @@ __global__ __launch_bounds__(kThreads) void rms_backward_kernel(RmsBackwardParam
 #pragma unroll
             for (int i = 0; i < 8; ++i) dw[j][i] = a[i / 4][i % 4] + dw[j][i];
           }
-          if (k < kTeams - 1) {
+          if (k < kTeams - kJoint) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) a[h] = v4f{dw[j][4 * h], dw[j][4 * h + 1], dw[j][4 * h + 2], dw[j][4 * h + 3]};
           }
         }
-        if (k == kTeams - 1) store_chunk<F32, EDGE>(to, at[j], C, dw[j]);
+        if (k == kTeams - kJoint) store_chunk<F32, EDGE>(to, at[j], C, dw[j]);
       }
     }
     if (kTeams > 1) __syncthreads();
   }
 }
 
-// dw from the workgroups' partial sums: 64 columns per workgroup, each of its 16 waves every sixteenth partial sum, then the waves in order.
+// dw from the workgroups' partial sums: 32 columns per workgroup, each of its 32 half waves every 32nd partial sum, then those in order.
 __global__ __launch_bounds__(1024) void rms_join_kernel(const float* __restrict__ partial, int count, int cols, void* __restrict__ dw, int wtype) {
-  __shared__ float parts[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+  __shared__ float parts[32][33];
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int64_t col = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.f;
   if (col < cols) {
-    int k = wave;
-    for (; k + 48 < count; k += 64) {
-      float v[4];
+    int k = part;
+    for (; k + 224 < count; k += 256) {
+      float v[8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = partial[(int64_t)(k + 16 * u) * cols + col];
+      for (int u = 0; u < 8; ++u) v[u] = partial[(int64_t)(k + 32 * u) * cols + col];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) s += v[u];
+      for (int u = 0; u < 8; ++u) s += v[u];
     }
-    for (; k < count; k += 16) s += partial[(int64_t)k * cols + col];
+    for (; k < count; k += 32) s += partial[(int64_t)k * cols + col];
   }
-  parts[wave][lane] = s;
+  parts[part][lane] = s;
   __syncthreads();
-  if (wave == 0 && col < cols) {
+  if (part == 0 && col < cols) {
     float total = 0.f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) total += parts[k][lane];
+    for (int k = 0; k < 32; ++k) total += parts[k][lane];
     if (wtype == HPFP8_OUT_BF16) ((uint16_t*)dw)[col] = from_f32<Bf16>(total);
     else if (wtype == HPFP8_TYPE_F16) ((_Float16*)dw)[col] = (_Float16)total;
     else ((float*)dw)[col] = total;
@@ -234,7 +246,7 @@ int hpfp8_rms_norm_backward(const void* dy, int64_t ld_dy, const void* s, int64_
     if (rc != HPFP8_OK) return rc;
   }
   if (dw) {            // (no rows: zeros)
-    rms_join_kernel<<<(unsigned)((cols + 63) / 64), 1024, 0, (hipStream_t)stream>>>(partial, (int)hpfp8_rms_norm_partials(rows, cols), (int)cols, dw, wtype);
+    rms_join_kernel<<<(unsigned)((cols + 31) / 32), 1024, 0, (hipStream_t)stream>>>(partial, (int)hpfp8_rms_norm_partials(rows, cols), (int)cols, dw, wtype);
     return check_launch("rms_norm_backward (join)");
   }
   return HPFP8_OK;
