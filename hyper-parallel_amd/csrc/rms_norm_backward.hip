@@ -35,9 +35,9 @@ __global__ __launch_bounds__(kThreads) void rms_backward_kernel(RmsBackwardParam
   using raw = typename E::raw;
   constexpr int kTeams = kThreads / TPR, kWaves = TPR < 64 ? 1 : TPR / 64, kChunks = TPR * NV;
   // Rows on their way while one is worked on, us with two / three / four, with ds': 16384 x 7168 bf16 166 / 163 / 162, x 2048 52 / 55 / 55, 65536 x 256
-  // 41 / 44 / 44; 4096 x 16384 with one / two 110 / 107 (without ds' 89 / 80).
-  constexpr int kAhead = sizeof(raw) == 4 ? (NV > 2 ? 1 : 2) : (TPR == 512 && NV == 2 ? 4 : (TPR == 256 && NV == 2 ? 3 : 2));
-  constexpr bool kEarlyDs = DS && NV <= 2;   // (of over 8192 values the third stream does not fit the registers)
+  // 41 / 44 / 44; 4096 x 16384 with one / two 89 / 80 without ds', with it two do not fit the registers.
+  constexpr int kAhead = sizeof(raw) == 4 ? (NV > 2 ? 1 : 2) : (NV > 2 ? (DS ? 1 : 2) : (TPR == 512 ? 4 : (TPR == 256 && NV == 2 ? 3 : 2)));
+  constexpr bool kEarlyDs = DS && (NV <= 2 || sizeof(raw) == 2);         // (of over 8192 fp32 values the third stream does not fit the registers)
   constexpr bool kHoldWeight = NV <= 2;      // (four steps' sums and rows fill the registers: the weight in LDS then)
   __shared__ float parts[2][kTeams][kWaves];
   __shared__ v4f joined[kTeams > 1 ? kChunks * 2 : 1];
