@@ -274,3 +274,79 @@ def test_more_than_2_31_elements(gpu):
     p.grad = t
     hpfp8.clip_grads_with_norm_(p, 6.5, torch.tensor(13.0, device=gpu))
     assert [float(t[i]) for i in (0, 1 << 30, n - 1)] == [1.5, 2.0, 6.0] and int((t != 0).sum()) == 3
+
+
+@pytest.mark.parametrize("p", [2.0, math.inf])
+def test_more_than_the_caches_hold(gpu, p):
+    """Streamed: over 256 MiB, in more tensors than a launch takes, odd sizes of every type, starts between vectors."""
+    import hpfp8
+    sizes = [40_000_003, 30_000_001, 33_333_333] + [1009 + 7 * i for i in range(170)]
+    flats = {d: torch.randn((sum(sizes[i::3]) + 1,), generator=torch.Generator().manual_seed(7)).to(d) for i, d in enumerate(TYPES)}
+    on = {d: t.to(gpu) for d, t in flats.items()}
+    before = {d: t.clone() for d, t in flats.items()}
+    ps, at = [], dict.fromkeys(TYPES, 1)
+    for i, n in enumerate(sizes):
+        d = TYPES[i % 3]
+        q = torch.nn.Parameter(torch.zeros((1,), dtype=d, device=gpu).expand(n))
+        q.grad = on[d][at[d]:at[d] + n]
+        at[d] += n
+        ps.append(q)
+    assert sum(q.grad.numel() * q.grad.element_size() for q in ps) > 256 << 20
+    want = norm64([t[1:] for t in flats.values()], p)
+    norm = hpfp8.get_total_norm([q.grad for q in ps], p)
+    near(norm, want)
+    assert torch.equal(hpfp8.clip_grad_norm_(ps, 10 * float(want), p), norm)
+    assert all(torch.equal(on[d].cpu(), before[d]) for d in TYPES)       # (the bound holds)
+    assert torch.equal(hpfp8.clip_grad_norm_(ps, 0.25 * float(want), p), norm)
+    for d in TYPES:
+        got = on[d].cpu()
+        assert torch.equal(got[1:], clipped([before[d][1:]], norm, 0.25 * float(want))[0]) and got[0] == before[d][0]
+
+
+def test_around_the_size_that_is_streamed(gpu):
+    """The same values in one form and in the other have the same norm and become the same."""
+    import hpfp8
+    n = (256 << 20) // 4
+    t = torch.randn((n + 5000,), device=gpu, generator=torch.Generator(device=gpu).manual_seed(8))
+    for m in (n - 1, n, n + 1, n + 4097):
+        part = t[:m].clone()
+        q = torch.nn.Parameter(torch.zeros((1,), device=gpu).expand(m))
+        q.grad = part
+        norm = hpfp8.clip_grad_norm_(q, 100.0)
+        assert abs(float(norm) - float(torch.linalg.vector_norm(t[:m].double()))) <= 2.0 ** -23 * float(norm)
+        factor = torch.tensor(100.0, device=gpu) / (norm + 1e-6)
+        assert torch.equal(part, t[:m] * factor)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_tensors_made_in_inference_mode(gpu, native, monkeypatch):
+    import hpfp8
+    from hpfp8 import ops
+    if not native:
+        monkeypatch.setattr(ops, "_native", None)
+    with torch.inference_mode():
+        g = torch.full((1000,), 2.0, device=gpu)
+        q = torch.nn.Parameter(torch.zeros(1000, device=gpu))
+        q.main_grad = g
+        near(hpfp8.clip_grad_norm_([q], 1e9), torch.tensor(2.0 * 1000 ** 0.5, dtype=torch.float64))
+        hpfp8.clip_grads_with_norm_([q], 1.0, torch.tensor(2.0, device=gpu))
+        assert torch.equal(g, torch.full_like(g, 2.0) * (1.0 / (torch.tensor(2.0, device=gpu) + 1e-6)))
+
+
+def test_half_a_parameters_gradient_in_each_place(gpu):
+    """Weights with main gradients beside biases with ordinary ones, in whatever containers."""
+    import hpfp8
+    linear = hpfp8.Fp8Linear(128, 256, device=gpu, apply_grad_on_fp32_main_grad=True)
+    x = torch.randn((32, 128), device=gpu).to(torch.bfloat16)
+    linear(x).float().square().sum().backward()
+    grads = [linear.weight.main_grad.clone(), linear.bias.grad.clone()]
+    want = norm64([t.cpu() for t in grads], 2.0)
+    for given in (linear.parameters(), tuple(linear.parameters()), [linear.bias, linear.weight], {p: 0 for p in linear.parameters()}):
+        near(hpfp8.clip_grad_norm_(given, 1e9), want)
+    norm = hpfp8.clip_grad_norm_(linear.parameters(), 1.0)
+    for got, t in zip((linear.weight.main_grad, linear.bias.grad), clipped([t.cpu() for t in grads], norm, 1.0)):
+        assert torch.equal(got.cpu(), t)
+    # the next backward adds onto what was clipped
+    before = linear.weight.main_grad.clone()
+    linear(x).float().square().sum().backward()
+    assert (linear.weight.main_grad - before - grads[0]).abs().max() <= 1e-5 * grads[0].abs().max()

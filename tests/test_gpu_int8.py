@@ -385,3 +385,81 @@ def test_refused(gpu):
         hpfp8.gemm_int8(w8.codes, w8.scale_inv, w8.codes, None, out_dtype=torch.float64)
     with torch.no_grad():
         assert hpfp8.int8_linear(x, w8, bias.clone().requires_grad_()).shape == (4, 128)
+
+
+def test_more_than_2_31_values_quantized_and_codes_of_a_weight_past_2_31(gpu):
+    import hpfp8
+    rows, cols = (1 << 31) // 4096 + 64, 4096
+    part = values(64, cols, torch.bfloat16, 1).to(gpu)
+    x = torch.empty((rows, cols), dtype=torch.bfloat16, device=gpu)
+    x.view(-1, 64, cols)[:] = part
+    by = torch.rand((cols,), device=gpu)
+    codes, scale = hpfp8.quantize_int8(x, column_scale=by)
+    want, want_scale = hpfp8.quantize_int8(part, column_scale=by)
+    for at in (0, rows - 64):
+        assert torch.equal(codes[at:at + 64], want) and torch.equal(scale[at:at + 64], want_scale)
+    del x
+    one = torch.ones((5,), device=gpu)
+    assert rows % 128 == 64
+    w = codes[:rows - 64]                                    # [524288, 4096]
+    for a in (want[:5], want):
+        s = torch.ones((a.shape[0],), device=gpu)
+        c = hpfp8.gemm_int8(a, s, w, None)
+        few = hpfp8.gemm_int8(a, s, want.repeat(2, 1), None)
+        for at in (0, w.shape[0] - 128):
+            assert torch.equal(c[:, at:at + 128], few)
+    del one
+
+
+def test_hooks_on_saved_tensors(gpu):
+    """What a hook hands back is looked at: as it was or packed elsewhere and back it is used, anything else is refused."""
+    import hpfp8
+    f, (x,), go = operator()
+    xl = x.clone().requires_grad_()
+    want, = torch.autograd.grad(f(xl), xl, go)
+    with torch.autograd.graph.save_on_cpu():
+        y = f(xl)
+    assert torch.equal(torch.autograd.grad(y, xl, go)[0], want)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t):
+        y = f(xl)
+    assert torch.equal(torch.autograd.grad(y, xl, go)[0], want)
+    for wrong in (lambda t: t.float(), lambda t: t[:-1], lambda t: t.cpu()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, wrong):
+            y = f(xl)
+        with pytest.raises((ValueError, TypeError)):
+            torch.autograd.grad(y, xl, go)
+
+
+def test_steps_of_several_threads_at_once(gpu):
+    import threading
+    import hpfp8
+    w8 = hpfp8.quantize_weight_int8(values(512, 1024, torch.bfloat16, 1).to(gpu))
+    norm_w = torch.ones(1024, dtype=torch.bfloat16, device=gpu)
+    xs = [values(200 + 50 * i, 1024, torch.bfloat16, 10 + i).to(gpu) for i in range(4)]
+
+    def run(i):
+        x = xs[i].clone().requires_grad_()
+        y, s = hpfp8.rms_norm(x, 1024, norm_w, residual=xs[i])
+        z = hpfp8.int8_linear(y, w8)
+        dx, = torch.autograd.grad((z, s), x, (torch.ones_like(z), torch.ones_like(s)))
+        p = torch.nn.Parameter(torch.zeros_like(x))
+        p.grad = dx.clone()
+        norm = hpfp8.clip_grad_norm_([p], 1.0)
+        return z.detach(), dx, norm, p.grad
+    want = [run(i) for i in range(4)]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i] = run(i)
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))

@@ -475,3 +475,45 @@ def test_more_than_2_31_values(gpu, form):
         want, want_scale = f(few)
         for at in (0, rows - 64):
             assert torch.equal(codes[at:at + 64].view(torch.uint8), want.view(torch.uint8)) and torch.equal(scale[at:at + 64], want_scale)
+
+
+def test_hooks_on_saved_tensors(gpu):
+    """What a hook hands back is looked at: as it was or packed elsewhere and back it is used, anything else is refused."""
+    import hpfp8
+    x, r, w, go, gs = (t.to(gpu) for t in make(32, 384, torch.bfloat16, torch.bfloat16, 15))
+    leaves = [t.requires_grad_() for t in (x, r, w)]
+    f = lambda: hpfp8.rms_norm(leaves[0], 384, leaves[2], residual=leaves[1])          # noqa: E731
+    want = torch.autograd.grad(f(), leaves, (go, gs))
+    with torch.autograd.graph.save_on_cpu():
+        out = f()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, (go, gs)), want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t):
+        out = f()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, (go, gs)), want))
+    for wrong in (lambda t: t.double(), lambda t: t[:-1], lambda t: t.cpu()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, wrong):
+            out = f()
+        with pytest.raises((ValueError, TypeError)):
+            torch.autograd.grad(out, leaves, (go, gs))
+
+
+def test_gradient_penalty_through_what_follows_and_accumulation(gpu):
+    """Two uses of the stream: their gradients add up before they reach the norm's node; .backward twice accumulates."""
+    import hpfp8
+    x, r, w, go, gs = (t.to(gpu) for t in make(40, 256, torch.float32, torch.float32, 16))
+    leaves = [t.requires_grad_() for t in (x, r, w)]
+    for t in leaves:
+        t.grad = None
+    for _ in range(2):
+        y, s = hpfp8.rms_norm(leaves[0], 256, leaves[2], EPS, residual=leaves[1])
+        y2, s2 = hpfp8.rms_norm(y, 256, leaves[2], EPS, residual=s)
+        ((y2 * go).sum() + (s2 * gs).sum() + (s * go).sum()).backward()
+    a, b, c = (t.detach().double().requires_grad_() for t in leaves)
+
+    def norm(v):
+        return v / torch.sqrt((v * v).mean(1, keepdim=True) + EPS) * c
+    s = a + b
+    s2 = norm(s) + s
+    ((norm(s2) * go.double()).sum() + (s2 * gs.double()).sum() + (s * go.double()).sum()).backward()
+    for t, u in zip(leaves, (a, b, c)):
+        assert (t.grad.double() - 2 * u.grad).norm() <= 1e-5 * u.grad.norm()       # (a few hundred roundings of 2^-24)
