@@ -319,7 +319,7 @@ int for_each_batch(const void* const* ptrs, const int64_t* numels, const int* ty
 int clip(void* const* ptrs, const int64_t* numels, const int* types, int64_t count, const float* norm, float max_norm, hipStream_t stream) {
   const bool streamed = all_bytes(numels, types, count) > kCached;
   return for_each_batch(ptrs, numels, types, count, kStep, [&](const GradBatch& b, unsigned parts, int64_t) {
-    if (streamed) grad_clip_kernel<true><<<parts, kThreads, 0, stream>>>(b, norm, max_norm);
+    if (streamed) grad_clip_kernel<true><<<std::min(parts, 1u << 22), kThreads, 0, stream>>>(b, norm, max_norm);
     else grad_clip_kernel<false><<<std::min(parts, kClipWorkgroups), kThreads, 0, stream>>>(b, norm, max_norm);
     return check_launch("grad_clip");
   });

@@ -167,7 +167,7 @@ int launch_forward(const RmsParams& p, int dtype, hipStream_t stream) {
     // one row sweep memory in a tighter order, which is worth more from a few rounds on.  us, staying / leaving, own type, E4M3, int8:
     //   16384 x 7168 bf16  162 / 154, 164 / 141, 147 / 133      65536 x 256  26.2 / 24.3, 24.6 / 22.7, 23.5 / 21.8      fp32 4096 x 7168  92 / 86, 80 / 72, 72 / 69
     //   1024 x 7168        12.1 / 14.1, 13.6 / 13.3, 12.8 / 12.6     4096 x 16384  97 / 90, 94 / 100, 81 / 79;   without a residual 78 / 80, 75 / 79, 65 / 67
-    const bool leave = p.residual && blocks > 2 * full && !(OUT == kE4m3 && nv > 2) && blocks < ((int64_t)1 << 31);
+    const bool leave = p.residual && blocks > 2 * full && !(OUT == kE4m3 && nv > 2) && blocks < ((int64_t)1 << 22);
     const dim3 grid((unsigned)(leave || blocks < full ? blocks : full));
     auto with = [&](auto edge) {
       if (p.residual) rms_forward_kernel<E, tpr, nv, OUT, true, edge><<<grid, kThreads, 0, stream>>>(p);

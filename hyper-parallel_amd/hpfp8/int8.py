@@ -15,7 +15,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 from .kept import _TYPES, _as_rows, _check_rows
-from .linear import _Fp8WeightCache, _hand_off
+from .linear import _hand_off
 
 MAX_FEATURES = 130944       # the sums of so many products of two codes fit 32 bits
 
@@ -211,47 +211,66 @@ def int8_linear(input: torch.Tensor, weight: Int8Weight, bias: Optional[torch.Te
 
 class Int8Linear(nn.Module):
     """A linear whose weight is frozen in 8-bit integers (buffers ``weight_codes``, ``weight_scale_inv`` and, with a bias, ``bias``), computed by
-    `int8_linear`.  Made of a trained layer by `from_linear`."""
+    `int8_linear`.  Made of a trained layer by `from_linear`.
 
-    def __init__(self, in_features: int, out_features: int, bias: bool = True, *, device=None, dtype=torch.bfloat16):
+    With ``with_transpose`` it also holds the transposed codes, which the input's gradient reads, as a buffer that is in no state dict; without
+    them, and after ``weight_codes`` was written or replaced, each backward makes them anew.  ``load_state_dict`` and `refresh` bring them up to
+    date (a write that the version counter does not see, through ``weight_codes.data``, needs the latter)."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, *, with_transpose: bool = False, device=None, dtype=torch.bfloat16):
         super().__init__()
         if in_features % ops.BLOCK or out_features % ops.BLOCK or not 0 < in_features <= MAX_FEATURES or not 0 < out_features <= MAX_FEATURES:
             raise ValueError(f"in_features and out_features must be multiples of 128 of at most {MAX_FEATURES}")
-        self.in_features, self.out_features = in_features, out_features
+        self.in_features, self.out_features, self.with_transpose = in_features, out_features, with_transpose
         self.register_buffer("weight_codes", torch.zeros((out_features, in_features), dtype=torch.int8, device=device))
         self.register_buffer("weight_scale_inv", torch.ones((out_features,), dtype=torch.float32, device=device))
         self.register_buffer("bias", torch.zeros((out_features,), dtype=dtype, device=device) if bias else None)
-        self._cache = _Fp8WeightCache(1)         # the transposed codes
-        self.register_load_state_dict_post_hook(lambda module, _keys: module.invalidate_cache())
+        self.register_buffer("weight_codes_t", None, persistent=False)
+        self.refresh()
+        self.register_load_state_dict_post_hook(lambda module, _keys: module.refresh())
 
     @classmethod
-    def from_linear(cls, linear: nn.Module) -> "Int8Linear":
+    def from_linear(cls, linear: nn.Module, *, with_transpose: bool = False) -> "Int8Linear":
         """Of a layer with a ``weight`` [out_features, in_features] and a ``bias`` or None: torch.nn.Linear, `Fp8Linear`."""
         weight, bias = linear.weight, linear.bias
         made = cls(weight.shape[1], weight.shape[0], bias is not None, device=weight.device, dtype=weight.dtype)
-        w8 = quantize_weight_int8(weight)
-        made.weight_codes, made.weight_scale_inv = w8.codes, w8.scale_inv
+        made.weight_codes, made.weight_scale_inv, _ = quantize_weight_int8(weight)
         if bias is not None:
             made.bias = bias.detach().clone()
+        made.with_transpose = with_transpose
+        made.refresh()
         return made
 
-    def invalidate_cache(self) -> None:
-        """Forget the transposed codes: the next backward's forward makes them again (they are refreshed by themselves when ``weight_codes`` is
-        replaced or written through torch)."""
-        self._cache.clear()
+    def _note_codes(self) -> None:
+        # (the tensor itself, not its address, which another could have later; one made in inference mode has no version to go by)
+        codes = self.weight_codes
+        self._transposed_of = None if codes.is_inference() else (codes, codes._version)
+
+    def _up_to_date(self) -> bool:
+        of = self._transposed_of
+        return of is not None and of[0] is self.weight_codes and of[1] == of[0]._version
+
+    def refresh(self) -> None:
+        """Make the transposed codes, where the layer holds them, of ``weight_codes`` as it is now."""
+        codes = self.weight_codes
+        self.weight_codes_t = None if not self.with_transpose else (_transposed(codes) if codes.is_cuda else codes.t().contiguous())
+        self._note_codes()
 
     def _apply(self, fn, recurse=True):
+        up_to_date = self._up_to_date()
         scale_inv = self.weight_scale_inv
         super()._apply(fn, recurse)
         if self.weight_scale_inv.dtype != torch.float32:            # (.to(torch.bfloat16) is meant for the bias)
             self.weight_scale_inv = scale_inv.to(self.weight_scale_inv.device)
-        self.invalidate_cache()
+        self._transposed_of = None
+        if up_to_date:
+            self._note_codes()
         return self
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
-        codes_t = None
-        if torch.is_grad_enabled() and input.requires_grad:
-            codes_t = self._cache.get(0, self.weight_codes, _transposed)
+        codes_t = self.weight_codes_t
+        if codes_t is not None and not self._up_to_date():
+            codes_t = None
         return int8_linear(input, Int8Weight(self.weight_codes, self.weight_scale_inv, codes_t), self.bias)
 
     def extra_repr(self) -> str:

@@ -246,30 +246,44 @@ def test_no_tokens(gpu):
         assert hpfp8.int8_linear(x, w8).shape == (0, 3, 128)
 
 
-def test_module_form(gpu):
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("with_transpose", [False, True])
+def test_module_form(gpu, bias, with_transpose):
     import hpfp8
-    for bias in (False, True):
-        linear = torch.nn.Linear(256, 384, bias=bias, device=gpu, dtype=torch.bfloat16)
-        made = hpfp8.Int8Linear.from_linear(linear)
-        x = values(40, 256, torch.bfloat16, 2).to(gpu).requires_grad_()
-        w8 = hpfp8.quantize_weight_int8(linear.weight)
-        y = made(x)
-        b = None if not bias else linear.bias.detach()
-        assert torch.equal(y, hpfp8.int8_linear(x, w8, b))
-        go = values(40, 384, torch.bfloat16, 3).to(gpu)
-        want, = torch.autograd.grad(hpfp8.int8_linear(x, w8, b), x, go)
-        assert torch.equal(torch.autograd.grad(y, x, go)[0], want)
-        other = hpfp8.Int8Linear(256, 384, bias=bias, device=gpu)
-        other(x)                                             # (its transposed codes are those of zeros)
-        other.load_state_dict(made.state_dict())
-        assert torch.equal(torch.autograd.grad(other(x), x, go)[0], want)
-        with torch.no_grad():
-            other.weight_codes.neg_()
-        assert torch.equal(torch.autograd.grad(other(x), x, go)[0], -want)
-        assert not list(made.parameters()) and "in_features=256" in repr(made)
-        half = made.to(torch.float16)
-        assert half.weight_scale_inv.dtype == torch.float32 and half.weight_codes.dtype == torch.int8
-        assert torch.equal(half(x.detach().half()), hpfp8.int8_linear(x.detach().half(), w8, None if b is None else b.half()))
+    linear = torch.nn.Linear(256, 384, bias=bias, device=gpu, dtype=torch.bfloat16)
+    made = hpfp8.Int8Linear.from_linear(linear, with_transpose=with_transpose)
+    x = values(40, 256, torch.bfloat16, 2).to(gpu).requires_grad_()
+    w8 = hpfp8.quantize_weight_int8(linear.weight)
+    y = made(x)
+    b = None if not bias else linear.bias.detach()
+    assert torch.equal(y, hpfp8.int8_linear(x, w8, b)) and (made.weight_codes_t is not None) == with_transpose
+    go = values(40, 384, torch.bfloat16, 3).to(gpu)
+    want, = torch.autograd.grad(hpfp8.int8_linear(x, w8, b), x, go)
+    assert torch.equal(torch.autograd.grad(y, x, go)[0], want)
+    assert list(made.state_dict()) == ["weight_codes", "weight_scale_inv"] + ["bias"] * bias
+    other = hpfp8.Int8Linear(256, 384, bias=bias, with_transpose=with_transpose, device=gpu)
+    other(x)                                                 # (its transposed codes are those of zeros)
+    other.load_state_dict(made.state_dict())
+    assert torch.equal(torch.autograd.grad(other(x), x, go)[0], want)
+    with torch.no_grad():
+        other.weight_codes.neg_()
+    assert torch.equal(torch.autograd.grad(other(x), x, go)[0], -want)
+    other.weight_codes = w8.codes.clone()
+    assert torch.equal(torch.autograd.grad(other(x), x, go)[0], want)
+    other.refresh()
+    assert torch.equal(torch.autograd.grad(other(x), x, go)[0], want)
+    assert not list(made.parameters()) and "in_features=256" in repr(made)
+    there = made.cpu().to(gpu)                               # (codes and transposed codes move together)
+    assert torch.equal(torch.autograd.grad(there(x), x, go)[0], want)
+    half = made.to(torch.float16)
+    assert half.weight_scale_inv.dtype == torch.float32 and half.weight_codes.dtype == torch.int8
+    assert torch.equal(half(x.detach().half()), hpfp8.int8_linear(x.detach().half(), w8, None if b is None else b.half()))
+    import copy
+    twin = copy.deepcopy(there).to(torch.bfloat16)
+    assert torch.equal(torch.autograd.grad(twin(x), x, go)[0], want)
+    with torch.inference_mode():
+        served = hpfp8.Int8Linear.from_linear(linear, with_transpose=with_transpose)
+        assert torch.equal(served(x.detach()), y)
     fp8 = hpfp8.Fp8Linear(256, 384, device=gpu)
     assert hpfp8.Int8Linear.from_linear(fp8)(x.detach()).shape == (40, 384)
 
