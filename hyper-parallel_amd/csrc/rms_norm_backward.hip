@@ -6,6 +6,8 @@
 // One pass over memory like the forward.  The workgroups stay for many rows and dw grows in their registers; at the end a workgroup's teams
 // are joined in LDS in their order, its sums leave as one row of partial sums, at most 256 of them (512 where rows are short), and a second
 // launch adds those up in a fixed order: the same bits every time.
+//
+// bf16: 4096 x 7168 with ds' 44 + 4 us, 5.3 TB/s; 16384 x 7168 161 us with both launches, 5.8 TB/s, without ds' 124, 5.7 TB/s.
 #include "norm_rows.h"
 
 namespace hpfp8 {

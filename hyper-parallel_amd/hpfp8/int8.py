@@ -181,10 +181,6 @@ def int8_linear(input: torch.Tensor, weight: Int8Weight, bias: Optional[torch.Te
     if not isinstance(weight, Int8Weight):
         raise TypeError("weight must be an Int8Weight (quantize_weight_int8)")
     codes, scale_inv, codes_t = weight
-    if codes_t is not None:
-        _check_codes(codes_t, "weight.codes_t")
-        if codes_t.shape != codes.shape[::-1]:
-            raise ValueError(f"weight.codes_t must be the transpose of weight.codes {tuple(codes.shape)}, got {tuple(codes_t.shape)}")
     if ops._gpu(input):
         device = ops._device()
         y = ops._native.int8_linear(input, codes, scale_inv, codes_t, bias, device, ops._raw_stream(device))
@@ -200,6 +196,10 @@ def int8_linear(input: torch.Tensor, weight: Int8Weight, bias: Optional[torch.Te
     ops._check_f32(scale_inv, "weight.scale_inv")
     if scale_inv.shape != (n,):
         raise ValueError(f"weight.scale_inv must have shape {(n,)}, got {tuple(scale_inv.shape)}")
+    if codes_t is not None:
+        _check_codes(codes_t, "weight.codes_t")
+        if codes_t.shape != codes.shape[::-1]:
+            raise ValueError(f"weight.codes_t must be the transpose of weight.codes {tuple(codes.shape)}, got {tuple(codes_t.shape)}")
     _check_bias(bias, n, input.dtype)
     if bias is not None and bias.requires_grad and torch.is_grad_enabled():
         raise ValueError("int8_linear has no gradient for a bias: detach it, or add it to the result")
