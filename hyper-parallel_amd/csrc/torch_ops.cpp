@@ -24,7 +24,6 @@
 
 #include <map>
 #include <mutex>
-#include <unordered_set>
 
 #include "../../include/hpfp8.h"
 
@@ -1433,13 +1432,25 @@ struct Gradients {
   // of a list of parameters, each gradient once: what grads._gradients finds of them
   bool of_parameters(PyObject* list, int64_t device) {
     if (!PyList_CheckExact(list)) return false;
-    std::unordered_set<const c10::TensorImpl*> seen;
-    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+    static PyObject* const name = PyUnicode_InternFromString("main_grad");
+    const Py_ssize_t n = PyList_GET_SIZE(list);
+    size_t slots = 64;
+    while (slots < 2 * (size_t)n) slots *= 2;
+    std::vector<const c10::TensorImpl*> seen(slots);       // (open addressing: at most half full)
+    tensors.reserve(n);
+    ptrs.reserve(n);
+    numels.reserve(n);
+    types.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
       const at::Tensor *p, *g;
       PyObject* const o = PyList_GET_ITEM(list, i);
       if (!plain(o, device, p)) return false;
       PyObject** const dict = _PyObject_GetDictPtr(o);
-      PyObject* const main_grad = dict && *dict ? PyDict_GetItemString(*dict, "main_grad") : nullptr;       // (borrowed; no error set where there is none)
+      PyObject* main_grad = nullptr;
+      if (dict && *dict) {
+        main_grad = PyDict_GetItemWithError(*dict, name);        // (borrowed)
+        if (!main_grad && PyErr_Occurred()) throw python_error();
+      }
       if (main_grad && main_grad != Py_None) {
         if (!plain(main_grad, device, g) || (p->grad().defined() && p->grad().unsafeGetTensorImpl() != g->unsafeGetTensorImpl())) return false;
       } else {
@@ -1448,7 +1459,11 @@ struct Gradients {
         if (!g->is_cuda() || g->get_device() != device || g->layout() != at::kStrided || at::isTensorSubclassLike(*g)) return false;
       }
       if (type_code(g->scalar_type()) < 0 || !g->is_contiguous()) return false;
-      if (!seen.insert(g->unsafeGetTensorImpl()).second) continue;
+      const c10::TensorImpl* const impl = g->unsafeGetTensorImpl();
+      size_t slot = ((uintptr_t)impl >> 6) * 0x9E3779B97F4A7C15u >> 20 & (slots - 1);
+      while (seen[slot] && seen[slot] != impl) slot = (slot + 1) & (slots - 1);
+      if (seen[slot] == impl) continue;
+      seen[slot] = impl;
       tensors.push_back(g);
       ptrs.push_back(g->data_ptr());
       numels.push_back(g->numel());
