@@ -23,7 +23,7 @@
 namespace hpfp8 {
 namespace {
 
-constexpr int kBatch = 160;               // tensors per launch: their table is a kernel argument, of which there are 4 KB
+constexpr int kBatch = 250;               // tensors per launch: their table is a kernel argument, of which there are 4 KB
 constexpr int kThreads = 256;
 constexpr int kStep = 16384;              // bytes that a workgroup takes at a time
 constexpr int64_t kNormParts = 8192;      // for all tensors together (and at most one more for each)
@@ -32,21 +32,23 @@ constexpr unsigned kClipWorkgroups = 1024;
 
 enum Power { kLargest = 0, kAbsolute = 1, kSquare = 2 };
 
+// A tensor is two words: its address with its element type above, and its first part (kPartBits) with its elements above.
+constexpr int kTypeShift = 56, kPartBits = 27;
+constexpr int64_t kMostElements = (int64_t)1 << (64 - kPartBits), kMostBytes = (int64_t)1 << 40;      // (so that all parts of 16 KB are counted in kPartBits)
 struct GradBatch {
-  void* ptr[kBatch];
-  int64_t numel[kBatch];
-  int wg_first[kBatch + 1];               // first workgroup of tensor e
-  uint8_t type[kBatch];
-  int64_t per;                            // bytes of a workgroup, a multiple of kStep
-  int count;
+  uint64_t where[kBatch], what[kBatch];
+  int64_t per;                            // bytes of a part, a multiple of kStep
+  int count, parts;
 };
 static_assert(sizeof(GradBatch) <= 4096 - 64, "kernel arguments");
+static_assert((kMostBytes / kStep + (1 << 20)) >> kPartBits == 0, "first parts");
 
-__device__ __forceinline__ int locate(const GradBatch& b, int wg) {
+__device__ __forceinline__ int locate(const GradBatch& b, int part) {
   const int lane = threadIdx.x & 63;
   int e = -1;
 #pragma unroll
-  for (int i = 0; i < kBatch; i += 64) e += __builtin_popcountll(__ballot(i + lane < b.count && b.wg_first[i + lane < kBatch ? i + lane : 0] <= wg));
+  for (int i = 0; i < kBatch; i += 64)
+    e += __builtin_popcountll(__ballot(i + lane < b.count && (int)(b.what[i + lane < kBatch ? i + lane : 0] & ((1 << kPartBits) - 1)) <= part));
   return __builtin_amdgcn_readfirstlane(e);
 }
 
@@ -57,9 +59,12 @@ struct Part {
   int type;
 };
 __device__ __forceinline__ Part part_of(const GradBatch& b, int part) {
-  const int e = locate(b, part), type = b.type[e], per_element = type == HPFP8_OUT_F32 ? 2 : 1;
-  const int64_t first = (int64_t)(part - b.wg_first[e]) * (b.per / 2), left = b.numel[e] * per_element - first;
-  return {(uint16_t*)b.ptr[e] + first, left < b.per / 2 ? left : b.per / 2, type};
+  const int e = locate(b, part);
+  const uint64_t where = b.where[e], what = b.what[e];
+  const int type = (int)(where >> kTypeShift);
+  const int64_t first = (int64_t)(part - (int)(what & ((1 << kPartBits) - 1))) * (b.per / 2);
+  const int64_t left = (int64_t)(what >> kPartBits) * (type == HPFP8_OUT_F32 ? 2 : 1) - first;
+  return {(uint16_t*)(where & (((uint64_t)1 << kTypeShift) - 1)) + first, left < b.per / 2 ? left : b.per / 2, type};
 }
 
 template <int POWER>
@@ -229,7 +234,7 @@ template <bool STREAM>
 __global__ __launch_bounds__(kThreads) void grad_clip_kernel(const GradBatch b, const float* __restrict__ norm, float max_norm) {
   const float factor = clip_factor(*norm, max_norm);
   if (factor >= 1.f) return;
-  for (int part = blockIdx.x; part < b.wg_first[b.count]; part += gridDim.x) {
+  for (int part = blockIdx.x; part < b.parts; part += gridDim.x) {
     const Part p = part_of(b, part);
     u32x4 w[U];
     load_part<STREAM>(p, w);
@@ -244,7 +249,7 @@ __global__ __launch_bounds__(1024) void grad_finish_and_clip_kernel(const GradBa
                                                                     float* __restrict__ norm, float max_norm) {
   constexpr int kQuarters = 1024 / kThreads;
   int part = blockIdx.x * kQuarters + __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
-  const int parts = b.wg_first[b.count];
+  const int parts = b.parts;
   Part p = {nullptr, 0, 0};
   u32x4 w[U];
   const bool once = parts <= (int)gridDim.x * kQuarters;       // (of more, the first parts would be a fifth of all, read for nothing where the bound holds)
@@ -280,13 +285,15 @@ int check(const char* what, const void* const* ptrs, const int64_t* numels, cons
   int64_t bytes = 0;
   for (int64_t e = 0; e < count; ++e) {
     HPFP8_REQUIRE(types[e] >= 0 && types[e] <= 2, HPFP8_ERR_ARG, "%s: unknown element type %d of tensor %lld", what, types[e], (long long)e);
-    HPFP8_REQUIRE(numels[e] >= 0 && numels[e] < ((int64_t)1 << 42) && bytes < ((int64_t)1 << 44), HPFP8_ERR_SHAPE, "%s: tensor %lld has %lld elements",
+    HPFP8_REQUIRE(numels[e] >= 0 && numels[e] < kMostElements && bytes < kMostBytes, HPFP8_ERR_SHAPE, "%s: tensor %lld has %lld elements",
                   what, (long long)e, (long long)numels[e]);
     HPFP8_REQUIRE(numels[e] == 0 || ptrs[e], HPFP8_ERR_ARG, "%s: tensor %lld is null", what, (long long)e);
+    HPFP8_REQUIRE((uint64_t)(uintptr_t)ptrs[e] >> kTypeShift == 0, HPFP8_ERR_ARG, "%s: tensor %lld has no address of this machine", what, (long long)e);
     HPFP8_REQUIRE(((uintptr_t)ptrs[e] & (element_bytes(types[e]) - 1)) == 0, HPFP8_ERR_ALIGN, "%s: tensor %lld is not aligned to its elements", what,
                   (long long)e);
     bytes += numels[e] * element_bytes(types[e]);
   }
+  HPFP8_REQUIRE(bytes < kMostBytes, HPFP8_ERR_SHAPE, "%s: %lld bytes", what, (long long)bytes);
   return HPFP8_OK;
 }
 
@@ -301,13 +308,11 @@ int for_each_batch(const void* const* ptrs, const int64_t* numels, const int* ty
     int64_t parts = 0;
     for (; e < count && b.count < kBatch; ++e) {
       if (numels[e] == 0) continue;
-      b.ptr[b.count] = const_cast<void*>(ptrs[e]);
-      b.numel[b.count] = numels[e];
-      b.type[b.count] = (uint8_t)types[e];
-      b.wg_first[b.count++] = (int)parts;
+      b.where[b.count] = (uint64_t)(uintptr_t)ptrs[e] | (uint64_t)types[e] << kTypeShift;
+      b.what[b.count++] = (uint64_t)parts | (uint64_t)numels[e] << kPartBits;
       parts += parts_of(numels[e], types[e], per);
     }
-    b.wg_first[b.count] = (int)parts;
+    b.parts = (int)parts;
     if (b.count == 0) break;
     const int rc = launch(b, (unsigned)parts, before);
     if (rc != HPFP8_OK) return rc;

@@ -1522,16 +1522,18 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// (tensors, norm, max_norm, device, stream) -> whether it was done
+// (tensors, or parameters, norm, max_norm, whether they are parameters, device, stream) -> whether it was done
 PyObject* grad_clip(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  expect(n_args, 5);
+  expect(n_args, 6);
   const Where at_ = where(args, n_args);
   const double max_norm = PyFloat_AsDouble(args[2]);
   if (PyErr_Occurred()) throw python_error();
   Gradients g;
   const at::Tensor* norm;
-  if (!no_modes() || !g.take(args[0], at_.device) || !floats(args[1], at_.device, norm) || norm->numel() != 1) Py_RETURN_FALSE;
+  const bool parameters = truth(args[3]);
+  if (!no_modes() || !floats(args[1], at_.device, norm) || norm->numel() != 1 ||
+      !(parameters ? g.of_parameters(args[0], at_.device) : g.take(args[0], at_.device))) Py_RETURN_FALSE;
   for (const at::Tensor* t : g.tensors) t->unsafeGetTensorImpl()->bump_version();
   Call call;
   HPFP8_CALL(call, hpfp8_grad_clip, g.ptrs.data(), g.numels.data(), g.types.data(), (int64_t)g.ptrs.size(), f32(*norm), (float)max_norm, at_.stream);

@@ -1,7 +1,7 @@
 """The global norm of a step's gradients, and their clipping by it: torch.nn.utils' three functions with their calling conventions.
 
 A parameter's gradient is its ``main_grad`` where `apply_grad_on_fp32_main_grad` has made one (which torch's functions know nothing of), otherwise
-its ``grad``.  The norm of all gradients is one pass over them and their clipping another, in one launch for each 160 tensors, with nothing read on
+its ``grad``.  The norm of all gradients is one pass over them and their clipping another, in one launch for each 250 tensors, with nothing read on
 the host; tensors of bfloat16, float16 and float32 go together.
 """
 from __future__ import annotations
@@ -105,7 +105,7 @@ def _clip(grads, max_norm, total_norm) -> None:
         return
     if ops._native is not None:
         device = ops._device()
-        if ops._native.grad_clip(grads, total_norm, max_norm, device, ops._raw_stream(device)):
+        if ops._native.grad_clip(grads, total_norm, max_norm, False, device, ops._raw_stream(device)):
             return
     _check(grads)
     device = torch.device("cuda", torch.cuda.current_device())
@@ -126,7 +126,12 @@ def _clip(grads, max_norm, total_norm) -> None:
 def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor) -> None:
     """torch.nn.utils.clip_grads_with_norm_: every gradient times min(1, max_norm / (total_norm + 1e-6)) in place, rounded once.  Where that is 1
     nothing is read or written.  Gradients must not share memory."""
-    _clip(_gradients(parameters), _bound(max_norm), total_norm)
+    parameters, max_norm = _list_of(parameters), _bound(max_norm)
+    if ops._native is not None and parameters and getattr(total_norm, "is_cuda", False):
+        device = ops._device()
+        if ops._native.grad_clip(parameters, total_norm, max_norm, True, device, ops._raw_stream(device)):
+            return
+    _clip(_gradients(parameters), max_norm, total_norm)
 
 
 @torch.no_grad()

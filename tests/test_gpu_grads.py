@@ -350,3 +350,22 @@ def test_half_a_parameters_gradient_in_each_place(gpu):
     before = linear.weight.main_grad.clone()
     linear(x).float().square().sum().backward()
     assert (linear.weight.main_grad - before - grads[0]).abs().max() <= 1e-5 * grads[0].abs().max()
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("count", [1, 249, 250, 251, 500, 501])
+def test_clipping_by_a_given_norm(gpu, count, native, monkeypatch):
+    """Tables of 250 tensors, tensors without elements among them; the norm in every form in which it comes; a parameter named twice is clipped once."""
+    import hpfp8
+    from hpfp8 import ops
+    if not native:
+        monkeypatch.setattr(ops, "_native", None)
+    ts = tensors([(e * 37) % 300 for e in range(1, count + 1)], 2)
+    norm = torch.tensor(7.0)
+    expected = clipped(ts, norm, 2.0)
+    for given in (norm.to(gpu), norm, norm.to(gpu, torch.bfloat16), norm.to(gpu).reshape(1), 7.0):
+        ps = params([t.to(gpu) for t in ts])
+        assert hpfp8.clip_grads_with_norm_(iter(ps + ps[:3]), 2.0, given) is None
+        for q, t in zip(ps, expected):
+            assert torch.equal((q.grad if q.grad is not None else q.main_grad).cpu(), t)
+    near(hpfp8.get_total_norm([q.grad if q.grad is not None else q.main_grad for q in ps]), norm64(expected, 2.0))
