@@ -209,6 +209,10 @@ def int8_linear(input: torch.Tensor, weight: Int8Weight, bias: Optional[torch.Te
     return gemm_int8(xq, sx, codes, scale_inv, bias, out_dtype=input.dtype)
 
 
+def _refresh(layer: "Int8Linear", _keys) -> None:           # (a function of the module's, so that a layer can be pickled)
+    layer.refresh()
+
+
 class Int8Linear(nn.Module):
     """A linear whose weight is frozen in 8-bit integers (buffers ``weight_codes``, ``weight_scale_inv`` and, with a bias, ``bias``), computed by
     `int8_linear`.  Made of a trained layer by `from_linear`.
@@ -227,7 +231,7 @@ class Int8Linear(nn.Module):
         self.register_buffer("bias", torch.zeros((out_features,), dtype=dtype, device=device) if bias else None)
         self.register_buffer("weight_codes_t", None, persistent=False)
         self.refresh()
-        self.register_load_state_dict_post_hook(lambda module, _keys: module.refresh())
+        self.register_load_state_dict_post_hook(_refresh)
 
     @classmethod
     def from_linear(cls, linear: nn.Module, *, with_transpose: bool = False) -> "Int8Linear":
@@ -249,6 +253,15 @@ class Int8Linear(nn.Module):
     def _up_to_date(self) -> bool:
         of = self._transposed_of
         return of is not None and of[0] is self.weight_codes and of[1] == of[0]._version
+
+    def __getstate__(self):             # (a copy's codes are another tensor, with a version of its own)
+        return {**self.__dict__, "_transposed_of": self._up_to_date()}
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        up_to_date, self._transposed_of = self._transposed_of, None
+        if up_to_date:
+            self._note_codes()
 
     def refresh(self) -> None:
         """Make the transposed codes, where the layer holds them, of ``weight_codes`` as it is now."""

@@ -180,3 +180,29 @@ def test_saved_tensors_that_a_hook_handed_back_as_something_else(as_if_on_the_gp
     for q, sc in ((codes[:64], scale), (codes.float(), scale), (codes, scale[:5]), (codes, scale.double())):
         with pytest.raises(ValueError, match="came back"):
             _int8_backward(torch.zeros(4, 128, dtype=BF16), q, sc, False, (4, 256))
+
+
+@pytest.mark.parametrize("way", ["deepcopy", "copy", "pickle"])
+@pytest.mark.parametrize("stale", [False, True])
+def test_a_copied_int8_layer_knows_whether_its_transposed_codes_are_its_codes(way, stale):
+    import copy
+    import pickle
+
+    import hpfp8
+    copied = {"deepcopy": copy.deepcopy, "copy": copy.copy, "pickle": lambda layer: pickle.loads(pickle.dumps(layer))}[way]
+    for writes in range(4):
+        layer = hpfp8.Int8Linear(128, 256, with_transpose=True)
+        layer.weight_codes.copy_(torch.arange(256 * 128).reshape(256, 128) % 251 - 125)
+        for _ in range(writes):
+            layer.weight_codes.add_(1)
+        layer.refresh()
+        if stale:
+            layer.weight_codes.add_(1)
+        there = copied(layer)
+        assert torch.equal(there.weight_codes, layer.weight_codes) and there._up_to_date() == (not stale)
+        there.load_state_dict(layer.state_dict())
+        assert torch.equal(there.weight_codes_t, layer.weight_codes.t()) and there._up_to_date()
+        there.weight_codes.add_(1)
+        assert not there._up_to_date()
+        if way != "copy":
+            assert layer._up_to_date() == (not stale)
