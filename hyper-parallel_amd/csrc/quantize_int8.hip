@@ -2,6 +2,9 @@
 //
 //   v = x[r, c] (times column_scale[c], rounded to fp32),   amax_r = max |v|,   code = rint(v * (127 / amax_r)),   scale_inv_r = amax_r / 127
 //
+// amax_r is at least 1e-12, as everywhere; with column scales at least 2^-118.  Those rows are a gradient's, which a loss averaged over many tokens
+// makes far smaller than 1e-12 before the scales, 1e-3 and less, are on it: all its codes would be 0.
+//
 // Bound by memory: x is read once, a row in the registers of a team of 16 to 512 threads while its largest value is found, the next row's
 // loads under way.  Rows longer than 16384 values are read twice, the second time through the L2.
 // bf16: 16384 x 7168 60 us, 5.8 TB/s; 4096 x 16384 36 us, 5.6 TB/s; 2048 x 40960 61 us, 4.1 TB/s; 8 x 7168 2.8 us.
@@ -11,6 +14,9 @@ namespace hpfp8 {
 namespace {
 
 constexpr int64_t kMaxInt8Cols = 130944;       // (the contraction that a product's 32-bit sums hold, codes of -128 among them)
+
+// the least amax whose two scales are normal numbers: 127 * 2^118 < 2^125, and 2^-118 / 127 > 2^-126
+constexpr float kLeastOfColumns = 0x1p-118f;
 
 struct Int8Params {
   const void* x;
@@ -70,7 +76,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void quantize_int8_kernel(In
     }
     if (row >= p.rows) continue;
     float scale, si;
-    int8_scales(top, scale, si);
+    int8_scales(top, scale, si, COLUMNS ? kLeastOfColumns : kAmaxEps);
     if (t == 0) p.scale_inv[row] = si;
 #pragma unroll
     for (int j = 0; j < NV; ++j) store_chunk_codes<kWhole>(p.q + row * C, at[j], C, int8_codes(v[j], scale, top < INFINITY));
@@ -109,7 +115,7 @@ __global__ __launch_bounds__(1024) void quantize_int8_long_kernel(Int8Params p) 
     const float top = __uint_as_float(m);
     __syncthreads();                                                          // (the next row writes it again)
     float scale, si;
-    int8_scales(top, scale, si);
+    int8_scales(top, scale, si, COLUMNS ? kLeastOfColumns : kAmaxEps);
     if (t == 0) p.scale_inv[row] = si;
     for (int col = t * 8; col < p.cols; col += 1024 * 8) {
       float v[8];

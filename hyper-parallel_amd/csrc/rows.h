@@ -214,8 +214,8 @@ __device__ __forceinline__ uint2 encode_group(const float v[8], float& scale_inv
 // ---- int8, one scale for a row: code = rint(v * (127 / amax)), amax the row's largest magnitude (no clamp: as above).  A row with an infinity
 // or a NaN has codes of 0 and that as its scale: what the codes stand for is NaN.
 constexpr float kInt8Max = 127.0f;
-__device__ __forceinline__ void int8_scales(float amax, float& scale, float& scale_inv) {
-  const float amc = amax < kAmaxEps ? kAmaxEps : amax;
+__device__ __forceinline__ void int8_scales(float amax, float& scale, float& scale_inv, float least = kAmaxEps) {
+  const float amc = amax < least ? least : amax;
   scale = amax < INFINITY ? kInt8Max / amc : 0.f;
   scale_inv = amc / kInt8Max;
 }

@@ -38,7 +38,9 @@ class Int8Weight(NamedTuple):
 
 def quantize_int8(x: torch.Tensor, *, column_scale: Optional[torch.Tensor] = None):
     """x[..., C] (bfloat16, float16 or float32, C a multiple of 128) -> (int8 codes, scale_inv[...]): one scale for each row.  With
-    ``column_scale`` (float32 [C]) of x * column_scale, rounded to fp32.  A row with an infinity or a NaN has codes of 0 and that for its scale."""
+    ``column_scale`` (float32 [C]) of x * column_scale, rounded to fp32.  A row with an infinity or a NaN has codes of 0 and that for its scale.
+
+    The largest magnitude that a row's scale is made from is at least 1e-12; with ``column_scale``, as a gradient's rows have, at least 2^-118."""
     if ops._gpu(x):
         device = ops._device()
         made = ops._native.quantize_int8(x, column_scale, device, ops._raw_stream(device))

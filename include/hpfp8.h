@@ -560,8 +560,9 @@ int hpfp8_rms_norm_backward(const void* dy, int64_t ld_dy, const void* s, int64_
 int64_t hpfp8_rms_norm_partials(int64_t rows, int64_t cols);
 
 /* Rows of x[rows, cols] (any of the three element types; cols a multiple of 128, at most 130944; row stride ld in elements) -> int8 codes q[rows, cols]
- * and scale_inv[rows]: v = x, or x * column_scale[c] rounded to fp32 (column_scale fp32 [cols], may be NULL); amax = max |v| of the row, at least 1e-12;
- * code = rint(v * (127 / amax)), scale_inv = amax / 127.  A row with an infinity or a NaN: codes 0 and that for its scale. */
+ * and scale_inv[rows]: v = x, or x * column_scale[c] rounded to fp32 (column_scale fp32 [cols], may be NULL); amax = max |v| of the row, at least 1e-12,
+ * with column_scale (a gradient's rows, which may be far smaller) at least 2^-118; code = rint(v * (127 / amax)), scale_inv = amax / 127.  A row with
+ * an infinity or a NaN: codes 0 and that for its scale. */
 int hpfp8_quantize_int8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, const float* column_scale, void* q, float* scale_inv,
                         hpfp8_stream_t stream);
 /* c[m, n] = (sum_k a[m, k] b[n, k]) sa[m] sb[n] + bias[n] of int8 codes, the sum exact; c and bias of element type out_type; bias may be NULL,

@@ -477,3 +477,53 @@ def test_steps_of_several_threads_at_once(gpu):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("with_transpose", [True, False])
+def test_small_gradients_scale_along(gpu, dtype, native, with_transpose, monkeypatch):
+    """Every step from dy to dx (times a scale, the row's largest, its codes, their integer sum times the row's scale) commutes with a power of two while
+    nothing is subnormal: the gradient of 2^-k dy is 2^-k times that of dy, bit for bit, each row by a k of its own."""
+    import hpfp8
+    from hpfp8 import ops
+    if not native:
+        monkeypatch.setattr(ops, "_native", None)
+    w8 = hpfp8.quantize_weight_int8((values(384, 256, torch.bfloat16, 1) * 0.02).to(gpu), with_transpose)
+    x = values(96, 256, dtype, 2).to(gpu).requires_grad_()
+    go = values(96, 384, dtype, 3).to(gpu)
+    # (2^-84 of dy, which is 1e-5 at its least, times a scale of 1e-3 is 1e-34: a normal number, and the row's largest is above 2^-118)
+    by = torch.exp2(-torch.arange(96, device=gpu).float() * 84 / 95).log2().round().exp2().unsqueeze(1)
+    want, = torch.autograd.grad(hpfp8.int8_linear(x, w8), x, go)
+    got, = torch.autograd.grad(hpfp8.int8_linear(x, w8), x, go * by.to(dtype))
+    assert by.min() == 2.0 ** -84 and (want != 0).any(1).all()
+    assert torch.equal(got, want * by.to(dtype))
+
+
+def test_gradients_of_zeros_subnormals_and_no_numbers(gpu):
+    import hpfp8
+    w8 = hpfp8.quantize_weight_int8((values(384, 256, torch.bfloat16, 1) * 0.02).to(gpu))
+    x = values(7, 256, torch.float32, 2).to(gpu).requires_grad_()
+    go = torch.zeros((7, 384), device=gpu)
+    go[1, 5], go[2], go[3, 1] = 1e-45, 2.0 ** -140, 1e-38
+    go[4, 0], go[5, 3], go[6] = math.inf, math.nan, 3e38
+    dx, = torch.autograd.grad(hpfp8.int8_linear(x, w8), x, go)
+    assert (dx[0] == 0).all() and torch.isfinite(dx[:4]).all() and dx[:4].abs().max() < 1e-35 and torch.isnan(dx[4:6]).all()
+    # the largest: 3e38 times the channels' scales, codes and one scale for the row, which an fp32 holds
+    wv = w8.dequantize(torch.float64)
+    assert torch.isfinite(dx[6][(wv.sum(0).abs() * 3e38) < 1e38]).all()
+
+
+@pytest.mark.parametrize("cols", [128, 2048, 16512])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_codes_of_small_rows_with_column_scales(gpu, cols, dtype):
+    """A row's largest value behind the columns' scales is held from below by 2^-118 alone, where 127 / amax and amax / 127 are both normal numbers."""
+    import hpfp8
+    x = values(6, cols, dtype, 1) * torch.tensor([0.0, 2.0 ** -34, 2.0 ** -60, 2.0 ** -90, 2.0 ** -110, 2.0 ** -120])[:, None].to(dtype)
+    by = torch.rand((cols,), generator=torch.Generator().manual_seed(2)) * 0.01
+    v = x.float().numpy() * by.numpy()[None, :]
+    amax = np.maximum(np.abs(v).max(1, keepdims=True), np.float32(2.0 ** -118))
+    codes = np.rint(v * (np.float32(127.0) / amax)).astype(np.int8)
+    got, scale = hpfp8.quantize_int8(x.to(gpu), column_scale=by.to(gpu))
+    assert same(got, torch.from_numpy(codes)) and same(scale, torch.from_numpy((amax / np.float32(127.0))[:, 0]))
+    assert got[1:5].abs().amax(1).eq(127).all() and not got[0].any()
