@@ -41,11 +41,18 @@ def quantize_int8(x: torch.Tensor, *, column_scale: Optional[torch.Tensor] = Non
     ``column_scale`` (float32 [C]) of x * column_scale, rounded to fp32.  A row with an infinity or a NaN has codes of 0 and that for its scale.
 
     The largest magnitude that a row's scale is made from is at least 1e-12; with ``column_scale``, as a gradient's rows have, at least 2^-118."""
+    return _quantize(x, column_scale, "quantize_int8")
+
+
+def _quantize(x, column_scale=None, name: Optional[str] = None):
+    """name: of the operator that a program calls; None inside another one, which has its place in a trace or refuses it."""
     if ops._gpu(x):
         device = ops._device()
         made = ops._native.quantize_int8(x, column_scale, device, ops._raw_stream(device))
         if made is not None:
             return made
+    if name is not None:
+        ops._refuse_trace(name, x, column_scale)
     _check_rows(x, "x")
     if x.dim() < 1:
         raise ValueError("x must have at least one dimension")
@@ -100,11 +107,18 @@ def gemm_int8(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: Optional[t
     exact; sa fp32, a scale for each row of a; sb fp32 [N], None for scales of 1; bias of ``out_dtype`` (bfloat16, float16 or float32)."""
     if out_dtype not in _TYPES:
         raise TypeError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
+    return _multiply(a, sa, b, sb, bias, out_dtype, "gemm_int8")
+
+
+def _multiply(a, sa, b, sb, bias, out_dtype, name: Optional[str] = None):
+    """name: as in `_quantize`."""
     if ops._gpu(a):
         device = ops._device()
         c = ops._native.gemm_int8(a, sa, b, sb, bias, _TYPES[out_dtype], device, ops._raw_stream(device))
         if c is not None:
             return c
+    if name is not None:
+        ops._refuse_trace(name, sa, sb, bias)
     if not isinstance(a, torch.Tensor) or a.dtype != torch.int8 or a.dim() < 1:
         raise TypeError("a must be an int8 tensor with at least one dimension")
     lead = a.shape[:-1]
@@ -144,8 +158,8 @@ def _check_bias(bias, n: int, dtype: torch.dtype) -> None:
 class _Int8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, codes, scale_inv, codes_t, bias):
-        xq, sx = quantize_int8(x)
-        y = gemm_int8(xq, sx, codes, scale_inv, bias, out_dtype=x.dtype)
+        xq, sx = _quantize(x)
+        y = _multiply(xq, sx, codes, scale_inv, bias, x.dtype)
         ctx.save_for_backward(codes if codes_t is None else codes_t, scale_inv)
         ctx.transposed, ctx.shape = codes_t is not None, x.shape
         return y
@@ -207,8 +221,8 @@ def int8_linear(input: torch.Tensor, weight: Int8Weight, bias: Optional[torch.Te
         raise ValueError("int8_linear has no gradient for a bias: detach it, or add it to the result")
     if ops._in_graph(input):
         return ops._apply(_Int8Linear, 1, input, codes, scale_inv, codes_t, bias)
-    xq, sx = quantize_int8(input)
-    return gemm_int8(xq, sx, codes, scale_inv, bias, out_dtype=input.dtype)
+    xq, sx = _quantize(input)
+    return _multiply(xq, sx, codes, scale_inv, bias, input.dtype)
 
 
 def _refresh(layer: "Int8Linear", _keys) -> None:           # (a function of the module's, so that a layer can be pickled)

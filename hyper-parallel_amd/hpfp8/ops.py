@@ -48,6 +48,17 @@ def _in_graph(*tensors) -> bool:
             or torch.jit.is_tracing())
 
 
+def _refuse_trace(name: str, *tensors) -> None:
+    """Raises for a call of an operator that has no autograd function where one would be needed: in a trace, which would keep its empty results and
+    none of its launches, and for a tangent of forward mode, which its kernels would drop."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{name} has no place in a trace: it would be replayed without its launches")
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no derivative in forward mode: call it on tensors without tangents")
+
+
 def _apply(function, level: int, *args):
     """function.apply(*args) for an autograd function whose saved tensors are left as they are by ``level``."""
     before, _saving.level = _saving.level, level

@@ -527,3 +527,25 @@ def test_codes_of_small_rows_with_column_scales(gpu, cols, dtype):
     got, scale = hpfp8.quantize_int8(x.to(gpu), column_scale=by.to(gpu))
     assert same(got, torch.from_numpy(codes)) and same(scale, torch.from_numpy((amax / np.float32(127.0))[:, 0]))
     assert got[1:5].abs().amax(1).eq(127).all() and not got[0].any()
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_traces_and_tangents_of_the_operators_by_themselves_are_refused(gpu, native, monkeypatch):
+    import hpfp8
+    import torch.autograd.forward_ad as fwAD
+    from hpfp8 import ops
+    if not native:
+        monkeypatch.setattr(ops, "_native", None)
+    x, w8 = values(48, 256, torch.bfloat16, 1).to(gpu), hpfp8.quantize_weight_int8(values(128, 256, torch.bfloat16, 2).to(gpu))
+    codes, scale = hpfp8.quantize_int8(x)
+    bias = torch.zeros((128,), dtype=torch.bfloat16, device=gpu)
+    for name, f, t in (("quantize_int8", hpfp8.quantize_int8, x), ("gemm_int8", lambda t: hpfp8.gemm_int8(codes, t, w8.codes, w8.scale_inv), scale),
+                       ("gemm_int8", lambda t: hpfp8.gemm_int8(codes, scale, w8.codes, w8.scale_inv, t), bias)):
+        with torch.no_grad(), pytest.raises(RuntimeError, match=f"{name} has no place in a trace"):
+            torch.jit.trace(f, (t,), check_trace=False)
+        with fwAD.dual_level():
+            with pytest.raises(RuntimeError, match="forward mode"):
+                f(fwAD.make_dual(t, torch.ones_like(t)))
+            inside = f(t)
+        after = f(t)
+        assert all(torch.equal(a, b) for a, b in zip(inside, after))

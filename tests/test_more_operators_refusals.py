@@ -206,3 +206,57 @@ def test_a_copied_int8_layer_knows_whether_its_transposed_codes_are_its_codes(wa
         assert not there._up_to_date()
         if way != "copy":
             assert layer._up_to_date() == (not stale)
+
+
+@pytest.fixture()
+def launched(as_if_on_the_gpu, monkeypatch):
+    """Launches written down instead of made."""
+    from hpfp8 import _lib, ops
+    seen = []
+    monkeypatch.setattr(ops, "_native", None)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_check_f32", lambda t, name: t)
+    monkeypatch.setattr(_lib, "call", lambda name, *a: seen.append(name))
+    return seen
+
+
+def int8_calls():
+    """(name, function of a tensor in 16 or 32 bits, that tensor)"""
+    import hpfp8
+    codes, scale = torch.zeros(128, 256, dtype=torch.int8), torch.ones(128)
+    return [("quantize_int8", hpfp8.quantize_int8, torch.zeros(128, 256, dtype=BF16)),
+            ("quantize_int8", lambda t: hpfp8.quantize_int8(torch.zeros(4, 256, dtype=BF16), column_scale=t), torch.ones(256)),
+            ("gemm_int8", lambda t: hpfp8.gemm_int8(codes, t, codes, scale), scale), ("gemm_int8", lambda t: hpfp8.gemm_int8(codes, scale, codes, t), scale),
+            ("gemm_int8", lambda t: hpfp8.gemm_int8(codes, scale, codes, None, t), torch.zeros(128, dtype=BF16))]
+
+
+@pytest.mark.parametrize("case", range(5))
+def test_int8_operators_have_no_place_in_a_trace_and_no_tangents(launched, case):
+    """A trace would keep their empty results and none of their launches."""
+    import torch.autograd.forward_ad as fwAD
+    name, f, t = int8_calls()[case]
+    with pytest.raises(RuntimeError, match=f"{name} has no place in a trace"):
+        torch.jit.trace(f, (t,), check_trace=False)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no place in a trace"):
+        torch.jit.trace(f, (t,), check_trace=False)
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), fwAD.dual_level():
+            with pytest.raises(RuntimeError, match=f"{name} .*forward mode"):
+                f(fwAD.make_dual(t, torch.ones_like(t)))
+            assert not launched
+            f(t)                                             # (a level without a tangent changes nothing)
+            assert launched.pop()
+    f(t)
+    assert launched
+
+
+def test_int8_linear_in_a_trace_launches_inside_its_function(launched):
+    import hpfp8
+    w8 = hpfp8.Int8Weight(torch.zeros(128, 256, dtype=torch.int8), torch.ones(128))
+    x = torch.zeros(4, 256, dtype=BF16)
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad):
+            traced = torch.jit.trace(lambda t: hpfp8.int8_linear(t, w8), (x,), check_trace=False)
+            launched.clear()
+            traced(x)
+        assert launched == ["hpfp8_quantize_int8", "hpfp8_gemm_int8"]
