@@ -1302,7 +1302,7 @@ PyObject* gemm_int8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (!int8_codes(args[0], at_.device, a) || a->dim() < 1 || !a->is_contiguous() || !int8_weight(args[2], at_.device, a->size(-1), b)) Py_RETURN_NONE;
   const int64_t k = a->size(-1), m = a->numel() / k, n = b->size(0);
   if (!floats(args[1], at_.device, sa) || sa->numel() != m || !sa->is_contiguous() || (args[3] != Py_None && !int8_vector(args[3], at_.device, n, at::kFloat, sb)) ||
-      (args[4] != Py_None && !int8_vector(args[4], at_.device, n, type_of((int)type), bias)) || !ordinary({a, sa, b, sb, bias}))
+      (args[4] != Py_None && !int8_vector(args[4], at_.device, n, type_of((int)type), bias)) || to_train({sa, sb, bias}) || !ordinary({a, sa, b, sb, bias}))
     Py_RETURN_NONE;
   at::Tensor c;
   Call call;
@@ -1377,7 +1377,7 @@ PyObject* int8_linear(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   const int64_t k = x->size(-1), m = x->numel() / k, n = w->size(0);
   if (n > kInt8MostFeatures || !int8_vector(args[2], at_.device, n, at::kFloat, sw) ||
       (args[3] != Py_None && (!int8_weight(args[3], at_.device, n, wt) || wt->size(0) != k)) ||
-      (args[4] != Py_None && !int8_vector(args[4], at_.device, n, x->scalar_type(), bias)) || to_train({bias}) || !ordinary({x, w, sw, bias}))
+      (args[4] != Py_None && !int8_vector(args[4], at_.device, n, x->scalar_type(), bias)) || to_train({sw, bias}) || !ordinary({x, w, sw, bias}))
     Py_RETURN_NONE;
   const bool train = to_train({x});
   Int8Made made;

@@ -104,7 +104,8 @@ def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 def gemm_int8(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: Optional[torch.Tensor], bias: Optional[torch.Tensor] = None, *,
               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """c[..., n] = (a[..., :] . b[n, :]) * sa[...] * sb[n] + bias[n] for int8 codes a[..., K] and b[N, K], both multiples of 128, the sum of products
-    exact; sa fp32, a scale for each row of a; sb fp32 [N], None for scales of 1; bias of ``out_dtype`` (bfloat16, float16 or float32)."""
+    exact; sa fp32, a scale for each row of a; sb fp32 [N], None for scales of 1; bias of ``out_dtype`` (bfloat16, float16 or float32).  It has no
+    gradients: scales or a bias that require one are refused."""
     if out_dtype not in _TYPES:
         raise TypeError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
     return _multiply(a, sa, b, sb, bias, out_dtype, "gemm_int8")
@@ -119,6 +120,9 @@ def _multiply(a, sa, b, sb, bias, out_dtype, name: Optional[str] = None):
             return c
     if name is not None:
         ops._refuse_trace(name, sa, sb, bias)
+        for what, t in (("sa", sa), ("sb", sb), ("bias", bias)):
+            if torch.is_grad_enabled() and isinstance(t, torch.Tensor) and t.requires_grad:
+                raise ValueError(f"gemm_int8 has no gradient for {what}: detach it")
     if not isinstance(a, torch.Tensor) or a.dtype != torch.int8 or a.dim() < 1:
         raise TypeError("a must be an int8 tensor with at least one dimension")
     lead = a.shape[:-1]
@@ -190,7 +194,7 @@ def int8_linear(input: torch.Tensor, weight: Int8Weight, bias: Optional[torch.Te
     """torch.nn.functional.linear with a weight in 8-bit integers: input [..., in_features] (bfloat16, float16 or float32), bias [out_features] of
     input's type; the result has that type too.  in_features and out_features are multiples of 128, the number of tokens is any.
 
-    Differentiable in input; the weight is frozen, and so is the bias."""
+    Differentiable in input; the weight is frozen, its codes and its scales, and so is the bias."""
     tensors = (input,) if bias is None else (input, bias)
     if torch.overrides.has_torch_function(tensors):
         return _hand_off(int8_linear, tensors, (input, weight, bias), {}, {})
@@ -217,6 +221,8 @@ def int8_linear(input: torch.Tensor, weight: Int8Weight, bias: Optional[torch.Te
         if codes_t.shape != codes.shape[::-1]:
             raise ValueError(f"weight.codes_t must be the transpose of weight.codes {tuple(codes.shape)}, got {tuple(codes_t.shape)}")
     _check_bias(bias, n, input.dtype)
+    if scale_inv.requires_grad and torch.is_grad_enabled():
+        raise ValueError("int8_linear has no gradient for the weight's scales: detach them")
     if bias is not None and bias.requires_grad and torch.is_grad_enabled():
         raise ValueError("int8_linear has no gradient for a bias: detach it, or add it to the result")
     if ops._in_graph(input):

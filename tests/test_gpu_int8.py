@@ -549,3 +549,25 @@ def test_traces_and_tangents_of_the_operators_by_themselves_are_refused(gpu, nat
             inside = f(t)
         after = f(t)
         assert all(torch.equal(a, b) for a, b in zip(inside, after))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_gradients_that_a_product_does_not_have_are_refused_and_not_lost(gpu, native, monkeypatch):
+    import hpfp8
+    from hpfp8 import ops
+    if not native:
+        monkeypatch.setattr(ops, "_native", None)
+    w8 = hpfp8.quantize_weight_int8(values(128, 256, torch.bfloat16, 1).to(gpu))
+    codes, scale = hpfp8.quantize_int8(values(8, 256, torch.bfloat16, 2).to(gpu))
+    bias = torch.ones((128,), dtype=torch.bfloat16, device=gpu)
+    want = hpfp8.gemm_int8(codes, scale, w8.codes, w8.scale_inv, bias)
+    learned = lambda t: t.clone().requires_grad_()           # noqa: E731
+    for sa, sb, b in ((learned(scale), w8.scale_inv, bias), (scale, learned(w8.scale_inv), bias), (scale, w8.scale_inv, learned(bias))):
+        with pytest.raises(ValueError, match="no gradient"):
+            hpfp8.gemm_int8(codes, sa, w8.codes, sb, b)
+        with torch.no_grad():
+            assert torch.equal(hpfp8.gemm_int8(codes, sa, w8.codes, sb, b), want)
+    x = values(8, 256, torch.bfloat16, 2).to(gpu)
+    for t in (x, learned(x)):
+        with pytest.raises(ValueError, match="no gradient"):
+            hpfp8.int8_linear(t, w8._replace(scale_inv=learned(w8.scale_inv)), bias)

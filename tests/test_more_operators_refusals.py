@@ -260,3 +260,22 @@ def test_int8_linear_in_a_trace_launches_inside_its_function(launched):
             launched.clear()
             traced(x)
         assert launched == ["hpfp8_quantize_int8", "hpfp8_gemm_int8"]
+
+
+@pytest.mark.parametrize("which", ["sa", "sb", "bias"])
+def test_int8_products_have_no_gradient_for_scales_and_bias(launched, which):
+    import hpfp8
+    codes = torch.zeros(128, 256, dtype=torch.int8)
+    given = dict(sa=torch.ones(128), sb=torch.ones(128), bias=torch.zeros(128, dtype=BF16))
+    given[which].requires_grad_()
+    with pytest.raises(ValueError, match=f"no gradient for {which}"):
+        hpfp8.gemm_int8(codes, given["sa"], codes, given["sb"], given["bias"])
+    assert not launched
+    with torch.no_grad():
+        assert not hpfp8.gemm_int8(codes, given["sa"], codes, given["sb"], given["bias"]).requires_grad
+    if which == "sb":
+        for x in (torch.zeros(4, 256, dtype=BF16), torch.zeros(4, 256, dtype=BF16).requires_grad_()):
+            with pytest.raises(ValueError, match="no gradient for the weight's scales"):
+                hpfp8.int8_linear(x, hpfp8.Int8Weight(codes, given["sb"]))
+            with torch.no_grad():
+                hpfp8.int8_linear(x, hpfp8.Int8Weight(codes, given["sb"]))
