@@ -1411,7 +1411,7 @@ struct Gradients {
   std::vector<void*> ptrs;
   std::vector<int64_t> numels;
   std::vector<int> types;
-  // of a list of dense, contiguous tensors of the three types; false where one is anything else
+  // of a list of dense, contiguous tensors of the three types without tangents; false where one is anything else
   bool take(PyObject* list, int64_t device) {
     if (!PyList_CheckExact(list)) return false;
     const Py_ssize_t n = PyList_GET_SIZE(list);
@@ -1421,7 +1421,7 @@ struct Gradients {
     types.resize(n);
     for (Py_ssize_t i = 0; i < n; ++i) {
       const at::Tensor* t;
-      if (!plain(PyList_GET_ITEM(list, i), device, t) || type_code(t->scalar_type()) < 0 || !t->is_contiguous()) return false;
+      if (!plain(PyList_GET_ITEM(list, i), device, t) || type_code(t->scalar_type()) < 0 || !t->is_contiguous() || t->_fw_grad(0).defined()) return false;
       tensors[i] = t;
       ptrs[i] = t->data_ptr();
       numels[i] = t->numel();
@@ -1458,7 +1458,7 @@ struct Gradients {
         if (!g->defined()) continue;
         if (!g->is_cuda() || g->get_device() != device || g->layout() != at::kStrided || at::isTensorSubclassLike(*g)) return false;
       }
-      if (type_code(g->scalar_type()) < 0 || !g->is_contiguous()) return false;
+      if (type_code(g->scalar_type()) < 0 || !g->is_contiguous() || g->_fw_grad(0).defined()) return false;
       const c10::TensorImpl* const impl = g->unsafeGetTensorImpl();
       size_t slot = ((uintptr_t)impl >> 6) * 0x9E3779B97F4A7C15u >> 20 & (slots - 1);
       while (seen[slot] && seen[slot] != impl) slot = (slot + 1) & (slots - 1);
@@ -1481,7 +1481,7 @@ PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   const int64_t power = PyLong_AsLongLong(args[1]);
   if (PyErr_Occurred()) throw python_error();
   Gradients g;
-  if (!no_modes() || !g.take(args[0], at_.device)) Py_RETURN_NONE;
+  if (!ordinary({}) || !g.take(args[0], at_.device)) Py_RETURN_NONE;
   at::Tensor norm;
   Call call;
   {
@@ -1505,7 +1505,7 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   const int64_t power = PyLong_AsLongLong(args[2]);
   if (PyErr_Occurred()) throw python_error();
   Gradients g;
-  if (!no_modes() || !g.of_parameters(args[0], at_.device)) Py_RETURN_NONE;
+  if (!ordinary({}) || !g.of_parameters(args[0], at_.device)) Py_RETURN_NONE;
   at::Tensor norm;
   Call call;
   {
@@ -1532,7 +1532,7 @@ PyObject* grad_clip(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   Gradients g;
   const at::Tensor* norm;
   const bool parameters = truth(args[3]);
-  if (!no_modes() || !floats(args[1], at_.device, norm) || norm->numel() != 1 ||
+  if (!floats(args[1], at_.device, norm) || norm->numel() != 1 || !ordinary({norm}) ||
       !(parameters ? g.of_parameters(args[0], at_.device) : g.take(args[0], at_.device))) Py_RETURN_FALSE;
   for (const at::Tensor* t : g.tensors) t->unsafeGetTensorImpl()->bump_version();
   Call call;

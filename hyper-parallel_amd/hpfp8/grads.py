@@ -79,6 +79,7 @@ def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_ty
         device = ops._device()
         norm = ops._native.grad_norm(tensors, power, device, ops._raw_stream(device))
     if norm is None:
+        ops._refuse_trace("get_total_norm", *tensors)
         _check(tensors)
         device = torch.device("cuda", torch.cuda.current_device())
         norm = torch.empty((), dtype=torch.float32, device=device)
@@ -131,7 +132,9 @@ def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]
         device = ops._device()
         if ops._native.grad_clip(parameters, total_norm, max_norm, True, device, ops._raw_stream(device)):
             return
-    _clip(_gradients(parameters), max_norm, total_norm)
+    grads = _gradients(parameters)
+    ops._refuse_trace("clip_grads_with_norm_", total_norm, *grads)
+    _clip(grads, max_norm, total_norm)
 
 
 @torch.no_grad()
@@ -146,6 +149,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
         if norm is not None:
             return norm
     grads = _gradients(parameters)
+    ops._refuse_trace("clip_grad_norm_", *grads)
     norm = get_total_norm(grads, norm_type, error_if_nonfinite)
     _clip(grads, max_norm, norm)
     return norm

@@ -369,3 +369,33 @@ def test_clipping_by_a_given_norm(gpu, count, native, monkeypatch):
         for q, t in zip(ps, expected):
             assert torch.equal((q.grad if q.grad is not None else q.main_grad).cpu(), t)
     near(hpfp8.get_total_norm([q.grad if q.grad is not None else q.main_grad for q in ps]), norm64(expected, 2.0))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_traces_and_tangents_are_refused(gpu, native, monkeypatch):
+    """A trace would keep an empty norm and no launch; a tangent would be dropped."""
+    import hpfp8
+    import torch.autograd.forward_ad as fwAD
+    from hpfp8 import ops
+    if not native:
+        monkeypatch.setattr(ops, "_native", None)
+
+    def clip(f):
+        def call(t):
+            p = torch.nn.Parameter(torch.zeros(8, device=gpu))
+            p.main_grad = t
+            f(p)
+            return t + 1
+        return call
+    two = torch.full((), 2.0, device=gpu)
+    for name, f in (("get_total_norm", lambda t: hpfp8.get_total_norm([t])), ("clip_grads_with_norm_", clip(lambda p: hpfp8.clip_grads_with_norm_(p, 1.0, two))),
+                    ("clip_grad_norm_", clip(lambda p: hpfp8.clip_grad_norm_(p, 1.0)))):
+        g = torch.ones(8, device=gpu)
+        with pytest.raises(RuntimeError, match=f"{name} has no place in a trace"):
+            torch.jit.trace(f, (g,), check_trace=False)
+        with fwAD.dual_level():
+            with pytest.raises(RuntimeError, match=f"{name} .*forward mode"):
+                f(fwAD.make_dual(g, torch.ones_like(g)))
+            assert (g == 1).all()
+            inside = f(g.clone())
+        assert torch.equal(inside, f(g.clone()))

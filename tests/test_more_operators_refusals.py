@@ -279,3 +279,23 @@ def test_int8_products_have_no_gradient_for_scales_and_bias(launched, which):
                 hpfp8.int8_linear(x, hpfp8.Int8Weight(codes, given["sb"]))
             with torch.no_grad():
                 hpfp8.int8_linear(x, hpfp8.Int8Weight(codes, given["sb"]))
+
+
+def test_gradients_norms_have_no_place_in_a_trace_and_no_tangents(launched):
+    import hpfp8
+    import torch.autograd.forward_ad as fwAD
+
+    def clip(f):
+        def call(t):
+            p = torch.nn.Parameter(torch.zeros(8))
+            p.main_grad = t
+            f(p)
+            return t + 1
+        return call
+    for name, f in (("get_total_norm", lambda t: hpfp8.get_total_norm([t])), ("clip_grads_with_norm_", clip(lambda p: hpfp8.clip_grads_with_norm_(p, 1.0, torch.ones(())))),
+                    ("clip_grad_norm_", clip(lambda p: hpfp8.clip_grad_norm_(p, 1.0)))):
+        with pytest.raises(RuntimeError, match=f"{name} has no place in a trace"):
+            torch.jit.trace(f, (torch.ones(8),), check_trace=False)
+        with fwAD.dual_level(), pytest.raises(RuntimeError, match=f"{name} .*forward mode"):
+            f(fwAD.make_dual(torch.ones(8), torch.ones(8)))
+    assert not launched
