@@ -43,10 +43,17 @@ def _gradients(parameters) -> List[torch.Tensor]:
     return list(found.values())
 
 
+def _local(t: torch.Tensor) -> torch.Tensor:
+    """This rank's part of a sharded tensor; any other as it is."""
+    return t.to_local() if hasattr(t, "to_local") else t
+
+
 def _check(tensors) -> None:
     for i, t in enumerate(tensors):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"tensor {i} must be a torch.Tensor")
+        if hasattr(t, "to_local"):
+            raise TypeError(f"tensor {i} is sharded: take the norm of this rank's shards (to_local()), then that over the ranks, then clip_grads_with_norm_")
         if t.layout != torch.strided or t.dtype not in _TYPES:
             raise TypeError(f"tensor {i} must be a dense tensor of bfloat16, float16 or float32, got {t.dtype}, {t.layout}")
         ops._check_device(t, f"tensor {i}")
@@ -109,6 +116,8 @@ def _clip(grads, max_norm, total_norm) -> None:
         if ops._native.grad_clip(grads, total_norm, max_norm, False, device, ops._raw_stream(device)):
             return
     _check(grads)
+    if hasattr(total_norm, "to_local"):
+        raise TypeError("total_norm must be a number or a local tensor (full_tensor())")
     device = torch.device("cuda", torch.cuda.current_device())
     if not isinstance(total_norm, torch.Tensor):
         total_norm = torch.full((), float(total_norm), dtype=torch.float32, device=device)
@@ -126,13 +135,13 @@ def _clip(grads, max_norm, total_norm) -> None:
 @torch.no_grad()
 def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor) -> None:
     """torch.nn.utils.clip_grads_with_norm_: every gradient times min(1, max_norm / (total_norm + 1e-6)) in place, rounded once.  Where that is 1
-    nothing is read or written.  Gradients must not share memory."""
+    nothing is read or written.  Gradients must not share memory.  Of a sharded gradient (one with ``to_local()``) this rank's shard is scaled."""
     parameters, max_norm = _list_of(parameters), _bound(max_norm)
     if ops._native is not None and parameters and getattr(total_norm, "is_cuda", False):
         device = ops._device()
         if ops._native.grad_clip(parameters, total_norm, max_norm, True, device, ops._raw_stream(device)):
             return
-    grads = _gradients(parameters)
+    grads = [_local(g) for g in _gradients(parameters)]
     ops._refuse_trace("clip_grads_with_norm_", total_norm, *grads)
     _clip(grads, max_norm, total_norm)
 
@@ -141,7 +150,8 @@ def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_ for gradients in ``grad`` and in ``main_grad``: their total norm (a 0-dim float32 tensor), and the gradients
-    scaled in place so that it is at most ``max_norm``."""
+    scaled in place so that it is at most ``max_norm``.  Sharded gradients have no norm on one rank: `get_total_norm` of the shards, a reduction over
+    the ranks and `clip_grads_with_norm_` take its place."""
     parameters, power, max_norm = _list_of(parameters), _power(norm_type), _bound(max_norm)
     if ops._native is not None and parameters and not error_if_nonfinite:
         device = ops._device()

@@ -399,3 +399,58 @@ def test_traces_and_tangents_are_refused(gpu, native, monkeypatch):
             assert (g == 1).all()
             inside = f(g.clone())
         assert torch.equal(inside, f(g.clone()))
+
+
+@pytest.fixture()
+def mesh(gpu):
+    """Two ranks of which this process is the first; nothing is ever sent."""
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.testing._internal.distributed.fake_pg import FakeStore
+    dist.init_process_group("fake", store=FakeStore(), rank=0, world_size=2)
+    try:
+        yield init_device_mesh("cuda", (2,))
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("kind", ["torch", "reference"])
+def test_shards(gpu, mesh, kind):
+    """The recipe for sharded gradients: the norm of the shards, that of the ranks' norms, and the parameters clipped by it, each gradient's own shard in
+    place.  torch's tensors over a mesh, and those that hand every call to a dispatcher; main gradients that are shards too; local gradients among them."""
+    import hpfp8
+    from torch.distributed.tensor import DTensor, Shard
+    import _hp_standin as S
+
+    def sharded(local):
+        if kind == "torch":
+            return DTensor.from_local(local, mesh, [Shard(0)], run_check=False)
+        return S.DTensor(local, S.Layout((2,), ("dp",))("dp", "None"))
+    S.DTensor.DISPATCHER = S.Dispatcher()
+    g = torch.Generator().manual_seed(3)
+    locals_ = [torch.randn(n, 6, generator=g).to(d).to(gpu) for n, d in ((40, torch.float32), (7, torch.bfloat16), (1, torch.float32))]
+    before = [t.cpu() for t in locals_]
+    with torch._C.DisableTorchFunctionSubclass():
+        grads = [sharded(t) for t in locals_[:2]] + [locals_[2]]
+        if kind == "torch":
+            a = torch.nn.Parameter(sharded(torch.zeros_like(locals_[0])))
+        else:
+            a = torch.nn.Parameter(torch.zeros_like(locals_[0]))
+        a.grad = grads[0]
+        b = torch.nn.Parameter(torch.zeros(3, device=gpu))
+        b.main_grad = grads[1]
+        c = torch.nn.Parameter(torch.zeros_like(locals_[2]))
+        c.grad = grads[2]
+    shards = [t.to_local() if hasattr(t, "to_local") else t for t in grads]
+    n = hpfp8.get_total_norm(shards)
+    near(n, norm64(before, 2.0))
+    n = (2 * n.square()).sqrt()                              # (the other rank's shards have the same norm)
+    for share in (2.0, 0.5):
+        assert hpfp8.clip_grads_with_norm_([a, b, c], share * float(n), n) is None
+        for t, w in zip(locals_, clipped(before, n, share * float(n))):
+            assert torch.equal(t.cpu(), w)
+    with pytest.raises((TypeError, RuntimeError), match="shard|parallel layout"):
+        hpfp8.clip_grad_norm_([a, b, c], 1.0)
+    with pytest.raises((TypeError, RuntimeError), match="shard|parallel layout"):
+        hpfp8.get_total_norm(grads)
+    assert all(torch.equal(t.cpu(), w) for t, w in zip(locals_, clipped(before, n, 0.5 * float(n))))

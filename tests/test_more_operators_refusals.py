@@ -299,3 +299,21 @@ def test_gradients_norms_have_no_place_in_a_trace_and_no_tangents(launched):
         with fwAD.dual_level(), pytest.raises(RuntimeError, match=f"{name} .*forward mode"):
             f(fwAD.make_dual(torch.ones(8), torch.ones(8)))
     assert not launched
+
+
+def test_sharded_gradients_without_a_norm_over_the_ranks_are_refused(launched):
+    import hpfp8
+
+    class Sharded(torch.Tensor):
+        def to_local(self):
+            return self.as_subclass(torch.Tensor)
+        __torch_function__ = torch._C._disabled_torch_function_impl
+    g = torch.zeros(8).as_subclass(Sharded)
+    p = torch.nn.Parameter(torch.zeros(8))
+    p.main_grad = g
+    for f in (lambda: hpfp8.get_total_norm([torch.zeros(8), g]), lambda: hpfp8.clip_grad_norm_(p, 1.0)):
+        with pytest.raises(TypeError, match="sharded"):
+            f()
+    with pytest.raises(TypeError, match="total_norm must be"):
+        hpfp8.clip_grads_with_norm_(p, 1.0, g)
+    assert not launched
