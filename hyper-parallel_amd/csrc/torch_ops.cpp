@@ -1324,6 +1324,13 @@ struct Int8Made {
   bool transposed;
 };
 
+// saved codes [rows, cols] as the forward takes them: rows may have a gap behind them, as the package's own transposed codes do
+bool int8_again(const at::Tensor& t, const at::Tensor& go, int64_t rows, int64_t cols) {
+  return t.defined() && t.is_cuda() && t.get_device() == go.get_device() && t.layout() == at::kStrided && !at::isTensorSubclassLike(t) &&
+         t.scalar_type() == at::kChar && t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.stride(1) == 1 && t.stride(0) >= cols &&
+         t.stride(0) % 16 == 0 && ((uintptr_t)t.data_ptr() & 15) == 0;
+}
+
 struct Int8Node : torch::autograd::Function<Int8Node> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const Int8Made& made) {
     ctx->save_for_backward({made.codes, made.scale_inv});
@@ -1338,8 +1345,8 @@ struct Int8Node : torch::autograd::Function<Int8Node> {
     const bool transposed = ctx->saved_data["transposed"].toBool();
     const int64_t k = shape.back(), n = grad.size(-1), m = grad.numel() / n;
     const bool as_made = no_modes() && grad.is_cuda() && grad.layout() == at::kStrided && !at::isTensorSubclassLike(grad) &&
-                         type_code(grad.scalar_type()) >= 0 && again(codes, grad, at::kChar, n * k) && codes.dim() == 2 && codes.size(0) == (transposed ? k : n) &&
-                         again(scale_inv, grad, at::kFloat, n) && scale_inv.dim() == 1 && ((uintptr_t)codes.data_ptr() & 15) == 0;
+                         type_code(grad.scalar_type()) >= 0 && int8_again(codes, grad, transposed ? k : n, transposed ? n : k) &&
+                         again(scale_inv, grad, at::kFloat, n) && scale_inv.dim() == 1;
     if (!as_made) {
       pybind11::gil_scoped_acquire held;
       return from_python(int8_backward_function, pybind11::make_tuple(grad, codes, scale_inv, transposed, as_tuple(shape)), 2);
@@ -1350,11 +1357,11 @@ struct Int8Node : torch::autograd::Function<Int8Node> {
     Int8Rows rows;
     quantize_rows_int8(go, &scale_inv, stream, rows, call);
     at::Tensor wt = codes;
-    int64_t ld = n;
+    int64_t ld = codes.stride(0);
     if (call.ok() && !transposed) {
       ld = padded_ld(n);
       wt = at::empty({k, ld}, codes.options());
-      HPFP8_CALL(call, hpfp8_transpose_codes, codes.data_ptr(), n, k, k, wt.data_ptr(), ld, stream);
+      HPFP8_CALL(call, hpfp8_transpose_codes, codes.data_ptr(), n, k, codes.stride(0), wt.data_ptr(), ld, stream);
     }
     at::Tensor dx;
     if (call.ok()) {

@@ -571,3 +571,38 @@ def test_gradients_that_a_product_does_not_have_are_refused_and_not_lost(gpu, na
     for t in (x, learned(x)):
         with pytest.raises(ValueError, match="no gradient"):
             hpfp8.int8_linear(t, w8._replace(scale_inv=learned(w8.scale_inv)), bias)
+
+
+@pytest.mark.parametrize("out", [256, 384])
+@pytest.mark.parametrize("form", ["transposed", "module", "plain", "strided"])
+def test_the_native_backward_takes_the_codes_that_the_package_makes(gpu, out, form):
+    """Transposed codes of an even multiple of 128 outputs have rows with a gap behind them; codes that are a slice have one too."""
+    import hpfp8
+    from hpfp8 import int8, ops
+    k = 512
+    w = (values(out, k, torch.bfloat16, 1) * 0.02).to(gpu)
+    w8 = hpfp8.quantize_weight_int8(w, with_transpose=form == "transposed")
+    assert form != "transposed" or w8.codes_t.is_contiguous() == (out == 384)
+    f = lambda t: hpfp8.int8_linear(t, w8)                   # noqa: E731
+    if form == "strided":
+        wide = torch.zeros((out, k + 256), dtype=torch.int8, device=gpu)
+        wide[:, 128:128 + k] = w8.codes
+        w8 = w8._replace(codes=wide[:, 128:128 + k])
+    elif form == "module":
+        linear = torch.nn.Linear(k, out, bias=False, device=gpu, dtype=torch.bfloat16)
+        linear.weight.data.copy_(w)
+        f = hpfp8.Int8Linear.from_linear(linear, with_transpose=True)
+        assert not f.weight_codes_t.is_contiguous() or out == 384
+    x, go = values(70, k, torch.bfloat16, 2).to(gpu).requires_grad_(), values(70, out, torch.bfloat16, 3).to(gpu)
+    codes, sw = quantized(w.float().cpu().numpy())
+    gq, sg = quantized(go.float().cpu().numpy() * sw[None, :])
+    want = product(gq, sg, np.ascontiguousarray(codes.T), None, None, torch.bfloat16)
+
+    def python(*a):
+        raise AssertionError("the native backward left this to Python")
+    ops._native.bind_int8_backward(python)
+    try:
+        dx, = torch.autograd.grad(f(x), x, go)
+    finally:
+        ops._native.bind_int8_backward(int8._int8_backward)
+    assert same(dx, want)
