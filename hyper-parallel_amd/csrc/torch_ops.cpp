@@ -1413,12 +1413,13 @@ PyObject* int8_linear(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
 }
 
 // ---- the norm of many gradients, and their clipping
+bool gapless(const at::Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }      // (grads._gapless)
 struct Gradients {
   std::vector<const at::Tensor*> tensors;
   std::vector<void*> ptrs;
   std::vector<int64_t> numels;
   std::vector<int> types;
-  // of a list of dense, contiguous tensors of the three types without tangents; false where one is anything else
+  // of a list of dense tensors of the three types, without gaps and without tangents; false where one is anything else
   bool take(PyObject* list, int64_t device) {
     if (!PyList_CheckExact(list)) return false;
     const Py_ssize_t n = PyList_GET_SIZE(list);
@@ -1428,7 +1429,7 @@ struct Gradients {
     types.resize(n);
     for (Py_ssize_t i = 0; i < n; ++i) {
       const at::Tensor* t;
-      if (!plain(PyList_GET_ITEM(list, i), device, t) || type_code(t->scalar_type()) < 0 || !t->is_contiguous() || t->_fw_grad(0).defined()) return false;
+      if (!plain(PyList_GET_ITEM(list, i), device, t) || type_code(t->scalar_type()) < 0 || !gapless(*t) || t->_fw_grad(0).defined()) return false;
       tensors[i] = t;
       ptrs[i] = t->data_ptr();
       numels[i] = t->numel();
@@ -1465,7 +1466,7 @@ struct Gradients {
         if (!g->defined()) continue;
         if (!g->is_cuda() || g->get_device() != device || g->layout() != at::kStrided || at::isTensorSubclassLike(*g)) return false;
       }
-      if (type_code(g->scalar_type()) < 0 || !g->is_contiguous() || g->_fw_grad(0).defined()) return false;
+      if (type_code(g->scalar_type()) < 0 || !gapless(*g) || g->_fw_grad(0).defined()) return false;
       const c10::TensorImpl* const impl = g->unsafeGetTensorImpl();
       size_t slot = ((uintptr_t)impl >> 6) * 0x9E3779B97F4A7C15u >> 20 & (slots - 1);
       while (seen[slot] && seen[slot] != impl) slot = (slot + 1) & (slots - 1);

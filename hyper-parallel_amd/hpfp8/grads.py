@@ -59,6 +59,18 @@ def _check(tensors) -> None:
         ops._check_device(t, f"tensor {i}")
 
 
+def _gapless(t: torch.Tensor) -> bool:
+    """Whether t's elements are the memory from its start on, each once, in whatever order: what a norm and a factor need to know."""
+    if t.is_contiguous():
+        return True
+    step = 1
+    for stride, size in sorted((stride, size) for size, stride in zip(t.shape, t.stride()) if size > 1):
+        if stride != step:
+            return False
+        step *= size
+    return True
+
+
 def _table(tensors):
     import ctypes
     n = max(len(tensors), 1)
@@ -90,7 +102,7 @@ def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_ty
         _check(tensors)
         device = torch.device("cuda", torch.cuda.current_device())
         norm = torch.empty((), dtype=torch.float32, device=device)
-        dense = [t.contiguous() for t in tensors]
+        dense = [t if _gapless(t) else t.contiguous() for t in tensors]
         table = _table(dense)
         partial = torch.empty((_lib.load().hpfp8_grad_norm_partials(*table[1:]),), dtype=torch.float64, device=device)
         _lib.call("hpfp8_grad_norm", *table, power, ops._ptr(partial), ops._ptr(norm), ops._stream())
@@ -124,7 +136,7 @@ def _clip(grads, max_norm, total_norm) -> None:
     if total_norm.numel() != 1:
         raise ValueError(f"total_norm must be one number, got {tuple(total_norm.shape)}")
     norm = total_norm.detach().to(device, torch.float32)
-    dense = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    dense = [g if _gapless(g) else g.contiguous() for g in grads]
     torch.autograd.graph.increment_version([g for g, d in zip(grads, dense) if d is g])
     _lib.call("hpfp8_grad_clip", *_table(dense), ops._ptr(norm), max_norm, ops._stream())
     for g, d in zip(grads, dense):
@@ -135,7 +147,8 @@ def _clip(grads, max_norm, total_norm) -> None:
 @torch.no_grad()
 def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor) -> None:
     """torch.nn.utils.clip_grads_with_norm_: every gradient times min(1, max_norm / (total_norm + 1e-6)) in place, rounded once.  Where that is 1
-    nothing is read or written.  Gradients must not share memory.  Of a sharded gradient (one with ``to_local()``) this rank's shard is scaled."""
+    nothing is read or written (but of gradients with gaps between their elements, which are copied and copied back).  Gradients must not share memory.
+    Of a sharded gradient (one with ``to_local()``) this rank's shard is scaled."""
     parameters, max_norm = _list_of(parameters), _bound(max_norm)
     if ops._native is not None and parameters and getattr(total_norm, "is_cuda", False):
         device = ops._device()

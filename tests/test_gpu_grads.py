@@ -454,3 +454,48 @@ def test_shards(gpu, mesh, kind):
     with pytest.raises((TypeError, RuntimeError), match="shard|parallel layout"):
         hpfp8.get_total_norm(grads)
     assert all(torch.equal(t.cpu(), w) for t, w in zip(locals_, clipped(before, n, 0.5 * float(n))))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_gradients_in_another_order_are_read_and_written_where_they_are(gpu, native, monkeypatch):
+    """Transposed and channels_last gradients are memory without gaps: no copy of one is made, whether there is something to clip or not; with gaps
+    between the elements, or elements that lie on one another, it is."""
+    import hpfp8
+    from hpfp8 import ops
+    if not native:
+        monkeypatch.setattr(ops, "_native", None)
+    g = torch.Generator().manual_seed(5)
+    grads = [torch.randn((1024, 2050), generator=g).to(gpu).t(), torch.randn((16, 64, 33, 35), generator=g).half().to(gpu).to(memory_format=torch.channels_last),
+             torch.randn((5, 7, 3, 1), generator=g).to(gpu).to(torch.bfloat16).permute(2, 3, 0, 1)]
+    cpu = [t.cpu() for t in grads]
+    ps = []
+    for t in grads:
+        p = torch.nn.Parameter(torch.zeros((1,), dtype=t.dtype, device=gpu).expand(t.shape))
+        p.grad = t
+        ps.append(p)
+    at = [(t.data_ptr(), t.stride()) for t in grads]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    norm = hpfp8.get_total_norm(grads)
+    held = hpfp8.clip_grad_norm_(ps, 1e9)
+    hpfp8.clip_grads_with_norm_(ps, 2e9, norm)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 17          # (the smallest two copies would be 2 MiB)
+    near(norm, norm64(cpu, 2.0))
+    assert torch.equal(held, norm) and all(torch.equal(t.cpu(), c) for t, c in zip(grads, cpu))
+    hpfp8.clip_grad_norm_(ps, 1.0)
+    hpfp8.clip_grads_with_norm_(ps, 1.0, torch.tensor(2.0, device=gpu))
+    assert torch.cuda.max_memory_allocated() - before < 1 << 17
+    want = clipped(clipped(cpu, norm, 1.0), torch.tensor(2.0), 1.0)
+    assert all(torch.equal(t.cpu(), w) for t, w in zip(grads, want)) and at == [(t.data_ptr(), t.stride()) for t in grads]
+    # gaps, and one value for a whole row: the norm counts elements, not memory
+    wide = torch.randn((64, 200), generator=g).to(gpu)
+    around = wide.clone()
+    apart = [wide.t()[3:90], wide[:, 100:101].expand(64, 9), wide[:, 120], torch.zeros((0, 4), device=gpu).t()]
+    near(hpfp8.get_total_norm(apart), norm64([t.cpu() for t in apart], 2.0))
+    q = torch.nn.Parameter(torch.zeros((1,), device=gpu).expand(87, 64))
+    q.grad = apart[0]
+    norm = hpfp8.clip_grad_norm_([q], 1.0)
+    near(norm, norm64([around.t()[3:90].cpu()], 2.0))
+    around.t()[3:90] = clipped([around.t()[3:90].cpu()], norm, 1.0)[0].to(gpu)
+    assert torch.equal(wide, around)
