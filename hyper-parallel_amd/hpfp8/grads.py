@@ -2,12 +2,13 @@
 
 A parameter's gradient is its ``main_grad`` where `apply_grad_on_fp32_main_grad` has made one (which torch's functions know nothing of), otherwise
 its ``grad``.  The norm of all gradients is one pass over them and their clipping another, in one launch for each 250 tensors, with nothing read on
-the host; tensors of bfloat16, float16 and float32 go together.
+the host; tensors of bfloat16, float16 and float32 go together.  Orders other than 1, 2 and inf are refused, and ``foreach``, which chooses between
+torch's two forms, is taken and changes nothing.
 """
 from __future__ import annotations
 
 import math
-from typing import Iterable, List, Union
+from typing import Iterable, List, Optional, Union
 
 import torch
 
@@ -85,14 +86,16 @@ def _raise_for_nonfinite(norm, norm_type) -> None:
 
 
 @torch.no_grad()
-def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+def get_total_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                   foreach: Optional[bool] = None) -> torch.Tensor:
     """torch.nn.utils.get_total_norm: the norm (of order 1, 2 or inf) of all elements of the tensors taken together, a 0-dim float32 tensor on the
     current GPU.  Sums are in 64 bits and in a fixed order: the same bits every time.  The norm over several ranks' shards is that of their norms
     (for order 2 the root of the sum of their squares): reduce it, then `clip_grads_with_norm_`."""
     tensors = _list_of(tensors)
     power = _power(norm_type)
     if torch.overrides.has_torch_function(tensors):
-        return torch.overrides.handle_torch_function(get_total_norm, tensors, tensors, norm_type, error_if_nonfinite)
+        return torch.overrides.handle_torch_function(get_total_norm, tensors, tensors, norm_type, error_if_nonfinite,
+                                                     **({} if foreach is None else dict(foreach=foreach)))
     norm = None
     if ops._native is not None and tensors:
         device = ops._device()
@@ -145,7 +148,8 @@ def _clip(grads, max_norm, total_norm) -> None:
 
 
 @torch.no_grad()
-def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor) -> None:
+def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor,
+                          foreach: Optional[bool] = None) -> None:
     """torch.nn.utils.clip_grads_with_norm_: every gradient times min(1, max_norm / (total_norm + 1e-6)) in place, rounded once.  Where that is 1
     nothing is read or written (but of gradients with gaps between their elements, which are copied and copied back).  Gradients must not share memory.
     Of a sharded gradient (one with ``to_local()``) this rank's shard is scaled."""
@@ -161,7 +165,7 @@ def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]
 
 @torch.no_grad()
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
-                    error_if_nonfinite: bool = False) -> torch.Tensor:
+                    error_if_nonfinite: bool = False, foreach: Optional[bool] = None) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_ for gradients in ``grad`` and in ``main_grad``: their total norm (a 0-dim float32 tensor), and the gradients
     scaled in place so that it is at most ``max_norm``.  Sharded gradients have no norm on one rank: `get_total_norm` of the shards, a reduction over
     the ranks and `clip_grads_with_norm_` take its place."""

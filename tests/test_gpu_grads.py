@@ -499,3 +499,17 @@ def test_gradients_in_another_order_are_read_and_written_where_they_are(gpu, nat
     near(norm, norm64([around.t()[3:90].cpu()], 2.0))
     around.t()[3:90] = clipped([around.t()[3:90].cpu()], norm, 1.0)[0].to(gpu)
     assert torch.equal(wide, around)
+
+
+@pytest.mark.parametrize("foreach", [None, True, False])
+def test_foreach_changes_nothing(gpu, foreach):
+    import hpfp8
+    ts = [t.to(gpu) for t in tensors([1000, 70, 5], 2)]
+    norm = hpfp8.get_total_norm(ts, foreach=foreach)
+    near(norm, norm64([t.cpu() for t in ts], 2.0))
+    one, other = params([t.clone() for t in ts]), params([t.clone() for t in ts])
+    assert torch.equal(hpfp8.clip_grad_norm_(one, 1.0, 2.0, False, foreach), norm)
+    hpfp8.clip_grads_with_norm_(other, 1.0, norm, foreach=foreach)
+    for a, b, w in zip(one, other, clipped([t.cpu() for t in ts], norm, 1.0)):
+        a, b = (q.grad if q.grad is not None else q.main_grad for q in (a, b))
+        assert torch.equal(a.cpu(), w) and torch.equal(b.cpu(), w)

@@ -317,3 +317,34 @@ def test_sharded_gradients_without_a_norm_over_the_ranks_are_refused(launched):
     with pytest.raises(TypeError, match="total_norm must be"):
         hpfp8.clip_grads_with_norm_(p, 1.0, g)
     assert not launched
+
+
+def test_the_gradients_functions_take_torchs_arguments(launched):
+    """By name and by place; foreach chooses between torch's own two forms and changes nothing here."""
+    import inspect
+    import hpfp8
+    for name in ("get_total_norm", "clip_grads_with_norm_", "clip_grad_norm_"):
+        ours, theirs = (inspect.signature(getattr(m, name)).parameters for m in (hpfp8, torch.nn.utils))
+        assert [(p.name, p.default, p.kind) for p in ours.values()] == [(p.name, p.default, p.kind) for p in theirs.values()]
+    x = torch.zeros(8, dtype=torch.float64)
+    p = torch.nn.Parameter(torch.zeros(8))
+    for foreach in (True, False, None):
+        for f in (lambda: hpfp8.get_total_norm([x], 2.0, False, foreach), lambda: hpfp8.get_total_norm([x], foreach=foreach)):
+            with pytest.raises(TypeError, match="tensor 0 must be a dense tensor"):
+                f()
+        assert hpfp8.clip_grads_with_norm_([p], 1.0, torch.ones(()), foreach) is None and hpfp8.clip_grads_with_norm_([p], 1.0, 1.0, foreach=foreach) is None
+    assert not launched
+
+
+def test_a_subclass_is_handed_the_norm_with_foreach():
+    import hpfp8
+    seen = []
+
+    class Recording(torch.Tensor):
+        @classmethod
+        def __torch_function__(cls, func, types, args=(), kwargs=None):
+            seen.append((func.__name__, args[1:], kwargs))
+            return "handed"
+    x = torch.zeros(4).as_subclass(Recording)
+    assert hpfp8.get_total_norm([x], 1.0) == "handed" and hpfp8.get_total_norm([x], 1.0, foreach=True) == "handed"
+    assert seen == [("get_total_norm", (1.0, False), {}), ("get_total_norm", (1.0, False), dict(foreach=True))]
