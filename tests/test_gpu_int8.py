@@ -606,3 +606,31 @@ def test_the_native_backward_takes_the_codes_that_the_package_makes(gpu, out, fo
     finally:
         ops._native.bind_int8_backward(int8._int8_backward)
     assert same(dx, want)
+
+
+@pytest.mark.parametrize("cols", [128, 512, 2048, 16512])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [9, 99])
+def test_products_of_rows_at_the_edges(gpu, cols, dtype, tokens):
+    """Bit for bit from the codes, with a weight whose rows cancel the largest values of a type or let them overflow to an infinity, as one rounding
+    to the type does; tokens: few rows, and tiles."""
+    import hpfp8
+    top = torch.finfo(dtype).max
+    x = torch.zeros((tokens, cols), dtype=torch.float64)
+    x[1, 3] = 1e-14
+    x[2, 5], x[2, 9] = -1e-39, 5e-40
+    x[3, 0], x[3, 1] = top, -top
+    x[4] = torch.arange(cols, dtype=torch.float64) % 255 - 127
+    x[5, 0], x[5, 1:5] = 127, torch.tensor([0.5, 1.5, -2.5, 126.5])
+    x[6, 0], x[6, 1] = top, top
+    x = x.to(dtype)
+    w = torch.ones((128, cols), dtype=dtype)
+    w[1::2, 1] = -1
+    w[2::4] *= 0.001
+    codes, scale = quantized(x.float().numpy())
+    wq, sw = quantized(w.float().numpy())
+    with np.errstate(over="ignore"):
+        want = product(codes, scale, wq, sw, None, dtype)
+    y = hpfp8.int8_linear(x.to(gpu), hpfp8.quantize_weight_int8(w.to(gpu)))
+    assert same(y, want)
+    assert (want[0] == 0).all() and torch.isinf(want[3, 1]) and want[3, 0] == 0 and torch.isfinite(want[[1, 2, 4, 5]].float()).all()
