@@ -39,9 +39,9 @@
 //     grouped along the contraction (MoE wgrad: an expert owns a range of k-blocks of both operands and
 //     its own c); bf16 or fp32 output, optionally added onto what c holds.
 //   * The same tiles multiply int8 codes (a k-block is two instructions of 64): sums are int32 and exact, so there is nothing to scale
-//     before a tile's end.  4096 x 36864 x 7168 760 to 800 us, 2.7 to 2.85 POP/s, bound by power: on random codes the matrix units are busy in 76 %
-//     of the cycles of a clock of 1.7 GHz and less, on zeros the same product takes 660 us; per tensor in E4M3 740.  1531 x 5120 x 2048 21 us, 1531 x
-//     2048 x 5120 25 to 28 us.
+//     before a tile's end.  4096 x 36864 x 7168 760 to 820 us, 2.6 to 2.85 POP/s, bound by power: on random codes the matrix units are busy in 76 %
+//     of the cycles of a clock of 1.7 GHz and less, on zeros the same product takes 660 us; per tensor in E4M3 740.  One behind the other it takes 780 us
+//     (uniform codes up to 60) to 960 (normally distributed, at the 1.43 GHz that are left).  1531 x 5120 x 2048 21 us, 1531 x 2048 x 5120 25 to 28 us.
 #include <atomic>
 #include <type_traits>
 
